@@ -68,6 +68,10 @@ extern "C" {
                                    /* masses place the target in no slice's own masses  */
                                    /* (states, masses and draw step from other inputs); */
                                    /* id -1, lp NaN                                     */
+#define DSV41_STATUS_REPEATED 64   /* a teacher's list names a token twice (loss NaN)   */
+#define DSV41_STATUS_BAD_TEACHER 128 /* teacher log-probs NaN or +inf, or without mass  */
+                                   /* to renormalize, or with more than 1.01 beside a   */
+                                   /* rest (loss NaN)                                   */
 
 /*
  * Row sampler.  For each row r of logits[rows, vocab]:
@@ -469,6 +473,121 @@ typedef struct dsv41_grpo_desc {
 #define DSV41_GRPO_M_APPROX_KL 5
 #define DSV41_GRPO_METRICS 6
 
+/*
+ * Scores of rows of logits [rows, vocab], whose distribution is p = softmax(x / temperature); x = -inf
+ * is a masked token, of probability 0:
+ *   out_logprob[r] = log p of targets[r]; out_rank[r] = 1 + the number of tokens before it in the order
+ *     (logit desc, index asc), with -0 equal to +0;
+ *   out_entropy[r] = -sum p log p;
+ *   out_top_ids / out_top_logprob[r, 0..top_k): the first tokens of that order; -1 and -inf past the
+ *     unmasked ones;
+ *   out_stats[r, 0..4): what dsv41_scores_grad_run needs (or NULL).
+ * A row with a NaN, a +inf or no unmasked token: NaN, ids -1, rank 0, DSV41_STATUS_NONFINITE.  A target
+ * outside [0, vocab): log-prob NaN, rank 0, DSV41_STATUS_BAD_TARGET.
+ * The reference's per-step log_softmax (dsv41_train/rl/rollout.py:144-150) and the token log-probs that
+ * rollout_manager/backends/vllm_actor.py:260 takes from an engine are the log-prob; the alternatives
+ * and ranks are that engine's `logprobs` output.
+ */
+typedef struct dsv41_scores_desc {
+  uint32_t struct_size; /* = sizeof(dsv41_scores_desc) */
+  int32_t rows;
+  int32_t vocab;             /* at most 2^21 */
+  int32_t logits_dtype;      /* DSV41_DTYPE_F32 or DSV41_DTYPE_BF16 */
+  int64_t logits_row_stride; /* in elements, >= vocab, or 0: every row the same */
+  const void* logits;        /* [rows, vocab] */
+  const int64_t* targets;    /* [rows] or NULL */
+  float temperature;         /* in [1e-30, 1e30] */
+  int32_t top_k;             /* in [0, min(vocab, 1024)] */
+  float* out_logprob;        /* [rows]; required with targets */
+  int64_t* out_rank;         /* [rows]; required with targets */
+  float* out_entropy;        /* [rows] */
+  int64_t* out_top_ids;      /* [rows, top_k] */
+  float* out_top_logprob;    /* [rows, top_k] */
+  int32_t* out_status;       /* [rows] */
+  double* out_stats;         /* [rows, 4] or NULL */
+} dsv41_scores_desc;
+
+/*
+ * Gradient of dsv41_scores_run with respect to the logits, in their dtype:
+ *   out_i = (1 / temperature) (grad_logprob ([i = target] - p_i) - grad_entropy p_i (log p_i + entropy)
+ *                              + sum_k grad_top_k ([i = top_ids_k] - p_i))
+ * NULL gradients count as zero; entries of top_ids below 0 carry none.  A row whose gradients are all
+ * zero is written as zeros and not read.
+ */
+typedef struct dsv41_scores_grad_desc {
+  uint32_t struct_size; /* = sizeof(dsv41_scores_grad_desc) */
+  int32_t rows;
+  int32_t vocab;
+  int32_t logits_dtype;
+  int64_t logits_row_stride;
+  const void* logits;        /* the forward's */
+  const int64_t* targets;    /* the forward's; required with grad_logprob */
+  const int64_t* top_ids;    /* the forward's [rows, top_k]; required with grad_top */
+  float temperature;
+  int32_t top_k;
+  const double* stats;       /* the forward's out_stats */
+  const float* grad_logprob; /* [rows] or NULL */
+  const float* grad_entropy; /* [rows] or NULL */
+  const float* grad_top;     /* [rows, top_k] or NULL */
+  void* out;                 /* [rows, vocab], rows vocab elements apart */
+} dsv41_scores_grad_desc;
+
+#define DSV41_TAIL_RENORMALIZE 0
+#define DSV41_TAIL_REST 1
+
+/*
+ * Divergence of a student's rows of logits from a teacher's top tokens (no reference counterpart: the
+ * learning losses beside it are dsv41_grpo_run and dsv41_token_tis_run).  p = softmax(x / temperature)
+ * over the vocabulary; the teacher's list of row r has the entries k with teacher_ids[r, k] >= 0, whose
+ * other values are ignored, too, where the id is negative.
+ *   DSV41_TAIL_RENORMALIZE: q = softmax of the list's teacher_logprob (logits divided by the
+ *     temperature do as well); out_loss[r] = sum_k q_k (log q_k - log p_k).
+ *   DSV41_TAIL_REST: q_k = exp(teacher_logprob), q_rest = 1 - sum q_k (below 2^-20: 0) and p_rest the
+ *     student's mass outside the list; out_loss[r] = sum_k q_k (log q_k - log p_k)
+ *     + q_rest (log q_rest - log p_rest).
+ * A row with an empty list: 0, and the logits are not read.  An id at or above vocab, a token named
+ * twice, teacher log-probs that are none: NaN and a status bit (BAD_TARGET, REPEATED, BAD_TEACHER).
+ * A loss that is not finite: DSV41_STATUS_NONFINITE.
+ */
+typedef struct dsv41_distill_desc {
+  uint32_t struct_size; /* = sizeof(dsv41_distill_desc) */
+  int32_t rows;
+  int32_t vocab;             /* at most 2^21 */
+  int32_t logits_dtype;      /* DSV41_DTYPE_F32 or DSV41_DTYPE_BF16 */
+  int64_t logits_row_stride; /* in elements, >= vocab, or 0: every row the same */
+  const void* logits;        /* [rows, vocab] */
+  const int64_t* teacher_ids;   /* [rows, top_k]; negative: no entry */
+  const float* teacher_logprob; /* [rows, top_k] */
+  float temperature;         /* in [1e-30, 1e30] */
+  int32_t top_k;             /* > 0 */
+  int32_t tail;              /* DSV41_TAIL_* */
+  float* out_loss;           /* [rows] */
+  int32_t* out_status;       /* [rows] */
+  double* out_stats;         /* [rows, 6] or NULL: what dsv41_distill_grad_run needs */
+} dsv41_distill_desc;
+
+/*
+ * Gradient of dsv41_distill_run with respect to the logits, in their dtype: with Q = sum q + q_rest,
+ *   grad_loss / temperature times (Q p_k - q_k) for the list's tokens and p_i (Q - q_rest / p_rest) for
+ *   the others (Q = 1 and q_rest = 0 when renormalized).
+ * A row with an empty list or a zero grad_loss is written as zeros and not read.
+ */
+typedef struct dsv41_distill_grad_desc {
+  uint32_t struct_size; /* = sizeof(dsv41_distill_grad_desc) */
+  int32_t rows;
+  int32_t vocab;
+  int32_t logits_dtype;
+  int64_t logits_row_stride;
+  const void* logits;           /* the forward's, like the lists */
+  const int64_t* teacher_ids;
+  const float* teacher_logprob;
+  float temperature;
+  int32_t top_k;
+  const double* stats;       /* the forward's out_stats */
+  const float* grad_loss;    /* [rows] */
+  void* out;                 /* [rows, vocab], rows vocab elements apart */
+} dsv41_distill_grad_desc;
+
 /* ABI identity. */
 int dsv41_abi_version(void);
 size_t dsv41_sampler_desc_size(void);
@@ -482,6 +601,10 @@ size_t dsv41_sampler_shard_desc_size(void);
 size_t dsv41_sampler_merge_desc_size(void);
 size_t dsv41_sampler_full_shard_desc_size(void);
 size_t dsv41_sampler_full_finish_desc_size(void);
+size_t dsv41_scores_desc_size(void);
+size_t dsv41_scores_grad_desc_size(void);
+size_t dsv41_distill_desc_size(void);
+size_t dsv41_distill_grad_desc_size(void);
 const char* dsv41_last_error(void);
 
 /* Sampler: replaces rollout.py:144-150 for a [rows, vocab] batch.
@@ -569,6 +692,20 @@ int dsv41_token_tis_run(const dsv41_token_tis_desc* desc, void* workspace, size_
 size_t dsv41_grpo_workspace_bytes(const dsv41_grpo_desc* desc);
 int dsv41_grpo_run(const dsv41_grpo_desc* desc, void* workspace, size_t workspace_bytes,
                    void* stream /* hipStream_t */);
+
+/* Scores of rows of logits, and their gradient.  Workspace (8-byte aligned, contents need no
+ * initialisation): rows * slices * (24 + 8 top_k) bytes where the rows are cut, none otherwise. */
+size_t dsv41_scores_workspace_bytes(const dsv41_scores_desc* desc);
+int dsv41_scores_run(const dsv41_scores_desc* desc, void* workspace, size_t workspace_bytes,
+                     void* stream /* hipStream_t */);
+int dsv41_scores_grad_run(const dsv41_scores_grad_desc* desc, void* stream /* hipStream_t */);
+
+/* Distillation from a teacher's top tokens, and its gradient.  Workspace (8-byte aligned, contents
+ * need no initialisation): rows * slices * 32 bytes where the rows are cut, none otherwise. */
+size_t dsv41_distill_workspace_bytes(const dsv41_distill_desc* desc);
+int dsv41_distill_run(const dsv41_distill_desc* desc, void* workspace, size_t workspace_bytes,
+                      void* stream /* hipStream_t */);
+int dsv41_distill_grad_run(const dsv41_distill_grad_desc* desc, void* stream /* hipStream_t */);
 
 /* What a checked call asks after its launches: returns 1 when some of the n statuses is
  * nonzero, plus 2 when some of the n_ids ids lies outside [0, limit) (0: neither), or a negative

@@ -24,4 +24,8 @@ extern "C" size_t dsv41_sampler_shard_desc_size(void) { return sizeof(dsv41_samp
 extern "C" size_t dsv41_sampler_merge_desc_size(void) { return sizeof(dsv41_sampler_merge_desc); }
 extern "C" size_t dsv41_sampler_full_shard_desc_size(void) { return sizeof(dsv41_sampler_full_shard_desc); }
 extern "C" size_t dsv41_sampler_full_finish_desc_size(void) { return sizeof(dsv41_sampler_full_finish_desc); }
+extern "C" size_t dsv41_scores_desc_size(void) { return sizeof(dsv41_scores_desc); }
+extern "C" size_t dsv41_scores_grad_desc_size(void) { return sizeof(dsv41_scores_grad_desc); }
+extern "C" size_t dsv41_distill_desc_size(void) { return sizeof(dsv41_distill_desc); }
+extern "C" size_t dsv41_distill_grad_desc_size(void) { return sizeof(dsv41_distill_grad_desc); }
 extern "C" const char* dsv41_last_error(void) { return dsv41::g_last_error.c_str(); }

@@ -1,0 +1,349 @@
+// distill.hip — divergence of a student's rows of logits from a teacher's top tokens, and its gradient.
+//
+// One row: student logits x [V], p = softmax(x / T); the teacher's list of tokens with log-probs lq
+// (entries with a negative id are none).  With m = max x, d_i = (x_i - m) / T, S = sum exp(d_i), and
+// S_rest the part of S outside the list:
+//   renormalize: q = softmax(lq) over the list;  L = sum_k q_k (log q_k - log p_k)
+//   rest: q_k = exp(lq_k), q_rest = 1 - sum q_k, p_rest = S_rest / S;
+//         L = sum_k q_k (lq_k - log p_k) + q_rest (log q_rest - log p_rest)
+//   dL/dx_k = (Q p_k - q_k) / T in the list, dL/dx_i = p_i (Q - q_rest / p_rest) / T outside,
+//   Q = sum q + q_rest (1, and q_rest 0, when renormalized).
+// p_rest may be many orders below 1, so S_rest is summed by itself: the list's tokens are bits of a map
+// in LDS that the pass over the row treats as masked.  What is left of nearly cancelling terms, the
+// divergence, is formed in fp64 from the list's logits.  fp32 log-probs do not carry a rest mass below
+// 2^-20, which counts as none.
+//
+// Forward: one read of the row; backward: one read, one write.
+#include <math.h>
+
+#include "row_scan.h"
+
+namespace dsv41 {
+namespace distill {
+
+using rows::bf16_t;
+using rows::Cut;
+using rows::Elem;
+using rows::GROUP;
+using rows::NT;
+using rows::Scale;
+using rows::State;
+using rows::WAVES;
+
+constexpr int MAX_LEN = 5120 * 32;  // elements of one slice: 20 KB of bits
+constexpr double REST_FLOOR = 0x1p-20;
+constexpr double MOST_MASS = 1.01;  // log-probs rounded to bf16 may add up to 1 + 2^-8 |lq| or so
+constexpr int STATS = 6;            // per row: m, S, others' factor, Q, log normalizer of the list, live
+
+struct SliceState {
+  State s;
+  int32_t flags, pad;
+};
+
+struct Params {
+  const void* logits;
+  int64_t stride;
+  const int64_t* ids;
+  const float* lq;
+  int rows, V, K, slices, len, rest;
+  Scale sc;
+  float* out_loss;
+  int32_t* out_status;
+  double* out_stats;
+  SliceState* states;  // [rows, slices]
+};
+
+struct Shared {
+  uint32_t named[MAX_LEN / 32];
+  double red[WAVES];
+  int flags;
+};
+constexpr int LIVE = 1 << 16;  // the list has an entry (above the status bits)
+
+__device__ void write_row(const Params& p, int row, float loss, int status, double m, double S, double others, double Q,
+                          double log_z, bool live) {
+  if (threadIdx.x) return;
+  p.out_loss[row] = loss;
+  p.out_status[row] = status;
+  if (p.out_stats) {
+    double* o = p.out_stats + (int64_t)row * STATS;
+    o[0] = m;
+    o[1] = S;
+    o[2] = others;
+    o[3] = Q;
+    o[4] = log_z;
+    o[5] = live ? 1.0 : 0.0;
+  }
+}
+
+// The row's divergence from the sums outside its list and the list itself.
+template <typename T>
+__device__ void finish(const Params& p, int row, State st, int flags, double* red) {
+  if (!(flags & LIVE)) {
+    write_row(p, row, 0.f, 0, 0.0, 1.0, 0.0, 0.0, 0.0, false);
+    return;
+  }
+  if (flags != LIVE) {
+    write_row(p, row, NAN, flags & ~LIVE, NAN, NAN, NAN, NAN, 0.0, true);
+    return;
+  }
+  const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.stride;
+  const int64_t* ids = p.ids + (int64_t)row * p.K;
+  const float* lq = p.lq + (int64_t)row * p.K;
+  double m = st.m, top = -INFINITY;
+  int bad = 0;
+  for (int k = threadIdx.x; k < p.K; k += NT)
+    if (ids[k] >= 0) {
+      m = fmax(m, (double)Elem<T>::one(x + ids[k]));
+      top = fmax(top, (double)lq[k]);
+      bad |= !(lq[k] < INFINITY);
+    }
+  m = rows::block_max<WAVES>(m, red);
+  top = p.rest ? 0.0 : rows::block_max<WAVES>(top, red);
+  bad = __syncthreads_or(bad || !(top > -INFINITY));
+  double Sn = 0.0, W = 0.0, WL = 0.0, WD = 0.0;
+  if (!bad)
+    for (int k = threadIdx.x; k < p.K; k += NT)
+      if (ids[k] >= 0) {
+        const double d = ((double)Elem<T>::one(x + ids[k]) - m) * p.sc.inv_t, l = (double)lq[k] - top, w = exp(l);
+        Sn += exp(d);
+        if (w > 0.0) {
+          W += w;
+          WL += w * l;
+          WD += w * d;
+        }
+      }
+  Sn = rows::block_sum<WAVES>(Sn, red);
+  W = rows::block_sum<WAVES>(W, red);
+  WL = rows::block_sum<WAVES>(WL, red);
+  WD = rows::block_sum<WAVES>(WD, red);
+  if (st.S == 0.0)
+    st.U = 0.0;
+  else
+    rows::rebase(st.S, st.U, st.m, m, p.sc);
+  const double S_rest = st.S + p.sc.kappa * st.U, S = S_rest + Sn, ln_s = log(S);
+  const bool nonfinite = !(S > 0.0 && S < INFINITY);
+  if (bad || (p.rest && W > MOST_MASS)) {
+    write_row(p, row, NAN, DSV41_STATUS_BAD_TEACHER, NAN, NAN, NAN, NAN, 0.0, true);
+    return;
+  }
+  double loss, others = 1.0, Q = 1.0, log_z = 0.0;
+  if (p.rest) {
+    double rest = 1.0 - W;
+    if (rest < REST_FLOOR) rest = 0.0;
+    loss = WL - WD + W * ln_s + (rest > 0.0 ? rest * (log(rest) - log(S_rest) + ln_s) : 0.0);
+    Q = W + rest;
+    others = S_rest > 0.0 ? Q - rest * S / S_rest : Q;
+  } else {
+    log_z = top + log(W);
+    loss = (WL - WD) / W - log(W) + ln_s;
+  }
+  const float l = nonfinite ? NAN : (float)loss;
+  write_row(p, row, l, nonfinite || !isfinite(l) ? DSV41_STATUS_NONFINITE : 0, m, nonfinite ? (double)NAN : S, others, Q,
+            log_z, true);
+}
+
+template <typename T>
+__global__ __launch_bounds__(NT) void distill_kernel(Params p) {
+  __shared__ Shared s;
+  const int row = blockIdx.x / p.slices, slice = blockIdx.x % p.slices, tid = threadIdx.x;
+  const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.stride;
+  const int begin = slice * p.len, len = min(p.len, p.V - begin);
+  const int64_t* ids = p.ids + (int64_t)row * p.K;
+  for (int i = tid; i < (len + 31) / 32; i += NT) s.named[i] = 0;
+  if (tid == 0) s.flags = 0;
+  __syncthreads();
+  int f = 0;
+  for (int k = tid; k < p.K; k += NT) {
+    const int64_t id = ids[k];
+    if (id < 0) continue;
+    f |= LIVE;
+    if (id >= p.V) f |= DSV41_STATUS_BAD_TARGET;
+    if (id >= begin && id < begin + len) {
+      const uint32_t i = (uint32_t)(id - begin), bit = 1u << (i & 31);
+      if (atomicOr(&s.named[i >> 5], bit) & bit) f |= DSV41_STATUS_REPEATED;
+    }
+  }
+  if (f) atomicOr(&s.flags, f);
+  __syncthreads();
+  const int flags = s.flags;
+  State st{0.0, 0.0, -INFINITY, 0};
+  if (flags == LIVE)
+    st = rows::scan<T, false, true>(x + begin, len, p.sc, INFINITY, 0, nullptr, s.named, s.red);
+  if (p.slices == 1) {
+    finish<T>(p, row, st, flags, s.red);
+  } else if (tid == 0) {
+    SliceState* o = p.states + (int64_t)row * p.slices + slice;
+    o->s = st;
+    o->flags = flags;
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(NT) void distill_join_kernel(Params p) {
+  __shared__ double red[WAVES];
+  __shared__ int flags;
+  const int row = blockIdx.x, tid = threadIdx.x;
+  SliceState in{{0.0, 0.0, -INFINITY, 0}, 0, 0};
+  if (tid == 0) flags = 0;
+  __syncthreads();
+  if (tid < p.slices) in = p.states[(int64_t)row * p.slices + tid];
+  if (in.flags) atomicOr(&flags, in.flags);
+  State st = in.s;
+  const double m = rows::block_max<WAVES>((double)st.m, red);
+  if (st.S == 0.0)
+    st.U = 0.0;
+  else
+    rows::rebase(st.S, st.U, st.m, m, p.sc);
+  st.m = (float)m;
+  st.S = rows::block_sum<WAVES>(st.S, red);
+  st.U = rows::block_sum<WAVES>(st.U, red);
+  finish<T>(p, row, st, flags, red);
+}
+
+struct GradParams {
+  const void* logits;
+  int64_t stride;
+  const int64_t* ids;
+  const float* lq;
+  int rows, V, K, slices, len;
+  Scale sc;
+  const double* stats;
+  const float* g;
+  void* out;  // [rows, V], rows V apart
+};
+
+// One read and one write of the row; the list's tokens are written again after the workgroup's barrier.
+// Rows whose list is empty or whose gradient is zero are zeros and are not read.
+template <typename T>
+__global__ __launch_bounds__(NT) void distill_grad_kernel(GradParams p) {
+  const int row = p.rows - 1 - (int)(blockIdx.x / p.slices), slice = blockIdx.x % p.slices;
+  const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.stride;
+  const int begin = slice * p.len, len = min(p.len, p.V - begin);
+  T* out = static_cast<T*>(p.out) + (int64_t)row * p.V + begin;
+  const double* st = p.stats + (int64_t)row * STATS;
+  const double g = (double)p.g[row] * p.sc.inv_t;
+  if (g == 0.0 || st[5] == 0.0) {
+    rows::fill_zero(out, len);
+    return;
+  }
+  const float m = (float)st[0];
+  const double S = st[1], Q = st[3], log_z = st[4];
+  const float A = (float)(g * st[2] / S);
+  rows::map(x + begin, out, len, [&](float v) { return A * __builtin_amdgcn_exp2f((v - m) * p.sc.c); });
+  __syncthreads();
+  const int64_t* ids = p.ids + (int64_t)row * p.K;
+  const float* lq = p.lq + (int64_t)row * p.K;
+  for (int k = threadIdx.x; k < p.K; k += NT) {
+    const int64_t i = ids[k] - begin;
+    if (ids[k] < 0 || i < 0 || i >= len) continue;
+    const double e = exp(((double)Elem<T>::one(x + begin + i) - m) * p.sc.inv_t);
+    rows::store_one(out + i, (float)(g * (Q * e / S - exp((double)lq[k] - log_z))));
+  }
+}
+
+Cut cut_of(int rows, int V) {
+  int64_t want = (1024 + rows - 1) / rows;
+  if (want > 64) want = 64;
+  if (want > V / 4096) want = V / 4096;
+  if (want < 1) want = 1;
+  int len = (int)(((V + want - 1) / want + GROUP - 1) / GROUP * GROUP);
+  if (len > MAX_LEN) len = MAX_LEN;
+  return {(V + len - 1) / len, len};
+}
+
+int check_desc(const dsv41_distill_desc* d) {
+  if (!d) return fail(DSV41_E_INVALID, "distillation descriptor is NULL");
+  if (d->struct_size != sizeof(dsv41_distill_desc))
+    return fail(DSV41_E_ABI, "dsv41_distill_desc size mismatch (rebuild the binding)");
+  if (int rc = rows::check_rows(d->rows, d->vocab, d->logits_dtype, d->logits_row_stride, d->logits, d->temperature)) return rc;
+  if (d->top_k <= 0) return fail(DSV41_E_INVALID, "teacher lists must have at least one entry");
+  if (!d->teacher_ids || !d->teacher_logprob) return fail(DSV41_E_INVALID, "teacher_ids and teacher_logprob are required");
+  if (d->tail != DSV41_TAIL_RENORMALIZE && d->tail != DSV41_TAIL_REST)
+    return fail(DSV41_E_INVALID, "tail must be DSV41_TAIL_RENORMALIZE or DSV41_TAIL_REST");
+  if (!d->out_loss || !d->out_status) return fail(DSV41_E_INVALID, "out_loss and out_status are required");
+  return rows::check_grid(d->rows, cut_of(d->rows, d->vocab));
+}
+
+size_t workspace_of(int rows, const Cut& c) { return c.slices == 1 ? 0 : (size_t)rows * c.slices * sizeof(SliceState); }
+
+}  // namespace distill
+}  // namespace dsv41
+
+using namespace dsv41;
+
+extern "C" size_t dsv41_distill_workspace_bytes(const dsv41_distill_desc* d) {
+  if (distill::check_desc(d)) return 0;
+  return distill::workspace_of(d->rows, distill::cut_of(d->rows, d->vocab));
+}
+
+extern "C" int dsv41_distill_run(const dsv41_distill_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = distill::check_desc(d)) return rc;
+  const rows::Cut c = distill::cut_of(d->rows, d->vocab);
+  const size_t need = distill::workspace_of(d->rows, c);
+  if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 8))
+    return fail(DSV41_E_WORKSPACE, "distillation workspace is missing, too small or not 8-byte aligned");
+  distill::Params p{};
+  p.logits = d->logits;
+  p.stride = d->logits_row_stride;
+  p.ids = d->teacher_ids;
+  p.lq = d->teacher_logprob;
+  p.rows = d->rows;
+  p.V = d->vocab;
+  p.K = d->top_k;
+  p.slices = c.slices;
+  p.len = c.len;
+  p.rest = d->tail == DSV41_TAIL_REST;
+  p.sc = rows::scale_of(d->temperature);
+  p.out_loss = d->out_loss;
+  p.out_status = d->out_status;
+  p.out_stats = d->out_stats;
+  p.states = static_cast<distill::SliceState*>(workspace);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const dim3 grid((unsigned)p.rows * (unsigned)p.slices), block(rows::NT);
+  if (d->logits_dtype == DSV41_DTYPE_F32) {
+    hipLaunchKernelGGL(distill::distill_kernel<float>, grid, block, 0, s, p);
+    if (p.slices > 1) hipLaunchKernelGGL(distill::distill_join_kernel<float>, dim3(p.rows), block, 0, s, p);
+  } else {
+    hipLaunchKernelGGL(distill::distill_kernel<rows::bf16_t>, grid, block, 0, s, p);
+    if (p.slices > 1) hipLaunchKernelGGL(distill::distill_join_kernel<rows::bf16_t>, dim3(p.rows), block, 0, s, p);
+  }
+  DSV41_HIP_CHECK(hipGetLastError());
+  return DSV41_OK;
+}
+
+extern "C" int dsv41_distill_grad_run(const dsv41_distill_grad_desc* d, void* stream) {
+  if (!d) return fail(DSV41_E_INVALID, "distillation gradient descriptor is NULL");
+  if (d->struct_size != sizeof(dsv41_distill_grad_desc))
+    return fail(DSV41_E_ABI, "dsv41_distill_grad_desc size mismatch (rebuild the binding)");
+  if (int rc = rows::check_rows(d->rows, d->vocab, d->logits_dtype, d->logits_row_stride, d->logits, d->temperature))
+    return rc;
+  if (d->top_k <= 0 || !d->teacher_ids || !d->teacher_logprob || !d->stats || !d->grad_loss || !d->out)
+    return fail(DSV41_E_INVALID, "teacher_ids, teacher_logprob, stats, grad_loss and out are required");
+  if ((uintptr_t)d->out % (d->logits_dtype == DSV41_DTYPE_F32 ? 4 : 2))
+    return fail(DSV41_E_INVALID, "out is not aligned to its type");
+  const rows::Cut c = rows::grad_cut(d->rows, d->vocab);
+  if (int rc = rows::check_grid(d->rows, c)) return rc;
+  distill::GradParams p{};
+  p.logits = d->logits;
+  p.stride = d->logits_row_stride;
+  p.ids = d->teacher_ids;
+  p.lq = d->teacher_logprob;
+  p.rows = d->rows;
+  p.V = d->vocab;
+  p.K = d->top_k;
+  p.slices = c.slices;
+  p.len = c.len;
+  p.sc = rows::scale_of(d->temperature);
+  p.stats = d->stats;
+  p.g = d->grad_loss;
+  p.out = d->out;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const dim3 grid((unsigned)p.rows * (unsigned)p.slices), block(rows::NT);
+  if (d->logits_dtype == DSV41_DTYPE_F32)
+    hipLaunchKernelGGL(distill::distill_grad_kernel<float>, grid, block, 0, s, p);
+  else
+    hipLaunchKernelGGL(distill::distill_grad_kernel<rows::bf16_t>, grid, block, 0, s, p);
+  DSV41_HIP_CHECK(hipGetLastError());
+  return DSV41_OK;
+}

@@ -79,13 +79,6 @@ constexpr int row_off(int i, int r) { return (i / 4) * (TL::BV / 2) + (i % 4) * 
 template <class TL>
 constexpr int col_off(int j) { return (j / 2) * (TL::BT / 2) + (j % 2) * 16; }
 
-// Two floats to bf16 (round to nearest even), packed low | high << 16.
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-  const bf16x2 v = {(__bf16)lo, (__bf16)hi};
-  return __builtin_bit_cast(uint32_t, v);
-}
-
 // Workgroup l of a grid padded to a multiple of 8 -> (block tb of n_tb, split of splits); false:
 // none.  Workgroups are dispatched round-robin over the 8 XCDs, and each XCD takes a run of
 // consecutive items, ordered so that the 32 it holds at a time form 8 blocks x 4 splits: they

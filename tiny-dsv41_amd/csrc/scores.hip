@@ -1,0 +1,531 @@
+// scores.hip — log-probs of given tokens from their logits, with rank, entropy and the top
+// alternatives, and the gradient of all of them with respect to the logits.
+//
+// For one row x [V] with p = softmax(x / T), m = max x and S = sum exp((x - m) / T):
+//   log p_i = (x_i - m) / T - log S,   H = log S - (1 / S) sum exp((x - m) / T) (x - m) / T
+// so one pass over the row (row_scan.h) gives everything but the alternatives.
+//
+// Alternatives.  The pass also leaves the maximum of each 32 consecutive elements in LDS.  Order the
+// elements by (logit desc, index asc) and the groups by (maximum desc, index asc): every element of the
+// top k lies in one of the first k groups.  For if its group G were not among them, k groups would come
+// before G, and each holds an element that comes before it: a larger one, or an equal one of a lower
+// index, since groups are index ranges.  So after the pass k groups at most are read again, whatever the
+// logits are, and those of their elements that reach the k-th group's maximum are sorted.
+//
+// A row of few is cut into slices, which leave their sums and their sorted lists in the workspace for a
+// second kernel.
+#include <math.h>
+
+#include "row_scan.h"
+
+namespace dsv41 {
+namespace scores {
+
+using rows::bf16_t;
+using rows::Cut;
+using rows::Elem;
+using rows::GROUP;
+using rows::NT;
+using rows::Scale;
+using rows::State;
+using rows::WAVES;
+
+constexpr int MAX_K = 1024;
+constexpr int MAX_GROUPS = 5120;                  // of one slice
+constexpr int MAX_LEN = MAX_GROUPS * GROUP;       // elements of one slice
+constexpr int LIST = MAX_K + MAX_K / 4 + 64;      // groups that are read again
+constexpr int BATCH = 2048;                       // elements or keys that one step may add to the buffer
+constexpr int BUF = 2 * BATCH;
+static_assert(BUF >= BATCH + MAX_K, "a compressed buffer takes a batch");
+static_assert(BUF * sizeof(uint64_t) >= MAX_GROUPS * sizeof(float), "the buffer stands over the group maxima");
+
+struct Params {
+  const void* logits;
+  int64_t stride;
+  const int64_t* targets;
+  int rows, V, K, slices, len;
+  Scale sc;
+  float* out_logprob;
+  int64_t* out_rank;
+  float* out_entropy;
+  int64_t* out_top_ids;
+  float* out_top_logprob;
+  int32_t* out_status;
+  double* out_stats;
+  State* states;   // [rows, slices]
+  uint64_t* keys;  // [rows, slices, K]
+};
+
+// A logit as an integer of the same order (-0 as +0), and back.
+__device__ __forceinline__ uint32_t order_of(float x) {
+  const uint32_t b = __float_as_uint(x + 0.0f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float logit_of(uint32_t o) {
+  return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
+}
+constexpr uint32_t ABOVE_MASKED = 0x00800000u;  // order_of(-inf) + 1
+// Element i of a row in (logit desc, index asc): larger keys come first.  0 is no element.
+__device__ __forceinline__ uint64_t key_of(float x, uint32_t i) { return (uint64_t)order_of(x) << 32 | (0xFFFFFFFFu - i); }
+
+struct Shared {
+  union {
+    uint64_t buf[BUF];
+    float group_max[MAX_GROUPS];
+  };
+  uint16_t list[LIST];
+  double red[WAVES];
+  int counts[2][WAVES];
+  int n;
+};
+
+// Descending bitonic sort of buf[0, n), padded with zeros to a power of two.  Every thread calls it.
+__device__ void sort_desc(uint64_t* buf, int n) {
+  int P = 64;
+  while (P < n) P <<= 1;
+  for (int i = n + threadIdx.x; i < P; i += NT) buf[i] = 0;
+  for (int k = 2; k <= P; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      __syncthreads();
+      for (int q = threadIdx.x; q < P / 2; q += NT) {
+        const int i = 2 * q - (q & (j - 1));
+        const uint64_t a = buf[i], b = buf[i + j];
+        if ((a < b) == ((i & k) == 0)) {
+          buf[i] = b;
+          buf[i + j] = a;
+        }
+      }
+    }
+  __syncthreads();
+}
+
+// Room for another batch: past BUF - BATCH keys, the first K in order are kept, and what follows has
+// to come before the last of them.  Every thread calls it behind a barrier.
+__device__ void make_room(Shared& s, int K, uint64_t& floor_key) {
+  const int n = s.n;
+  __syncthreads();
+  if (n <= BUF - BATCH) return;
+  sort_desc(s.buf, n);
+  floor_key = s.buf[K - 1];
+  __syncthreads();
+  if (threadIdx.x == 0) s.n = K;
+  __syncthreads();
+}
+
+__device__ __forceinline__ void push(Shared& s, uint64_t key) { s.buf[atomicAdd(&s.n, 1)] = key; }
+
+// How many of the workgroup's keys are at least `at`.
+template <int J>
+__device__ __forceinline__ int count_from(const uint32_t (&key)[J], uint32_t at, int* counts) {
+  int c = 0;
+#pragma unroll
+  for (int j = 0; j < J; ++j) c += __popcll(__ballot(key[j] >= at));
+  if ((threadIdx.x & 63) == 0) counts[threadIdx.x >> 6] = c;
+  __syncthreads();
+  c = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) c += counts[w];
+  return c;
+}
+
+// s.list = at least the first K groups in (maximum desc, index asc) of those that hold an unmasked
+// element, or all of them; returns their number, and in `least` a bound that the K-th reaches.
+__device__ int select_groups(Shared& s, int n, int K, float m, uint32_t& least) {
+  constexpr int J = MAX_GROUPS / NT;
+  uint32_t key[J];
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const int i = j * NT + (int)threadIdx.x;
+    key[j] = i < n ? order_of(s.group_max[i]) : 0u;
+  }
+  const int most = K + max(16, K / 4);
+  uint32_t lo = ABOVE_MASKED, hi = order_of(m) + 1u;
+  int turn = 0;
+  int c = count_from(key, lo, s.counts[0]);
+  while (c > most && hi - lo > 1u) {
+    const uint32_t mid = lo + ((hi - lo) >> 1);
+    turn ^= 1;
+    const int got = count_from(key, mid, s.counts[turn]);
+    if (got >= K) {
+      lo = mid;
+      c = got;
+    } else {
+      hi = mid;
+    }
+  }
+  least = lo;
+  if (threadIdx.x == 0) s.n = 0;
+  __syncthreads();
+  // those above `lo` in any order, and at most as many at `lo` as are wanted, from the lowest index
+  const bool all = c <= most;
+  const uint32_t from = all ? lo : hi;
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+    if (key[j] >= from) {
+      const int at = atomicAdd(&s.n, 1);
+      if (at < LIST) s.list[at] = (uint16_t)(j * NT + threadIdx.x);
+    }
+  __syncthreads();
+  int taken = min(s.n, LIST);
+  if (!all) {
+    for (int j = 0; j < J && j * NT < n && taken < K; ++j) {
+      const bool tie = key[j] == lo;
+      const uint64_t b = __ballot(tie);
+      const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+      __syncthreads();
+      if (lane == 0) s.counts[0][wave] = __popcll(b);
+      __syncthreads();
+      int before = taken, total = 0;
+      for (int w = 0; w < WAVES; ++w) {
+        if (w < wave) before += s.counts[0][w];
+        total += s.counts[0][w];
+      }
+      before += __popcll(b & ((1ull << lane) - 1ull));
+      if (tie && before < K) s.list[before] = (uint16_t)(j * NT + threadIdx.x);
+      taken = min(K, taken + total);
+    }
+  }
+  __syncthreads();
+  return taken;
+}
+
+// s.buf = the first K elements of x[0, len) in order (or as many as are not masked); returns their
+// number.  `first`: the index of x[0] in its row.
+template <typename T>
+__device__ int top_of(Shared& s, const T* x, int len, int first, int K, float m) {
+  constexpr int VEC = Elem<T>::VEC, LANES = GROUP / VEC, AT_ONCE = BATCH / GROUP;
+  uint32_t least;
+  const int groups = select_groups(s, (len + GROUP - 1) / GROUP, K, m, least);
+  if (threadIdx.x == 0) s.n = 0;
+  __syncthreads();
+  uint64_t floor_key = 0;
+  for (int b = 0; b < groups; b += AT_ONCE) {
+    make_room(s, K, floor_key);
+    const int g = b + (int)threadIdx.x / LANES;
+    if ((int)threadIdx.x < AT_ONCE * LANES && g < groups) {
+      const int i = (int)s.list[g] * LANES + (int)threadIdx.x % LANES;
+      float v[VEC];
+      if ((i + 1) * VEC <= len)
+        rows::load_full(x, i, v);
+      else
+        rows::load_edge(x, len, i, v);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const uint64_t key = key_of(v[j], (uint32_t)(first + i * VEC + j));
+        if ((uint32_t)(key >> 32) >= least && key > floor_key) push(s, key);
+      }
+    }
+    __syncthreads();
+  }
+  const int n = s.n;
+  sort_desc(s.buf, n);
+  return min(n, K);
+}
+
+// The row's outputs from its sums and its sorted list.
+__device__ void write_row(const Params& p, int row, State st, float xt, int64_t target, const uint64_t* top, int n_top) {
+  const double S = st.S + p.sc.kappa * st.U;
+  const bool bad = !(S > 0.0 && S < INFINITY);
+  const double m = st.m, ln_s = log(S);
+  const double entropy = bad ? (double)NAN : fmax(ln_s - st.U * (p.sc.inv_t / p.sc.c) / S, 0.0);
+  for (int i = threadIdx.x; i < p.K; i += NT) {
+    const uint64_t key = i < n_top ? top[i] : 0;
+    const int64_t at = (int64_t)row * p.K + i;
+    const bool none = bad || key == 0;
+    p.out_top_ids[at] = none ? -1 : (int64_t)(0xFFFFFFFFu - (uint32_t)key);
+    p.out_top_logprob[at] =
+        bad ? NAN : none ? -INFINITY : (float)(((double)logit_of((uint32_t)(key >> 32)) - m) * p.sc.inv_t - ln_s);
+  }
+  if (threadIdx.x) return;
+  int status = bad ? DSV41_STATUS_NONFINITE : 0;
+  if (p.targets) {
+    const bool outside = target < 0 || target >= p.V;
+    if (outside) status |= DSV41_STATUS_BAD_TARGET;
+    p.out_logprob[row] = bad || outside ? NAN : (float)(((double)xt - m) * p.sc.inv_t - ln_s);
+    p.out_rank[row] = bad || outside ? 0 : 1 + (int64_t)st.before;
+  }
+  p.out_entropy[row] = (float)entropy;
+  p.out_status[row] = status;
+  if (p.out_stats) {
+    double* o = p.out_stats + (int64_t)row * 4;
+    o[0] = m;
+    o[1] = bad ? (double)NAN : S;
+    o[2] = ln_s;
+    o[3] = entropy;
+  }
+}
+
+template <typename T, bool TOP>
+__global__ __launch_bounds__(NT) void scores_kernel(Params p) {
+  __shared__ Shared s;
+  const int row = blockIdx.x / p.slices, slice = blockIdx.x % p.slices;
+  const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.stride;
+  const int begin = slice * p.len, len = min(p.len, p.V - begin);
+  int64_t target = -1;
+  float xt = INFINITY;
+  if (p.targets) {
+    target = p.targets[row];
+    if (target >= 0 && target < p.V) xt = Elem<T>::one(x + target);
+  }
+  const State st =
+      rows::scan<T, TOP, false>(x + begin, len, p.sc, xt, target - begin, s.group_max, nullptr, s.red);
+  int n = 0;
+  if constexpr (TOP) n = top_of(s, x + begin, len, begin, p.K, st.m);
+  if (p.slices == 1) {
+    write_row(p, row, st, xt, target, s.buf, n);
+    return;
+  }
+  const int64_t at = (int64_t)row * p.slices + slice;
+  if (threadIdx.x == 0) p.states[at] = st;
+  for (int i = threadIdx.x; i < p.K; i += NT) p.keys[at * p.K + i] = i < n ? s.buf[i] : 0;
+}
+
+// Joins the slices of a row.
+template <typename T>
+__global__ __launch_bounds__(NT) void scores_join_kernel(Params p) {
+  __shared__ Shared s;
+  const int row = blockIdx.x, tid = threadIdx.x;
+  const State* states = p.states + (int64_t)row * p.slices;
+  State st{0.0, 0.0, -INFINITY, 0};
+  if (tid < p.slices) st = states[tid];
+  const double m = rows::block_max<WAVES>((double)st.m, s.red);
+  if (st.S == 0.0)
+    st.U = 0.0;
+  else
+    rows::rebase(st.S, st.U, st.m, m, p.sc);
+  st.m = (float)m;
+  st.S = rows::block_sum<WAVES>(st.S, s.red);
+  st.U = rows::block_sum<WAVES>(st.U, s.red);
+  st.before = (int32_t)rows::block_sum<WAVES>((double)st.before, s.red);
+  int n = 0;
+  if (p.K) {
+    // each list holds K elements that come no later than its last, so the row's K-th comes no later
+    // than any of these lasts
+    const uint64_t* keys = p.keys + (int64_t)row * p.slices * p.K;
+    uint64_t least = 1;
+    for (int i = 0; i < p.slices; ++i) least = max(least, keys[(int64_t)i * p.K + p.K - 1]);
+    const int total = p.slices * p.K;
+    if (tid == 0) s.n = 0;
+    __syncthreads();
+    uint64_t floor_key = 0;
+    for (int b = 0; b < total; b += BATCH) {
+      make_room(s, p.K, floor_key);
+      for (int i = b + tid; i < min(total, b + BATCH); i += NT) {
+        const uint64_t key = keys[i];
+        if (key >= least && key > floor_key) push(s, key);
+      }
+      __syncthreads();
+    }
+    n = s.n;
+    sort_desc(s.buf, n);
+    n = min(n, p.K);
+  }
+  int64_t target = -1;
+  float xt = INFINITY;
+  if (p.targets) {
+    target = p.targets[row];
+    if (target >= 0 && target < p.V) xt = Elem<T>::one(static_cast<const T*>(p.logits) + (int64_t)row * p.stride + target);
+  }
+  write_row(p, row, st, xt, target, s.buf, n);
+}
+
+// ------------------------------------------------------------------------------------ gradient
+struct GradParams {
+  const void* logits;
+  int64_t stride;
+  const int64_t* targets;
+  const int64_t* top_ids;
+  int rows, V, K, slices, len;
+  Scale sc;
+  const double* stats;
+  const float* g_logprob;
+  const float* g_entropy;
+  const float* g_top;
+  void* out;  // [rows, V], rows V apart
+};
+
+// dx_i = (1 / T) (-(G + g_H (log p_i + H)) p_i + g_lp [i = t] + sum_k g_k [i = id_k]),  G = g_lp + sum_k g_k,
+// as e_i (A + B d_i) with e_i = 2^d_i and d_i = (x_i - m) c: one read and one write of the row.  The
+// tokens that have a gradient of their own are written again after the workgroup's barrier.
+template <typename T>
+__global__ __launch_bounds__(NT) void scores_grad_kernel(GradParams p) {
+  __shared__ double red[WAVES];
+  const int row = p.rows - 1 - (int)(blockIdx.x / p.slices), slice = blockIdx.x % p.slices;
+  const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.stride;
+  const int begin = slice * p.len, len = min(p.len, p.V - begin);
+  T* out = static_cast<T*>(p.out) + (int64_t)row * p.V + begin;
+  const int tid = threadIdx.x;
+  const int64_t t = p.targets && p.g_logprob ? p.targets[row] : -1;
+  const double g_lp = p.targets && p.g_logprob ? p.g_logprob[row] : 0.0, g_h = p.g_entropy ? p.g_entropy[row] : 0.0;
+  const int64_t* ids = p.g_top ? p.top_ids + (int64_t)row * p.K : nullptr;
+  const float* g_top = p.g_top ? p.g_top + (int64_t)row * p.K : nullptr;
+  double G = 0.0;
+  int any = g_lp != 0.0 || g_h != 0.0;
+  if (p.g_top) {
+    for (int k = tid; k < p.K; k += NT)
+      if (ids[k] >= 0) {
+        G += g_top[k];
+        any |= g_top[k] != 0.f;
+      }
+    G = rows::block_sum<WAVES>(G, red);
+    any = __syncthreads_or(any);
+  }
+  G += g_lp != 0.0 && (t < 0 || t >= p.V) ? (double)NAN : g_lp;
+  if (!any) {
+    rows::fill_zero(out, len);
+    return;
+  }
+  const double* st = p.stats + (int64_t)row * 4;
+  const float m = (float)st[0];
+  const double S = st[1];
+  const float A = (float)(-(G + g_h * (st[3] - st[2])) * p.sc.inv_t / S);
+  const float B = (float)(-g_h * p.sc.inv_t * p.sc.inv_t / (p.sc.c * S));
+  auto dense = [&](float v) {
+    const float d = (v - m) * p.sc.c;
+    return __builtin_amdgcn_exp2f(d) * __builtin_fmaf(B, fmaxf(d, -1000.f), A);
+  };
+  rows::map(x + begin, out, len, dense);
+  __syncthreads();
+  const float inv_t = (float)p.sc.inv_t;
+  int listed = 0;
+  if (p.g_top)
+    for (int k = tid; k < p.K; k += NT) {
+      const int64_t i = ids[k] - begin;
+      if (ids[k] < 0) continue;
+      listed |= ids[k] == t;
+      if (i >= 0 && i < len) {
+        const double own = (double)g_top[k] + (ids[k] == t ? g_lp : 0.0);
+        rows::store_one(out + i, dense(Elem<T>::one(x + begin + i)) + (float)(own * p.sc.inv_t));
+      }
+    }
+  listed = __syncthreads_or(listed);
+  if (!listed && tid == 0 && t >= begin && t < begin + len)
+    rows::store_one(out + (t - begin), dense(Elem<T>::one(x + t)) + (float)g_lp * inv_t);
+}
+
+// ---------------------------------------------------------------------------------------- host
+// Rows are cut where there are too few of them to occupy the GPU: into slices of at least 4096
+// elements, whose lists are at most an eighth of them, until there are 1024 workgroups.
+Cut cut_of(int rows, int V, int K) {
+  const int least = K * 8 > 4096 ? K * 8 : 4096;
+  int64_t want = (1024 + rows - 1) / rows;
+  if (want > 64) want = 64;
+  if (want > V / least) want = V / least;
+  if (want < 1) want = 1;
+  int len = (int)((V + want - 1) / want);
+  len = (len + GROUP - 1) / GROUP * GROUP;
+  if (len > MAX_LEN) len = MAX_LEN;
+  return {(V + len - 1) / len, len};
+}
+
+size_t workspace_of(int rows, int K, const Cut& c) {
+  return c.slices == 1 ? 0 : (size_t)rows * c.slices * (sizeof(State) + (size_t)K * sizeof(uint64_t));
+}
+
+template <typename T>
+void launch(const Params& p, hipStream_t s) {
+  const dim3 grid((unsigned)p.rows * (unsigned)p.slices);
+  if (p.K)
+    hipLaunchKernelGGL((scores_kernel<T, true>), grid, dim3(NT), 0, s, p);
+  else
+    hipLaunchKernelGGL((scores_kernel<T, false>), grid, dim3(NT), 0, s, p);
+  if (p.slices > 1) hipLaunchKernelGGL(scores_join_kernel<T>, dim3(p.rows), dim3(NT), 0, s, p);
+}
+
+int check_desc(const dsv41_scores_desc* d) {
+  if (!d) return fail(DSV41_E_INVALID, "scores descriptor is NULL");
+  if (d->struct_size != sizeof(dsv41_scores_desc))
+    return fail(DSV41_E_ABI, "dsv41_scores_desc size mismatch (rebuild the binding)");
+  if (int rc = rows::check_rows(d->rows, d->vocab, d->logits_dtype, d->logits_row_stride, d->logits, d->temperature)) return rc;
+  if (d->top_k < 0 || d->top_k > d->vocab) return fail(DSV41_E_INVALID, "top_k must lie in [0, vocabulary_size]");
+  if (d->top_k > MAX_K) return fail(DSV41_E_UNSUPPORTED, "top_k above 1024 is not supported");
+  if (!d->out_entropy || !d->out_status) return fail(DSV41_E_INVALID, "out_entropy and out_status are required");
+  if (d->targets && (!d->out_logprob || !d->out_rank))
+    return fail(DSV41_E_INVALID, "targets need out_logprob and out_rank");
+  if (d->top_k && (!d->out_top_ids || !d->out_top_logprob))
+    return fail(DSV41_E_INVALID, "top_k needs out_top_ids and out_top_logprob");
+  return rows::check_grid(d->rows, cut_of(d->rows, d->vocab, d->top_k));
+}
+
+}  // namespace scores
+}  // namespace dsv41
+
+using namespace dsv41;
+
+extern "C" size_t dsv41_scores_workspace_bytes(const dsv41_scores_desc* d) {
+  if (scores::check_desc(d)) return 0;
+  return scores::workspace_of(d->rows, d->top_k, scores::cut_of(d->rows, d->vocab, d->top_k));
+}
+
+extern "C" int dsv41_scores_run(const dsv41_scores_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = scores::check_desc(d)) return rc;
+  const rows::Cut c = scores::cut_of(d->rows, d->vocab, d->top_k);
+  const size_t need = scores::workspace_of(d->rows, d->top_k, c);
+  if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 8))
+    return fail(DSV41_E_WORKSPACE, "scores workspace is missing, too small or not 8-byte aligned");
+  scores::Params p{};
+  p.logits = d->logits;
+  p.stride = d->logits_row_stride;
+  p.targets = d->targets;
+  p.rows = d->rows;
+  p.V = d->vocab;
+  p.K = d->top_k;
+  p.slices = c.slices;
+  p.len = c.len;
+  p.sc = rows::scale_of(d->temperature);
+  p.out_logprob = d->out_logprob;
+  p.out_rank = d->out_rank;
+  p.out_entropy = d->out_entropy;
+  p.out_top_ids = d->out_top_ids;
+  p.out_top_logprob = d->out_top_logprob;
+  p.out_status = d->out_status;
+  p.out_stats = d->out_stats;
+  p.states = static_cast<rows::State*>(workspace);
+  p.keys = reinterpret_cast<uint64_t*>(p.states + (c.slices > 1 ? (int64_t)d->rows * c.slices : 0));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (d->logits_dtype == DSV41_DTYPE_F32)
+    scores::launch<float>(p, s);
+  else
+    scores::launch<rows::bf16_t>(p, s);
+  DSV41_HIP_CHECK(hipGetLastError());
+  return DSV41_OK;
+}
+
+extern "C" int dsv41_scores_grad_run(const dsv41_scores_grad_desc* d, void* stream) {
+  if (!d) return fail(DSV41_E_INVALID, "scores gradient descriptor is NULL");
+  if (d->struct_size != sizeof(dsv41_scores_grad_desc))
+    return fail(DSV41_E_ABI, "dsv41_scores_grad_desc size mismatch (rebuild the binding)");
+  if (int rc = rows::check_rows(d->rows, d->vocab, d->logits_dtype, d->logits_row_stride, d->logits, d->temperature))
+    return rc;
+  if (!d->stats || !d->out) return fail(DSV41_E_INVALID, "stats and out are required");
+  if ((uintptr_t)d->out % (d->logits_dtype == DSV41_DTYPE_F32 ? 4 : 2))
+    return fail(DSV41_E_INVALID, "out is not aligned to its type");
+  if (d->grad_logprob && !d->targets) return fail(DSV41_E_INVALID, "grad_logprob needs targets");
+  if (d->grad_top && (!d->top_ids || d->top_k <= 0)) return fail(DSV41_E_INVALID, "grad_top needs top_ids and top_k");
+  const rows::Cut c = rows::grad_cut(d->rows, d->vocab);
+  if (int rc = rows::check_grid(d->rows, c)) return rc;
+  scores::GradParams p{};
+  p.logits = d->logits;
+  p.stride = d->logits_row_stride;
+  p.targets = d->targets;
+  p.top_ids = d->top_ids;
+  p.rows = d->rows;
+  p.V = d->vocab;
+  p.K = d->grad_top ? d->top_k : 0;
+  p.slices = c.slices;
+  p.len = c.len;
+  p.sc = rows::scale_of(d->temperature);
+  p.stats = d->stats;
+  p.g_logprob = d->grad_logprob;
+  p.g_entropy = d->grad_entropy;
+  p.g_top = d->grad_top;
+  p.out = d->out;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const dim3 grid((unsigned)p.rows * (unsigned)p.slices);
+  if (d->logits_dtype == DSV41_DTYPE_F32)
+    hipLaunchKernelGGL(scores::scores_grad_kernel<float>, grid, dim3(rows::NT), 0, s, p);
+  else
+    hipLaunchKernelGGL(scores::scores_grad_kernel<rows::bf16_t>, grid, dim3(rows::NT), 0, s, p);
+  DSV41_HIP_CHECK(hipGetLastError());
+  return DSV41_OK;
+}

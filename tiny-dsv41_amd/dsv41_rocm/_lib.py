@@ -31,6 +31,11 @@ STATUS_BAD_UNIFORM = 4
 STATUS_RATIO_ZERO = 8
 STATUS_BAD_TARGET = 16
 STATUS_BAD_SLICES = 32
+STATUS_REPEATED = 64
+STATUS_BAD_TEACHER = 128
+
+TAIL_RENORMALIZE = 0
+TAIL_REST = 1
 
 
 class SamplerDesc(ctypes.Structure):
@@ -271,6 +276,79 @@ class SamplerFullFinishDesc(ctypes.Structure):
     ]
 
 
+# the fields that the descriptors of scores and distillation begin with
+_ROW_FIELDS = [
+    ("struct_size", ctypes.c_uint32),
+    ("rows", ctypes.c_int32),
+    ("vocab", ctypes.c_int32),
+    ("logits_dtype", ctypes.c_int32),
+    ("logits_row_stride", ctypes.c_int64),
+    ("logits", ctypes.c_void_p),
+]
+
+
+class ScoresDesc(ctypes.Structure):
+    """Mirror of dsv41_scores_desc."""
+
+    _fields_ = _ROW_FIELDS + [
+        ("targets", ctypes.c_void_p),
+        ("temperature", ctypes.c_float),
+        ("top_k", ctypes.c_int32),
+        ("out_logprob", ctypes.c_void_p),
+        ("out_rank", ctypes.c_void_p),
+        ("out_entropy", ctypes.c_void_p),
+        ("out_top_ids", ctypes.c_void_p),
+        ("out_top_logprob", ctypes.c_void_p),
+        ("out_status", ctypes.c_void_p),
+        ("out_stats", ctypes.c_void_p),
+    ]
+
+
+class ScoresGradDesc(ctypes.Structure):
+    """Mirror of dsv41_scores_grad_desc."""
+
+    _fields_ = _ROW_FIELDS + [
+        ("targets", ctypes.c_void_p),
+        ("top_ids", ctypes.c_void_p),
+        ("temperature", ctypes.c_float),
+        ("top_k", ctypes.c_int32),
+        ("stats", ctypes.c_void_p),
+        ("grad_logprob", ctypes.c_void_p),
+        ("grad_entropy", ctypes.c_void_p),
+        ("grad_top", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+    ]
+
+
+class DistillDesc(ctypes.Structure):
+    """Mirror of dsv41_distill_desc."""
+
+    _fields_ = _ROW_FIELDS + [
+        ("teacher_ids", ctypes.c_void_p),
+        ("teacher_logprob", ctypes.c_void_p),
+        ("temperature", ctypes.c_float),
+        ("top_k", ctypes.c_int32),
+        ("tail", ctypes.c_int32),
+        ("out_loss", ctypes.c_void_p),
+        ("out_status", ctypes.c_void_p),
+        ("out_stats", ctypes.c_void_p),
+    ]
+
+
+class DistillGradDesc(ctypes.Structure):
+    """Mirror of dsv41_distill_grad_desc."""
+
+    _fields_ = _ROW_FIELDS + [
+        ("teacher_ids", ctypes.c_void_p),
+        ("teacher_logprob", ctypes.c_void_p),
+        ("temperature", ctypes.c_float),
+        ("top_k", ctypes.c_int32),
+        ("stats", ctypes.c_void_p),
+        ("grad_loss", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+    ]
+
+
 FULL_DRAW_CDF = 0
 FULL_DRAW_RACE = 1
 FULL_DRAW_GREEDY = 2
@@ -292,6 +370,10 @@ EXPORTS = (
     "dsv41_sampler_merge_desc_size",
     "dsv41_sampler_full_shard_desc_size",
     "dsv41_sampler_full_finish_desc_size",
+    "dsv41_scores_desc_size",
+    "dsv41_scores_grad_desc_size",
+    "dsv41_distill_desc_size",
+    "dsv41_distill_grad_desc_size",
     "dsv41_last_error",
     "dsv41_sampler_workspace_bytes",
     "dsv41_sampler_run",
@@ -316,6 +398,12 @@ EXPORTS = (
     "dsv41_head_dx_workspace_bytes",
     "dsv41_head_dx_run",
     "dsv41_head_dw_run",
+    "dsv41_scores_workspace_bytes",
+    "dsv41_scores_run",
+    "dsv41_scores_grad_run",
+    "dsv41_distill_workspace_bytes",
+    "dsv41_distill_run",
+    "dsv41_distill_grad_run",
 )
 
 _lock = threading.Lock()
@@ -384,6 +472,16 @@ def _bind(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.dsv41_head_dw_run.restype = ctypes.c_int
     lib.dsv41_head_dw_run.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int,
                                       ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]
+    for name, forward, backward in (("scores", ScoresDesc, ScoresGradDesc), ("distill", DistillDesc, DistillGradDesc)):
+        getattr(lib, f"dsv41_{name}_desc_size").restype = ctypes.c_size_t
+        getattr(lib, f"dsv41_{name}_grad_desc_size").restype = ctypes.c_size_t
+        size = getattr(lib, f"dsv41_{name}_workspace_bytes")
+        size.restype, size.argtypes = ctypes.c_size_t, [ctypes.POINTER(forward)]
+        run = getattr(lib, f"dsv41_{name}_run")
+        run.restype = ctypes.c_int
+        run.argtypes = [ctypes.POINTER(forward), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+        grad = getattr(lib, f"dsv41_{name}_grad_run")
+        grad.restype, grad.argtypes = ctypes.c_int, [ctypes.POINTER(backward), ctypes.c_void_p]
     lib.dsv41_check_wait.restype = ctypes.c_int
     lib.dsv41_check_wait.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
                                     ctypes.c_void_p, ctypes.c_void_p]
@@ -400,7 +498,11 @@ def load() -> ctypes.CDLL:
             raise RuntimeError(
                 f"{LIB_PATH} is missing: build it with `make -C {LIB_PATH.parent.parent}` "
                 "(or __graft_entry__.build()); there is no CPU fallback")
-        lib = _bind(ctypes.CDLL(os.fspath(LIB_PATH)))
+        lib = ctypes.CDLL(os.fspath(LIB_PATH))
+        missing = [name for name in EXPORTS if not hasattr(lib, name)]
+        if missing:
+            raise RuntimeError(f"{LIB_PATH} lacks {', '.join(missing)}: build it with `make -C {LIB_PATH.parent.parent}`")
+        lib = _bind(lib)
         if lib.dsv41_abi_version() != ABI_VERSION:
             raise RuntimeError(f"{LIB_PATH} has ABI {lib.dsv41_abi_version()}, expected {ABI_VERSION}")
         if lib.dsv41_sampler_desc_size() != ctypes.sizeof(SamplerDesc):
@@ -425,6 +527,10 @@ def load() -> ctypes.CDLL:
             raise RuntimeError("dsv41_sampler_full_shard_desc layout differs between library and binding")
         if lib.dsv41_sampler_full_finish_desc_size() != ctypes.sizeof(SamplerFullFinishDesc):
             raise RuntimeError("dsv41_sampler_full_finish_desc layout differs between library and binding")
+        for name, cls in (("scores", ScoresDesc), ("scores_grad", ScoresGradDesc), ("distill", DistillDesc),
+                          ("distill_grad", DistillGradDesc)):
+            if getattr(lib, f"dsv41_{name}_desc_size")() != ctypes.sizeof(cls):
+                raise RuntimeError(f"dsv41_{name}_desc layout differs between library and binding")
         _lib = lib
         return lib
 

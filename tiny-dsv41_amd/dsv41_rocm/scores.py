@@ -1,0 +1,206 @@
+"""Scores of rows of logits on MI355X: log-probs and ranks of given tokens, entropy and the top
+alternatives, differentiable in the logits.
+
+Reference (paths relative to the Tiny-DSV41 tree): ``dsv41_train/rl/rollout.py:144-150`` forms a step's
+``log_softmax(logits.float() / T)`` and takes the token's entry; ``rollout_manager/backends/
+vllm_actor.py:260`` takes a token's log-prob from an engine whose ``logprobs`` output also names the top
+alternatives and the token's rank.  Here one pass over each row gives all of them, where the logits are
+at hand; ``selected_log_probs`` does it from hidden states, without alternatives.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from . import _lib
+from ._check import any_set
+from .logprob import first_order
+from .sampling import validate_temperature
+
+MAX_TOP_K = 1024
+
+
+@dataclass
+class LogitScores:
+    """Per-row outputs of :func:`logit_scores`: the targets' log-probs (fp32) and ranks (int64, 1 = the
+    most likely token), both None without targets; entropies (fp32); the top alternatives' ids (int64,
+    -1 past the unmasked tokens) and log-probs (fp32, -inf there), ``[rows, top_k]``."""
+
+    log_probs: Optional[torch.Tensor]
+    ranks: Optional[torch.Tensor]
+    entropy: torch.Tensor
+    top_ids: torch.Tensor
+    top_log_probs: torch.Tensor
+
+
+def rows_of_logits(logits, temperature):
+    """Validated fp32 or bf16 logits [rows, V] whose rows are contiguous."""
+    validate_temperature(temperature)
+    if not isinstance(logits, torch.Tensor) or logits.ndim != 2 or logits.shape[1] == 0:
+        raise ValueError("logits must have shape [rows, vocabulary_size]")
+    if not logits.is_cuda:
+        raise ValueError("logits must be on the GPU (libdsv41hip has no CPU path)")
+    if logits.dtype not in (torch.float32, torch.bfloat16):
+        logits = logits.float()
+    # rows that overlap without being one and the same (stride 0) have no place for the kernels' row stride
+    if logits.stride(1) != 1 and logits.shape[1] > 1 or 0 < logits.stride(0) < logits.shape[1]:
+        logits = logits.contiguous()
+    return logits
+
+
+def refuse_capture(check: bool) -> None:
+    if check and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("a checked call waits for its answer and cannot be captured: pass check=False")
+
+
+def fill_rows(d, logits, temperature) -> None:
+    """The fields that every descriptor over rows of logits has."""
+    d.struct_size = ctypes.sizeof(type(d))
+    d.rows, d.vocab = logits.shape
+    d.logits_dtype = _lib.DTYPE_F32 if logits.dtype == torch.float32 else _lib.DTYPE_BF16
+    d.logits_row_stride = logits.stride(0) if logits.shape[0] > 1 else logits.shape[1]
+    d.logits = logits.data_ptr()
+    d.temperature = temperature
+
+
+def grad_vector(g, shape, device):
+    """An upstream gradient in kernel form, or None."""
+    return None if g is None else g.to(device=device, dtype=torch.float32).expand(shape).contiguous()
+
+
+def _forward(logits, targets, top_k, temperature, want_stats):
+    rows, dev = logits.shape[0], logits.device
+    f32, i64 = torch.float32, torch.int64
+    lp = torch.empty(rows if targets is not None else 0, dtype=f32, device=dev)
+    rank = torch.empty(rows if targets is not None else 0, dtype=i64, device=dev)
+    entropy = torch.empty(rows, dtype=f32, device=dev)
+    top_ids = torch.empty(rows, top_k, dtype=i64, device=dev)
+    top_lp = torch.empty(rows, top_k, dtype=f32, device=dev)
+    status = torch.empty(rows, dtype=torch.int32, device=dev)
+    stats = torch.empty(rows, 4, dtype=torch.float64, device=dev) if want_stats else None
+    if rows == 0:
+        return lp, rank, entropy, top_ids, top_lp, status, stats
+    d = _lib.ScoresDesc()
+    fill_rows(d, logits, temperature)
+    d.top_k = top_k
+    if targets is not None:
+        d.targets, d.out_logprob, d.out_rank = targets.data_ptr(), lp.data_ptr(), rank.data_ptr()
+    d.out_entropy, d.out_status = entropy.data_ptr(), status.data_ptr()
+    if top_k:
+        d.out_top_ids, d.out_top_logprob = top_ids.data_ptr(), top_lp.data_ptr()
+    d.out_stats = None if stats is None else stats.data_ptr()
+    lib = _lib.load()
+    size = lib.dsv41_scores_workspace_bytes(ctypes.byref(d))
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    with torch.cuda.device(dev):
+        rc = lib.dsv41_scores_run(ctypes.byref(d), None if ws is None else ws.data_ptr(), size,
+                                  torch.cuda.current_stream(dev).cuda_stream)
+    _lib.check(rc)
+    return lp, rank, entropy, top_ids, top_lp, status, stats
+
+
+def scores_backward(logits, targets, top_ids, temperature, stats, g_log_probs, g_entropy, g_top):
+    """dL/dlogits of :func:`logit_scores`, in the logits' dtype; gradients that are None count as zero."""
+    rows, vocab = logits.shape
+    dev = logits.device
+    out = torch.empty(rows, vocab, dtype=logits.dtype, device=dev)
+    if rows == 0:
+        return out
+    g_log_probs = grad_vector(g_log_probs if targets is not None else None, (rows,), dev)
+    g_entropy = grad_vector(g_entropy, (rows,), dev)
+    g_top = grad_vector(g_top, top_ids.shape, dev) if top_ids.shape[1] else None
+    d = _lib.ScoresGradDesc()
+    fill_rows(d, logits, temperature)
+    if targets is not None:
+        d.targets = targets.data_ptr()
+    d.stats, d.out = stats.data_ptr(), out.data_ptr()
+    if g_log_probs is not None:
+        d.grad_logprob = g_log_probs.data_ptr()
+    if g_entropy is not None:
+        d.grad_entropy = g_entropy.data_ptr()
+    if g_top is not None:
+        d.top_k, d.top_ids, d.grad_top = top_ids.shape[1], top_ids.data_ptr(), g_top.data_ptr()
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        rc = lib.dsv41_scores_grad_run(ctypes.byref(d), torch.cuda.current_stream(dev).cuda_stream)
+    _lib.check(rc)
+    return out
+
+
+class _LogitScores(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, top_k, temperature):
+        lp, rank, entropy, top_ids, top_lp, status, stats = _forward(logits, targets, top_k, temperature, True)
+        ctx.temperature = temperature
+        ctx.save_for_backward(logits, targets, top_ids, stats)
+        ctx.mark_non_differentiable(rank, top_ids, status)
+        ctx.set_materialize_grads(False)
+        return lp, rank, entropy, top_ids, top_lp, status
+
+    @staticmethod
+    def backward(ctx, g_lp, g_rank, g_entropy, g_ids, g_top, g_status):
+        logits, targets, top_ids, stats = ctx.saved_tensors
+        if g_lp is None and g_entropy is None and g_top is None:
+            return None, None, None, None
+        grad = scores_backward(logits, targets, top_ids, ctx.temperature, stats, g_lp, g_entropy, g_top)
+        sources = [t for t in (logits, g_lp, g_entropy, g_top) if t is not None]
+        return first_order(grad, *sources), None, None, None
+
+
+def _status_error(status: torch.Tensor) -> None:
+    bits = 0
+    for v in status.unique().tolist():
+        bits |= int(v)
+    if bits & _lib.STATUS_BAD_TARGET:
+        raise ValueError("target token ID is outside the model vocabulary")
+    if bits & _lib.STATUS_NONFINITE:
+        raise ValueError("logits leave a row without a distribution (NaN, +inf or every token masked)")
+
+
+def logit_scores(
+    logits: torch.Tensor,
+    targets: Optional[torch.Tensor] = None,
+    *,
+    top_k: int = 0,
+    temperature: float = 1.0,
+    check: bool = True,
+) -> LogitScores:
+    """Log-probs under ``softmax(logits / temperature)`` of one given token per row, its rank, the row's
+    entropy and the ``top_k`` most likely tokens with their log-probs.
+
+    ``logits [rows, V]`` are fp32 or bf16 on the GPU (other dtypes are converted to fp32), rows at any
+    stride; ``-inf`` is a masked token, of probability 0.  ``targets [rows]`` int64.  Tokens order by
+    (logit desc, index asc), with -0 equal to +0; a rank is 1 plus the number of tokens before the target.
+    ``top_k`` is at most 1024 and V.
+
+    Differentiable in ``logits``: log-probs, entropy and the alternatives' log-probs (with the
+    alternatives held fixed), once (no second derivatives).  A row whose upstream gradients are all zero
+    gets zeros.
+
+    With ``check`` the call synchronises and raises ``ValueError`` for a target outside the vocabulary,
+    or a row with a NaN, a +inf or no unmasked token; without, such a row holds NaN (ids -1, rank 0).
+    """
+    logits = rows_of_logits(logits, temperature)
+    rows, vocab = logits.shape
+    if isinstance(top_k, bool) or not isinstance(top_k, int) or not 0 <= top_k <= vocab:
+        raise ValueError("top_k must be an integer in [0, vocabulary_size]")
+    if targets is not None:
+        if targets.is_floating_point() or targets.dtype == torch.bool:
+            raise ValueError("targets must be integers")
+        targets = targets.to(device=logits.device, dtype=torch.int64).reshape(-1).contiguous()
+        if targets.numel() != rows:
+            raise ValueError("one target is required per row")
+    refuse_capture(check)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        lp, rank, entropy, top_ids, top_lp, status = _LogitScores.apply(logits, targets, top_k, temperature)
+    else:
+        lp, rank, entropy, top_ids, top_lp, status, _ = _forward(logits, targets, top_k, temperature, False)
+    if check and any_set(status)[0]:
+        _status_error(status)
+    if targets is None:
+        lp = rank = None
+    return LogitScores(lp, rank, entropy, top_ids, top_lp)
