@@ -217,12 +217,10 @@ def _plain_distill(case, x, ids, lq, g):
 
 
 def _calls():
-    path = str(Path(__file__).resolve().parents[1] / "tiny-dsv41_amd")
-    if path not in sys.path:
-        sys.path.insert(0, path)
-    import dsv41_rocm
-
-    return dsv41_rocm
+    if "dsv41_rocm" not in sys.modules:
+        sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "tiny-dsv41_amd"))
+        import dsv41_rocm  # noqa: F401
+    return sys.modules["dsv41_rocm"]
 
 
 def _own_scores(case, state):
