@@ -55,7 +55,7 @@ struct Params {
 
 struct Shared {
   uint32_t named[MAX_LEN / 32];
-  double red[WAVES];
+  double red[4 * WAVES];
   int flags;
 };
 constexpr int LIVE = 1 << 16;  // the list has an entry (above the status bits)
@@ -76,9 +76,25 @@ __device__ void write_row(const Params& p, int row, float loss, int status, doub
   }
 }
 
+// A thread's first entry of a list: read ahead of the pass over the row, whose loads hide its own.
+struct Entry {
+  int64_t id;
+  float x, lq;
+};
+template <typename T>
+__device__ __forceinline__ Entry entry_of(const Params& p, int row, int k) {
+  Entry e{-1, -INFINITY, 0.f};
+  if (k < p.K) {
+    e.id = p.ids[(int64_t)row * p.K + k];
+    e.lq = p.lq[(int64_t)row * p.K + k];
+    if (e.id >= 0 && e.id < p.V) e.x = Elem<T>::one(static_cast<const T*>(p.logits) + (int64_t)row * p.stride + e.id);
+  }
+  return e;
+}
+
 // The row's divergence from the sums outside its list and the list itself.
 template <typename T>
-__device__ void finish(const Params& p, int row, State st, int flags, double* red) {
+__device__ __forceinline__ void finish(const Params& p, int row, State st, int flags, const Entry& mine, double* red) {
   if (!(flags & LIVE)) {
     write_row(p, row, 0.f, 0, 0.0, 1.0, 0.0, 0.0, 0.0, false);
     return;
@@ -87,41 +103,38 @@ __device__ void finish(const Params& p, int row, State st, int flags, double* re
     write_row(p, row, NAN, flags & ~LIVE, NAN, NAN, NAN, NAN, 0.0, true);
     return;
   }
-  const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.stride;
-  const int64_t* ids = p.ids + (int64_t)row * p.K;
-  const float* lq = p.lq + (int64_t)row * p.K;
-  double m = st.m, top = -INFINITY;
+  float mf = st.m, top = -INFINITY;
   int bad = 0;
-  for (int k = threadIdx.x; k < p.K; k += NT)
-    if (ids[k] >= 0) {
-      m = fmax(m, (double)Elem<T>::one(x + ids[k]));
-      top = fmax(top, (double)lq[k]);
-      bad |= !(lq[k] < INFINITY);
+  Entry e = mine;
+  for (int k = threadIdx.x; k < p.K; k += NT) {
+    if (k >= NT) e = entry_of<T>(p, row, k);
+    if (e.id >= 0) {
+      mf = fmaxf(mf, e.x);
+      top = fmaxf(top, e.lq);
+      bad |= !(e.lq < INFINITY);
     }
-  m = rows::block_max<WAVES>(m, red);
-  top = p.rest ? 0.0 : rows::block_max<WAVES>(top, red);
+  }
+  const double m = rows::block_max(mf, red);
+  top = p.rest ? 0.f : rows::block_max(top, red);
   bad = __syncthreads_or(bad || !(top > -INFINITY));
-  double Sn = 0.0, W = 0.0, WL = 0.0, WD = 0.0;
-  if (!bad)
-    for (int k = threadIdx.x; k < p.K; k += NT)
-      if (ids[k] >= 0) {
-        const double d = ((double)Elem<T>::one(x + ids[k]) - m) * p.sc.inv_t, l = (double)lq[k] - top, w = exp(l);
-        Sn += exp(d);
-        if (w > 0.0) {
-          W += w;
-          WL += w * l;
-          WD += w * d;
-        }
+  double sum[4] = {0.0, 0.0, 0.0, 0.0};
+  e = mine;
+  for (int k = threadIdx.x; k < p.K && !bad; k += NT) {
+    if (k >= NT) e = entry_of<T>(p, row, k);
+    if (e.id >= 0) {
+      const double d = ((double)e.x - m) * p.sc.inv_t, l = (double)e.lq - top, w = exp(l);
+      sum[0] += exp(d);
+      if (w > 0.0) {
+        sum[1] += w;
+        sum[2] += w * l;
+        sum[3] += w * d;
       }
-  Sn = rows::block_sum<WAVES>(Sn, red);
-  W = rows::block_sum<WAVES>(W, red);
-  WL = rows::block_sum<WAVES>(WL, red);
-  WD = rows::block_sum<WAVES>(WD, red);
-  if (st.S == 0.0)
-    st.U = 0.0;
-  else
-    rows::rebase(st.S, st.U, st.m, m, p.sc);
-  const double S_rest = st.S + p.sc.kappa * st.U, S = S_rest + Sn, ln_s = log(S);
+    }
+  }
+  rows::block_sums(sum, red);
+  const double Sn = sum[0], W = sum[1], WL = sum[2], WD = sum[3];
+  if (st.S != 0.0) rows::rebase(st.S, st.U, ((double)st.m - m) * p.sc.cd);
+  const double S_rest = st.S, S = S_rest + Sn, ln_s = log(S);
   const bool nonfinite = !(S > 0.0 && S < INFINITY);
   if (bad || (p.rest && W > MOST_MASS)) {
     write_row(p, row, NAN, DSV41_STATUS_BAD_TEACHER, NAN, NAN, NAN, NAN, 0.0, true);
@@ -143,19 +156,19 @@ __device__ void finish(const Params& p, int row, State st, int flags, double* re
             log_z, true);
 }
 
-template <typename T>
-__global__ __launch_bounds__(NT) void distill_kernel(Params p) {
+template <typename T, bool ONCE>
+__global__ __launch_bounds__(NT, 8) void distill_kernel(Params p) {
   __shared__ Shared s;
   const int row = blockIdx.x / p.slices, slice = blockIdx.x % p.slices, tid = threadIdx.x;
   const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.stride;
   const int begin = slice * p.len, len = min(p.len, p.V - begin);
-  const int64_t* ids = p.ids + (int64_t)row * p.K;
+  const Entry mine = entry_of<T>(p, row, tid);
   for (int i = tid; i < (len + 31) / 32; i += NT) s.named[i] = 0;
   if (tid == 0) s.flags = 0;
   __syncthreads();
   int f = 0;
   for (int k = tid; k < p.K; k += NT) {
-    const int64_t id = ids[k];
+    const int64_t id = k < NT ? mine.id : p.ids[(int64_t)row * p.K + k];
     if (id < 0) continue;
     f |= LIVE;
     if (id >= p.V) f |= DSV41_STATUS_BAD_TARGET;
@@ -168,10 +181,11 @@ __global__ __launch_bounds__(NT) void distill_kernel(Params p) {
   __syncthreads();
   const int flags = s.flags;
   State st{0.0, 0.0, -INFINITY, 0};
+  float own[4];
   if (flags == LIVE)
-    st = rows::scan<T, false, true>(x + begin, len, p.sc, INFINITY, 0, nullptr, s.named, s.red);
+    st = rows::scan<T, ONCE, false, true>(x + begin, len, p.sc, INFINITY, 0, nullptr, s.named, s.red, own);
   if (p.slices == 1) {
-    finish<T>(p, row, st, flags, s.red);
+    finish<T>(p, row, st, flags, mine, s.red);
   } else if (tid == 0) {
     SliceState* o = p.states + (int64_t)row * p.slices + slice;
     o->s = st;
@@ -181,24 +195,21 @@ __global__ __launch_bounds__(NT) void distill_kernel(Params p) {
 
 template <typename T>
 __global__ __launch_bounds__(NT) void distill_join_kernel(Params p) {
-  __shared__ double red[WAVES];
+  __shared__ double red[4 * WAVES];
   __shared__ int flags;
   const int row = blockIdx.x, tid = threadIdx.x;
+  const Entry mine = entry_of<T>(p, row, tid);
   SliceState in{{0.0, 0.0, -INFINITY, 0}, 0, 0};
   if (tid == 0) flags = 0;
   __syncthreads();
   if (tid < p.slices) in = p.states[(int64_t)row * p.slices + tid];
   if (in.flags) atomicOr(&flags, in.flags);
   State st = in.s;
-  const double m = rows::block_max<WAVES>((double)st.m, red);
-  if (st.S == 0.0)
-    st.U = 0.0;
-  else
-    rows::rebase(st.S, st.U, st.m, m, p.sc);
-  st.m = (float)m;
-  st.S = rows::block_sum<WAVES>(st.S, red);
-  st.U = rows::block_sum<WAVES>(st.U, red);
-  finish<T>(p, row, st, flags, red);
+  const float m = rows::block_max(st.m, red);
+  if (st.S != 0.0) rows::rebase(st.S, st.U, ((double)st.m - (double)m) * p.sc.cd);
+  double sum[1] = {st.S};
+  rows::block_sums(sum, red);
+  finish<T>(p, row, State{sum[0], 0.0, m, 0}, flags, mine, red);
 }
 
 struct GradParams {
@@ -240,6 +251,16 @@ __global__ __launch_bounds__(NT) void distill_grad_kernel(GradParams p) {
     const double e = exp(((double)Elem<T>::one(x + begin + i) - m) * p.sc.inv_t);
     rows::store_one(out + i, (float)(g * (Q * e / S - exp((double)lq[k] - log_z))));
   }
+}
+
+template <typename T>
+void launch(const Params& p, hipStream_t s) {
+  const dim3 grid((unsigned)p.rows * (unsigned)p.slices);
+  if (rows::read_once(p.rows, p.V, sizeof(T)))
+    hipLaunchKernelGGL((distill_kernel<T, true>), grid, dim3(NT), 0, s, p);
+  else
+    hipLaunchKernelGGL((distill_kernel<T, false>), grid, dim3(NT), 0, s, p);
+  if (p.slices > 1) hipLaunchKernelGGL(distill_join_kernel<T>, dim3(p.rows), dim3(NT), 0, s, p);
 }
 
 Cut cut_of(int rows, int V) {
@@ -294,20 +315,16 @@ extern "C" int dsv41_distill_run(const dsv41_distill_desc* d, void* workspace, s
   p.slices = c.slices;
   p.len = c.len;
   p.rest = d->tail == DSV41_TAIL_REST;
-  p.sc = rows::scale_of(d->temperature);
+  p.sc = rows::scale_of(d->temperature, true);
   p.out_loss = d->out_loss;
   p.out_status = d->out_status;
   p.out_stats = d->out_stats;
   p.states = static_cast<distill::SliceState*>(workspace);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)p.rows * (unsigned)p.slices), block(rows::NT);
-  if (d->logits_dtype == DSV41_DTYPE_F32) {
-    hipLaunchKernelGGL(distill::distill_kernel<float>, grid, block, 0, s, p);
-    if (p.slices > 1) hipLaunchKernelGGL(distill::distill_join_kernel<float>, dim3(p.rows), block, 0, s, p);
-  } else {
-    hipLaunchKernelGGL(distill::distill_kernel<rows::bf16_t>, grid, block, 0, s, p);
-    if (p.slices > 1) hipLaunchKernelGGL(distill::distill_join_kernel<rows::bf16_t>, dim3(p.rows), block, 0, s, p);
-  }
+  if (d->logits_dtype == DSV41_DTYPE_F32)
+    distill::launch<float>(p, s);
+  else
+    distill::launch<rows::bf16_t>(p, s);
   DSV41_HIP_CHECK(hipGetLastError());
   return DSV41_OK;
 }
@@ -334,7 +351,7 @@ extern "C" int dsv41_distill_grad_run(const dsv41_distill_grad_desc* d, void* st
   p.K = d->top_k;
   p.slices = c.slices;
   p.len = c.len;
-  p.sc = rows::scale_of(d->temperature);
+  p.sc = rows::scale_of(d->temperature, false);
   p.stats = d->stats;
   p.g = d->grad_loss;
   p.out = d->out;

@@ -2,14 +2,18 @@
 // rows of any alignment, the pass over a row (or a slice of it) with its running softmax sums, and
 // sums over a workgroup.
 //
-// Sums.  With c = log2(e) / T and a reference r that a thread raises when it meets a larger logit, the
-// pass keeps
-//   S = sum 2^((x - r) c)   and   U = sum 2^((x - r) c) (x - r) c
-// in fp32 over the thread's few hundred elements; the threads' sums are brought to the row's maximum
-// and added in fp64.  c itself is rounded to fp32, which would put the same relative error into every
-// exponent; to first order that is S (1 + kappa U / S) with kappa = ln 2 (c - fp32(c)) / fp32(c), so the
-// joined S takes kappa U more.  x = -inf is a masked token: it adds nothing to either sum.  A NaN or
-// +inf makes S NaN.
+// Sums.  With c = log2(e) / T and a reference that a thread raises when it meets a larger logit, a pass
+// keeps sums of exponentials in fp32 over the thread's few hundred elements; the threads' sums are
+// brought to the largest logit and added in fp64.
+//   For scores, S = sum 2^d and U = sum 2^d d with d = (x - r) c.  The difference is what keeps a row with
+// one likely token exact: that token's term is 1, and S - 1 has the others' precision.  c is rounded to
+// fp32, which puts the same relative error into every exponent; to first order it is made up for by
+// kappa U, kappa = ln 2 (c - fp32(c)) / fp32(c), which S takes in the end.
+//   For the mass outside a list, S = sum 2^(x c - r) alone: c as a sum of two and one multiply-add for
+// each, so there is nothing to make up for and r may be any number.  Where the largest x c leaves the
+// range that this is safe in (logits all at their type's lowest value, say), the sum is formed again as
+// 2^((x - m) c).
+//   x = -inf is a masked token: it adds nothing to any sum.  A NaN or +inf makes S NaN.
 #pragma once
 
 #include <math.h>
@@ -31,22 +35,14 @@ struct bf16_t {
 // 16 bytes of a row; rows begin at any element, so the loads assume the element's alignment only
 // (global_load_dwordx4 takes any).
 template <typename T>
-struct Raw;
-template <>
-struct __attribute__((packed, aligned(4))) Raw<float> {
-  uint32_t w[4];
-};
-template <>
-struct __attribute__((packed, aligned(2))) Raw<bf16_t> {
-  uint32_t w[4];
-};
-
-template <typename T>
 struct Elem;
 template <>
 struct Elem<float> {
   static constexpr int VEC = 4;
+  typedef uint32_t Raw __attribute__((ext_vector_type(4), aligned(4)));
+  static constexpr uint32_t MASKED = 0xFF800000u;  // -inf
   static __device__ __forceinline__ float one(const float* p) { return *p; }
+  static __device__ __forceinline__ void put(uint32_t (&w)[4], int j, float v) { w[j] = __float_as_uint(v); }
   static __device__ __forceinline__ void unpack(const uint32_t (&w)[4], float (&x)[4]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) x[j] = __uint_as_float(w[j]);
@@ -55,7 +51,12 @@ struct Elem<float> {
 template <>
 struct Elem<bf16_t> {
   static constexpr int VEC = 8;
+  typedef uint32_t Raw __attribute__((ext_vector_type(4), aligned(2)));
+  static constexpr uint32_t MASKED = 0xFF80FF80u;  // twice -inf
   static __device__ __forceinline__ float one(const bf16_t* p) { return bf16_to_f32(p->v); }
+  static __device__ __forceinline__ void put(uint32_t (&w)[4], int j, bf16_t v) {
+    w[j >> 1] = j & 1 ? (w[j >> 1] & 0xFFFFu) | (uint32_t)v.v << 16 : (w[j >> 1] & 0xFFFF0000u) | v.v;
+  }
   static __device__ __forceinline__ void unpack(const uint32_t (&w)[4], float (&x)[8]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -65,20 +66,38 @@ struct Elem<bf16_t> {
   }
 };
 
-// The elements [i VEC, i VEC + VEC) of x[0, len), -inf where they lie outside.
-template <typename T>
-__device__ __forceinline__ void load_edge(const T* x, int len, int i, float (&v)[Elem<T>::VEC]) {
+// 16 bytes at p.  ONCE: nontemporal, for rows that are read once and do not stay in a cache.
+template <bool ONCE, typename T>
+__device__ __forceinline__ void load16(const T* p, uint32_t (&w)[4]) {
+  using Raw = typename Elem<T>::Raw;
+  Raw r;
+  if constexpr (ONCE)
+    r = __builtin_nontemporal_load(reinterpret_cast<const Raw*>(p));
+  else
+    r = *reinterpret_cast<const Raw*>(p);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = r[j];
+}
+// The elements [i VEC, i VEC + VEC) of x[0, len) as 16 bytes, -inf where they lie outside; i < 0: none.
+template <bool ONCE, typename T>
+__device__ __forceinline__ void load_some(const T* x, int len, int i, uint32_t (&w)[4]) {
   constexpr int VEC = Elem<T>::VEC;
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) {
-    const int64_t at = (int64_t)i * VEC + j;
-    v[j] = at < len ? Elem<T>::one(x + at) : -INFINITY;
+  for (int j = 0; j < 4; ++j) w[j] = Elem<T>::MASKED;
+  if (i >= 0 && i < len / VEC) {
+    load16<ONCE>(x + (int64_t)i * VEC, w);
+  } else if (i == len / VEC) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const int at = i * VEC + j;
+      if (at < len) Elem<T>::put(w, j, x[at]);
+    }
   }
 }
-template <typename T>
+template <bool ONCE = false, typename T>
 __device__ __forceinline__ void load_full(const T* x, int i, float (&v)[Elem<T>::VEC]) {
-  const Raw<T> r = *reinterpret_cast<const Raw<T>*>(x + (int64_t)i * Elem<T>::VEC);
-  const uint32_t w[4] = {r.w[0], r.w[1], r.w[2], r.w[3]};
+  uint32_t w[4];
+  load16<ONCE>(x + (int64_t)i * Elem<T>::VEC, w);
   Elem<T>::unpack(w, v);
 }
 
@@ -86,16 +105,16 @@ __device__ __forceinline__ void load_full(const T* x, int i, float (&v)[Elem<T>:
 __device__ __forceinline__ void store_one(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_one(bf16_t* p, float v) { p->v = (uint16_t)pack_bf16(v, 0.f); }
 __device__ __forceinline__ void store_full(float* out, int i, const float (&v)[4]) {
-  Raw<float> r;
+  Elem<float>::Raw r;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) r.w[j] = __float_as_uint(v[j]);
-  *reinterpret_cast<Raw<float>*>(out + (int64_t)i * 4) = r;
+  for (int j = 0; j < 4; ++j) r[j] = __float_as_uint(v[j]);
+  *reinterpret_cast<Elem<float>::Raw*>(out + (int64_t)i * 4) = r;
 }
 __device__ __forceinline__ void store_full(bf16_t* out, int i, const float (&v)[8]) {
-  Raw<bf16_t> r;
+  Elem<bf16_t>::Raw r;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) r.w[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
-  *reinterpret_cast<Raw<bf16_t>*>(out + (int64_t)i * 8) = r;
+  for (int j = 0; j < 4; ++j) r[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+  *reinterpret_cast<Elem<bf16_t>::Raw*>(out + (int64_t)i * 8) = r;
 }
 template <typename T, class F>
 __device__ __forceinline__ void map(const T* x, T* out, int len, F f) {
@@ -131,48 +150,60 @@ __device__ __forceinline__ void fill_zero(T* out, int len) {
   for (int i = full * VEC + (int)threadIdx.x; i < len; i += NT) store_one(out + i, 0.f);
 }
 
-// ---- sums and maxima over the workgroup, the same value in every thread.  `s`: WAVES values of LDS.
-template <int W>
-__device__ __forceinline__ double block_sum(double v, double* s) {
-  v = wave_total_d(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = 0.0;
+// ---- sums and maxima over the workgroup, the same value in every thread.  `s`: LDS, WAVES values for
+// each value that is joined.
+template <int N>
+__device__ __forceinline__ void block_sums(double (&v)[N], double* s) {
 #pragma unroll
-  for (int w = 0; w < W; ++w) v += s[w];
-  return v;
+  for (int i = 0; i < N; ++i) v[i] = wave_total_d(v[i]);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0)
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i * WAVES + (threadIdx.x >> 6)] = v[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    v[i] = 0.0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) v[i] += s[i * WAVES + w];
+  }
 }
-template <int W>
-__device__ __forceinline__ double block_max(double v, double* s) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o));
+__device__ __forceinline__ float block_max(float v, double* s) {
+  v = wave_max_dpp(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
   __syncthreads();
-  v = s[0];
+  v = (float)s[0];
 #pragma unroll
-  for (int w = 1; w < W; ++w) v = fmax(v, s[w]);
+  for (int w = 1; w < WAVES; ++w) v = fmaxf(v, (float)s[w]);
   return v;
 }
 
 // The scale of a temperature, computed on the host.
 struct Scale {
-  float c;       // log2(e) / T in fp32
-  float margin;  // how far a logit may exceed the reference: two powers of two
-  double inv_t;  // 1 / T
-  double kappa;  // ln 2 (log2(e) / T - c) / c
+  float c, c_lo;  // log2(e) / T in fp32, or as a sum of two
+  float margin;   // how far a logit may exceed the reference: two powers of two
+  double cd;      // what c and c_lo say
+  double inv_t;   // 1 / T
+  double kappa;   // ln 2 (log2(e) / T - cd) / cd
 };
-inline Scale scale_of(float temperature) {
+inline Scale scale_of(float temperature, bool split) {
   Scale s;
   const double c = 1.4426950408889634 / (double)temperature;
   s.c = (float)c;
+  s.c_lo = 0.f;
+  if (split) {
+    // c_lo above zero, so that -inf stays -inf in both products
+    while ((double)s.c >= c || (float)(c - (double)s.c) == 0.f) s.c = nextafterf(s.c, 0.f);
+    s.c_lo = (float)(c - (double)s.c);
+  }
+  s.cd = (double)s.c + (double)s.c_lo;
   s.margin = (float)(2.0 / c);
   s.inv_t = 1.0 / (double)temperature;
-  s.kappa = 0.6931471805599453 * (c - (double)s.c) / (double)s.c;
+  s.kappa = 0.6931471805599453 * (c - s.cd) / s.cd;
   return s;
 }
-// Temperatures whose c or margin leave fp32's normal numbers are refused.
+// Temperatures whose c or c_lo leave fp32's range are refused.
 inline bool scale_ok(float temperature) { return temperature >= 1e-30f && temperature <= 1e30f; }
 
 // What a slice of a row (or the whole row) adds up to: its largest logit, S and U against it, and how
@@ -182,121 +213,175 @@ struct State {
   float m;
   int32_t before;
 };
-// The join of two: S and U against the larger maximum.
-__device__ __forceinline__ void rebase(double& S, double& U, float from, double to, const Scale& sc) {
-  const double d = fmax(((double)from - to) * sc.c, -2000.0);
+// S and U from one reference to another, d = the first less the second as an exponent.
+__device__ __forceinline__ void rebase(double& S, double& U, double d) {
+  d = fmax(d, -2000.0);
   const double f = exp2(d);
   U = f * (U + d * S);
   S = f * S;
 }
 
-// Largest of N values and a running one.  v_max3_f32 by itself: fmaxf would first quiet each operand.
-template <int N>
-__device__ __forceinline__ float max_of(const float (&x)[N]) {
+// Largest of a chunk.  v_max3_f32 by itself: fmaxf would first quiet each operand.
+__device__ __forceinline__ float max3(float a, float b, float c) {
   float m;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(x[0]), "v"(x[1]), "v"(x[2]));
-  if constexpr (N == 4) {
-    asm("v_max_f32 %0, %1, %2\n\ts_nop 1" : "=v"(m) : "v"(m), "v"(x[3]));
-  } else {
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(m), "v"(x[3]), "v"(x[4]));
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(m), "v"(x[5]), "v"(x[6]));
-    asm("v_max_f32 %0, %1, %2\n\ts_nop 1" : "=v"(m) : "v"(m), "v"(x[7]));
-  }
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(a), "v"(b), "v"(c));
   return m;
 }
-
-template <int CTRL>
-__device__ __forceinline__ float max_dpp(float v) {
-  return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true)));
+__device__ __forceinline__ float max_of(const float (&x)[4]) {
+  const float m = max3(x[0], x[1], x[2]);
+  return max3(m, x[3], x[3]);
+}
+__device__ __forceinline__ float max_of(const float (&x)[8]) {
+  const float a = max3(x[0], x[1], x[2]), b = max3(x[3], x[4], x[5]);
+  return max3(max3(a, x[6], x[7]), b, b);
 }
 
-struct Thread {
-  float r, m, S, U;
-  int before;
-};
+// Two chunk maxima become the maxima of their groups of LANES lanes (8 or 4), in every lane of them.  A
+// DPP read needs two wait states after the instruction that wrote its register.
+template <int LANES>
+__device__ __forceinline__ void group_max2(float& g, float& h) {
+#define DSV41_DPP2(ctrl)                                                                        \
+  "s_nop 0\n\t"                                                                                 \
+  "v_max_f32_dpp %0, %0, %0 " ctrl " row_mask:0xf bank_mask:0xf bound_ctrl:1\n\t"               \
+  "v_max_f32_dpp %1, %1, %1 " ctrl " row_mask:0xf bank_mask:0xf bound_ctrl:1\n\t"
+  asm("s_nop 1\n\t" DSV41_DPP2("quad_perm:[1,0,3,2]") DSV41_DPP2("quad_perm:[2,3,0,1]") "s_nop 1" : "+v"(g), "+v"(h));
+  if constexpr (LANES == 8) asm("s_nop 1\n\t" DSV41_DPP2("row_half_mirror") "s_nop 1" : "+v"(g), "+v"(h));
+#undef DSV41_DPP2
+}
+
+constexpr float SAFE = 1e30f;  // the largest |m c| that x c - r is formed with
 
 // One pass over x[0, len) by the workgroup, whose threads take 16 bytes in turn.
 //   TOP: group_max[g] = the largest of the elements [32 g, 32 g + 32).
-//   NAMED: elements whose bit in `named` is set count as masked.
+//   NAMED: the sum outside a list: elements whose bit in `named` is set count as masked.
 //   xt, t: the target's logit (+inf: no target) and index, from x's begin.
-template <typename T, bool TOP, bool NAMED>
-__device__ __forceinline__ State scan(const T* x, int len, const Scale& sc, float xt, int64_t t, float* group_max,
-                                      const uint32_t* named, double* red) {
-  constexpr int VEC = Elem<T>::VEC, U = 4, LANES = GROUP / VEC;
+//   own: the largest elements of the thread's four shares of the row.
+template <typename T, bool ONCE, bool TOP, bool NAMED>
+__device__ __forceinline__ State scan(const T* x, int len, const Scale& sc, float xt, int t, float* group_max,
+                                      const uint32_t* named, double* red, float (&own)[4]) {
+  constexpr int VEC = Elem<T>::VEC, LANES = GROUP / VEC;
   const int full = len / VEC, n = (len + VEC - 1) / VEC;
   const int tid = threadIdx.x;
-  Thread a{LOWEST, -INFINITY, 0.f, 0.f, 0};
-
-  auto take = [&](float(&v)[VEC], int i) {
-    if constexpr (NAMED) {
-      const uint32_t bits = i < n ? (named[(i * VEC) >> 5] >> ((i * VEC) & 31)) & ((1u << VEC) - 1u) : 0u;
-      if (bits) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j)
-          if (bits >> j & 1) v[j] = -INFINITY;
+  for (int u = 0; u < 4; ++u) own[u] = -INFINITY;
+  float r = LOWEST, S[2] = {0.f, 0.f}, Us[2] = {0.f, 0.f}, margin = NAMED ? 2.f : sc.margin;
+  asm("" : "+v"(margin));  // (a scalar register short, the compiler would load it in every step)
+  int before = 0;
+
+  using Tile = uint32_t[2][4];  // two chunks a thread
+  constexpr int STEP = 2 * NT;
+  auto load = [&](Tile& w, int base) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) load16<ONCE>(x + (int64_t)(base + u * NT + tid) * VEC, w[u]);
+  };
+  auto take = [&](const Tile& w, int base, float& own0, float& own1) {
+    float v[2][VEC], cm[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      Elem<T>::unpack(w[u], v[u]);
+      if constexpr (NAMED) {
+        const int i = base + u * NT + tid;
+        const uint32_t bits = i < n ? (named[(i * VEC) >> 5] >> ((i * VEC) & 31)) & ((1u << VEC) - 1u) : 0u;
+        if (bits) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+            if (bits >> j & 1) v[u][j] = -INFINITY;
+        }
+      }
+      cm[u] = max_of(v[u]);
+    }
+    own0 = fmaxf(own0, cm[0]);
+    own1 = fmaxf(own1, cm[1]);
+    const float tm = max3(cm[0], cm[1], cm[1]);
+    if (!NAMED && tm >= xt) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int below = t - (base + u * NT + tid) * VEC;  // elements of the chunk with a lower index
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) before += (v[u][j] > xt || (v[u][j] == xt && j < below)) ? 1 : 0;
       }
     }
-    const float cm = max_of(v);
     if constexpr (TOP) {
-      float g = max_dpp<0xB1>(cm);                   // quad_perm [1,0,3,2]
-      g = max_dpp<0x4E>(g);                          // quad_perm [2,3,0,1]
-      if constexpr (LANES == 8) g = max_dpp<0x141>(g);  // row_half_mirror
-      if ((tid & (LANES - 1)) == 0 && i < n) group_max[i / LANES] = g;
+      group_max2<LANES>(cm[0], cm[1]);
+      if ((tid & (LANES - 1)) == 0) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int i = base + u * NT + tid;
+          if (i < n) group_max[i / LANES] = cm[u];
+        }
+      }
     }
-    if (cm >= xt) {
+    if constexpr (NAMED) {
+      const float mc = tm * sc.c;
+      if (mc > r + margin) {
+        const float f = __builtin_amdgcn_exp2f(r - mc);
+        S[0] *= f;
+        S[1] *= f;
+        r = mc;
+      }
+    } else if (tm > r + margin) {
+      const float d = fmaxf((r - tm) * sc.c, -1000.f), f = __builtin_amdgcn_exp2f(d);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        Us[q] = f * (Us[q] + d * S[q]);
+        S[q] = f * S[q];
+      }
+      r = tm;
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        const int64_t at = (int64_t)i * VEC + j;
-        a.before += (v[j] > xt || (v[j] == xt && at < t)) ? 1 : 0;
+        if constexpr (NAMED) {
+          const float d = __builtin_fmaf(v[u][j], sc.c_lo, __builtin_fmaf(v[u][j], sc.c, -r));
+          S[j & 1] += __builtin_amdgcn_exp2f(d);
+        } else {
+          const float d = (v[u][j] - r) * sc.c, e = __builtin_amdgcn_exp2f(d);
+          S[j & 1] += e;
+          Us[j & 1] = __builtin_fmaf(e, fmaxf(d, -1000.f), Us[j & 1]);
+        }
       }
-    }
-    a.m = fmaxf(a.m, cm);
-    if (cm > a.r + sc.margin) {
-      const float d = fmaxf((a.r - cm) * sc.c, -1000.f);
-      const float f = __builtin_amdgcn_exp2f(d);
-      a.U = f * (a.U + d * a.S);
-      a.S = f * a.S;
-      a.r = cm;
-    }
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const float d = (v[j] - a.r) * sc.c;
-      const float e = __builtin_amdgcn_exp2f(d);
-      a.S += e;
-      a.U = __builtin_fmaf(e, fmaxf(d, -1000.f), a.U);
-    }
   };
-
-  int base = 0;
-  for (; base + U * NT <= full; base += U * NT) {
-    float v[U][VEC];
-#pragma unroll
-    for (int u = 0; u < U; ++u) load_full(x, base + u * NT + tid, v[u]);
-#pragma unroll
-    for (int u = 0; u < U; ++u) take(v[u], base + u * NT + tid);
+  // the whole steps, each one's loads in flight while the one before it is taken
+  Tile a, b;
+  const int steps = full / STEP;
+  if (steps > 0) load(a, 0);
+  for (int i = 0; i < steps; i += 2) {
+    if (i + 1 < steps) load(b, (i + 1) * STEP);
+    take(a, i * STEP, own[0], own[1]);
+    if (i + 1 == steps) break;
+    if (i + 2 < steps) load(a, (i + 2) * STEP);
+    take(b, (i + 1) * STEP, own[2], own[3]);
   }
-  for (; base < n; base += NT) {
-    const int i = base + tid;
-    float v[VEC];
-    if (i < full)
-      load_full(x, i, v);
-    else
-      load_edge(x, i < n ? len : 0, i, v);
-    take(v, i);
+  if (steps * STEP < n) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) load_some<ONCE>(x, len, steps * STEP + u * NT + tid, a[u]);
+    take(a, steps * STEP, own[2], own[3]);
   }
 
   // to the largest logit of all threads
   State s;
-  const double m = block_max<WAVES>((double)a.m, red);
-  s.m = (float)m;
-  double S = a.S, Ud = a.U;
-  rebase(S, Ud, a.r, m, sc);
-  if (a.S == 0.f) S = Ud = 0.0;  // nothing met (its reference means nothing); a NaN stays
-  s.S = block_sum<WAVES>(S, red);
-  s.U = block_sum<WAVES>(Ud, red);
-  s.before = (int32_t)block_sum<WAVES>((double)a.before, red);
+  s.m = block_max(fmaxf(fmaxf(own[0], own[1]), fmaxf(own[2], own[3])), red);
+  double sum[3] = {(double)S[0] + S[1], (double)Us[0] + Us[1], (double)before};
+  if (NAMED && fabsf(s.m * sc.c) > SAFE && s.m > -INFINITY) {
+    sum[0] = 0.0;
+    for (int i = tid; i < len; i += NT)
+      if (!(named[i >> 5] >> (i & 31) & 1)) sum[0] += exp2(((double)Elem<T>::one(x + i) - (double)s.m) * sc.cd);
+  } else if (sum[0] == 0.0) {
+    sum[1] = 0.0;  // nothing met: its reference means nothing
+  } else {
+    rebase(sum[0], sum[1], (NAMED ? (double)r - (double)s.m * sc.cd : ((double)r - (double)s.m) * sc.cd));
+  }
+  block_sums(sum, red);
+  s.S = sum[0];
+  s.U = sum[1];
+  s.before = (int32_t)sum[2];
   return s;
 }
+
+// ---- host: whether rows are read past the caches.  256 MB of cache lie between the L2s and the memory:
+// @ONCE@
+inline bool read_once(int rows, int V, int esize) { return (double)rows * V * esize > 256e6; }
 
 // ---- host: how a batch of rows is cut, and what every call checks
 struct Cut {

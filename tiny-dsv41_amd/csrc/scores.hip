@@ -14,6 +14,7 @@
 //
 // A row of few is cut into slices, which leave their sums and their sorted lists in the workspace for a
 // second kernel.
+#include <limits.h>
 #include <math.h>
 
 #include "row_scan.h"
@@ -74,20 +75,48 @@ struct Shared {
     float group_max[MAX_GROUPS];
   };
   uint16_t list[LIST];
-  double red[WAVES];
-  int counts[2][WAVES];
+  double red[3 * WAVES];
+  int counts[2][7 * WAVES];
+  uint64_t least;
+  State state;
+  int64_t target;
+  float xt;
   int n;
 };
 
-// Descending bitonic sort of buf[0, n), padded with zeros to a power of two.  Every thread calls it.
+// Descending order of buf[0, n), n <= BUF.  Every thread calls it, behind a barrier.
 __device__ void sort_desc(uint64_t* buf, int n) {
-  int P = 64;
+  const int tid = threadIdx.x;
+  if (n <= 128) {
+    // each key's place is the number of larger ones, counted by 4 threads
+    const int i = tid >> 2;
+    const uint64_t key = i < n ? buf[i] : 0;
+    int before = 0;
+    for (int q = tid & 3; q < n; q += 4) before += buf[q] > key;
+    before += __shfl_xor(before, 1);
+    before += __shfl_xor(before, 2);
+    __syncthreads();
+    if (i < n && (tid & 3) == 0) buf[before] = key;
+    __syncthreads();
+    return;
+  }
+  // bitonic over the next power of two, padded with zeros.  Threads 64 w to 64 w + 63 take the pairs
+  // of 128 elements that no other wave touches while the pairs are at most 64 apart: those steps
+  // need no barrier.
+  int P = 256;
   while (P < n) P <<= 1;
-  for (int i = n + threadIdx.x; i < P; i += NT) buf[i] = 0;
+  for (int i = n + tid; i < P; i += NT) buf[i] = 0;
+  int last = P;
   for (int k = 2; k <= P; k <<= 1)
     for (int j = k >> 1; j > 0; j >>= 1) {
-      __syncthreads();
-      for (int q = threadIdx.x; q < P / 2; q += NT) {
+      if (j > 64 || last > 64) {
+        __syncthreads();
+      } else {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      }
+      last = j;
+      for (int q = tid; q < P / 2; q += NT) {
         const int i = 2 * q - (q & (j - 1));
         const uint64_t a = buf[i], b = buf[i + j];
         if ((a < b) == ((i & k) == 0)) {
@@ -114,64 +143,149 @@ __device__ void make_room(Shared& s, int K, uint64_t& floor_key) {
 
 __device__ __forceinline__ void push(Shared& s, uint64_t key) { s.buf[atomicAdd(&s.n, 1)] = key; }
 
-// How many of the workgroup's keys are at least `at`.
-template <int J>
-__device__ __forceinline__ int count_from(const uint32_t (&key)[J], uint32_t at, int* counts) {
-  int c = 0;
+template <int CTRL>
+__device__ __forceinline__ int dpp_i(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, true);
+}
+
+// c[w] summed over the workgroup's waves.
+template <int W>
+__device__ __forceinline__ void join_counts(int (&c)[W], int* counts) {
+  if ((threadIdx.x & 63) == 0)
 #pragma unroll
-  for (int j = 0; j < J; ++j) c += __popcll(__ballot(key[j] >= at));
-  if ((threadIdx.x & 63) == 0) counts[threadIdx.x >> 6] = c;
+    for (int w = 0; w < W; ++w) counts[w * WAVES + (threadIdx.x >> 6)] = c[w];
   __syncthreads();
-  c = 0;
+  // lane 8 w + i takes wave i's count of at[w]
+  static_assert(WAVES == 8 && W <= 8, "a lane for every count");
+  const int lane = threadIdx.x & 63;
+  int v = lane < W * WAVES ? counts[lane] : 0;
+  v += dpp_i<0xB1>(v);   // quad_perm [1,0,3,2]
+  v += dpp_i<0x4E>(v);   // quad_perm [2,3,0,1]
+  v += dpp_i<0x141>(v);  // row_half_mirror
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) c += counts[w];
+  for (int w = 0; w < W; ++w) c[w] = __builtin_amdgcn_readlane(v, 8 * w);
+}
+
+// Raises `lo`, an order that c >= K values reach, until at most `most` do, as far as ties let it; `hi`
+// is an order that fewer than K reach.  W + 1 intervals at a time, three times of the logits between the
+// two, then of their orders; count(at, c) counts the wave's values.
+template <class Count>
+__device__ __forceinline__ void search(uint32_t& lo, uint32_t& hi, int& c, int K, int most, int (*counts)[7 * WAVES],
+                                       Count count) {
+  constexpr int W = 7;
+  for (int turn = 0; c > most && hi - lo > 1u; ++turn) {
+    uint32_t at[W];
+    float value[W];
+    int got[W];
+    const float from = logit_of(lo), part = (logit_of(hi - 1u) - from) / (W + 1);
+    const uint32_t step = (hi - lo) / (W + 1);
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      at[w] = lo + (step ? step * (w + 1) : 1u);
+      if (turn < 3 && part < INFINITY) at[w] = min(max(order_of(from + part * (w + 1)), lo + 1u), hi - 1u);
+      value[w] = logit_of(at[w]);
+    }
+    count(value, got);
+    join_counts(got, counts[turn & 1]);
+    uint32_t above = hi;
+#pragma unroll
+    for (int w = W - 1; w >= 0; --w) {
+      if (at[w] >= above) continue;
+      if (got[w] >= K) {
+        lo = at[w];
+        c = got[w];
+        break;
+      }
+      above = at[w];
+    }
+    hi = above;
+  }
+}
+
+// Appends the groups whose maximum is at least `bound` to s.list, as many as it holds, and returns
+// their number.
+__device__ __forceinline__ int list_groups(Shared& s, int n, float bound) {
+  const int tid = threadIdx.x;
+  if (tid == 0) s.n = 0;
+  __syncthreads();
+  for (int j = tid; j < n; j += NT)
+    if (s.group_max[j] >= bound) {
+      const int at = atomicAdd(&s.n, 1);
+      if (at < LIST) s.list[at] = (uint16_t)j;
+    }
+  __syncthreads();
+  const int c = s.n;
+  __syncthreads();
   return c;
 }
 
 // s.list = at least the first K groups in (maximum desc, index asc) of those that hold an unmasked
-// element, or all of them; returns their number, and in `least` a bound that the K-th reaches.
-__device__ int select_groups(Shared& s, int n, int K, float m, uint32_t& least) {
-  constexpr int J = MAX_GROUPS / NT;
-  uint32_t key[J];
+// element, or all of them; returns their number, and in `least` (order_of) a bound that the row's K-th
+// element reaches.  own: the largest of the thread's shares, m: the row's largest.
+__device__ __forceinline__ int select_groups(Shared& s, int n, int K, const float (&own)[4], float m, uint32_t& least) {
+  constexpr int W = 7;
+  const int tid = threadIdx.x, most = K + max(16, K / 4);
+  const uint32_t top = order_of(m) + 1u;
+  uint32_t lo = ABOVE_MASKED;
+  int c;
+  // The K-th largest of the shares' maxima bounds the row's K-th element from below, and few more
+  // groups than K reach it where K is at most half of the shares: in rows of no special order, 68 groups
+  // the 64th of 512, 710 the 512th of 1024.
+  {
+    const float a = fmaxf(own[0], own[1]), b = fmaxf(own[2], own[3]), ab = fmaxf(a, b);
+    auto count = [&](const float(&at)[W], int(&got)[W]) {
 #pragma unroll
-  for (int j = 0; j < J; ++j) {
-    const int i = j * NT + (int)threadIdx.x;
-    key[j] = i < n ? order_of(s.group_max[i]) : 0u;
-  }
-  const int most = K + max(16, K / 4);
-  uint32_t lo = ABOVE_MASKED, hi = order_of(m) + 1u;
-  int turn = 0;
-  int c = count_from(key, lo, s.counts[0]);
-  while (c > most && hi - lo > 1u) {
-    const uint32_t mid = lo + ((hi - lo) >> 1);
-    turn ^= 1;
-    const int got = count_from(key, mid, s.counts[turn]);
-    if (got >= K) {
-      lo = mid;
-      c = got;
-    } else {
-      hi = mid;
+      for (int w = 0; w < W; ++w) {
+        if (K <= NT / 2)
+          got[w] = __popcll(__ballot(ab >= at[w]));
+        else if (K <= NT)
+          got[w] = __popcll(__ballot(a >= at[w])) + __popcll(__ballot(b >= at[w]));
+        else
+          got[w] = __popcll(__ballot(own[0] >= at[w])) + __popcll(__ballot(own[1] >= at[w])) +
+                   __popcll(__ballot(own[2] >= at[w])) + __popcll(__ballot(own[3] >= at[w]));
+      }
+    };
+    // (a share that met nothing but masked tokens is none; the others begin at the smallest of them)
+    const float least_own = fminf(fminf(own[0] > -INFINITY ? own[0] : INFINITY, own[1] > -INFINITY ? own[1] : INFINITY),
+                                  fminf(own[2] > -INFINITY ? own[2] : INFINITY, own[3] > -INFINITY ? own[3] : INFINITY));
+    const uint32_t first = max(order_of(-rows::block_max(-least_own, s.red)), ABOVE_MASKED);
+    const float at[W] = {logit_of(first), INFINITY, INFINITY, INFINITY, INFINITY, INFINITY, INFINITY};
+    int got[W];
+    count(at, got);
+    join_counts(got, s.counts[0]);
+    c = got[0];
+    __syncthreads();
+    if (c >= K) {
+      uint32_t hi = top;
+      lo = first;
+      search(lo, hi, c, K, most, s.counts, count);
     }
   }
   least = lo;
-  if (threadIdx.x == 0) s.n = 0;
-  __syncthreads();
+  c = list_groups(s, n, logit_of(lo));
+  if (c <= min(2 * most, LIST)) return c;
+
+  // too many: the bound is searched among the groups' maxima, and what is left at the end are ties
+  uint32_t hi = top;
+  search(lo, hi, c, K, most, s.counts, [&](const float(&at)[W], int(&got)[W]) {
+#pragma unroll
+    for (int w = 0; w < W; ++w) got[w] = 0;
+    for (int j = 0; j < n; j += NT) {
+      const float v = j + tid < n ? s.group_max[j + tid] : -INFINITY;
+#pragma unroll
+      for (int w = 0; w < W; ++w) got[w] += __popcll(__ballot(v >= at[w]));
+    }
+  });
+  least = lo;
   // those above `lo` in any order, and at most as many at `lo` as are wanted, from the lowest index
   const bool all = c <= most;
-  const uint32_t from = all ? lo : hi;
-#pragma unroll
-  for (int j = 0; j < J; ++j)
-    if (key[j] >= from) {
-      const int at = atomicAdd(&s.n, 1);
-      if (at < LIST) s.list[at] = (uint16_t)(j * NT + threadIdx.x);
-    }
-  __syncthreads();
-  int taken = min(s.n, LIST);
+  const float bound = logit_of(lo);
+  int taken = min(list_groups(s, n, all ? bound : logit_of(hi)), LIST);
   if (!all) {
-    for (int j = 0; j < J && j * NT < n && taken < K; ++j) {
-      const bool tie = key[j] == lo;
+    const int wave = tid >> 6, lane = tid & 63;
+    for (int j = 0; j < n && taken < K; j += NT) {
+      const bool tie = j + tid < n && s.group_max[j + tid] == bound;
       const uint64_t b = __ballot(tie);
-      const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
       __syncthreads();
       if (lane == 0) s.counts[0][wave] = __popcll(b);
       __syncthreads();
@@ -181,7 +295,7 @@ __device__ int select_groups(Shared& s, int n, int K, float m, uint32_t& least) 
         total += s.counts[0][w];
       }
       before += __popcll(b & ((1ull << lane) - 1ull));
-      if (tie && before < K) s.list[before] = (uint16_t)(j * NT + threadIdx.x);
+      if (tie && before < K) s.list[before] = (uint16_t)(j + tid);
       taken = min(K, taken + total);
     }
   }
@@ -192,30 +306,45 @@ __device__ int select_groups(Shared& s, int n, int K, float m, uint32_t& least) 
 // s.buf = the first K elements of x[0, len) in order (or as many as are not masked); returns their
 // number.  `first`: the index of x[0] in its row.
 template <typename T>
-__device__ int top_of(Shared& s, const T* x, int len, int first, int K, float m) {
+__device__ __forceinline__ int top_of(Shared& s, const T* x, int len, int first, int K, const float (&own)[4], float m) {
   constexpr int VEC = Elem<T>::VEC, LANES = GROUP / VEC, AT_ONCE = BATCH / GROUP;
   uint32_t least;
-  const int groups = select_groups(s, (len + GROUP - 1) / GROUP, K, m, least);
+  const int n_groups = (len + GROUP - 1) / GROUP;
+  const int groups = select_groups(s, n_groups, K, own, m, least);
   if (threadIdx.x == 0) s.n = 0;
   __syncthreads();
   uint64_t floor_key = 0;
-  for (int b = 0; b < groups; b += AT_ONCE) {
-    make_room(s, K, floor_key);
-    const int g = b + (int)threadIdx.x / LANES;
-    if ((int)threadIdx.x < AT_ONCE * LANES && g < groups) {
-      const int i = (int)s.list[g] * LANES + (int)threadIdx.x % LANES;
+  constexpr int AHEAD = 4;  // batches whose loads are in flight at once
+  const int lane = (int)threadIdx.x % LANES, first_group = (int)threadIdx.x / LANES;
+  for (int b = 0; b < groups; b += AHEAD * AT_ONCE) {
+    uint32_t w[AHEAD][4];
+    int at[AHEAD];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const int g = b + a * AT_ONCE + first_group;
+      at[a] = first_group < AT_ONCE && g < groups ? (int)s.list[g] * LANES + lane : -1;
+      rows::load_some<false>(x, len, at[a], w[a]);
+    }
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      if (b + a * AT_ONCE >= groups) break;
+      make_room(s, K, floor_key);
       float v[VEC];
-      if ((i + 1) * VEC <= len)
-        rows::load_full(x, i, v);
-      else
-        rows::load_edge(x, len, i, v);
+      Elem<T>::unpack(w[a], v);
+      uint32_t pass = 0;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        const uint64_t key = key_of(v[j], (uint32_t)(first + i * VEC + j));
-        if ((uint32_t)(key >> 32) >= least && key > floor_key) push(s, key);
+        const uint64_t key = key_of(v[j], (uint32_t)(first + at[a] * VEC + j));
+        pass |= (uint32_t)((uint32_t)(key >> 32) >= least && key > floor_key) << j;
       }
+      if (pass) {
+        int to = atomicAdd(&s.n, __popc(pass));
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (pass >> j & 1) s.buf[to++] = key_of(v[j], (uint32_t)(first + at[a] * VEC + j));
+      }
+      __syncthreads();
     }
-    __syncthreads();
   }
   const int n = s.n;
   sort_desc(s.buf, n);
@@ -223,11 +352,13 @@ __device__ int top_of(Shared& s, const T* x, int len, int first, int K, float m)
 }
 
 // The row's outputs from its sums and its sorted list.
-__device__ void write_row(const Params& p, int row, State st, float xt, int64_t target, const uint64_t* top, int n_top) {
+__device__ __forceinline__ void write_row(const Params& p, int row, const Shared& s, int n_top) {
+  const State st = s.state;
+  const uint64_t* top = s.buf;
   const double S = st.S + p.sc.kappa * st.U;
   const bool bad = !(S > 0.0 && S < INFINITY);
   const double m = st.m, ln_s = log(S);
-  const double entropy = bad ? (double)NAN : fmax(ln_s - st.U * (p.sc.inv_t / p.sc.c) / S, 0.0);
+  const double entropy = bad ? (double)NAN : fmax(ln_s - st.U * (p.sc.inv_t / p.sc.cd) / S, 0.0);
   for (int i = threadIdx.x; i < p.K; i += NT) {
     const uint64_t key = i < n_top ? top[i] : 0;
     const int64_t at = (int64_t)row * p.K + i;
@@ -239,6 +370,8 @@ __device__ void write_row(const Params& p, int row, State st, float xt, int64_t 
   if (threadIdx.x) return;
   int status = bad ? DSV41_STATUS_NONFINITE : 0;
   if (p.targets) {
+    const int64_t target = s.target;
+    const float xt = s.xt;
     const bool outside = target < 0 || target >= p.V;
     if (outside) status |= DSV41_STATUS_BAD_TARGET;
     p.out_logprob[row] = bad || outside ? NAN : (float)(((double)xt - m) * p.sc.inv_t - ln_s);
@@ -255,8 +388,8 @@ __device__ void write_row(const Params& p, int row, State st, float xt, int64_t 
   }
 }
 
-template <typename T, bool TOP>
-__global__ __launch_bounds__(NT) void scores_kernel(Params p) {
+template <typename T, bool ONCE, bool TOP>
+__global__ __launch_bounds__(NT, 8) void scores_kernel(Params p) {
   __shared__ Shared s;
   const int row = blockIdx.x / p.slices, slice = blockIdx.x % p.slices;
   const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.stride;
@@ -267,66 +400,92 @@ __global__ __launch_bounds__(NT) void scores_kernel(Params p) {
     target = p.targets[row];
     if (target >= 0 && target < p.V) xt = Elem<T>::one(x + target);
   }
+  float own[4];
   const State st =
-      rows::scan<T, TOP, false>(x + begin, len, p.sc, xt, target - begin, s.group_max, nullptr, s.red);
+      rows::scan<T, ONCE, TOP, false>(x + begin, len, p.sc, xt, (int)(target - begin), s.group_max, nullptr, s.red, own);
+  if (threadIdx.x == 0) {  // (registers that would be kept over the selection)
+    s.state = st;
+    s.target = target;
+    s.xt = xt;
+  }
   int n = 0;
-  if constexpr (TOP) n = top_of(s, x + begin, len, begin, p.K, st.m);
+  if constexpr (TOP)
+    n = top_of(s, x + begin, len, begin, p.K, own, st.m);
+  else
+    __syncthreads();
   if (p.slices == 1) {
-    write_row(p, row, st, xt, target, s.buf, n);
+    write_row(p, row, s, n);
     return;
   }
   const int64_t at = (int64_t)row * p.slices + slice;
-  if (threadIdx.x == 0) p.states[at] = st;
+  if (threadIdx.x == 0) p.states[at] = s.state;
   for (int i = threadIdx.x; i < p.K; i += NT) p.keys[at * p.K + i] = i < n ? s.buf[i] : 0;
 }
 
-// Joins the slices of a row.
+// Joins the slices of a row, at most 64.
 template <typename T>
 __global__ __launch_bounds__(NT) void scores_join_kernel(Params p) {
   __shared__ Shared s;
   const int row = blockIdx.x, tid = threadIdx.x;
-  const State* states = p.states + (int64_t)row * p.slices;
-  State st{0.0, 0.0, -INFINITY, 0};
-  if (tid < p.slices) st = states[tid];
-  const double m = rows::block_max<WAVES>((double)st.m, s.red);
-  if (st.S == 0.0)
-    st.U = 0.0;
-  else
-    rows::rebase(st.S, st.U, st.m, m, p.sc);
-  st.m = (float)m;
-  st.S = rows::block_sum<WAVES>(st.S, s.red);
-  st.U = rows::block_sum<WAVES>(st.U, s.red);
-  st.before = (int32_t)rows::block_sum<WAVES>((double)st.before, s.red);
-  int n = 0;
-  if (p.K) {
-    // each list holds K elements that come no later than its last, so the row's K-th comes no later
-    // than any of these lasts
-    const uint64_t* keys = p.keys + (int64_t)row * p.slices * p.K;
-    uint64_t least = 1;
-    for (int i = 0; i < p.slices; ++i) least = max(least, keys[(int64_t)i * p.K + p.K - 1]);
-    const int total = p.slices * p.K;
-    if (tid == 0) s.n = 0;
-    __syncthreads();
-    uint64_t floor_key = 0;
-    for (int b = 0; b < total; b += BATCH) {
-      make_room(s, p.K, floor_key);
-      for (int i = b + tid; i < min(total, b + BATCH); i += NT) {
-        const uint64_t key = keys[i];
-        if (key >= least && key > floor_key) push(s, key);
-      }
-      __syncthreads();
-    }
-    n = s.n;
-    sort_desc(s.buf, n);
-    n = min(n, p.K);
-  }
+  const uint64_t* keys = p.keys + (int64_t)row * p.slices * p.K;
+  const int total = p.slices * p.K;
+  constexpr int EACH = BATCH / NT;
+  uint64_t key[EACH];
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) key[e] = e * NT + tid < total ? keys[e * NT + tid] : 0;
   int64_t target = -1;
   float xt = INFINITY;
   if (p.targets) {
     target = p.targets[row];
     if (target >= 0 && target < p.V) xt = Elem<T>::one(static_cast<const T*>(p.logits) + (int64_t)row * p.stride + target);
   }
-  write_row(p, row, st, xt, target, s.buf, n);
+  if (tid < 64) {
+    State st{0.0, 0.0, -INFINITY, 0};
+    uint64_t least = 1;
+    if (tid < p.slices) {
+      st = p.states[(int64_t)row * p.slices + tid];
+      // each list holds K elements that come no later than its last, so the row's K-th comes no later
+      // than any of these lasts
+      if (p.K) least = max(least, keys[(int64_t)tid * p.K + p.K - 1]);
+    }
+    const float m = wave_max_dpp(st.m);
+    if (st.S == 0.0)
+      st.U = 0.0;
+    else
+      rows::rebase(st.S, st.U, ((double)st.m - (double)m) * p.sc.cd);
+    const double S = wave_total_d(st.S), U = wave_total_d(st.U);
+    const int before = wave_sum_i(st.before);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) least = max(least, (uint64_t)__shfl_xor((unsigned long long)least, o));
+    if (tid == 0) {
+      s.state = State{S, U, m, before};
+      s.target = target;
+      s.xt = xt;
+      s.least = least;
+      s.n = 0;
+    }
+  }
+  __syncthreads();
+  int n = 0;
+  if (p.K) {
+    const uint64_t least = s.least;
+    uint64_t floor_key = 0;
+    for (int b = 0; b < total; b += BATCH) {
+      if (b) {
+        make_room(s, p.K, floor_key);
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) key[e] = b + e * NT + tid < total ? keys[b + e * NT + tid] : 0;
+      }
+#pragma unroll
+      for (int e = 0; e < EACH; ++e)
+        if (key[e] >= least && key[e] > floor_key) push(s, key[e]);
+      __syncthreads();
+    }
+    n = s.n;
+    sort_desc(s.buf, n);
+    n = min(n, p.K);
+  }
+  write_row(p, row, s, n);
 }
 
 // ------------------------------------------------------------------------------------ gradient
@@ -349,7 +508,7 @@ struct GradParams {
 // tokens that have a gradient of their own are written again after the workgroup's barrier.
 template <typename T>
 __global__ __launch_bounds__(NT) void scores_grad_kernel(GradParams p) {
-  __shared__ double red[WAVES];
+  __shared__ double red[3 * WAVES];
   const int row = p.rows - 1 - (int)(blockIdx.x / p.slices), slice = blockIdx.x % p.slices;
   const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.stride;
   const int begin = slice * p.len, len = min(p.len, p.V - begin);
@@ -367,7 +526,9 @@ __global__ __launch_bounds__(NT) void scores_grad_kernel(GradParams p) {
         G += g_top[k];
         any |= g_top[k] != 0.f;
       }
-    G = rows::block_sum<WAVES>(G, red);
+    double sum[1] = {G};
+    rows::block_sums(sum, red);
+    G = sum[0];
     any = __syncthreads_or(any);
   }
   G += g_lp != 0.0 && (t < 0 || t >= p.V) ? (double)NAN : g_lp;
@@ -422,14 +583,21 @@ size_t workspace_of(int rows, int K, const Cut& c) {
   return c.slices == 1 ? 0 : (size_t)rows * c.slices * (sizeof(State) + (size_t)K * sizeof(uint64_t));
 }
 
-template <typename T>
+template <typename T, bool ONCE>
 void launch(const Params& p, hipStream_t s) {
   const dim3 grid((unsigned)p.rows * (unsigned)p.slices);
   if (p.K)
-    hipLaunchKernelGGL((scores_kernel<T, true>), grid, dim3(NT), 0, s, p);
+    hipLaunchKernelGGL((scores_kernel<T, ONCE, true>), grid, dim3(NT), 0, s, p);
   else
-    hipLaunchKernelGGL((scores_kernel<T, false>), grid, dim3(NT), 0, s, p);
+    hipLaunchKernelGGL((scores_kernel<T, ONCE, false>), grid, dim3(NT), 0, s, p);
   if (p.slices > 1) hipLaunchKernelGGL(scores_join_kernel<T>, dim3(p.rows), dim3(NT), 0, s, p);
+}
+template <typename T>
+void launch(const Params& p, hipStream_t s) {
+  if (rows::read_once(p.rows, p.V, sizeof(T)))
+    launch<T, true>(p, s);
+  else
+    launch<T, false>(p, s);
 }
 
 int check_desc(const dsv41_scores_desc* d) {
@@ -472,7 +640,7 @@ extern "C" int dsv41_scores_run(const dsv41_scores_desc* d, void* workspace, siz
   p.K = d->top_k;
   p.slices = c.slices;
   p.len = c.len;
-  p.sc = rows::scale_of(d->temperature);
+  p.sc = rows::scale_of(d->temperature, false);
   p.out_logprob = d->out_logprob;
   p.out_rank = d->out_rank;
   p.out_entropy = d->out_entropy;
@@ -514,7 +682,7 @@ extern "C" int dsv41_scores_grad_run(const dsv41_scores_grad_desc* d, void* stre
   p.K = d->grad_top ? d->top_k : 0;
   p.slices = c.slices;
   p.len = c.len;
-  p.sc = rows::scale_of(d->temperature);
+  p.sc = rows::scale_of(d->temperature, false);
   p.stats = d->stats;
   p.g_logprob = d->grad_logprob;
   p.g_entropy = d->grad_entropy;
