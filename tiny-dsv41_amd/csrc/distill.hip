@@ -54,7 +54,7 @@ struct Params {
 };
 
 struct Shared {
-  uint32_t named[MAX_LEN / 32];
+  alignas(16) uint32_t named[MAX_LEN / 32];  // whole 16 bytes
   double red[4 * WAVES];
   int flags;
 };
@@ -103,33 +103,35 @@ __device__ __forceinline__ void finish(const Params& p, int row, State st, int f
     write_row(p, row, NAN, flags & ~LIVE, NAN, NAN, NAN, NAN, 0.0, true);
     return;
   }
+  // (a list of more than NT entries is read again here; the first entries stay in registers, and the
+  // code for them apart, which the constants of a loop would push into memory)
   float mf = st.m, top = -INFINITY;
   int bad = 0;
-  Entry e = mine;
-  for (int k = threadIdx.x; k < p.K; k += NT) {
-    if (k >= NT) e = entry_of<T>(p, row, k);
-    if (e.id >= 0) {
-      mf = fmaxf(mf, e.x);
-      top = fmaxf(top, e.lq);
-      bad |= !(e.lq < INFINITY);
-    }
-  }
+  const auto meet = [&](const Entry& e) {
+    if (e.id < 0) return;
+    mf = fmaxf(mf, e.x);
+    top = fmaxf(top, e.lq);
+    bad |= !(e.lq < INFINITY);
+  };
+  meet(mine);
+  for (int k = threadIdx.x + NT; k < p.K; k += NT) meet(entry_of<T>(p, row, k));
   const double m = rows::block_max(mf, red);
   top = p.rest ? 0.f : rows::block_max(top, red);
   bad = __syncthreads_or(bad || !(top > -INFINITY));
   double sum[4] = {0.0, 0.0, 0.0, 0.0};
-  e = mine;
-  for (int k = threadIdx.x; k < p.K && !bad; k += NT) {
-    if (k >= NT) e = entry_of<T>(p, row, k);
-    if (e.id >= 0) {
-      const double d = ((double)e.x - m) * p.sc.inv_t, l = (double)e.lq - top, w = exp(l);
-      sum[0] += exp(d);
-      if (w > 0.0) {
-        sum[1] += w;
-        sum[2] += w * l;
-        sum[3] += w * d;
-      }
+  const auto add = [&](const Entry& e) {
+    if (e.id < 0) return;
+    const double d = ((double)e.x - m) * p.sc.inv_t, l = (double)e.lq - top, w = exp(l);
+    sum[0] += exp(d);
+    if (w > 0.0) {
+      sum[1] += w;
+      sum[2] += w * l;
+      sum[3] += w * d;
     }
+  };
+  if (!bad) {
+    add(mine);
+    for (int k = threadIdx.x + NT; k < p.K; k += NT) add(entry_of<T>(p, row, k));
   }
   rows::block_sums(sum, red);
   const double Sn = sum[0], W = sum[1], WL = sum[2], WD = sum[3];
@@ -162,28 +164,31 @@ __global__ __launch_bounds__(NT, 8) void distill_kernel(Params p) {
   const int row = blockIdx.x / p.slices, slice = blockIdx.x % p.slices, tid = threadIdx.x;
   const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.stride;
   const int begin = slice * p.len, len = min(p.len, p.V - begin);
-  const Entry mine = entry_of<T>(p, row, tid);
-  for (int i = tid; i < (len + 31) / 32; i += NT) s.named[i] = 0;
-  if (tid == 0) s.flags = 0;
-  __syncthreads();
-  int f = 0;
-  for (int k = tid; k < p.K; k += NT) {
-    const int64_t id = k < NT ? mine.id : p.ids[(int64_t)row * p.K + k];
-    if (id < 0) continue;
-    f |= LIVE;
-    if (id >= p.V) f |= DSV41_STATUS_BAD_TARGET;
-    if (id >= begin && id < begin + len) {
-      const uint32_t i = (uint32_t)(id - begin), bit = 1u << (i & 31);
-      if (atomicOr(&s.named[i >> 5], bit) & bit) f |= DSV41_STATUS_REPEATED;
+  Entry mine;
+  int flags;
+  const auto before = [&](float&, int&) {
+    mine = entry_of<T>(p, row, tid);
+    for (int i = 4 * tid; i < (len + 31) / 32; i += 4 * NT) *reinterpret_cast<uint4*>(s.named + i) = make_uint4(0, 0, 0, 0);
+    if (tid == 0) s.flags = 0;
+    __syncthreads();
+    int f = 0;
+    for (int k = tid; k < p.K; k += NT) {
+      const int64_t id = k < NT ? mine.id : p.ids[(int64_t)row * p.K + k];
+      if (id < 0) continue;
+      f |= LIVE;
+      if (id >= p.V) f |= DSV41_STATUS_BAD_TARGET;
+      if (id >= begin && id < begin + len) {
+        const uint32_t i = (uint32_t)(id - begin), bit = 1u << (i & 31);
+        if (atomicOr(&s.named[i >> 5], bit) & bit) f |= DSV41_STATUS_REPEATED;
+      }
     }
-  }
-  if (f) atomicOr(&s.flags, f);
-  __syncthreads();
-  const int flags = s.flags;
-  State st{0.0, 0.0, -INFINITY, 0};
+    if (f) atomicOr(&s.flags, f);
+    __syncthreads();
+    flags = s.flags;
+    return flags == LIVE;
+  };
   float own[4];
-  if (flags == LIVE)
-    st = rows::scan<T, ONCE, false, true>(x + begin, len, p.sc, INFINITY, 0, nullptr, s.named, s.red, own);
+  const State st = rows::scan<T, ONCE, false, true>(x + begin, len, p.sc, before, nullptr, s.named, s.red, own);
   if (p.slices == 1) {
     finish<T>(p, row, st, flags, mine, s.red);
   } else if (tid == 0) {

@@ -150,33 +150,48 @@ __device__ __forceinline__ void fill_zero(T* out, int len) {
   for (int i = full * VEC + (int)threadIdx.x; i < len; i += NT) store_one(out + i, 0.f);
 }
 
-// ---- sums and maxima over the workgroup, the same value in every thread.  `s`: LDS, WAVES values for
-// each value that is joined.
+// ---- sums and maxima over the workgroup, the same value in every thread, in scalar registers.  `s`: LDS,
+// WAVES values for each value that is joined.  Eight lanes take the waves' values of each.
+static_assert(WAVES == 8, "a lane for every wave's value");
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xF, 0xF, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xF, 0xF, true);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double lane_d(double v, int lane) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, lane);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
 template <int N>
 __device__ __forceinline__ void block_sums(double (&v)[N], double* s) {
+  static_assert(N <= 8, "a lane for every value");
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = wave_total_d(v[i]);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0)
+  const int lane = threadIdx.x & 63;
+  if (lane == 0)
 #pragma unroll
     for (int i = 0; i < N; ++i) s[i * WAVES + (threadIdx.x >> 6)] = v[i];
   __syncthreads();
+  double a = lane < N * WAVES ? s[lane] : 0.0;
+  a += dpp_d<0xB1>(a);   // quad_perm [1,0,3,2]
+  a += dpp_d<0x4E>(a);   // quad_perm [2,3,0,1]
+  a += dpp_d<0x141>(a);  // row_half_mirror
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    v[i] = 0.0;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) v[i] += s[i * WAVES + w];
-  }
+  for (int i = 0; i < N; ++i) v[i] = lane_d(a, 8 * i);
 }
 __device__ __forceinline__ float block_max(float v, double* s) {
   v = wave_max_dpp(v);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+  const int lane = threadIdx.x & 63;
+  if (lane == 0) s[threadIdx.x >> 6] = v;
   __syncthreads();
-  v = (float)s[0];
-#pragma unroll
-  for (int w = 1; w < WAVES; ++w) v = fmaxf(v, (float)s[w]);
-  return v;
+  const float w = wave_max_dpp((float)s[lane & (WAVES - 1)]);
+  return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(w)));
 }
 
 // The scale of a temperature, computed on the host.
@@ -254,10 +269,11 @@ constexpr float SAFE = 1e30f;  // the largest |m c| that x c - r is formed with
 // One pass over x[0, len) by the workgroup, whose threads take 16 bytes in turn.
 //   TOP: group_max[g] = the largest of the elements [32 g, 32 g + 32).
 //   NAMED: the sum outside a list: elements whose bit in `named` is set count as masked.
-//   xt, t: the target's logit (+inf: no target) and index, from x's begin.
+//   before(xt, t): called once, with the first loads in flight; it may use barriers, gives the target's
+//     logit (+inf: no target) and index, from x's begin, and says whether there is a pass to make.
 //   own: the largest elements of the thread's four shares of the row.
-template <typename T, bool ONCE, bool TOP, bool NAMED>
-__device__ __forceinline__ State scan(const T* x, int len, const Scale& sc, float xt, int t, float* group_max,
+template <typename T, bool ONCE, bool TOP, bool NAMED, class Before>
+__device__ __forceinline__ State scan(const T* x, int len, const Scale& sc, Before before, float* group_max,
                                       const uint32_t* named, double* red, float (&own)[4]) {
   constexpr int VEC = Elem<T>::VEC, LANES = GROUP / VEC;
   const int full = len / VEC, n = (len + VEC - 1) / VEC;
@@ -266,7 +282,8 @@ __device__ __forceinline__ State scan(const T* x, int len, const Scale& sc, floa
   for (int u = 0; u < 4; ++u) own[u] = -INFINITY;
   float r = LOWEST, S[2] = {0.f, 0.f}, Us[2] = {0.f, 0.f}, margin = NAMED ? 2.f : sc.margin;
   asm("" : "+v"(margin));  // (a scalar register short, the compiler would load it in every step)
-  int before = 0;
+  int ahead = 0, t = 0;
+  float xt = INFINITY;
 
   using Tile = uint32_t[2][4];  // two chunks a thread
   constexpr int STEP = 2 * NT;
@@ -298,7 +315,7 @@ __device__ __forceinline__ State scan(const T* x, int len, const Scale& sc, floa
       for (int u = 0; u < 2; ++u) {
         const int below = t - (base + u * NT + tid) * VEC;  // elements of the chunk with a lower index
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) before += (v[u][j] > xt || (v[u][j] == xt && j < below)) ? 1 : 0;
+        for (int j = 0; j < VEC; ++j) ahead += (v[u][j] > xt || (v[u][j] == xt && j < below)) ? 1 : 0;
       }
     }
     if constexpr (TOP) {
@@ -345,7 +362,13 @@ __device__ __forceinline__ State scan(const T* x, int len, const Scale& sc, floa
   // the whole steps, each one's loads in flight while the one before it is taken
   Tile a, b;
   const int steps = full / STEP;
-  if (steps > 0) load(a, 0);
+  if (steps > 0) {
+    load(a, 0);
+  } else {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) load_some<ONCE>(x, len, u * NT + tid, a[u]);
+  }
+  if (!before(xt, t)) return State{0.0, 0.0, -INFINITY, 0};
   for (int i = 0; i < steps; i += 2) {
     if (i + 1 < steps) load(b, (i + 1) * STEP);
     take(a, i * STEP, own[0], own[1]);
@@ -354,15 +377,17 @@ __device__ __forceinline__ State scan(const T* x, int len, const Scale& sc, floa
     take(b, (i + 1) * STEP, own[2], own[3]);
   }
   if (steps * STEP < n) {
+    if (steps > 0) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) load_some<ONCE>(x, len, steps * STEP + u * NT + tid, a[u]);
+      for (int u = 0; u < 2; ++u) load_some<ONCE>(x, len, steps * STEP + u * NT + tid, a[u]);
+    }
     take(a, steps * STEP, own[2], own[3]);
   }
 
   // to the largest logit of all threads
   State s;
   s.m = block_max(fmaxf(fmaxf(own[0], own[1]), fmaxf(own[2], own[3])), red);
-  double sum[3] = {(double)S[0] + S[1], (double)Us[0] + Us[1], (double)before};
+  double sum[3] = {(double)S[0] + S[1], (double)Us[0] + Us[1], (double)ahead};
   if (NAMED && fabsf(s.m * sc.c) > SAFE && s.m > -INFINITY) {
     sum[0] = 0.0;
     for (int i = tid; i < len; i += NT)
