@@ -187,8 +187,8 @@ __global__ __launch_bounds__(NT, 8) void distill_kernel(Params p) {
     flags = s.flags;
     return flags == LIVE;
   };
-  float own[4];
-  const State st = rows::scan<T, ONCE, false, true>(x + begin, len, p.sc, before, nullptr, s.named, s.red, own);
+  const State st = rows::scan<T, ONCE, false, true>(
+      x + begin, len, p.sc, nullptr, s.named, s.red, before, [](const float(&)[4]) {}, [](float) {});
   if (p.slices == 1) {
     finish<T>(p, row, st, flags, mine, s.red);
   } else if (tid == 0) {

@@ -166,12 +166,13 @@ __device__ __forceinline__ double lane_d(double v, int lane) {
   const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane);
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
-template <int N>
+// FRESH: `s` has not been read since the last barrier, so none is needed before it is written.
+template <bool FRESH = false, int N>
 __device__ __forceinline__ void block_sums(double (&v)[N], double* s) {
   static_assert(N <= 8, "a lane for every value");
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = wave_total_d(v[i]);
-  __syncthreads();
+  if (!FRESH) __syncthreads();
   const int lane = threadIdx.x & 63;
   if (lane == 0)
 #pragma unroll
@@ -184,9 +185,10 @@ __device__ __forceinline__ void block_sums(double (&v)[N], double* s) {
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = lane_d(a, 8 * i);
 }
+template <bool FRESH = false>
 __device__ __forceinline__ float block_max(float v, double* s) {
   v = wave_max_dpp(v);
-  __syncthreads();
+  if (!FRESH) __syncthreads();
   const int lane = threadIdx.x & 63;
   if (lane == 0) s[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -271,15 +273,16 @@ constexpr float SAFE = 1e30f;  // the largest |m c| that x c - r is formed with
 //   NAMED: the sum outside a list: elements whose bit in `named` is set count as masked.
 //   before(xt, t): called once, with the first loads in flight; it may use barriers, gives the target's
 //     logit (+inf: no target) and index, from x's begin, and says whether there is a pass to make.
-//   own: the largest elements of the thread's four shares of the row.
-template <typename T, bool ONCE, bool TOP, bool NAMED, class Before>
-__device__ __forceinline__ State scan(const T* x, int len, const Scale& sc, Before before, float* group_max,
-                                      const uint32_t* named, double* red, float (&own)[4]) {
+//   met(own): called with the largest elements of the thread's four shares, before a barrier; found(m)
+//     with the largest of all, behind it and before the last one.
+//   red: LDS of 4 WAVES values that nothing else uses in the meantime.
+template <typename T, bool ONCE, bool TOP, bool NAMED, class Before, class Met, class Found>
+__device__ __forceinline__ State scan(const T* x, int len, const Scale& sc, float* group_max, const uint32_t* named,
+                                      double* red, Before before, Met met, Found found) {
   constexpr int VEC = Elem<T>::VEC, LANES = GROUP / VEC;
   const int full = len / VEC, n = (len + VEC - 1) / VEC;
   const int tid = threadIdx.x;
-#pragma unroll
-  for (int u = 0; u < 4; ++u) own[u] = -INFINITY;
+  float own[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
   float r = LOWEST, S[2] = {0.f, 0.f}, Us[2] = {0.f, 0.f}, margin = NAMED ? 2.f : sc.margin;
   asm("" : "+v"(margin));  // (a scalar register short, the compiler would load it in every step)
   int ahead = 0, t = 0;
@@ -386,7 +389,8 @@ __device__ __forceinline__ State scan(const T* x, int len, const Scale& sc, Befo
 
   // to the largest logit of all threads
   State s;
-  s.m = block_max(fmaxf(fmaxf(own[0], own[1]), fmaxf(own[2], own[3])), red);
+  met(own);
+  s.m = block_max<true>(fmaxf(fmaxf(own[0], own[1]), fmaxf(own[2], own[3])), red);
   double sum[3] = {(double)S[0] + S[1], (double)Us[0] + Us[1], (double)ahead};
   if (NAMED && fabsf(s.m * sc.c) > SAFE && s.m > -INFINITY) {
     sum[0] = 0.0;
@@ -397,7 +401,8 @@ __device__ __forceinline__ State scan(const T* x, int len, const Scale& sc, Befo
   } else {
     rebase(sum[0], sum[1], (NAMED ? (double)r - (double)s.m * sc.cd : ((double)r - (double)s.m) * sc.cd));
   }
-  block_sums(sum, red);
+  found(s.m);
+  block_sums<true>(sum, red + WAVES);
   s.S = sum[0];
   s.U = sum[1];
   s.before = (int32_t)sum[2];

@@ -38,7 +38,7 @@ constexpr int LIST = MAX_K + MAX_K / 4 + 64;      // groups that are read again
 constexpr int BATCH = 2048;                       // elements or keys that one step may add to the buffer
 constexpr int BUF = 2 * BATCH;
 constexpr int BUCKETS = NT;                       // of a sort
-constexpr int CROWD = 64;                         // keys of one bucket that are placed by counting
+constexpr int CROWD = 256;                        // keys of one bucket that are placed by counting
 static_assert(BUF >= BATCH + MAX_K, "a compressed buffer takes a batch");
 static_assert(BUF * sizeof(uint64_t) >= MAX_GROUPS * sizeof(float), "the buffer stands over the group maxima");
 
@@ -78,13 +78,13 @@ struct Shared {
   };
   uint16_t list[LIST];
   int bucket[BUCKETS];
-  double red[3 * WAVES];
+  double red[4 * WAVES];
   int counts[2][7 * WAVES];
   uint64_t least;
   State state;
   int64_t target;
-  float xt;
-  int n;
+  float xt, bound;
+  int n, listed;
 };
 
 // Descending bitonic sort of buf[0, n), over the next power of two, padded with zeros.  Threads 64 w to
@@ -179,6 +179,7 @@ __device__ __forceinline__ void sort_desc(Shared& s, int n, float low, float m) 
     if (!key[e]) continue;
     const int b = s.bucket[bucket_of(key[e])], first = b & 0xFFFF, end = first + (b >> 16);
     int at = first;
+#pragma unroll 4
     for (int q = first; q < end; ++q) at += buf[q] > key[e];
     slot[e] = at;
   }
@@ -231,11 +232,9 @@ __device__ __forceinline__ void join_counts(int (&c)[W], int* counts) {
 
 // Raises `lo`, an order that c >= K values reach, until at most `most` do, as far as ties let it; `hi`
 // is an order that fewer than K reach.  W + 1 intervals at a time, three times of the logits between the
-// two, then of their orders; count(at, c) counts the wave's values.
-template <class Count>
-__device__ __forceinline__ void search(uint32_t& lo, uint32_t& hi, int& c, int K, int most, int (*counts)[7 * WAVES],
-                                       Count count) {
-  constexpr int W = 7;
+// two, then of their orders; count(at, got) gives how many reach each at[w].
+template <int W, class Count>
+__device__ __forceinline__ void search(uint32_t& lo, uint32_t& hi, int& c, int K, int most, Count count) {
   for (int turn = 0; c > most && hi - lo > 1u; ++turn) {
     uint32_t at[W];
     float value[W];
@@ -249,7 +248,6 @@ __device__ __forceinline__ void search(uint32_t& lo, uint32_t& hi, int& c, int K
       value[w] = logit_of(at[w]);
     }
     count(value, got);
-    join_counts(got, counts[turn & 1]);
     uint32_t above = hi;
 #pragma unroll
     for (int w = W - 1; w >= 0; --w) {
@@ -265,72 +263,104 @@ __device__ __forceinline__ void search(uint32_t& lo, uint32_t& hi, int& c, int K
   }
 }
 
-// Appends the groups whose maximum is at least `bound` to s.list, as many as it holds, and returns
-// their number.
-__device__ __forceinline__ int list_groups(Shared& s, int n, float bound) {
-  const int tid = threadIdx.x;
-  if (tid == 0) s.n = 0;
+// The selection begins within the pass: what the threads met bounds the row's K-th element.  The K-th
+// largest of the shares' maxima is such a bound, and few more groups than K reach it where K is at most
+// half of the shares: in rows of no special order, 68 groups the 64th of 512, 710 the 512th of 1024.
+// Up to K = 256 one wave searches among the 512 threads' maxima by itself, without a barrier (0.9 us,
+// 3.4 by all waves); above, all search among 1024 or 2048 (search_shares).
+constexpr int ALONE = NT / 2;
+__device__ __forceinline__ void met_shares(Shared& s, const float (&own)[4], int K) {
+  if (K <= ALONE) s.bucket[threadIdx.x] = __float_as_int(fmaxf(fmaxf(own[0], own[1]), fmaxf(own[2], own[3])));
+}
+__device__ __forceinline__ void search_alone(Shared& s, int K, float m) {
+  if (threadIdx.x >= 64) return;
+  constexpr int EACH = NT / 64, W = 3;
+  float v[EACH], least = INFINITY;
+  int c = 0;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    v[e] = __int_as_float(s.bucket[e * 64 + threadIdx.x]);
+    c += __popcll(__ballot(v[e] > -INFINITY));
+    least = fminf(least, v[e] > -INFINITY ? v[e] : INFINITY);
+  }
+  uint32_t lo = ABOVE_MASKED;
+  if (c >= K) {
+    // (the smallest: a maximum with the signs turned)
+    lo = max(order_of(-wave_max_dpp(-least)), ABOVE_MASKED);
+    uint32_t hi = order_of(m) + 1u;
+    search<W>(lo, hi, c, K, K + max(16, K / 4), [&](const float(&at)[W], int(&got)[W]) {
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        got[w] = 0;
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) got[w] += __popcll(__ballot(v[e] >= at[w]));
+      }
+    });
+  }
+  if (threadIdx.x == 0) {
+    s.bound = logit_of(lo);
+    s.listed = s.n = 0;
+  }
+}
+__device__ __forceinline__ void search_shares(Shared& s, const float (&own)[4], int K, float m) {
+  constexpr int W = 7;
+  const float a = fmaxf(own[0], own[1]), b = fmaxf(own[2], own[3]);
+  int turn = 0;
+  const auto count = [&](const float(&at)[W], int(&got)[W]) {
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+      got[w] = K <= NT ? __popcll(__ballot(a >= at[w])) + __popcll(__ballot(b >= at[w]))
+                       : __popcll(__ballot(own[0] >= at[w])) + __popcll(__ballot(own[1] >= at[w])) +
+                             __popcll(__ballot(own[2] >= at[w])) + __popcll(__ballot(own[3] >= at[w]));
+    join_counts(got, s.counts[turn]);
+    turn ^= 1;
+  };
+  float least = INFINITY;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) least = fminf(least, own[u] > -INFINITY ? own[u] : INFINITY);
+  const uint32_t first = max(order_of(-rows::block_max(-least, s.red)), ABOVE_MASKED);
+  const float at[W] = {logit_of(first), INFINITY, INFINITY, INFINITY, INFINITY, INFINITY, INFINITY};
+  int got[W];
+  count(at, got);
+  int c = got[0];
+  uint32_t lo = ABOVE_MASKED, hi = order_of(m) + 1u;
+  if (c >= K) {
+    lo = first;
+    search<W>(lo, hi, c, K, K + K / 4, count);
+  }
+  if (threadIdx.x == 0) {
+    s.bound = logit_of(lo);
+    s.listed = s.n = 0;
+  }
   __syncthreads();
-  for (int j = tid; j < n; j += NT)
+}
+
+// Appends the groups whose maximum is at least `bound` to s.list, from s.listed = 0 on, as many as it
+// holds, and returns their number.
+__device__ __forceinline__ int list_groups(Shared& s, int n, float bound) {
+  for (int j = threadIdx.x; j < n; j += NT)
     if (s.group_max[j] >= bound) {
-      const int at = atomicAdd(&s.n, 1);
+      const int at = atomicAdd(&s.listed, 1);
       if (at < LIST) s.list[at] = (uint16_t)j;
     }
   __syncthreads();
-  const int c = s.n;
-  __syncthreads();
-  return c;
+  return s.listed;
 }
 
 // s.list = at least the first K groups in (maximum desc, index asc) of those that hold an unmasked
 // element, or all of them; returns their number, and in `bound` a logit that the row's K-th element
-// reaches.  own: the largest of the thread's shares, m: the row's largest.
-__device__ __forceinline__ int select_groups(Shared& s, int n, int K, const float (&own)[4], float m, float& bound) {
+// reaches, which comes as s.bound.
+__device__ __forceinline__ int select_groups(Shared& s, int n, int K, float m, float& bound) {
   constexpr int W = 7;
   const int tid = threadIdx.x, most = K + max(16, K / 4);
-  const uint32_t top = order_of(m) + 1u;
-  uint32_t lo = ABOVE_MASKED;
-  int c;
-  // The K-th largest of the shares' maxima bounds the row's K-th element from below, and few more
-  // groups than K reach it where K is at most half of the shares: in rows of no special order, 68 groups
-  // the 64th of 512, 710 the 512th of 1024.
-  {
-    const float a = fmaxf(own[0], own[1]), b = fmaxf(own[2], own[3]), ab = fmaxf(a, b);
-    auto count = [&](const float(&at)[W], int(&got)[W]) {
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        if (K <= NT / 2)
-          got[w] = __popcll(__ballot(ab >= at[w]));
-        else if (K <= NT)
-          got[w] = __popcll(__ballot(a >= at[w])) + __popcll(__ballot(b >= at[w]));
-        else
-          got[w] = __popcll(__ballot(own[0] >= at[w])) + __popcll(__ballot(own[1] >= at[w])) +
-                   __popcll(__ballot(own[2] >= at[w])) + __popcll(__ballot(own[3] >= at[w]));
-      }
-    };
-    // (a share that met nothing but masked tokens is none; the others begin at the smallest of them)
-    const float least_own = fminf(fminf(own[0] > -INFINITY ? own[0] : INFINITY, own[1] > -INFINITY ? own[1] : INFINITY),
-                                  fminf(own[2] > -INFINITY ? own[2] : INFINITY, own[3] > -INFINITY ? own[3] : INFINITY));
-    const uint32_t first = max(order_of(-rows::block_max(-least_own, s.red)), ABOVE_MASKED);
-    const float at[W] = {logit_of(first), INFINITY, INFINITY, INFINITY, INFINITY, INFINITY, INFINITY};
-    int got[W];
-    count(at, got);
-    join_counts(got, s.counts[0]);
-    c = got[0];
-    __syncthreads();
-    if (c >= K) {
-      uint32_t hi = top;
-      lo = first;
-      search(lo, hi, c, K, most, s.counts, count);
-    }
-  }
-  bound = logit_of(lo);
-  c = list_groups(s, n, bound);
-  if (c <= min(2 * most, LIST)) return c;
+  bound = s.bound;
+  int c = list_groups(s, n, bound);
+  if (c <= (bound > logit_of(ABOVE_MASKED) ? min(2 * most, LIST) : most)) return c;
 
   // too many: the bound is searched among the groups' maxima, and what is left at the end are ties
-  uint32_t hi = top;
-  search(lo, hi, c, K, most, s.counts, [&](const float(&at)[W], int(&got)[W]) {
+  uint32_t lo = order_of(bound), hi = order_of(m) + 1u;
+  int turn = 0;
+  search<W>(lo, hi, c, K, most, [&](const float(&at)[W], int(&got)[W]) {
 #pragma unroll
     for (int w = 0; w < W; ++w) got[w] = 0;
     for (int j = 0; j < n; j += NT) {
@@ -338,10 +368,15 @@ __device__ __forceinline__ int select_groups(Shared& s, int n, int K, const floa
 #pragma unroll
       for (int w = 0; w < W; ++w) got[w] += __popcll(__ballot(v >= at[w]));
     }
+    join_counts(got, s.counts[turn]);
+    turn ^= 1;
   });
   bound = logit_of(lo);
   // those above `lo` in any order, and at most as many at `lo` as are wanted, from the lowest index
   const bool all = c <= most;
+  __syncthreads();
+  if (tid == 0) s.listed = 0;
+  __syncthreads();
   int taken = min(list_groups(s, n, all ? bound : logit_of(hi)), LIST);
   if (!all) {
     const int wave = tid >> 6, lane = tid & 63;
@@ -368,13 +403,11 @@ __device__ __forceinline__ int select_groups(Shared& s, int n, int K, const floa
 // s.buf = the first K elements of x[0, len) in order (or as many as are not masked); returns their
 // number.  `first`: the index of x[0] in its row.
 template <typename T>
-__device__ __forceinline__ int top_of(Shared& s, const T* x, int len, int first, int K, const float (&own)[4], float m) {
+__device__ __forceinline__ int top_of(Shared& s, const T* x, int len, int first, int K, float m) {
   constexpr int VEC = Elem<T>::VEC, LANES = GROUP / VEC, AT_ONCE = BATCH / GROUP;
   float bound;
   const int n_groups = (len + GROUP - 1) / GROUP;
-  const int groups = select_groups(s, n_groups, K, own, m, bound);
-  if (threadIdx.x == 0) s.n = 0;
-  __syncthreads();
+  const int groups = select_groups(s, n_groups, K, m, bound);
   // (a lane takes 16 bytes of a group; `to` is where its elements that reach the bound go)
   const int lane = (int)threadIdx.x % LANES;
   const auto element_key = [&](float v, int at, int j) { return key_of(v, (uint32_t)(first + at * VEC + j)); };
@@ -493,7 +526,21 @@ __global__ __launch_bounds__(NT, 8) void scores_kernel(Params p) {
     return true;
   };
   float own[4];
-  const State st = rows::scan<T, ONCE, TOP, false>(x + begin, len, p.sc, before, s.group_max, nullptr, s.red, own);
+  const auto met = [&](const float(&o)[4]) {
+    if constexpr (TOP) {
+      met_shares(s, o, p.K);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) own[u] = o[u];
+    }
+  };
+  const auto found = [&](float m) {
+    if constexpr (TOP)
+      if (p.K <= ALONE) search_alone(s, p.K, m);
+  };
+  const State st =
+      rows::scan<T, ONCE, TOP, false>(x + begin, len, p.sc, s.group_max, nullptr, s.red, before, met, found);
+  if constexpr (TOP)
+    if (p.K > ALONE) search_shares(s, own, p.K, st.m);
   if (threadIdx.x == 0) {  // (registers that would be kept over the selection)
     s.state = st;
     s.target = target;
@@ -501,7 +548,7 @@ __global__ __launch_bounds__(NT, 8) void scores_kernel(Params p) {
   }
   int n = 0;
   if constexpr (TOP)
-    n = top_of(s, x + begin, len, begin, p.K, own, st.m);
+    n = top_of(s, x + begin, len, begin, p.K, st.m);
   else
     __syncthreads();
   if (p.slices == 1) {
