@@ -15,7 +15,7 @@ import torch
 from . import _lib
 from ._check import any_set
 from .logprob import first_order
-from .scores import fill_rows, grad_vector, refuse_capture, rows_of_logits
+from .scores import launch, refuse_capture, row_fields, rows_of_logits, vector
 
 _TAILS = {"renormalize": _lib.TAIL_RENORMALIZE, "rest": _lib.TAIL_REST}
 
@@ -25,39 +25,26 @@ def _forward(logits, ids, lq, temperature, tail, want_stats):
     loss = torch.empty(rows, dtype=torch.float32, device=dev)
     status = torch.empty(rows, dtype=torch.int32, device=dev)
     stats = torch.empty(rows, 6, dtype=torch.float64, device=dev) if want_stats else None
-    if rows == 0:
-        return loss, status, stats
-    d = _lib.DistillDesc()
-    fill_rows(d, logits, temperature)
-    d.teacher_ids, d.teacher_logprob, d.top_k, d.tail = ids.data_ptr(), lq.data_ptr(), ids.shape[1], tail
-    d.out_loss, d.out_status = loss.data_ptr(), status.data_ptr()
-    d.out_stats = None if stats is None else stats.data_ptr()
-    lib = _lib.load()
-    size = lib.dsv41_distill_workspace_bytes(ctypes.byref(d))
-    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    with torch.cuda.device(dev):
-        rc = lib.dsv41_distill_run(ctypes.byref(d), None if ws is None else ws.data_ptr(), size,
-                                   torch.cuda.current_stream(dev).cuda_stream)
-    _lib.check(rc)
+    if rows:
+        d = _lib.DistillDesc(*row_fields(_lib.DistillDesc, logits), ids.data_ptr(), lq.data_ptr(), temperature, ids.shape[1],
+                             tail, loss.data_ptr(), status.data_ptr(), None if stats is None else stats.data_ptr())
+        lib = _lib.load()
+        ref = ctypes.byref(d)
+        size = lib.dsv41_distill_workspace_bytes(ref)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+        launch(lib.dsv41_distill_run, dev, ref, None if ws is None else ws.data_ptr(), size)
     return loss, status, stats
 
 
 def distillation_backward(logits, ids, lq, temperature, stats, g_loss):
     """dL/dlogits of :func:`distillation_loss`, in the logits' dtype."""
     rows, vocab = logits.shape
-    dev = logits.device
-    out = torch.empty(rows, vocab, dtype=logits.dtype, device=dev)
-    if rows == 0:
-        return out
-    g_loss = grad_vector(g_loss, (rows,), dev)
-    d = _lib.DistillGradDesc()
-    fill_rows(d, logits, temperature)
-    d.teacher_ids, d.teacher_logprob, d.top_k = ids.data_ptr(), lq.data_ptr(), ids.shape[1]
-    d.stats, d.grad_loss, d.out = stats.data_ptr(), g_loss.data_ptr(), out.data_ptr()
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        rc = lib.dsv41_distill_grad_run(ctypes.byref(d), torch.cuda.current_stream(dev).cuda_stream)
-    _lib.check(rc)
+    out = torch.empty(rows, vocab, dtype=logits.dtype, device=logits.device)
+    if rows:
+        g_loss = vector(g_loss, torch.float32, (rows,), logits.device)
+        d = _lib.DistillGradDesc(*row_fields(_lib.DistillGradDesc, logits), ids.data_ptr(), lq.data_ptr(), temperature,
+                                 ids.shape[1], stats.data_ptr(), g_loss.data_ptr(), out.data_ptr())
+        launch(_lib.load().dsv41_distill_grad_run, logits.device, ctypes.byref(d))
     return out
 
 
@@ -133,8 +120,8 @@ def distillation_loss(
         raise ValueError("one teacher log probability is required per teacher ID")
     if teacher_ids.is_floating_point() or teacher_ids.dtype == torch.bool:
         raise ValueError("teacher_ids must be integers")
-    ids = teacher_ids.to(device=logits.device, dtype=torch.int64).contiguous()
-    lq = teacher_log_probs.detach().to(device=logits.device, dtype=torch.float32).contiguous()
+    ids = vector(teacher_ids, torch.int64, teacher_ids.shape, logits.device)
+    lq = vector(teacher_log_probs.detach(), torch.float32, teacher_ids.shape, logits.device)
     if ids.shape[1] == 0:  # no row has an entry
         ids, lq = ids.new_full((rows, 1), -1), lq.new_zeros(rows, 1)
     refuse_capture(check)

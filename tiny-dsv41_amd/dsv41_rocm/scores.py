@@ -57,49 +57,59 @@ def refuse_capture(check: bool) -> None:
         raise RuntimeError("a checked call waits for its answer and cannot be captured: pass check=False")
 
 
-def fill_rows(d, logits, temperature) -> None:
-    """The fields that every descriptor over rows of logits has."""
-    d.struct_size = ctypes.sizeof(type(d))
-    d.rows, d.vocab = logits.shape
-    d.logits_dtype = _lib.DTYPE_F32 if logits.dtype == torch.float32 else _lib.DTYPE_BF16
-    d.logits_row_stride = logits.stride(0) if logits.shape[0] > 1 else logits.shape[1]
-    d.logits = logits.data_ptr()
-    d.temperature = temperature
+def row_fields(cls, logits) -> tuple:
+    """The fields that every descriptor over rows of logits begins with."""
+    rows, vocab = logits.shape
+    return (ctypes.sizeof(cls), rows, vocab, _lib.DTYPE_F32 if logits.dtype == torch.float32 else _lib.DTYPE_BF16,
+            logits.stride(0) if rows > 1 else vocab, logits.data_ptr())
 
 
-def grad_vector(g, shape, device):
-    """An upstream gradient in kernel form, or None."""
-    return None if g is None else g.to(device=device, dtype=torch.float32).expand(shape).contiguous()
+def launch(call, device, *args) -> None:
+    """``call(*args, stream)`` on the device's current stream, with its error raised."""
+    if torch.cuda.current_device() == device.index:
+        rc = call(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = call(*args, torch.cuda.current_stream(device).cuda_stream)
+    _lib.check(rc)
+
+
+def vector(t, dtype, shape, device):
+    """A contiguous tensor of that dtype and shape on the device, ``t`` itself where it is one."""
+    if t.dtype != dtype or t.device != device:
+        t = t.to(device=device, dtype=dtype)
+    if t.shape != shape:
+        t = t.expand(shape)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
 
 
 def _forward(logits, targets, top_k, temperature, want_stats):
     rows, dev = logits.shape[0], logits.device
     f32, i64 = torch.float32, torch.int64
-    lp = torch.empty(rows if targets is not None else 0, dtype=f32, device=dev)
-    rank = torch.empty(rows if targets is not None else 0, dtype=i64, device=dev)
+    lp = rank = stats = ws = None
+    if targets is not None:
+        lp = torch.empty(rows, dtype=f32, device=dev)
+        rank = torch.empty(rows, dtype=i64, device=dev)
     entropy = torch.empty(rows, dtype=f32, device=dev)
     top_ids = torch.empty(rows, top_k, dtype=i64, device=dev)
     top_lp = torch.empty(rows, top_k, dtype=f32, device=dev)
     status = torch.empty(rows, dtype=torch.int32, device=dev)
-    stats = torch.empty(rows, 4, dtype=torch.float64, device=dev) if want_stats else None
-    if rows == 0:
-        return lp, rank, entropy, top_ids, top_lp, status, stats
-    d = _lib.ScoresDesc()
-    fill_rows(d, logits, temperature)
-    d.top_k = top_k
-    if targets is not None:
-        d.targets, d.out_logprob, d.out_rank = targets.data_ptr(), lp.data_ptr(), rank.data_ptr()
-    d.out_entropy, d.out_status = entropy.data_ptr(), status.data_ptr()
-    if top_k:
-        d.out_top_ids, d.out_top_logprob = top_ids.data_ptr(), top_lp.data_ptr()
-    d.out_stats = None if stats is None else stats.data_ptr()
-    lib = _lib.load()
-    size = lib.dsv41_scores_workspace_bytes(ctypes.byref(d))
-    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    with torch.cuda.device(dev):
-        rc = lib.dsv41_scores_run(ctypes.byref(d), None if ws is None else ws.data_ptr(), size,
-                                  torch.cuda.current_stream(dev).cuda_stream)
-    _lib.check(rc)
+    if want_stats:
+        stats = torch.empty(rows, 4, dtype=torch.float64, device=dev)
+    if rows:
+        d = _lib.ScoresDesc(*row_fields(_lib.ScoresDesc, logits), _ptr(targets), temperature, top_k, _ptr(lp), _ptr(rank),
+                            entropy.data_ptr(), top_ids.data_ptr() if top_k else None, top_lp.data_ptr() if top_k else None,
+                            status.data_ptr(), _ptr(stats))
+        lib = _lib.load()
+        ref = ctypes.byref(d)
+        size = lib.dsv41_scores_workspace_bytes(ref)
+        if size:
+            ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        launch(lib.dsv41_scores_run, dev, ref, _ptr(ws), size)
     return lp, rank, entropy, top_ids, top_lp, status, stats
 
 
@@ -110,24 +120,14 @@ def scores_backward(logits, targets, top_ids, temperature, stats, g_log_probs, g
     out = torch.empty(rows, vocab, dtype=logits.dtype, device=dev)
     if rows == 0:
         return out
-    g_log_probs = grad_vector(g_log_probs if targets is not None else None, (rows,), dev)
-    g_entropy = grad_vector(g_entropy, (rows,), dev)
-    g_top = grad_vector(g_top, top_ids.shape, dev) if top_ids.shape[1] else None
-    d = _lib.ScoresGradDesc()
-    fill_rows(d, logits, temperature)
-    if targets is not None:
-        d.targets = targets.data_ptr()
-    d.stats, d.out = stats.data_ptr(), out.data_ptr()
-    if g_log_probs is not None:
-        d.grad_logprob = g_log_probs.data_ptr()
-    if g_entropy is not None:
-        d.grad_entropy = g_entropy.data_ptr()
-    if g_top is not None:
-        d.top_k, d.top_ids, d.grad_top = top_ids.shape[1], top_ids.data_ptr(), g_top.data_ptr()
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        rc = lib.dsv41_scores_grad_run(ctypes.byref(d), torch.cuda.current_stream(dev).cuda_stream)
-    _lib.check(rc)
+    g_log_probs = None if g_log_probs is None or targets is None else vector(g_log_probs, torch.float32, (rows,), dev)
+    g_entropy = None if g_entropy is None else vector(g_entropy, torch.float32, (rows,), dev)
+    top_k = top_ids.shape[1]
+    g_top = None if g_top is None or not top_k else vector(g_top, torch.float32, top_ids.shape, dev)
+    d = _lib.ScoresGradDesc(*row_fields(_lib.ScoresGradDesc, logits), _ptr(targets), _ptr(top_ids) if top_k else None,
+                            temperature, top_k, stats.data_ptr(), _ptr(g_log_probs), _ptr(g_entropy), _ptr(g_top),
+                            out.data_ptr())
+    launch(_lib.load().dsv41_scores_grad_run, dev, ctypes.byref(d))
     return out
 
 
@@ -137,7 +137,7 @@ class _LogitScores(torch.autograd.Function):
         lp, rank, entropy, top_ids, top_lp, status, stats = _forward(logits, targets, top_k, temperature, True)
         ctx.temperature = temperature
         ctx.save_for_backward(logits, targets, top_ids, stats)
-        ctx.mark_non_differentiable(rank, top_ids, status)
+        ctx.mark_non_differentiable(*(t for t in (rank, top_ids, status) if t is not None))
         ctx.set_materialize_grads(False)
         return lp, rank, entropy, top_ids, top_lp, status
 
@@ -191,9 +191,9 @@ def logit_scores(
     if targets is not None:
         if targets.is_floating_point() or targets.dtype == torch.bool:
             raise ValueError("targets must be integers")
-        targets = targets.to(device=logits.device, dtype=torch.int64).reshape(-1).contiguous()
         if targets.numel() != rows:
             raise ValueError("one target is required per row")
+        targets = vector(targets.reshape(rows), torch.int64, (rows,), logits.device)
     refuse_capture(check)
     if torch.is_grad_enabled() and logits.requires_grad:
         lp, rank, entropy, top_ids, top_lp, status = _LogitScores.apply(logits, targets, top_k, temperature)
@@ -201,6 +201,4 @@ def logit_scores(
         lp, rank, entropy, top_ids, top_lp, status, _ = _forward(logits, targets, top_k, temperature, False)
     if check and any_set(status)[0]:
         _status_error(status)
-    if targets is None:
-        lp = rank = None
     return LogitScores(lp, rank, entropy, top_ids, top_lp)
