@@ -427,3 +427,32 @@ def test_agrees_with_the_sampler():
     assert torch.equal(s.top_ids[:, 0], r.ids) and bool((s.ranks == 1).all())
     assert float((s.log_probs - r.logprobs).abs().max()) <= 1e-4
     assert torch.equal(s.log_probs, s.top_log_probs[:, 0])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,V,k", [(2, 3000, 700), (1, 6000, 1024), (600, 5000, 600), (2, 9000, 513), (1, 40000, 1024)])
+def test_many_alternatives_of_few_tokens(rows, V, k, dtype):
+    # more alternatives than groups of 32 tokens, or not far from it; and values that crowd together
+    logits, t = make(rows, V, dtype, V + k, scale=1.0)
+    check(logits, t, k, 1.0)
+    g = torch.Generator().manual_seed(k)
+    near = (5 + 0.01 * torch.rand(rows, V, generator=g)).to(dtype).to(DEV)
+    near[0, V // 2] = 900.0
+    check(near, t, k, 1.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("k", [5, 64, 400])
+def test_top_tokens_that_lie_together(dtype, k):
+    # all of one thread's share, all of one slice, all of one group, every 512th chunk
+    V = 65536
+    g = torch.Generator().manual_seed(k)
+    x = torch.randn(4, V, generator=g)
+    x[0, torch.arange(0, V, 4096)] += 50
+    x[1, 30000:31000] += 50
+    x[2, 64:96] += 50
+    vec = 4 if dtype == torch.float32 else 8
+    x[3, (torch.arange(V) // vec) % 512 == 7] += 50
+    t = torch.tensor([4096, 30500, 70, 7 * vec], device=DEV)
+    check(x.to(dtype).to(DEV), t, k, 1.0)
+    check(x.to(dtype).to(DEV).repeat(150, 1), t.repeat(150), k, 1.0)

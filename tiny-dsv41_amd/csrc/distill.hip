@@ -268,10 +268,12 @@ void launch(const Params& p, hipStream_t s) {
   if (p.slices > 1) hipLaunchKernelGGL(distill_join_kernel<T>, dim3(p.rows), dim3(NT), 0, s, p);
 }
 
+// As the scores' (GPU time of a call in a graph, rest of a 64-token list, bf16: 48 rows of 151851 16.7 us
+// with 512 workgroups, 20.5 with 1024; 600 rows of 151936 49.3 and 52.0).
 Cut cut_of(int rows, int V) {
-  int64_t want = (1024 + rows - 1) / rows;
+  int64_t want = (512 + rows - 1) / rows;
   if (want > 64) want = 64;
-  if (want > V / 4096) want = V / 4096;
+  if (want > V / 6144) want = V / 6144;
   if (want < 1) want = 1;
   int len = (int)(((V + want - 1) / want + GROUP - 1) / GROUP * GROUP);
   if (len > MAX_LEN) len = MAX_LEN;

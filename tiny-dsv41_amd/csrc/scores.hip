@@ -408,42 +408,76 @@ __device__ __forceinline__ int top_of(Shared& s, const T* x, int len, int first,
   float bound;
   const int n_groups = (len + GROUP - 1) / GROUP;
   const int groups = select_groups(s, n_groups, K, m, bound);
-  // (a lane takes 16 bytes of a group; `to` is where its elements that reach the bound go)
+  // calls f(w, at) for the 16 bytes w at chunk `at` of each listed group, or masked ones; every thread of a
+  // wave as often as the others
   const int lane = (int)threadIdx.x % LANES;
-  const auto element_key = [&](float v, int at, int j) { return key_of(v, (uint32_t)(first + at * VEC + j)); };
-  constexpr int AHEAD = 4;  // loads in flight at once
-  for (int b = (int)threadIdx.x / LANES; b < groups; b += AHEAD * (NT / LANES)) {
-    uint32_t w[AHEAD][4];
-    int at[AHEAD];
+  const auto each_chunk = [&](auto&& f) {
+    constexpr int AHEAD = 4;  // loads in flight at once
+    for (int b = 0; b < groups; b += AHEAD * (NT / LANES)) {
+      uint32_t w[AHEAD][4];
+      int at[AHEAD];
 #pragma unroll
-    for (int a = 0; a < AHEAD; ++a) {
-      const int g = b + a * (NT / LANES);
-      at[a] = g < groups ? (int)s.list[g] * LANES + lane : -1;
-      rows::load_some<false>(x, len, at[a], w[a]);
+      for (int a = 0; a < AHEAD; ++a) {
+        const int g = b + a * (NT / LANES) + (int)threadIdx.x / LANES;
+        at[a] = g < groups ? (int)s.list[g] * LANES + lane : -1;
+        rows::load_some<false>(x, len, at[a], w[a]);
+      }
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) f(w[a], at[a]);
     }
-#pragma unroll
-    for (int a = 0; a < AHEAD; ++a) {
+  };
+  const auto element_key = [&](float v, int at, int j) { return key_of(v, (uint32_t)(first + at * VEC + j)); };
+  const auto gather = [&](float from) {
+    each_chunk([&](const uint32_t(&w)[4], int at) {
       float v[VEC];
-      Elem<T>::unpack(w[a], v);
+      Elem<T>::unpack(w, v);
       uint32_t pass = 0;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) pass |= (uint32_t)(v[j] >= bound) << j;
+      for (int j = 0; j < VEC; ++j) pass |= (uint32_t)(v[j] >= from) << j;
       if (pass) {
         int to = atomicAdd(&s.n, __popc(pass));
 #pragma unroll
         for (int j = 0; j < VEC; ++j)
           if (pass >> j & 1) {
-            if (to < BUF) s.buf[to] = element_key(v[j], at[a], j);
+            if (to < BUF) s.buf[to] = element_key(v[j], at, j);
             ++to;
           }
       }
-    }
-  }
-  __syncthreads();
-  int n = s.n;
-  __syncthreads();
+    });
+    __syncthreads();
+    const int n = s.n;
+    __syncthreads();
+    return n;
+  };
+  int n = gather(bound);
   if (n > BUF) {
-    // the groups hold more elements that reach the bound than the buffer: a batch at a time
+    // few groups for many alternatives: the bound is searched among their elements
+    constexpr int W = 7;
+    uint32_t lo = order_of(bound), hi = order_of(m) + 1u;
+    int turn = 0;
+    search<W>(lo, hi, n, K, BUF, [&](const float(&at)[W], int(&got)[W]) {
+#pragma unroll
+      for (int q = 0; q < W; ++q) got[q] = 0;
+      each_chunk([&](const uint32_t(&w)[4], int) {
+        float v[VEC];
+        Elem<T>::unpack(w, v);
+#pragma unroll
+        for (int q = 0; q < W; ++q)
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) got[q] += __popcll(__ballot(v[j] >= at[q]));
+      });
+      join_counts(got, s.counts[turn]);
+      turn ^= 1;
+    });
+    bound = logit_of(lo);
+    __syncthreads();
+    if (threadIdx.x == 0) s.n = 0;
+    __syncthreads();
+    n = gather(bound);
+  }
+  if (n > BUF) {
+    // ties
+    // more ties at the bound than the buffer holds: a batch at a time
     if (threadIdx.x == 0) s.n = 0;
     __syncthreads();
     uint64_t floor_key = 0;
@@ -565,12 +599,15 @@ template <typename T>
 __global__ __launch_bounds__(NT) void scores_join_kernel(Params p) {
   __shared__ Shared s;
   const int row = blockIdx.x, tid = threadIdx.x;
+  // the lists' first keys before their second ones and so on, so that what is left below the bound need
+  // not be read
   const uint64_t* keys = p.keys + (int64_t)row * p.slices * p.K;
   const int total = p.slices * p.K;
+  const auto key_at = [&](int i) { return i < total ? keys[(int64_t)(i % p.slices) * p.K + i / p.slices] : 0; };
   constexpr int EACH = BATCH / NT;
   uint64_t key[EACH];
 #pragma unroll
-  for (int e = 0; e < EACH; ++e) key[e] = e * NT + tid < total ? keys[e * NT + tid] : 0;
+  for (int e = 0; e < EACH; ++e) key[e] = key_at(e * NT + tid);
   int64_t target = -1;
   float xt = INFINITY;
   if (p.targets) {
@@ -579,12 +616,15 @@ __global__ __launch_bounds__(NT) void scores_join_kernel(Params p) {
   }
   if (tid < 64) {
     State st{0.0, 0.0, -INFINITY, 0};
-    uint64_t least = 1;
+    // Two bounds of the row's K-th key.  Each list holds K keys that come no later than its last; and
+    // all hold ceil(K / slices) that come no later than the last of these.
+    uint64_t last = 1, share = ~0ull;
     if (tid < p.slices) {
       st = p.states[(int64_t)row * p.slices + tid];
-      // each list holds K elements that come no later than its last, so the row's K-th comes no later
-      // than any of these lasts
-      if (p.K) least = max(least, keys[(int64_t)tid * p.K + p.K - 1]);
+      if (p.K) {
+        last = max(last, keys[(int64_t)tid * p.K + p.K - 1]);
+        share = keys[(int64_t)tid * p.K + (p.K + p.slices - 1) / p.slices - 1];
+      }
     }
     const float m = wave_max_dpp(st.m);
     if (st.S == 0.0)
@@ -594,12 +634,15 @@ __global__ __launch_bounds__(NT) void scores_join_kernel(Params p) {
     const double S = wave_total_d(st.S), U = wave_total_d(st.U);
     const int before = wave_sum_i(st.before);
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) least = max(least, (uint64_t)__shfl_xor((unsigned long long)least, o));
+    for (int o = 32; o > 0; o >>= 1) {
+      last = max(last, (uint64_t)__shfl_xor((unsigned long long)last, o));
+      share = min(share, (uint64_t)__shfl_xor((unsigned long long)share, o));
+    }
     if (tid == 0) {
       s.state = State{S, U, m, before};
       s.target = target;
       s.xt = xt;
-      s.least = least;
+      s.least = max(last, share);
       s.n = 0;
     }
   }
@@ -612,12 +655,16 @@ __global__ __launch_bounds__(NT) void scores_join_kernel(Params p) {
       if (b) {
         make_room(s, p.K, floor_key);
 #pragma unroll
-        for (int e = 0; e < EACH; ++e) key[e] = b + e * NT + tid < total ? keys[b + e * NT + tid] : 0;
+        for (int e = 0; e < EACH; ++e) key[e] = key_at(b + e * NT + tid);
       }
+      bool any = false;
 #pragma unroll
       for (int e = 0; e < EACH; ++e)
-        if (key[e] >= least && key[e] > floor_key) push(s, key[e]);
-      __syncthreads();
+        if (key[e] >= least && key[e] > floor_key) {
+          push(s, key[e]);
+          any = true;
+        }
+      if (!__syncthreads_or(any)) break;
     }
     n = s.n;
     sort_desc(s, n, logit_of((uint32_t)(least >> 32)), s.state.m);
@@ -703,11 +750,14 @@ __global__ __launch_bounds__(NT) void scores_grad_kernel(GradParams p) {
 }
 
 // ---------------------------------------------------------------------------------------- host
-// Rows are cut where there are too few of them to occupy the GPU: into slices of at least 4096
-// elements, whose lists are at most an eighth of them, until there are 1024 workgroups.
-Cut cut_of(int rows, int V, int K) {
-  const int least = K * 8 > 4096 ? K * 8 : 4096;
-  int64_t want = (1024 + rows - 1) / rows;
+// Rows are cut where there are too few of them to occupy the GPU: into slices of at least 6144 elements
+// until there are 512 workgroups.  (Measured, GPU time of a call in a graph, fp32: 48 rows of 151851, top 20,
+// 22.0 us with 512, 24.4 with 1024, 21.4 with 256; 331 rows of 129280, top 64, 48.9, 51.9 and 46.4; one
+// row of 129280 without alternatives 7.4 in slices of 6144, 7.3 of 4096, 7.8 of 8192.)  More than 256
+// alternatives take slices whose threads meet four chunks each, whose maxima bound them.
+Cut cut_of(int rows, int V, int K, int esize) {
+  const int least = K > ALONE ? 4 * NT * (16 / esize) : 6144;
+  int64_t want = (512 + rows - 1) / rows;
   if (want > 64) want = 64;
   if (want > V / least) want = V / least;
   if (want < 1) want = 1;
@@ -750,7 +800,7 @@ int check_desc(const dsv41_scores_desc* d) {
     return fail(DSV41_E_INVALID, "targets need out_logprob and out_rank");
   if (d->top_k && (!d->out_top_ids || !d->out_top_logprob))
     return fail(DSV41_E_INVALID, "top_k needs out_top_ids and out_top_logprob");
-  return rows::check_grid(d->rows, cut_of(d->rows, d->vocab, d->top_k));
+  return rows::check_grid(d->rows, cut_of(d->rows, d->vocab, d->top_k, d->logits_dtype == DSV41_DTYPE_F32 ? 4 : 2));
 }
 
 }  // namespace scores
@@ -760,12 +810,12 @@ using namespace dsv41;
 
 extern "C" size_t dsv41_scores_workspace_bytes(const dsv41_scores_desc* d) {
   if (scores::check_desc(d)) return 0;
-  return scores::workspace_of(d->rows, d->top_k, scores::cut_of(d->rows, d->vocab, d->top_k));
+  return scores::workspace_of(d->rows, d->top_k, scores::cut_of(d->rows, d->vocab, d->top_k, d->logits_dtype == DSV41_DTYPE_F32 ? 4 : 2));
 }
 
 extern "C" int dsv41_scores_run(const dsv41_scores_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = scores::check_desc(d)) return rc;
-  const rows::Cut c = scores::cut_of(d->rows, d->vocab, d->top_k);
+  const rows::Cut c = scores::cut_of(d->rows, d->vocab, d->top_k, d->logits_dtype == DSV41_DTYPE_F32 ? 4 : 2);
   const size_t need = scores::workspace_of(d->rows, d->top_k, c);
   if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 8))
     return fail(DSV41_E_WORKSPACE, "scores workspace is missing, too small or not 8-byte aligned");
