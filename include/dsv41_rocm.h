@@ -545,7 +545,7 @@ typedef struct dsv41_scores_grad_desc {
  *   DSV41_TAIL_REST: q_k = exp(teacher_logprob), q_rest = 1 - sum q_k (below 2^-20: 0) and p_rest the
  *     student's mass outside the list; out_loss[r] = sum_k q_k (log q_k - log p_k)
  *     + q_rest (log q_rest - log p_rest).
- * A row with an empty list: 0, and the logits are not read.  An id at or above vocab, a token named
+ * A row with an empty list: 0, whatever its logits.  An id at or above vocab, a token named
  * twice, teacher log-probs that are none: NaN and a status bit (BAD_TARGET, REPEATED, BAD_TEACHER).
  * A loss that is not finite: DSV41_STATUS_NONFINITE.
  */
@@ -563,7 +563,7 @@ typedef struct dsv41_distill_desc {
   int32_t tail;              /* DSV41_TAIL_* */
   float* out_loss;           /* [rows] */
   int32_t* out_status;       /* [rows] */
-  double* out_stats;         /* [rows, 6] or NULL: what dsv41_distill_grad_run needs */
+  double* out_stats;         /* [rows, 7] or NULL: what dsv41_distill_grad_run needs */
 } dsv41_distill_desc;
 
 /*

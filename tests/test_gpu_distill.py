@@ -139,6 +139,25 @@ def test_student_far_more_certain_than_its_rest():
     assert float(loss.min()) > 0
 
 
+@pytest.mark.parametrize("tail", ["renormalize", "rest"])
+def test_rest_far_below_the_list(tail):
+    # 200 and 600 nats below: p_rest is no fp32 number, but the loss and the gradient are
+    V, k = 3000, 6
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(3, V, generator=g)
+    x[0, :k] += 200.0
+    x[1, :k] += 600.0
+    x[2, :k] += 95.0
+    lq = torch.log_softmax(torch.randn(3, k, generator=g), 1) + math.log(0.9)
+    ids = torch.arange(k).expand(3, k)
+    loss, grad = compare(x.to(DEV), ids.to(DEV), lq.to(DEV), 1.0, tail, g=torch.tensor([1.0, 1.0, 2.0 ** 16]))
+    if tail == "rest":
+        assert abs(float(grad[0, k:].sum()) + 0.1) < 1e-5 and abs(float(grad[1, k:].sum()) + 0.1) < 1e-5
+    else:
+        # e^-95 is below 2^-126, and 2^16 times that is above it
+        assert float(grad[2, k:].min()) > 0.0
+
+
 def test_confident_teacher_has_no_rest():
     # log-probs whose mass rounds to 1 (or to just above it): the rest is none, the loss finite
     V, k = 300, 5
@@ -212,6 +231,8 @@ def test_refused_rows(rows):
 
     case("outside the model vocabulary", i=(3, V))
     case("outside the model vocabulary", i=(0, 1 << 40))
+    loss, grad = case("non-finite", x=([i for i in range(V) if i not in ids[2].tolist()], torch.finfo(torch.float32).min))
+    assert float(loss) == math.inf and bool(grad.isfinite().all())
     for tail in ("rest", "renormalize"):
         case("names a token twice", tail, i=(3, ids[2, 1].item()))
         case("do not form", tail, l=(2, math.nan))

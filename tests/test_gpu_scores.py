@@ -324,6 +324,18 @@ def test_gradient_of_masked_tokens_and_missing_alternatives():
     assert float(got[0, 3:].abs().max()) == 0.0 and float(got[1, ::3].abs().max()) == 0.0
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradient_of_probabilities_below_the_smallest_normal_number(dtype):
+    V = 2048
+    x = torch.full((1, V), -92.0)
+    x[0, 5] = 0.0
+    leaf = x.to(dtype).to(DEV).requires_grad_()
+    s = logit_scores(leaf, torch.tensor([5], device=DEV))
+    (got,) = torch.autograd.grad(s.log_probs, leaf, torch.tensor([2.0 ** 20], device=DEV))
+    want = -math.exp(float(leaf[0, 7].detach())) * 2.0 ** 20  # (the other tokens change S by less than 1e-36)
+    assert 0 < -want < 2.0 ** -104 and abs(float(got[0, 7]) / want - 1) <= 2.0 ** -8
+
+
 def test_gradient_against_differences():
     # the plain gradient itself, by central differences in 64 bits
     V, k, T = 50, 6, 0.9

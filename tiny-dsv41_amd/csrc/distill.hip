@@ -33,7 +33,7 @@ using rows::WAVES;
 constexpr int MAX_LEN = 5120 * 32;  // elements of one slice: 20 KB of bits
 constexpr double REST_FLOOR = 0x1p-20;
 constexpr double MOST_MASS = 1.01;  // log-probs rounded to bf16 may add up to 1 + 2^-8 |lq| or so
-constexpr int STATS = 6;            // per row: m, S, others' factor, Q, log normalizer of the list, live
+constexpr int STATS = 7;            // per row, see write_row
 
 struct SliceState {
   State s;
@@ -60,20 +60,18 @@ struct Shared {
 };
 constexpr int LIVE = 1 << 16;  // the list has an entry (above the status bits)
 
-__device__ void write_row(const Params& p, int row, float loss, int status, double m, double S, double others, double Q,
-                          double log_z, bool live) {
+// What the gradient needs of a row: p_k = exp((x_k - m) / T) / S in its list; p_i (Q - q_rest / p_rest) =
+// others exp((x_i - base) / T) outside, with the largest of these logits as base, since p_rest may lie
+// below what fp32 holds; Q; q_k = exp(lq_k - log_z); whether there is anything to do.
+struct Stats {
+  double m, S, base, others, Q, log_z, live;
+};
+static_assert(sizeof(Stats) == STATS * sizeof(double), "the layout of out_stats");
+__device__ __forceinline__ void write_row(const Params& p, int row, float loss, int status, const Stats& st) {
   if (threadIdx.x) return;
   p.out_loss[row] = loss;
   p.out_status[row] = status;
-  if (p.out_stats) {
-    double* o = p.out_stats + (int64_t)row * STATS;
-    o[0] = m;
-    o[1] = S;
-    o[2] = others;
-    o[3] = Q;
-    o[4] = log_z;
-    o[5] = live ? 1.0 : 0.0;
-  }
+  if (p.out_stats) reinterpret_cast<Stats*>(p.out_stats)[row] = st;
 }
 
 // A thread's first entry of a list: read ahead of the pass over the row, whose loads hide its own.
@@ -96,11 +94,11 @@ __device__ __forceinline__ Entry entry_of(const Params& p, int row, int k) {
 template <typename T>
 __device__ __forceinline__ void finish(const Params& p, int row, State st, int flags, const Entry& mine, double* red) {
   if (!(flags & LIVE)) {
-    write_row(p, row, 0.f, 0, 0.0, 1.0, 0.0, 0.0, 0.0, false);
+    write_row(p, row, 0.f, 0, Stats{0.0, 1.0, 0.0, 0.0, 0.0, 0.0, 0.0});
     return;
   }
   if (flags != LIVE) {
-    write_row(p, row, NAN, flags & ~LIVE, NAN, NAN, NAN, NAN, 0.0, true);
+    write_row(p, row, NAN, flags & ~LIVE, Stats{NAN, NAN, NAN, NAN, NAN, 0.0, 1.0});
     return;
   }
   // (a list of more than NT entries is read again here; the first entries stay in registers, and the
@@ -135,27 +133,34 @@ __device__ __forceinline__ void finish(const Params& p, int row, State st, int f
   }
   rows::block_sums(sum, red);
   const double Sn = sum[0], W = sum[1], WL = sum[2], WD = sum[3];
-  if (st.S != 0.0) rows::rebase(st.S, st.U, ((double)st.m - m) * p.sc.cd);
-  const double S_rest = st.S, S = S_rest + Sn, ln_s = log(S);
+  // S_rest against m, by `down` from the sum against its own largest logit
+  const double down = st.S != 0.0 ? exp2(fmax(((double)st.m - m) * p.sc.cd, -2000.0)) : 0.0;
+  const double S_rest = st.S * down, S = S_rest + Sn, ln_s = log(S);
   const bool nonfinite = !(S > 0.0 && S < INFINITY);
   if (bad || (p.rest && W > MOST_MASS)) {
-    write_row(p, row, NAN, DSV41_STATUS_BAD_TEACHER, NAN, NAN, NAN, NAN, 0.0, true);
+    write_row(p, row, NAN, DSV41_STATUS_BAD_TEACHER, Stats{NAN, NAN, NAN, NAN, NAN, 0.0, 1.0});
     return;
   }
-  double loss, others = 1.0, Q = 1.0, log_z = 0.0;
+  double loss, rest = 0.0, Q = 1.0, log_z = 0.0;
   if (p.rest) {
-    double rest = 1.0 - W;
+    rest = 1.0 - W;
     if (rest < REST_FLOOR) rest = 0.0;
-    loss = WL - WD + W * ln_s + (rest > 0.0 ? rest * (log(rest) - log(S_rest) + ln_s) : 0.0);
+    // (the sum against its own largest logit, whose distance from m counts in full; a mass that fp64
+    // does not hold is none)
+    const double log_rest = S_rest > 0.0 ? log(st.S) + ((double)st.m - m) * p.sc.inv_t - ln_s : -(double)INFINITY;
+    loss = WL - WD + W * ln_s + (rest > 0.0 ? rest * (log(rest) - log_rest) : 0.0);
     Q = W + rest;
-    others = S_rest > 0.0 ? Q - rest * S / S_rest : Q;
   } else {
     log_z = top + log(W);
     loss = (WL - WD) / W - log(W) + ln_s;
   }
   const float l = nonfinite ? NAN : (float)loss;
-  write_row(p, row, l, nonfinite || !isfinite(l) ? DSV41_STATUS_NONFINITE : 0, m, nonfinite ? (double)NAN : S, others, Q,
-            log_z, true);
+  Stats out{m, nonfinite ? (double)NAN : S, m, 0.0, Q, log_z, 1.0};
+  if (st.S != 0.0) {
+    out.base = st.m;
+    out.others = Q * down / S - (rest > 0.0 ? rest / st.S : 0.0);
+  }
+  write_row(p, row, l, nonfinite || !isfinite(l) ? DSV41_STATUS_NONFINITE : 0, out);
 }
 
 template <typename T, bool ONCE>
@@ -237,24 +242,25 @@ __global__ __launch_bounds__(NT) void distill_grad_kernel(GradParams p) {
   const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.stride;
   const int begin = slice * p.len, len = min(p.len, p.V - begin);
   T* out = static_cast<T*>(p.out) + (int64_t)row * p.V + begin;
-  const double* st = p.stats + (int64_t)row * STATS;
+  const Stats st = reinterpret_cast<const Stats*>(p.stats)[row];
   const double g = (double)p.g[row] * p.sc.inv_t;
-  if (g == 0.0 || st[5] == 0.0) {
+  if (g == 0.0 || st.live == 0.0) {
     rows::fill_zero(out, len);
     return;
   }
-  const float m = (float)st[0];
-  const double S = st[1], Q = st[3], log_z = st[4];
-  const float A = (float)(g * st[2] / S);
-  rows::map(x + begin, out, len, [&](float v) { return A * __builtin_amdgcn_exp2f((v - m) * p.sc.c); });
+  const rows::Lift lift(g * st.others);
+  const float base = (float)st.base, A = (float)(g * st.others * lift.down);
+  // (a row whose sums are NaN has NaN for S: its gradient is, too)
+  const float bad = st.S == st.S ? 0.f : NAN;
+  rows::map(x + begin, out, len, [&](float v) { return __builtin_fmaf(A, lift.exp2(v - base, p.sc.c), bad); });
   __syncthreads();
   const int64_t* ids = p.ids + (int64_t)row * p.K;
   const float* lq = p.lq + (int64_t)row * p.K;
   for (int k = threadIdx.x; k < p.K; k += NT) {
     const int64_t i = ids[k] - begin;
     if (ids[k] < 0 || i < 0 || i >= len) continue;
-    const double e = exp(((double)Elem<T>::one(x + begin + i) - m) * p.sc.inv_t);
-    rows::store_one(out + i, (float)(g * (Q * e / S - exp((double)lq[k] - log_z))));
+    const double e = exp(((double)Elem<T>::one(x + begin + i) - st.m) * p.sc.inv_t);
+    rows::store_one(out + i, (float)(g * (st.Q * e / st.S - exp((double)lq[k] - st.log_z))));
   }
 }
 

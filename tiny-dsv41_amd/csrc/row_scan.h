@@ -116,6 +116,17 @@ __device__ __forceinline__ void store_full(bf16_t* out, int i, const float (&v)[
   for (int j = 0; j < 4; ++j) r[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
   *reinterpret_cast<Elem<bf16_t>::Raw*>(out + (int64_t)i * 8) = r;
 }
+// A factor times 2^(d c), d c <= 0.  v_exp_f32 returns zero below 2^-126, where fp32 and bf16 still hold
+// values; a factor that brings such a power back above them gives 2^32 of its size to the exponent.
+struct Lift {
+  float up, down;  // what the exponent takes, and 2^-up
+  __device__ __forceinline__ explicit Lift(double factor) {
+    const bool large = fabs(factor) >= 0x1p-60;
+    up = large ? 32.f : 0.f;
+    down = large ? 0x1p-32f : 1.f;
+  }
+  __device__ __forceinline__ float exp2(float d, float c) const { return __builtin_amdgcn_exp2f(__builtin_fmaf(d, c, up)); }
+};
 template <typename T, class F>
 __device__ __forceinline__ void map(const T* x, T* out, int len, F f) {
   constexpr int VEC = Elem<T>::VEC, U = 4;

@@ -724,11 +724,12 @@ __global__ __launch_bounds__(NT) void scores_grad_kernel(GradParams p) {
   const double* st = p.stats + (int64_t)row * 4;
   const float m = (float)st[0];
   const double S = st[1];
-  const float A = (float)(-(G + g_h * (st[3] - st[2])) * p.sc.inv_t / S);
-  const float B = (float)(-g_h * p.sc.inv_t * p.sc.inv_t / (p.sc.c * S));
+  const double a = -(G + g_h * (st[3] - st[2])) * p.sc.inv_t / S, b = -g_h * p.sc.inv_t * p.sc.inv_t / (p.sc.c * S);
+  const rows::Lift lift(fabs(a) + fabs(b));
+  const float A = (float)(a * lift.down), B = (float)(b * lift.down), c = p.sc.c;
   auto dense = [&](float v) {
-    const float d = (v - m) * p.sc.c;
-    return __builtin_amdgcn_exp2f(d) * __builtin_fmaf(B, fmaxf(d, -1000.f), A);
+    const float d = v - m;
+    return lift.exp2(d, c) * __builtin_fmaf(B, fmaxf(d * c, -1000.f), A);
   };
   rows::map(x + begin, out, len, dense);
   __syncthreads();

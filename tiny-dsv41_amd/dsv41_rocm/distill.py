@@ -24,7 +24,7 @@ def _forward(logits, ids, lq, temperature, tail, want_stats):
     rows, dev = logits.shape[0], logits.device
     loss = torch.empty(rows, dtype=torch.float32, device=dev)
     status = torch.empty(rows, dtype=torch.int32, device=dev)
-    stats = torch.empty(rows, 6, dtype=torch.float64, device=dev) if want_stats else None
+    stats = torch.empty(rows, 7, dtype=torch.float64, device=dev) if want_stats else None
     if rows:
         d = _lib.DistillDesc(*row_fields(_lib.DistillDesc, logits), ids.data_ptr(), lq.data_ptr(), temperature, ids.shape[1],
                              tail, loss.data_ptr(), status.data_ptr(), None if stats is None else stats.data_ptr())
