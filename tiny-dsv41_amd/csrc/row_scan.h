@@ -420,9 +420,12 @@ __device__ __forceinline__ State scan(const T* x, int len, const Scale& sc, floa
   return s;
 }
 
-// ---- host: whether rows are read past the caches.  256 MB of cache lie between the L2s and the memory:
-// @ONCE@
-inline bool read_once(int rows, int V, int esize) { return (double)rows * V * esize > 256e6; }
+// ---- host: whether a pass reads its rows with nontemporal loads, which leave the caches as they are.
+// Entropies alone, fp32 rows of 151936: 4096 rows 371 us, 442 otherwise; 331 rows (201 MB) just written
+// 45 and 42, but 43 and 72 behind other work that filled the 256 MB cache with what has to be written
+// back.  Pass and gradient in turn, whose second read the caches serve: 600 rows 218 and 239, bf16 124 and
+// 132; 100 bf16 rows of 129280 (26 MB) 36 and 32.
+inline bool read_once(int rows, int V, int esize) { return (double)rows * V * esize > 64e6; }
 
 // ---- host: how a batch of rows is cut, and what every call checks
 struct Cut {
