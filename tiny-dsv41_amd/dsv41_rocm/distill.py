@@ -17,17 +17,39 @@ from ._check import any_set
 from .logprob import first_order
 from .scores import launch, refuse_capture, row_fields, rows_of_logits, vector
 
+STATS = 7  # fp64 values of a row that the backward needs of the forward
 _TAILS = {"renormalize": _lib.TAIL_RENORMALIZE, "rest": _lib.TAIL_REST}
 
 
-def _forward(logits, ids, lq, temperature, tail, want_stats):
+def prepare(logits, teacher_ids, teacher_log_probs, temperature, tail):
+    """Validated arguments in kernel form."""
+    logits = rows_of_logits(logits, temperature)
+    rows = logits.shape[0]
+    if tail not in _TAILS:
+        raise ValueError("tail must be 'renormalize' or 'rest'")
+    for t in (teacher_ids, teacher_log_probs):
+        if not isinstance(t, torch.Tensor) or t.ndim != 2 or t.shape[0] != rows:
+            raise ValueError("teacher_ids and teacher_log_probs must have shape [rows, entries]")
+    if teacher_ids.shape != teacher_log_probs.shape:
+        raise ValueError("one teacher log probability is required per teacher ID")
+    if teacher_ids.is_floating_point() or teacher_ids.dtype == torch.bool:
+        raise ValueError("teacher_ids must be integers")
+    ids = vector(teacher_ids, torch.int64, teacher_ids.shape, logits.device)
+    lq = vector(teacher_log_probs.detach(), torch.float32, teacher_ids.shape, logits.device)
+    if ids.shape[1] == 0:  # no row has an entry
+        ids, lq = ids.new_full((rows, 1), -1), lq.new_zeros(rows, 1)
+    return logits, ids, lq
+
+
+def forward(logits, ids, lq, temperature, tail, want_stats):
+    """One dsv41_distill_run; returns (loss, statuses, stats or None)."""
     rows, dev = logits.shape[0], logits.device
     loss = torch.empty(rows, dtype=torch.float32, device=dev)
     status = torch.empty(rows, dtype=torch.int32, device=dev)
-    stats = torch.empty(rows, 7, dtype=torch.float64, device=dev) if want_stats else None
+    stats = torch.empty(rows, STATS, dtype=torch.float64, device=dev) if want_stats else None
     if rows:
         d = _lib.DistillDesc(*row_fields(_lib.DistillDesc, logits), ids.data_ptr(), lq.data_ptr(), temperature, ids.shape[1],
-                             tail, loss.data_ptr(), status.data_ptr(), None if stats is None else stats.data_ptr())
+                             _TAILS[tail], loss.data_ptr(), status.data_ptr(), None if stats is None else stats.data_ptr())
         lib = _lib.load()
         ref = ctypes.byref(d)
         size = lib.dsv41_distill_workspace_bytes(ref)
@@ -51,7 +73,7 @@ def distillation_backward(logits, ids, lq, temperature, stats, g_loss):
 class _Distillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, lq, temperature, tail):
-        loss, status, stats = _forward(logits, ids, lq, temperature, tail, True)
+        loss, status, stats = forward(logits, ids, lq, temperature, tail, True)
         ctx.temperature = temperature
         ctx.save_for_backward(logits, ids, lq, stats)
         ctx.mark_non_differentiable(status)
@@ -109,26 +131,12 @@ def distillation_loss(
     1.01 of it with ``"rest"``) or a loss that is not finite (a masked token that the teacher gives mass,
     NaN or +inf logits); without, such a row's loss is NaN, or inf.
     """
-    logits = rows_of_logits(logits, temperature)
-    rows = logits.shape[0]
-    if tail not in _TAILS:
-        raise ValueError("tail must be 'renormalize' or 'rest'")
-    for t in (teacher_ids, teacher_log_probs):
-        if not isinstance(t, torch.Tensor) or t.ndim != 2 or t.shape[0] != rows:
-            raise ValueError("teacher_ids and teacher_log_probs must have shape [rows, entries]")
-    if teacher_ids.shape != teacher_log_probs.shape:
-        raise ValueError("one teacher log probability is required per teacher ID")
-    if teacher_ids.is_floating_point() or teacher_ids.dtype == torch.bool:
-        raise ValueError("teacher_ids must be integers")
-    ids = vector(teacher_ids, torch.int64, teacher_ids.shape, logits.device)
-    lq = vector(teacher_log_probs.detach(), torch.float32, teacher_ids.shape, logits.device)
-    if ids.shape[1] == 0:  # no row has an entry
-        ids, lq = ids.new_full((rows, 1), -1), lq.new_zeros(rows, 1)
+    logits, ids, lq = prepare(logits, teacher_ids, teacher_log_probs, temperature, tail)
     refuse_capture(check)
     if torch.is_grad_enabled() and logits.requires_grad:
-        loss, status = _Distillation.apply(logits, ids, lq, temperature, _TAILS[tail])
+        loss, status = _Distillation.apply(logits, ids, lq, temperature, tail)
     else:
-        loss, status, _ = _forward(logits, ids, lq, temperature, _TAILS[tail], False)
+        loss, status, _ = forward(logits, ids, lq, temperature, tail, False)
     if check and any_set(status)[0]:
         _status_error(status)
     return loss

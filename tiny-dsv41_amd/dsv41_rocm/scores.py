@@ -87,7 +87,24 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
-def _forward(logits, targets, top_k, temperature, want_stats):
+def prepare(logits, targets, top_k, temperature):
+    """Validated arguments in kernel form."""
+    logits = rows_of_logits(logits, temperature)
+    rows, vocab = logits.shape
+    if isinstance(top_k, bool) or not isinstance(top_k, int) or not 0 <= top_k <= vocab:
+        raise ValueError("top_k must be an integer in [0, vocabulary_size]")
+    if targets is not None:
+        if targets.is_floating_point() or targets.dtype == torch.bool:
+            raise ValueError("targets must be integers")
+        if targets.numel() != rows:
+            raise ValueError("one target is required per row")
+        targets = vector(targets.reshape(rows), torch.int64, (rows,), logits.device)
+    return logits, targets
+
+
+def forward(logits, targets, top_k, temperature, want_stats):
+    """One dsv41_scores_run; returns (log-probs, ranks, entropy, ids, log-probs, statuses, stats), None for
+    what is not asked for."""
     rows, dev = logits.shape[0], logits.device
     f32, i64 = torch.float32, torch.int64
     lp = rank = stats = ws = None
@@ -134,7 +151,7 @@ def scores_backward(logits, targets, top_ids, temperature, stats, g_log_probs, g
 class _LogitScores(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top_k, temperature):
-        lp, rank, entropy, top_ids, top_lp, status, stats = _forward(logits, targets, top_k, temperature, True)
+        lp, rank, entropy, top_ids, top_lp, status, stats = forward(logits, targets, top_k, temperature, True)
         ctx.temperature = temperature
         ctx.save_for_backward(logits, targets, top_ids, stats)
         ctx.mark_non_differentiable(*(t for t in (rank, top_ids, status) if t is not None))
@@ -184,21 +201,12 @@ def logit_scores(
     With ``check`` the call synchronises and raises ``ValueError`` for a target outside the vocabulary,
     or a row with a NaN, a +inf or no unmasked token; without, such a row holds NaN (ids -1, rank 0).
     """
-    logits = rows_of_logits(logits, temperature)
-    rows, vocab = logits.shape
-    if isinstance(top_k, bool) or not isinstance(top_k, int) or not 0 <= top_k <= vocab:
-        raise ValueError("top_k must be an integer in [0, vocabulary_size]")
-    if targets is not None:
-        if targets.is_floating_point() or targets.dtype == torch.bool:
-            raise ValueError("targets must be integers")
-        if targets.numel() != rows:
-            raise ValueError("one target is required per row")
-        targets = vector(targets.reshape(rows), torch.int64, (rows,), logits.device)
+    logits, targets = prepare(logits, targets, top_k, temperature)
     refuse_capture(check)
     if torch.is_grad_enabled() and logits.requires_grad:
         lp, rank, entropy, top_ids, top_lp, status = _LogitScores.apply(logits, targets, top_k, temperature)
     else:
-        lp, rank, entropy, top_ids, top_lp, status, _ = _forward(logits, targets, top_k, temperature, False)
+        lp, rank, entropy, top_ids, top_lp, status, _ = forward(logits, targets, top_k, temperature, False)
     if check and any_set(status)[0]:
         _status_error(status)
     return LogitScores(lp, rank, entropy, top_ids, top_lp)
