@@ -234,8 +234,9 @@ struct GradParams {
   void* out;  // [rows, V], rows V apart
 };
 
-// One read and one write of the row; the list's tokens are written again after the workgroup's barrier.
-// Rows whose list is empty or whose gradient is zero are zeros and are not read.
+// One read and one write of the row; the list's tokens are written again after the workgroup's barrier,
+// with values that the threads form first, while the other waves already read.  Rows whose list is empty
+// or whose gradient is zero are zeros and are not read.
 template <typename T>
 __global__ __launch_bounds__(NT) void distill_grad_kernel(GradParams p) {
   const int row = p.rows - 1 - (int)(blockIdx.x / p.slices), slice = blockIdx.x % p.slices;
@@ -248,19 +249,27 @@ __global__ __launch_bounds__(NT) void distill_grad_kernel(GradParams p) {
     rows::fill_zero(out, len);
     return;
   }
+  // entry k's place in the slice (below 0: none of this slice's) and gradient
+  const auto entry = [&](int k, float& v) {
+    const int64_t id = p.ids[(int64_t)row * p.K + k], i = id - begin;
+    if (id < 0 || i < 0 || i >= len) return -1;
+    const double e = exp(((double)Elem<T>::one(x + id) - st.m) * p.sc.inv_t);
+    v = (float)(g * (st.Q * e / st.S - exp((double)p.lq[(int64_t)row * p.K + k] - st.log_z)));
+    return (int)i;
+  };
+  float mine = 0.f;
+  const int at = (int)threadIdx.x < p.K ? entry(threadIdx.x, mine) : -1;
   const rows::Lift lift(g * st.others);
   const float base = (float)st.base, A = (float)(g * st.others * lift.down);
   // (a row whose sums are NaN has NaN for S: its gradient is, too)
   const float bad = st.S == st.S ? 0.f : NAN;
   rows::map(x + begin, out, len, [&](float v) { return __builtin_fmaf(A, lift.exp2(v - base, p.sc.c), bad); });
   __syncthreads();
-  const int64_t* ids = p.ids + (int64_t)row * p.K;
-  const float* lq = p.lq + (int64_t)row * p.K;
-  for (int k = threadIdx.x; k < p.K; k += NT) {
-    const int64_t i = ids[k] - begin;
-    if (ids[k] < 0 || i < 0 || i >= len) continue;
-    const double e = exp(((double)Elem<T>::one(x + begin + i) - st.m) * p.sc.inv_t);
-    rows::store_one(out + i, (float)(g * (st.Q * e / st.S - exp((double)lq[k] - st.log_z))));
+  if (at >= 0) rows::store_one(out + at, mine);
+  for (int k = (int)threadIdx.x + NT; k < p.K; k += NT) {
+    float v;
+    const int i = entry(k, v);
+    if (i >= 0) rows::store_one(out + i, v);
   }
 }
 

@@ -733,21 +733,23 @@ __global__ __launch_bounds__(NT) void scores_grad_kernel(GradParams p) {
   };
   rows::map(x + begin, out, len, dense);
   __syncthreads();
-  const float inv_t = (float)p.sc.inv_t;
+  // the tokens with a gradient of their own, in fp64, since 1 - p_t is what is left of a likely target's
+  const auto write = [&](int64_t id, double g) {
+    const int64_t i = id - begin;
+    if (id < 0 || i < 0 || i >= len) return;
+    const double d = ((double)Elem<T>::one(x + id) - st[0]) * p.sc.inv_t;
+    // (b goes with exponents of 2; a masked token has a power of 0, and a row without sums NaN)
+    const double e = d > -INFINITY ? exp(d) * (a + b * d * (p.sc.c / p.sc.inv_t)) : 0.0 * S;
+    rows::store_one(out + i, (float)(e + g * p.sc.inv_t));
+  };
   int listed = 0;
   if (p.g_top)
     for (int k = tid; k < p.K; k += NT) {
-      const int64_t i = ids[k] - begin;
-      if (ids[k] < 0) continue;
       listed |= ids[k] == t;
-      if (i >= 0 && i < len) {
-        const double own = (double)g_top[k] + (ids[k] == t ? g_lp : 0.0);
-        rows::store_one(out + i, dense(Elem<T>::one(x + begin + i)) + (float)(own * p.sc.inv_t));
-      }
+      write(ids[k], (double)g_top[k] + (ids[k] == t ? g_lp : 0.0));
     }
   listed = __syncthreads_or(listed);
-  if (!listed && tid == 0 && t >= begin && t < begin + len)
-    rows::store_one(out + (t - begin), dense(Elem<T>::one(x + t)) + (float)g_lp * inv_t);
+  if (!listed && tid == 0) write(t, g_lp);
 }
 
 // ---------------------------------------------------------------------------------------- host
