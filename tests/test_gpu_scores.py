@@ -468,3 +468,22 @@ def test_top_tokens_that_lie_together(dtype, k):
     t = torch.tensor([4096, 30500, 70, 7 * vec], device=DEV)
     check(x.to(dtype).to(DEV), t, k, 1.0)
     check(x.to(dtype).to(DEV).repeat(150, 1), t.repeat(150), k, 1.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_ranks_of_every_token(dtype):
+    # ties within the target's chunk, before and behind it, zeros of both signs, masked targets, and
+    # the neighbours of each value
+    V = 1037
+    g = torch.Generator().manual_seed(3)
+    x = torch.randint(-3, 4, (1, V), generator=g).float() * 0.5
+    x[0, torch.randperm(V, generator=g)[:200]] = -0.0
+    x[0, torch.randperm(V, generator=g)[:150]] = -math.inf
+    x[0, 100:103] = torch.tensor([torch.finfo(dtype).tiny, -torch.finfo(dtype).tiny, torch.finfo(dtype).min])
+    x[0, 103:105] = torch.tensor([1.5 + 2 * torch.finfo(dtype).eps, 1.5 - 2 * torch.finfo(dtype).eps])
+    rows = x.to(dtype).expand(V, V).contiguous().to(DEV)
+    check(rows, torch.arange(V, device=DEV), 0, 1.0)
+    # and in slices: the same row, long
+    long = torch.cat([x] * 30, 1).to(dtype).to(DEV)
+    t = torch.randint(0, long.shape[1], (40,), generator=g).to(DEV)
+    check(long.expand(40, -1), t, 3, 1.0)

@@ -277,6 +277,14 @@ __device__ __forceinline__ void group_max2(float& g, float& h) {
 #undef DSV41_DPP2
 }
 
+// The largest number below x that is not equal to it (-0 equals +0); NaN, which no number is at most,
+// below -inf.
+__device__ __forceinline__ float next_below(float x) {
+  const uint32_t b = __float_as_uint(x);
+  if (x == 0.f) return __uint_as_float(0x80000001u);
+  return __uint_as_float(x > 0.f ? b - 1u : b + 1u);
+}
+
 constexpr float SAFE = 1e30f;  // the largest |m c| that x c - r is formed with
 
 // One pass over x[0, len) by the workgroup, whose threads take 16 bytes in turn.
@@ -296,9 +304,11 @@ __device__ __forceinline__ State scan(const T* x, int len, const Scale& sc, floa
   float own[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
   float r = LOWEST, S[2] = {0.f, 0.f}, Us[2] = {0.f, 0.f}, margin = NAMED ? 2.f : sc.margin;
   asm("" : "+v"(margin));  // (a scalar register short, the compiler would load it in every step)
-  int ahead = 0, t = 0;
+  int ahead = 0, t = 0;  // (ahead: the wave's count)
   float xt = INFINITY;
 
+  int target_chunk = 0;
+  float below = INFINITY;
   using Tile = uint32_t[2][4];  // two chunks a thread
   constexpr int STEP = 2 * NT;
   auto load = [&](Tile& w, int base) {
@@ -324,12 +334,14 @@ __device__ __forceinline__ State scan(const T* x, int len, const Scale& sc, floa
     own0 = fmaxf(own0, cm[0]);
     own1 = fmaxf(own1, cm[1]);
     const float tm = max3(cm[0], cm[1], cm[1]);
-    if (!NAMED && tm >= xt) {
+    // elements before the target: those above its logit, and in chunks before its own also the equal
+    // ones, which are above the next smaller number
+    if (!NAMED && __ballot(tm >= xt)) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int below = t - (base + u * NT + tid) * VEC;  // elements of the chunk with a lower index
+        const float at_most = base + u * NT + tid < target_chunk ? below : xt;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) ahead += (v[u][j] > xt || (v[u][j] == xt && j < below)) ? 1 : 0;
+        for (int j = 0; j < VEC; ++j) ahead += __popcll(__ballot(!(v[u][j] <= at_most)));
       }
     }
     if constexpr (TOP) {
@@ -383,6 +395,14 @@ __device__ __forceinline__ State scan(const T* x, int len, const Scale& sc, floa
     for (int u = 0; u < 2; ++u) load_some<ONCE>(x, len, u * NT + tid, a[u]);
   }
   if (!before(xt, t)) return State{0.0, 0.0, -INFINITY, 0};
+  if constexpr (!NAMED) {
+    target_chunk = t >= 0 ? min(t / VEC, n) : 0;  // (behind the slice: all of its chunks, and none past them)
+    below = next_below(xt);
+    if (t >= 0 && t < len && xt < INFINITY) {
+      const int at = target_chunk * VEC + tid;  // equal ones of the target's own chunk
+      ahead += __popcll(__ballot(at < t && Elem<T>::one(x + min(at, t)) == xt));
+    }
+  }
   for (int i = 0; i < steps; i += 2) {
     if (i + 1 < steps) load(b, (i + 1) * STEP);
     take(a, i * STEP, own[0], own[1]);
@@ -402,7 +422,7 @@ __device__ __forceinline__ State scan(const T* x, int len, const Scale& sc, floa
   State s;
   met(own);
   s.m = block_max<true>(fmaxf(fmaxf(own[0], own[1]), fmaxf(own[2], own[3])), red);
-  double sum[3] = {(double)S[0] + S[1], (double)Us[0] + Us[1], (double)ahead};
+  double sum[3] = {(double)S[0] + S[1], (double)Us[0] + Us[1], (tid & 63) == 0 ? (double)ahead : 0.0};
   if (NAMED && fabsf(s.m * sc.c) > SAFE && s.m > -INFINITY) {
     sum[0] = 0.0;
     for (int i = tid; i < len; i += NT)
