@@ -132,6 +132,7 @@ __device__ __forceinline__ void finish(const Params& p, int row, State st, int f
     for (int k = threadIdx.x + NT; k < p.K; k += NT) add(entry_of<T>(p, row, k));
   }
   rows::block_sums(sum, red);
+  if (threadIdx.x >= 64) return;  // (one thread writes)
   const double Sn = sum[0], W = sum[1], WL = sum[2], WD = sum[3];
   // S_rest against m, by `down` from the sum against its own largest logit
   const double down = st.S != 0.0 ? exp2(fmax(((double)st.m - m) * p.sc.cd, -2000.0)) : 0.0;

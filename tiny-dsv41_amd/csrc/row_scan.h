@@ -430,7 +430,12 @@ __device__ __forceinline__ State scan(const T* x, int len, const Scale& sc, floa
   } else if (sum[0] == 0.0) {
     sum[1] = 0.0;  // nothing met: its reference means nothing
   } else {
-    rebase(sum[0], sum[1], (NAMED ? (double)r - (double)s.m * sc.cd : ((double)r - (double)s.m) * sc.cd));
+    // as rebase, with v_exp_f32: off by 2^-23 of the thread's share, and exact for the one that holds m
+    const double d = fmax(NAMED ? (double)r - (double)s.m * sc.cd : ((double)r - (double)s.m) * sc.cd, -1000.0);
+    const float near = (float)d;
+    const double f = (double)__builtin_amdgcn_exp2f(near) * (1.0 + 0.6931471805599453 * (d - (double)near));
+    sum[1] = f * (sum[1] + d * sum[0]);
+    sum[0] *= f;
   }
   found(s.m);
   block_sums<true>(sum, red + WAVES);

@@ -506,6 +506,7 @@ __device__ __forceinline__ int top_of(Shared& s, const T* x, int len, int first,
 
 // The row's outputs from its sums and its sorted list.
 __device__ __forceinline__ void write_row(const Params& p, int row, const Shared& s, int n_top) {
+  if ((int)(threadIdx.x & ~63u) > p.K) return;  // waves without an alternative to write
   const State st = s.state;
   const uint64_t* top = s.buf;
   const double S = st.S + p.sc.kappa * st.U;
