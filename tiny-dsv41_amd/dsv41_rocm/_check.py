@@ -46,10 +46,13 @@ def any_set(status: Optional[torch.Tensor], ids: Optional[torch.Tensor] = None, 
         return n > 0 and bool((status != 0).any()), n_ids > 0 and bool(((ids < 0) | (ids >= limit)).any())
     if _word.ptr is None:
         _word.make()
-    device = t.device
-    with torch.cuda.device(device):
-        got = _lib.load().dsv41_check_wait(status.data_ptr() if n else None, n, ids.data_ptr() if n_ids else None,
-                                           n_ids, limit, _word.ptr, torch.cuda.current_stream(device).cuda_stream)
+    index = t.device.index
+    args = (status.data_ptr() if n else None, n, ids.data_ptr() if n_ids else None, n_ids, limit, _word.ptr)
+    if torch.cuda.current_device() == index:
+        got = _lib.load().dsv41_check_wait(*args, _lib.stream(index))
+    else:
+        with torch.cuda.device(index):
+            got = _lib.load().dsv41_check_wait(*args, _lib.stream(index))
     if got < 0:
         _left.append(_word.host)
         _word.make()

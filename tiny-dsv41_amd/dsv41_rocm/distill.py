@@ -15,7 +15,7 @@ import torch
 from . import _lib
 from ._check import any_set
 from .logprob import first_order
-from .scores import launch, refuse_capture, row_fields, rows_of_logits, vector
+from .scores import INTEGERS, launch, refuse_capture, row_fields, rows_of_logits, vector
 
 STATS = 7  # fp64 values of a row that the backward needs of the forward
 _TAILS = {"renormalize": _lib.TAIL_RENORMALIZE, "rest": _lib.TAIL_REST}
@@ -27,16 +27,17 @@ def prepare(logits, teacher_ids, teacher_log_probs, temperature, tail):
     rows = logits.shape[0]
     if tail not in _TAILS:
         raise ValueError("tail must be 'renormalize' or 'rest'")
+    shape, device = teacher_ids.shape, logits.device
     for t in (teacher_ids, teacher_log_probs):
-        if not isinstance(t, torch.Tensor) or t.ndim != 2 or t.shape[0] != rows:
+        if t.ndim != 2 or t.shape[0] != rows:
             raise ValueError("teacher_ids and teacher_log_probs must have shape [rows, entries]")
-    if teacher_ids.shape != teacher_log_probs.shape:
+    if teacher_log_probs.shape != shape:
         raise ValueError("one teacher log probability is required per teacher ID")
-    if teacher_ids.is_floating_point() or teacher_ids.dtype == torch.bool:
+    if teacher_ids.dtype not in INTEGERS:
         raise ValueError("teacher_ids must be integers")
-    ids = vector(teacher_ids, torch.int64, teacher_ids.shape, logits.device)
-    lq = vector(teacher_log_probs.detach(), torch.float32, teacher_ids.shape, logits.device)
-    if ids.shape[1] == 0:  # no row has an entry
+    ids = vector(teacher_ids, torch.int64, shape, device)
+    lq = vector(teacher_log_probs.detach() if teacher_log_probs.requires_grad else teacher_log_probs, torch.float32, shape, device)
+    if shape[1] == 0:  # no row has an entry
         ids, lq = ids.new_full((rows, 1), -1), lq.new_zeros(rows, 1)
     return logits, ids, lq
 

@@ -21,7 +21,7 @@ from ._check import any_set
 from .logprob import first_order
 from .sampling import validate_temperature
 
-MAX_TOP_K = 1024
+INTEGERS = frozenset((torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8))
 
 
 @dataclass
@@ -37,6 +37,9 @@ class LogitScores:
     top_log_probs: torch.Tensor
 
 
+_KERNEL_DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
+
+
 def rows_of_logits(logits, temperature):
     """Validated fp32 or bf16 logits [rows, V] whose rows are contiguous."""
     validate_temperature(temperature)
@@ -44,10 +47,12 @@ def rows_of_logits(logits, temperature):
         raise ValueError("logits must have shape [rows, vocabulary_size]")
     if not logits.is_cuda:
         raise ValueError("logits must be on the GPU (libdsv41hip has no CPU path)")
-    if logits.dtype not in (torch.float32, torch.bfloat16):
+    if logits.dtype not in _KERNEL_DTYPES:
         logits = logits.float()
     # rows that overlap without being one and the same (stride 0) have no place for the kernels' row stride
-    if logits.stride(1) != 1 and logits.shape[1] > 1 or 0 < logits.stride(0) < logits.shape[1]:
+    step, unit = logits.stride()
+    vocab = logits.shape[1]
+    if unit != 1 and vocab > 1 or 0 < step < vocab:
         logits = logits.contiguous()
     return logits
 
@@ -60,18 +65,20 @@ def refuse_capture(check: bool) -> None:
 def row_fields(cls, logits) -> tuple:
     """The fields that every descriptor over rows of logits begins with."""
     rows, vocab = logits.shape
-    return (ctypes.sizeof(cls), rows, vocab, _lib.DTYPE_F32 if logits.dtype == torch.float32 else _lib.DTYPE_BF16,
-            logits.stride(0) if rows > 1 else vocab, logits.data_ptr())
+    return (ctypes.sizeof(cls), rows, vocab, _KERNEL_DTYPES[logits.dtype], logits.stride(0) if rows > 1 else vocab,
+            logits.data_ptr())
 
 
 def launch(call, device, *args) -> None:
     """``call(*args, stream)`` on the device's current stream, with its error raised."""
-    if torch.cuda.current_device() == device.index:
-        rc = call(*args, torch.cuda.current_stream(device).cuda_stream)
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = call(*args, _lib.stream(index))
     else:
-        with torch.cuda.device(device):
-            rc = call(*args, torch.cuda.current_stream(device).cuda_stream)
-    _lib.check(rc)
+        with torch.cuda.device(index):
+            rc = call(*args, _lib.stream(index))
+    if rc:
+        _lib.check(rc)
 
 
 def vector(t, dtype, shape, device):
@@ -94,11 +101,13 @@ def prepare(logits, targets, top_k, temperature):
     if isinstance(top_k, bool) or not isinstance(top_k, int) or not 0 <= top_k <= vocab:
         raise ValueError("top_k must be an integer in [0, vocabulary_size]")
     if targets is not None:
-        if targets.is_floating_point() or targets.dtype == torch.bool:
+        if targets.dtype not in INTEGERS:
             raise ValueError("targets must be integers")
         if targets.numel() != rows:
             raise ValueError("one target is required per row")
-        targets = vector(targets.reshape(rows), torch.int64, (rows,), logits.device)
+        if targets.ndim != 1:
+            targets = targets.reshape(rows)
+        targets = vector(targets, torch.int64, targets.shape, logits.device)
     return logits, targets
 
 
