@@ -267,6 +267,15 @@ def test_refused_arguments():
         distillation_loss(torch.zeros(1, (1 << 21) + 1, device=DEV), ids[:1], lq[:1])
 
 
+def test_sizes_past_32_bits_are_refused():
+    one, ids, lq = torch.zeros(1, 1, device=DEV), torch.zeros(1, 1, dtype=torch.int64, device=DEV), torch.zeros(1, 1, device=DEV)
+    n = 2 ** 32 + 1
+    for x, i, q in ((one.expand(n, 1), ids.expand(n, 1), lq.expand(n, 1)), (one.expand(1, n), ids, lq),
+                    (one, ids.expand(1, n), lq.expand(1, n))):
+        with pytest.raises(NotImplementedError, match="2\\^31"):
+            distillation_loss(x, i, q)
+
+
 def test_layouts():
     logits, ids, lq = make(12, 800, 6, torch.float32, 9)
     want = distillation_loss(logits, ids, lq, tail="rest")

@@ -208,6 +208,16 @@ def test_refusals():
         logit_scores(logits.cpu())
 
 
+def test_sizes_past_32_bits_are_refused():
+    # (views of one element: a wrapped size would pass for a small batch)
+    one = torch.zeros(1, 1, device=DEV)
+    for shape in ((2 ** 32 + 1, 1), (1, 2 ** 32 + 5), (2 ** 31, 1)):
+        with pytest.raises(NotImplementedError, match="2\\^31"):
+            logit_scores(one.expand(shape))
+        with pytest.raises(NotImplementedError, match="2\\^31"):
+            torch.ops.dsv41_rocm.logit_scores(one.expand(shape), None, 0, 1.0)
+
+
 def test_empty_batch_and_other_layouts():
     s = logit_scores(torch.empty(0, 50, device=DEV), torch.empty(0, dtype=torch.int64, device=DEV), top_k=3)
     assert s.log_probs.shape == (0,) and s.top_ids.shape == (0, 3)

@@ -15,7 +15,7 @@ import torch
 from . import _lib
 from ._check import any_set
 from .logprob import first_order
-from .scores import INTEGERS, launch, refuse_capture, row_fields, rows_of_logits, vector
+from .scores import INTEGERS, fit_int32, launch, refuse_capture, row_fields, rows_of_logits, vector
 
 STATS = 7  # fp64 values of a row that the backward needs of the forward
 _TAILS = {"renormalize": _lib.TAIL_RENORMALIZE, "rest": _lib.TAIL_REST}
@@ -28,6 +28,7 @@ def prepare(logits, teacher_ids, teacher_log_probs, temperature, tail):
     if tail not in _TAILS:
         raise ValueError("tail must be 'renormalize' or 'rest'")
     shape, device = teacher_ids.shape, logits.device
+    fit_int32(*shape)
     for t in (teacher_ids, teacher_log_probs):
         if t.ndim != 2 or t.shape[0] != rows:
             raise ValueError("teacher_ids and teacher_log_probs must have shape [rows, entries]")

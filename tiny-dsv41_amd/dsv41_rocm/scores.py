@@ -40,6 +40,12 @@ class LogitScores:
 _KERNEL_DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 
 
+def fit_int32(*sizes) -> None:
+    """Refuses sizes that a descriptor's int32 would wrap."""
+    if max(sizes) > 0x7FFFFFFF:
+        raise NotImplementedError("sizes above 2^31 - 1 are not supported")
+
+
 def rows_of_logits(logits, temperature):
     """Validated fp32 or bf16 logits [rows, V] whose rows are contiguous."""
     validate_temperature(temperature)
@@ -47,6 +53,7 @@ def rows_of_logits(logits, temperature):
         raise ValueError("logits must have shape [rows, vocabulary_size]")
     if not logits.is_cuda:
         raise ValueError("logits must be on the GPU (libdsv41hip has no CPU path)")
+    fit_int32(*logits.shape)
     if logits.dtype not in _KERNEL_DTYPES:
         logits = logits.float()
     # rows that overlap without being one and the same (stride 0) have no place for the kernels' row stride
