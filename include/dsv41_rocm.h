@@ -32,6 +32,10 @@
  *                         differentiates it (dsv41_train/rl/distributed_grpo.py:352-375 over
  *                         native_lora.py:120-122 / model.py:735-738): the gradient with
  *                         respect to the lm_head output, in that output's dtype (bf16).
+ *   dsv41_scores_run   <- an engine's logprobs output, of which rollout_manager/backends/
+ *                         vllm_actor.py:260 takes the sampled token's: over rows of logits at hand,
+ *                         with ranks, entropies and alternatives; dsv41_scores_grad_run is its gradient.
+ * dsv41_distill_run and dsv41_distill_grad_run (divergence from a teacher's top tokens) replace nothing.
  */
 #ifndef DSV41_ROCM_H
 #define DSV41_ROCM_H

@@ -387,3 +387,68 @@ def test_streams_graphs_and_repeats():
         for a, b in zip(got, want[i]):
             assert torch.equal(a, b)
         distillation_loss(batches[0][0], batches[0][1], batches[0][2])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tail", ["renormalize", "rest"])
+def test_lists_longer_than_the_threads_over_slices(tail, dtype):
+    # more entries than a workgroup has threads, some of them none, of rows that are cut
+    logits, ids, lq = make(3, 30000, 1100, dtype, 81, ragged=True, pad=3, shift=1)
+    compare(logits, ids, lq, 1.0, tail)
+    # as many entries as tokens, and more with the empty ones
+    logits, ids, lq = make(2, 700, 700, dtype, 82)
+    ids = torch.cat([ids.new_full((2, 50), -7), ids], 1)
+    lq = torch.cat([lq.new_full((2, 50), math.inf), lq], 1)
+    compare(logits, ids, lq, 1.0, tail)
+
+
+def test_offsets_above_32_bits():
+    rows, V = 15000, 151936
+    logits = torch.zeros(rows, V, dtype=torch.bfloat16, device=DEV)
+    logits[-1, 100000], logits[-1, 7] = 9.0, 8.0
+    ids = torch.tensor([[100000, 151935]], device=DEV).expand(rows, 2)
+    lq = torch.log(torch.tensor([[0.5, 0.25]], device=DEV)).expand(rows, 2)
+    print("case: distillation_loss 15000 x 151936 bf16", flush=True)
+    leaf = logits.requires_grad_()
+    loss = distillation_loss(leaf, ids, lq, tail="rest")
+    g = torch.zeros(rows, device=DEV)
+    g[-1] = 1.0
+    (grad,) = torch.autograd.grad(loss, leaf, g)
+    few = [0, rows - 1]
+    want, slope, _, _ = plain(logits.detach()[few].float(), ids[few], lq[few], 1.0, "rest")
+    assert float((loss.detach()[few].cpu().double() - want).abs().max()) <= H * 2.1 * (48 + V / 512) + 4 * H * 12
+    assert float((grad[-1].cpu().double() - slope[1]).norm() / slope[1].norm()) <= 2.0 ** -8
+    assert float(grad[-2].abs().max()) == 0.0 and float(grad[0].abs().max()) == 0.0
+
+
+def test_two_streams_at_once():
+    batches = [make(15, 30000 + 500 * i, 70, torch.float32, 90 + i, ragged=True) for i in range(4)]
+
+    def step(x, ids, lq):
+        leaf = x.detach().requires_grad_()
+        loss = distillation_loss(leaf, ids, lq, tail="rest", check=False)
+        return loss.detach(), torch.autograd.grad(loss.sum(), leaf)[0]
+
+    want = [step(*b) for b in batches]
+    sides = [torch.cuda.Stream(DEV) for _ in range(2)]
+    for s in sides:
+        s.wait_stream(torch.cuda.current_stream(DEV))
+    got = []
+    for turn in range(3):
+        for i, b in enumerate(batches):
+            with torch.cuda.stream(sides[i % 2]):
+                got.append((i, step(*b)))
+    torch.cuda.synchronize()
+    for i, out in got:
+        for a, b in zip(out, want[i]):
+            assert torch.equal(a, b)
+
+
+def test_what_was_saved_is_not_changed_unseen():
+    logits, ids, lq = make(3, 2000, 9, torch.float32, 95)
+    for change in (lambda ids, lq: ids.fill_(-1), lambda ids, lq: lq.zero_()):
+        leaf, i, q = logits.clone().requires_grad_(), ids.clone(), lq.clone()
+        loss = distillation_loss(leaf, i, q)
+        change(i, q)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.sum().backward()

@@ -497,3 +497,110 @@ def test_ranks_of_every_token(dtype):
     long = torch.cat([x] * 30, 1).to(dtype).to(DEV)
     t = torch.randint(0, long.shape[1], (40,), generator=g).to(DEV)
     check(long.expand(40, -1), t, 3, 1.0)
+
+
+@pytest.mark.parametrize("rows,V,k", [(2, 9000, 1024), (3, 40000, 700)])
+def test_gradient_of_more_alternatives_than_threads(rows, V, k):
+    T = 0.6
+    logits, t = make(rows, V, torch.float32, V + k)
+    order = logits.argsort(1, descending=True)
+    t[0], t[1] = order[0, 600], order[1, 3]  # among the alternatives, in a thread's second and first
+    g = torch.Generator().manual_seed(5)
+    g_lp, g_h, g_top = torch.randn(rows, generator=g), torch.randn(rows, generator=g), torch.randn(rows, k, generator=g)
+    leaf = logits.detach().requires_grad_()
+    s, ref = check(leaf, t, k, T)
+    (got,) = torch.autograd.grad([s.log_probs, s.entropy, s.top_log_probs], leaf, [g_lp.to(DEV), g_h.to(DEV), g_top.to(DEV)])
+    want, size = plain_grad(ref, t, T, g_lp, g_h, g_top)
+    # the sum of k gradients in fp64 of fp32 values adds nothing; a scaled sum's rounding is in `size`
+    close(got, want, grad_tolerance(size, want, torch.float32, ref, T, V), "gradient")
+
+
+def test_two_streams_and_two_threads_at_once():
+    import threading
+
+    batches = [make(20 + i, 30000 + 1000 * i, torch.bfloat16, 60 + i) for i in range(4)]
+
+    def step(x, t, check):
+        leaf = x.detach().requires_grad_()
+        s = logit_scores(leaf, t, top_k=40, check=check)
+        (grad,) = torch.autograd.grad(s.log_probs.sum() + s.top_log_probs.sum(), leaf)
+        return s.log_probs.detach(), s.ranks, s.entropy.detach(), s.top_ids, s.top_log_probs.detach(), grad
+
+    want = [step(*b, True) for b in batches]
+    # unchecked calls in turn on two streams, with nothing between them
+    sides = [torch.cuda.Stream(DEV) for _ in range(2)]
+    for s in sides:
+        s.wait_stream(torch.cuda.current_stream(DEV))
+    got = []
+    for turn in range(3):
+        for i, b in enumerate(batches):
+            with torch.cuda.stream(sides[i % 2]):
+                got.append((i, step(*b, False)))
+    torch.cuda.synchronize()
+    # checked calls from two threads, each on its own stream
+    failed = []
+
+    def work(n):
+        try:
+            with torch.cuda.stream(sides[n]):
+                for turn in range(3):
+                    for i in (n, 2 + n):
+                        out = step(*batches[i], True)
+                        sides[n].synchronize()
+                        got.append((i, out))
+        except Exception as e:  # shown by the test's own thread
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join(60)
+    torch.cuda.synchronize()
+    assert not failed and len(got) == 24
+    for i, out in got:
+        for a, b in zip(out, want[i]):
+            assert torch.equal(a, b)
+
+
+def test_two_graphs_replayed_at_once():
+    batches = [make(6, 50000, torch.float32, 70 + i) for i in range(2)]
+    want = [logit_scores(*b, top_k=300) for b in batches]
+    graphs, outs = [], []
+    for b in batches:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(logit_scores(*b, top_k=300, check=False))
+        graphs.append(graph)
+    sides = [torch.cuda.Stream(DEV) for _ in range(2)]
+    for turn in range(4):
+        for s, graph, out in zip(sides, graphs, outs):
+            for t in (out.entropy, out.top_log_probs, out.log_probs):
+                t.zero_()
+            s.wait_stream(torch.cuda.current_stream(DEV))
+        for s, graph in zip(sides, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+                graph.replay()
+        torch.cuda.synchronize()
+        for out, w in zip(outs, want):
+            for name in ("log_probs", "ranks", "entropy", "top_ids", "top_log_probs"):
+                assert torch.equal(getattr(out, name), getattr(w, name)), name
+
+
+def test_what_was_saved_is_not_changed_unseen():
+    logits, t = make(3, 2000, torch.float32, 5)
+    for change in (lambda leaf, t, s: t.zero_(), lambda leaf, t, s: s.top_ids.zero_()):
+        leaf, t2 = logits.clone().requires_grad_(), t.clone()
+        s = logit_scores(leaf, t2, top_k=4)
+        change(leaf, t2, s)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            s.log_probs.sum().backward()
+    # outputs that nothing saves may be edited, and targets of any integer type or shape given
+    leaf = logits.clone().requires_grad_()
+    s = logit_scores(leaf, t.to(torch.int16).view(3, 1), top_k=4)
+    s.ranks.zero_()
+    (got,) = torch.autograd.grad((s.log_probs * 2.0).sum(), leaf)
+    leaf2 = logits.clone().requires_grad_()
+    (want,) = torch.autograd.grad(logit_scores(leaf2, t).log_probs.sum(), leaf2)
+    assert torch.equal(got, 2.0 * want)

@@ -14,6 +14,11 @@
 //
 // A row of few is cut into slices, which leave their sums and their sorted lists in the workspace for a
 // second kernel.
+//
+// What bounds it.  4096 fp32 rows of 151936 with 64 alternatives take 381 us, 6.5 TB/s (7.0 is what
+// nontemporal reads reach): memory, and the selections, which fall together on the workgroups of a CU.
+// 1000 bf16 rows of 129280 with ranks take 50 us, 5.2 TB/s: 10.8 vector instructions an element, of which
+// the exponential counts twice.  A single row, 7.3 us and 4.6 to join, is a chain of latencies.
 #include <limits.h>
 #include <math.h>
 
@@ -119,7 +124,7 @@ __device__ __forceinline__ void sort_bitonic(uint64_t* buf, int n) {
 
 // Descending order of s.buf[0, n), n <= BUF, of logits in [low, m].  Every thread calls it, behind a
 // barrier.  Up to 128 keys are placed by counting the larger ones.  More are dealt into BUCKETS intervals of
-// the logits, and placed by counting within their bucket: 710 keys of a row's tail in 3.3 us beside three
+// the logits, and placed by counting within their bucket: 710 keys of a row's tail in 4.6 us beside three
 // other workgroups, 15 by the bitonic sort, which is left for logits that crowd into few buckets.
 __device__ __forceinline__ void sort_desc(Shared& s, int n, float low, float m) {
   const int tid = threadIdx.x;
@@ -266,8 +271,9 @@ __device__ __forceinline__ void search(uint32_t& lo, uint32_t& hi, int& c, int K
 // The selection begins within the pass: what the threads met bounds the row's K-th element.  The K-th
 // largest of the shares' maxima is such a bound, and few more groups than K reach it where K is at most
 // half of the shares: in rows of no special order, 68 groups the 64th of 512, 710 the 512th of 1024.
-// Up to K = 256 one wave searches among the 512 threads' maxima by itself, without a barrier (0.9 us,
-// 3.4 by all waves); above, all search among 1024 or 2048 (search_shares).
+// Up to K = 256 one wave searches among the 512 threads' maxima by itself, without a barrier, while the
+// others join their sums (one row's top 5: 7.4 us instead of 8.7; 48 rows' top 20: 18.3 instead of 22.6);
+// above, all search among 1024 or 2048 (search_shares).
 constexpr int ALONE = NT / 2;
 __device__ __forceinline__ void met_shares(Shared& s, const float (&own)[4], int K) {
   if (K <= ALONE) s.bucket[threadIdx.x] = __float_as_int(fmaxf(fmaxf(own[0], own[1]), fmaxf(own[2], own[3])));
@@ -476,7 +482,6 @@ __device__ __forceinline__ int top_of(Shared& s, const T* x, int len, int first,
     n = gather(bound);
   }
   if (n > BUF) {
-    // ties
     // more ties at the bound than the buffer holds: a batch at a time
     if (threadIdx.x == 0) s.n = 0;
     __syncthreads();
@@ -691,7 +696,9 @@ struct GradParams {
 
 // dx_i = (1 / T) (-(G + g_H (log p_i + H)) p_i + g_lp [i = t] + sum_k g_k [i = id_k]),  G = g_lp + sum_k g_k,
 // as e_i (A + B d_i) with e_i = 2^d_i and d_i = (x_i - m) c: one read and one write of the row.  The
-// tokens that have a gradient of their own are written again after the workgroup's barrier.
+// tokens that have a gradient of their own are written again after the workgroup's barrier.  Bound by memory:
+// 1000 bf16 rows of 151851 in 103-120 us, 5.1-5.9 TB/s (a copy: 5.1-5.5).  The last rows come first: the
+// forward read them last, and the caches may still hold them.
 template <typename T>
 __global__ __launch_bounds__(NT) void scores_grad_kernel(GradParams p) {
   __shared__ double red[3 * WAVES];
