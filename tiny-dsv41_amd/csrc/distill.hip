@@ -286,17 +286,8 @@ void launch(const Params& p, hipStream_t s) {
   if (p.slices > 1) hipLaunchKernelGGL(distill_join_kernel<T>, dim3(p.rows), dim3(NT), 0, s, p);
 }
 
-// As the scores' (GPU time of a call in a graph, rest of a 64-token list, bf16: 48 rows of 151851 16.7 us
-// with 512 workgroups, 20.5 with 1024; 600 rows of 151936 49.3 and 52.0).
-Cut cut_of(int rows, int V) {
-  int64_t want = (512 + rows - 1) / rows;
-  if (want > 64) want = 64;
-  if (want > V / 6144) want = V / 6144;
-  if (want < 1) want = 1;
-  int len = (int)(((V + want - 1) / want + GROUP - 1) / GROUP * GROUP);
-  if (len > MAX_LEN) len = MAX_LEN;
-  return {(V + len - 1) / len, len};
-}
+Cut cut_of(int rows, int V, int esize) { return rows::cut_rows(rows, V, 0, esize, 6144, MAX_LEN); }
+int esize_of(const dsv41_distill_desc* d) { return d->logits_dtype == DSV41_DTYPE_F32 ? 4 : 2; }
 
 int check_desc(const dsv41_distill_desc* d) {
   if (!d) return fail(DSV41_E_INVALID, "distillation descriptor is NULL");
@@ -308,7 +299,7 @@ int check_desc(const dsv41_distill_desc* d) {
   if (d->tail != DSV41_TAIL_RENORMALIZE && d->tail != DSV41_TAIL_REST)
     return fail(DSV41_E_INVALID, "tail must be DSV41_TAIL_RENORMALIZE or DSV41_TAIL_REST");
   if (!d->out_loss || !d->out_status) return fail(DSV41_E_INVALID, "out_loss and out_status are required");
-  return rows::check_grid(d->rows, cut_of(d->rows, d->vocab));
+  return rows::check_grid(d->rows, cut_of(d->rows, d->vocab, esize_of(d)));
 }
 
 size_t workspace_of(int rows, const Cut& c) { return c.slices == 1 ? 0 : (size_t)rows * c.slices * sizeof(SliceState); }
@@ -320,12 +311,12 @@ using namespace dsv41;
 
 extern "C" size_t dsv41_distill_workspace_bytes(const dsv41_distill_desc* d) {
   if (distill::check_desc(d)) return 0;
-  return distill::workspace_of(d->rows, distill::cut_of(d->rows, d->vocab));
+  return distill::workspace_of(d->rows, distill::cut_of(d->rows, d->vocab, distill::esize_of(d)));
 }
 
 extern "C" int dsv41_distill_run(const dsv41_distill_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = distill::check_desc(d)) return rc;
-  const rows::Cut c = distill::cut_of(d->rows, d->vocab);
+  const rows::Cut c = distill::cut_of(d->rows, d->vocab, distill::esize_of(d));
   const size_t need = distill::workspace_of(d->rows, c);
   if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 8))
     return fail(DSV41_E_WORKSPACE, "distillation workspace is missing, too small or not 8-byte aligned");

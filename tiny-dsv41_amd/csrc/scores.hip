@@ -761,21 +761,9 @@ __global__ __launch_bounds__(NT) void scores_grad_kernel(GradParams p) {
 }
 
 // ---------------------------------------------------------------------------------------- host
-// Rows are cut where there are too few of them to occupy the GPU: into slices of at least 6144 elements
-// until there are 512 workgroups.  (Measured, GPU time of a call in a graph, fp32: 48 rows of 151851, top 20,
-// 22.0 us with 512, 24.4 with 1024, 21.4 with 256; 331 rows of 129280, top 64, 48.9, 51.9 and 46.4; one
-// row of 129280 without alternatives 7.4 in slices of 6144, 7.3 of 4096, 7.8 of 8192.)  More than 256
-// alternatives take slices whose threads meet four chunks each, whose maxima bound them.
+// More than 256 alternatives take slices whose threads meet four chunks each, whose maxima bound them.
 Cut cut_of(int rows, int V, int K, int esize) {
-  const int least = K > ALONE ? 4 * NT * (16 / esize) : 6144;
-  int64_t want = (512 + rows - 1) / rows;
-  if (want > 64) want = 64;
-  if (want > V / least) want = V / least;
-  if (want < 1) want = 1;
-  int len = (int)((V + want - 1) / want);
-  len = (len + GROUP - 1) / GROUP * GROUP;
-  if (len > MAX_LEN) len = MAX_LEN;
-  return {(V + len - 1) / len, len};
+  return rows::cut_rows(rows, V, K, esize, K > ALONE ? 4 * NT * (16 / esize) : 6144, MAX_LEN);
 }
 
 size_t workspace_of(int rows, int K, const Cut& c) {
