@@ -437,17 +437,23 @@ __device__ __forceinline__ int top_of(Shared& s, const T* x, int len, int first,
     each_chunk([&](const uint32_t(&w)[4], int at) {
       float v[VEC];
       Elem<T>::unpack(w, v);
-      uint32_t pass = 0;
+      // the wave's elements one after the other: one addition for all of them
+      uint64_t pass[VEC];
+      int total = 0;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) pass |= (uint32_t)(v[j] >= from) << j;
-      if (pass) {
-        int to = atomicAdd(&s.n, __popc(pass));
+      for (int j = 0; j < VEC; ++j) {
+        pass[j] = __ballot(v[j] >= from);
+        total += __popcll(pass[j]);
+      }
+      if (total == 0) return;
+      int to = 0;
+      if ((threadIdx.x & 63) == 0) to = atomicAdd(&s.n, total);
+      to = __builtin_amdgcn_readfirstlane(to);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j)
-          if (pass >> j & 1) {
-            if (to < BUF) s.buf[to] = element_key(v[j], at, j);
-            ++to;
-          }
+      for (int j = 0; j < VEC; ++j) {
+        const int mine = to + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(pass[j] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)pass[j], 0));
+        if (v[j] >= from && mine < BUF) s.buf[mine] = element_key(v[j], at, j);
+        to += __popcll(pass[j]);
       }
     });
     __syncthreads();
