@@ -237,9 +237,9 @@ struct GradParams {
   void* out;  // [rows, V], rows V apart
 };
 
-// One read and one write of the row; the list's tokens are written again after the workgroup's barrier,
-// with values that the threads form first, while the other waves already read.  Rows whose list is empty
-// or whose gradient is zero are zeros and are not read.
+// One read and one write of the row; then the list's tokens are written again, with values that the threads
+// form first, while the other waves already read.  Rows whose list is empty or whose gradient is zero are
+// zeros and are not read.
 template <typename T>
 __global__ __launch_bounds__(NT) void distill_grad_kernel(GradParams p) {
   const int row = p.rows - 1 - (int)(blockIdx.x / p.slices), slice = blockIdx.x % p.slices;
@@ -260,19 +260,22 @@ __global__ __launch_bounds__(NT) void distill_grad_kernel(GradParams p) {
     v = (float)(g * (st.Q * e / st.S - exp((double)p.lq[(int64_t)row * p.K + k] - st.log_z)));
     return (int)i;
   };
-  float mine = 0.f;
-  const int at = (int)threadIdx.x < p.K ? entry(threadIdx.x, mine) : -1;
+  __shared__ rows::Again again;
+  const int tid = threadIdx.x;
+  again.at[tid] = tid < p.K ? entry(tid, again.v[tid]) : -1;
   const rows::Lift lift(g * st.others);
   const float base = (float)st.base, A = (float)(g * st.others * lift.down);
   // (a row whose sums are NaN has NaN for S: its gradient is, too)
   const float bad = st.S == st.S ? 0.f : NAN;
   rows::map(x + begin, out, len, [&](float v) { return __builtin_fmaf(A, lift.exp2(v - base, p.sc.c), bad); });
-  __syncthreads();
-  if (at >= 0) rows::store_one(out + at, mine);
-  for (int k = (int)threadIdx.x + NT; k < p.K; k += NT) {
-    float v;
-    const int i = entry(k, v);
-    if (i >= 0) rows::store_one(out + i, v);
+  rows::own_stores_in_order();
+  rows::lds_barrier();
+  rows::store_again(again, min(p.K, NT), out, len);
+  for (int k = NT; k < p.K; k += NT) {
+    rows::lds_barrier();
+    again.at[tid] = k + tid < p.K ? entry(k + tid, again.v[tid]) : -1;
+    rows::lds_barrier();
+    rows::store_again(again, min(p.K - k, NT), out, len);
   }
 }
 

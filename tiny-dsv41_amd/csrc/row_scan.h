@@ -153,6 +153,38 @@ __device__ __forceinline__ void map(const T* x, T* out, int len, F f) {
   }
   for (int i = full * VEC + tid; i < len; i += NT) store_one(out + i, f(Elem<T>::one(x + i)));
 }
+// Some elements of a row that `map` wrote are written again, by the wave that wrote them: its stores to one
+// address stay in order, so no wave waits for those of the others, nor for its own, which a barrier of
+// all memory would have it do.  `wrote` says whether element i of out[0, len) is this wave's.
+template <typename T>
+__device__ __forceinline__ bool wrote(int i, int len) {
+  constexpr int VEC = Elem<T>::VEC;
+  const int at = i < len / VEC * VEC ? i / VEC % NT : 0;  // (the few behind the last chunk are the first wave's)
+  return at >> 6 == (int)threadIdx.x >> 6;
+}
+__device__ __forceinline__ void own_stores_in_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+// A barrier for what the threads wrote to LDS, with stores to memory left in flight.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+// Values for the elements at[k] (below 0: none) of out[0, len), k < n: a thread's entry is formed before the row
+// is mapped, then each wave stores those of its own elements.
+struct Again {
+  int at[NT];
+  float v[NT];
+};
+template <typename T>
+__device__ __forceinline__ void store_again(const Again& a, int n, T* out, int len) {
+  for (int k = (int)threadIdx.x & 63; k < n; k += 64) {
+    const int i = a.at[k];
+    if (i >= 0 && wrote<T>(i, len)) store_one(out + i, a.v[k]);
+  }
+}
 template <typename T>
 __device__ __forceinline__ void fill_zero(T* out, int len) {
   constexpr int VEC = Elem<T>::VEC;

@@ -702,11 +702,11 @@ struct GradParams {
 
 // dx_i = (1 / T) (-(G + g_H (log p_i + H)) p_i + g_lp [i = t] + sum_k g_k [i = id_k]),  G = g_lp + sum_k g_k,
 // as e_i (A + B d_i) with e_i = 2^d_i and d_i = (x_i - m) c: one read and one write of the row.  The
-// tokens that have a gradient of their own are written again after the workgroup's barrier.  Bound by memory:
+// tokens that have a gradient of their own are written again by the waves that wrote them.  Bound by memory:
 // 1000 bf16 rows of 151851 in 103-120 us, 5.1-5.9 TB/s (a copy: 5.1-5.5).  The last rows come first: the
 // forward read them last, and the caches may still hold them.
 template <typename T>
-__global__ __launch_bounds__(NT) void scores_grad_kernel(GradParams p) {
+__global__ __launch_bounds__(NT, 8) void scores_grad_kernel(GradParams p) {
   __shared__ double red[3 * WAVES];
   const int row = p.rows - 1 - (int)(blockIdx.x / p.slices), slice = blockIdx.x % p.slices;
   const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.stride;
@@ -745,25 +745,45 @@ __global__ __launch_bounds__(NT) void scores_grad_kernel(GradParams p) {
     const float d = v - m;
     return lift.exp2(d, c) * __builtin_fmaf(B, fmaxf(d * c, -1000.f), A);
   };
-  rows::map(x + begin, out, len, dense);
-  __syncthreads();
   // the tokens with a gradient of their own, in fp64, since 1 - p_t is what is left of a likely target's
-  const auto write = [&](int64_t id, double g) {
-    const int64_t i = id - begin;
-    if (id < 0 || i < 0 || i >= len) return;
+  const auto value = [&](int64_t id, double g) {
     const double d = ((double)Elem<T>::one(x + id) - st[0]) * p.sc.inv_t;
     // (b goes with exponents of 2; a masked token has a power of 0, and a row without sums NaN)
     const double e = d > -INFINITY ? exp(d) * (a + b * d * (p.sc.c / p.sc.inv_t)) : 0.0 * S;
-    rows::store_one(out + i, (float)(e + g * p.sc.inv_t));
+    return (float)(e + g * p.sc.inv_t);
   };
+  const auto place = [&](int64_t id) { return id >= begin && id < begin + len ? (int)(id - begin) : -1; };
+  if (!p.g_top) {
+    rows::map(x + begin, out, len, dense);
+    rows::own_stores_in_order();
+    const int i = place(t);
+    if (i >= 0 && rows::wrote<T>(i, len) && (tid & 63) == 0) rows::store_one(out + i, value(t, g_lp));
+    return;
+  }
+  // the alternatives, and the target where it is none of them
+  __shared__ rows::Again again;
   int listed = 0;
-  if (p.g_top)
-    for (int k = tid; k < p.K; k += NT) {
-      listed |= ids[k] == t;
-      write(ids[k], (double)g_top[k] + (ids[k] == t ? g_lp : 0.0));
-    }
+  const auto entry = [&](int k) {
+    const int64_t id = k < p.K ? ids[k] : -1;
+    listed |= id >= 0 && id == t;
+    const int i = place(id);
+    if (i >= 0) again.v[tid] = value(id, (double)g_top[k] + (id == t ? g_lp : 0.0));
+    again.at[tid] = i;
+  };
+  entry(tid);
+  rows::map(x + begin, out, len, dense);
+  rows::own_stores_in_order();
+  rows::lds_barrier();
+  rows::store_again(again, min(p.K, NT), out, len);
+  for (int k = NT; k < p.K; k += NT) {
+    rows::lds_barrier();
+    entry(k + tid);
+    rows::lds_barrier();
+    rows::store_again(again, min(p.K - k, NT), out, len);
+  }
   listed = __syncthreads_or(listed);
-  if (!listed && tid == 0) write(t, g_lp);
+  const int i = place(t);
+  if (!listed && i >= 0 && rows::wrote<T>(i, len) && (tid & 63) == 0) rows::store_one(out + i, value(t, g_lp));
 }
 
 // ---------------------------------------------------------------------------------------- host
