@@ -128,29 +128,32 @@ struct Lift {
   }
   __device__ __forceinline__ float exp2(float d, float c) const { return __builtin_amdgcn_exp2f(__builtin_fmaf(d, c, up)); }
 };
+// U chunks a thread from `base` on, the loads of all of them in flight; of the last U only `rest` threads'.
+template <int U, typename T, class F>
+__device__ __forceinline__ void map_some(const T* x, T* out, int base, int rest, F f) {
+  constexpr int VEC = Elem<T>::VEC;
+  const int tid = threadIdx.x;
+  float v[U][VEC];
+#pragma unroll
+  for (int u = 0; u < U; ++u) load_full(x, base + u * NT + (u + 1 < U ? tid : min(tid, rest - 1)), v[u]);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[u][j] = f(v[u][j]);
+    if (u + 1 < U || tid < rest) store_full(out, base + u * NT + tid, v[u]);
+  }
+}
 template <typename T, class F>
 __device__ __forceinline__ void map(const T* x, T* out, int len, F f) {
   constexpr int VEC = Elem<T>::VEC, U = 4;
   const int full = len / VEC, tid = threadIdx.x;
   int base = 0;
-  for (; base + U * NT <= full; base += U * NT) {
-    float v[U][VEC];
-#pragma unroll
-    for (int u = 0; u < U; ++u) load_full(x, base + u * NT + tid, v[u]);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v[u][j] = f(v[u][j]);
-      store_full(out, base + u * NT + tid, v[u]);
-    }
-  }
-  for (int i = base + tid; i < full; i += NT) {
-    float v[VEC];
-    load_full(x, i, v);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = f(v[j]);
-    store_full(out, i, v);
-  }
+  for (; base + U * NT <= full; base += U * NT) map_some<U>(x, out, base, NT, f);
+  const int left = full - base;
+  if (left > 3 * NT) map_some<4>(x, out, base, left - 3 * NT, f);
+  else if (left > 2 * NT) map_some<3>(x, out, base, left - 2 * NT, f);
+  else if (left > NT) map_some<2>(x, out, base, left - NT, f);
+  else if (left > 0) map_some<1>(x, out, base, left, f);
   for (int i = full * VEC + tid; i < len; i += NT) store_one(out + i, f(Elem<T>::one(x + i)));
 }
 // Some elements of a row that `map` wrote are written again, by the wave that wrote them: its stores to one
