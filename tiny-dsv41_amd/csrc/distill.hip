@@ -358,7 +358,7 @@ extern "C" int dsv41_distill_grad_run(const dsv41_distill_grad_desc* d, void* st
     return fail(DSV41_E_INVALID, "teacher_ids, teacher_logprob, stats, grad_loss and out are required");
   if ((uintptr_t)d->out % (d->logits_dtype == DSV41_DTYPE_F32 ? 4 : 2))
     return fail(DSV41_E_INVALID, "out is not aligned to its type");
-  const rows::Cut c = rows::grad_cut(d->rows, d->vocab);
+  const rows::Cut c = rows::grad_cut(d->rows, d->vocab, d->logits_dtype == DSV41_DTYPE_F32 ? 4 : 2);
   if (int rc = rows::check_grid(d->rows, c)) return rc;
   distill::GradParams p{};
   p.logits = d->logits;

@@ -883,7 +883,7 @@ extern "C" int dsv41_scores_grad_run(const dsv41_scores_grad_desc* d, void* stre
     return fail(DSV41_E_INVALID, "out is not aligned to its type");
   if (d->grad_logprob && !d->targets) return fail(DSV41_E_INVALID, "grad_logprob needs targets");
   if (d->grad_top && (!d->top_ids || d->top_k <= 0)) return fail(DSV41_E_INVALID, "grad_top needs top_ids and top_k");
-  const rows::Cut c = rows::grad_cut(d->rows, d->vocab);
+  const rows::Cut c = rows::grad_cut(d->rows, d->vocab, d->logits_dtype == DSV41_DTYPE_F32 ? 4 : 2);
   if (int rc = rows::check_grid(d->rows, c)) return rc;
   scores::GradParams p{};
   p.logits = d->logits;
