@@ -703,7 +703,7 @@ struct GradParams {
 // dx_i = (1 / T) (-(G + g_H (log p_i + H)) p_i + g_lp [i = t] + sum_k g_k [i = id_k]),  G = g_lp + sum_k g_k,
 // as e_i (A + B d_i) with e_i = 2^d_i and d_i = (x_i - m) c: one read and one write of the row.  The
 // tokens that have a gradient of their own are written again by the waves that wrote them.  Bound by memory:
-// 1000 bf16 rows of 151851 in 103-120 us, 5.1-5.9 TB/s (a copy: 5.1-5.5).  The last rows come first: the
+// 1000 bf16 rows of 151851 in 100-114 us, 5.3-6.0 TB/s of read and write.  The last rows come first: the
 // forward read them last, and the caches may still hold them.
 template <typename T>
 __global__ __launch_bounds__(NT, 8) void scores_grad_kernel(GradParams p) {
