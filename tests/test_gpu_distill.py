@@ -452,3 +452,26 @@ def test_what_was_saved_is_not_changed_unseen():
         change(i, q)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             loss.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,V", [(2, 33003), (40, 40001), (3, 5), (1, 151851)])
+def test_listed_tokens_at_the_ends_of_slices_and_chunks(rows, V, dtype):
+    # wherever the gradient's slices of whole 32 elements end, their first and last tokens are listed in some
+    # row, and so are the few behind the last 16 bytes
+    logits, _, _ = make(rows, V, 1, dtype, V + 5, pad=1, shift=1)
+    edges = [i for n in range(1, 41) for b in (-(-(-(-V // n)) // 32) * 32,) for j in range(1, n) for i in (j * b - 1, j * b)]
+    edges = sorted({i for i in edges if 0 <= i < V} | set(range(max(0, V - 9), V)) | {0})
+    k = min(len(edges), 500)
+    g = torch.Generator().manual_seed(3)
+    ids = torch.stack([torch.tensor(edges)[torch.randperm(len(edges), generator=g)[:k]] for _ in range(rows)])
+    lq = torch.log_softmax(torch.randn(rows, k, generator=g), 1) - 0.1
+    ids, lq = ids.to(DEV), lq.to(DEV)
+    if k == V:
+        # the teacher's rest, 1 - exp(-0.1), has no token left to go to: q (log q - log 0) is infinite
+        assert bool(plain(logits.float(), ids, lq, 1.0, "rest")[0].isinf().all())
+        with pytest.raises(ValueError, match="non-finite"):
+            distillation_loss(logits, ids, lq, tail="rest")
+        compare(logits, ids, lq, 1.0, "renormalize")
+        return
+    compare(logits, ids, lq, 1.0, "rest")

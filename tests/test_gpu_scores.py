@@ -604,3 +604,21 @@ def test_what_was_saved_is_not_changed_unseen():
     leaf2 = logits.clone().requires_grad_()
     (want,) = torch.autograd.grad(logit_scores(leaf2, t).log_probs.sum(), leaf2)
     assert torch.equal(got, 2.0 * want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [33003, 8192, 16385])
+def test_gradient_of_targets_at_the_ends_of_slices_and_chunks(V, dtype):
+    # a row for each place where a slice of whole 32 elements may end, and for the last elements
+    edges = [i for n in range(1, 9) for b in (-(-(-(-V // n)) // 32) * 32,) for j in range(1, n) for i in (j * b - 1, j * b)]
+    edges = sorted({i for i in edges if 0 <= i < V} | set(range(V - 9, V)) | {0, 2047, 2048, 4095, 4096})
+    rows, T = len(edges), 1.0
+    logits, _ = make(rows, V, dtype, V + 9, pad=1, shift=1)
+    t = torch.tensor(edges, device=DEV)
+    g = torch.Generator().manual_seed(6)
+    g_lp, g_h, g_top = torch.randn(rows, generator=g), torch.randn(rows, generator=g), torch.zeros(rows, 0)
+    leaf = logits.detach().requires_grad_()
+    s, ref = check(leaf, t, 0, T)
+    (got,) = torch.autograd.grad([s.log_probs, s.entropy], leaf, [g_lp.to(DEV), g_h.to(DEV)])
+    want, size = plain_grad(ref, t, T, g_lp, g_h, g_top)
+    close(got, want, grad_tolerance(size, want, dtype, ref, T, V), "gradient")
