@@ -622,3 +622,38 @@ def test_gradient_of_targets_at_the_ends_of_slices_and_chunks(V, dtype):
     (got,) = torch.autograd.grad([s.log_probs, s.entropy], leaf, [g_lp.to(DEV), g_h.to(DEV)])
     want, size = plain_grad(ref, t, T, g_lp, g_h, g_top)
     close(got, want, grad_tolerance(size, want, dtype, ref, T, V), "gradient")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shift", range(0, 70, 3))
+def test_rows_that_begin_anywhere_in_a_line(shift, dtype):
+    # rows of an odd stride, cut into slices whose ends lie inside 16 bytes; few values, so that most
+    # comparisons are ties, masked tokens at the slices' ends, and masked targets; NaN around the rows
+    rows, V, k = 6, 25003, 30
+    g = torch.Generator().manual_seed(shift)
+    x = torch.randint(0, 4, (rows, V), generator=g).float()
+    x[torch.rand(rows, V, generator=g) < 0.3] = -math.inf
+    for n in range(1, 5):
+        b = -(-(-(-V // n)) // 32) * 32
+        for j in range(1, n):
+            x[0::2, j * b - 3:j * b + 5] = -math.inf
+    t = torch.randint(0, V, (rows,), generator=g)
+    t[0], t[1], t[2] = V - 1, 0, V // 2
+    x[0, V - 1] = x[2, V // 2] = -math.inf
+    x[1, 0] = 0.0
+    buf = torch.full((rows * (V + 2) + shift,), math.nan, dtype=dtype)
+    view = buf[shift:].view(rows, V + 2)
+    view[:, :V] = x.to(dtype)
+    logits = buf.to(DEV)[shift:].view(rows, V + 2)[:, :V]
+    assert logits.data_ptr() % 128 == shift * buf.element_size() % 128
+    leaf = logits.detach().requires_grad_()
+    s, ref = check(leaf, t.to(DEV), k, 1.0)
+    up = torch.zeros(rows)
+    up[3:] = 1.0  # (the rows with masked targets aside)
+    (got,) = torch.autograd.grad([s.log_probs, s.entropy], leaf, [up.to(DEV), up.to(DEV)])
+    ref["top_ids"] = ref["top_ids"][:, :0]
+    want, size = plain_grad(ref, t, 1.0, up, up, torch.zeros(rows, 0))
+    want = torch.where((x == -math.inf) & (torch.arange(V) != t[:, None]), torch.zeros_like(want), want)
+    got, want, size = got[3:], want[3:], size[3:]
+    ref = {key: value[3:] for key, value in ref.items()}
+    close(got, want, grad_tolerance(size, want, dtype, ref, 1.0, V), "gradient")

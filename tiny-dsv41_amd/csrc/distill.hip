@@ -32,7 +32,8 @@ using rows::Scale;
 using rows::State;
 using rows::WAVES;
 
-constexpr int MAX_LEN = 5120 * 32;  // elements of one slice: 20 KB of bits
+constexpr int MAP = 5120 * 32;                     // bits of the map: 20 KB
+constexpr int MAX_LEN = MAP - rows::MOST_SKEW;  // elements of one slice
 constexpr double REST_FLOOR = 0x1p-20;
 constexpr double MOST_MASS = 1.01;  // log-probs rounded to bf16 may add up to 1 + 2^-8 |lq| or so
 constexpr int STATS = 7;            // per row, see write_row
@@ -56,7 +57,7 @@ struct Params {
 };
 
 struct Shared {
-  alignas(16) uint32_t named[MAX_LEN / 32];  // whole 16 bytes
+  alignas(16) uint32_t named[MAP / 32];  // whole 16 bytes
   double red[4 * WAVES];
   int flags;
 };
@@ -171,7 +172,7 @@ __global__ __launch_bounds__(NT, 8) void distill_kernel(Params p) {
   __shared__ Shared s;
   const int row = blockIdx.x / p.slices, slice = blockIdx.x % p.slices, tid = threadIdx.x;
   const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.stride;
-  const int begin = slice * p.len, len = min(p.len, p.V - begin);
+  const int skew = rows::skew_of(x + slice * p.len), begin = slice * p.len - skew, len = min(p.len, p.V - slice * p.len) + skew;
   Entry mine;
   int flags;
   const auto before = [&](float&, int&) {
@@ -185,7 +186,7 @@ __global__ __launch_bounds__(NT, 8) void distill_kernel(Params p) {
       if (id < 0) continue;
       f |= LIVE;
       if (id >= p.V) f |= DSV41_STATUS_BAD_TARGET;
-      if (id >= begin && id < begin + len) {
+      if (id >= begin + skew && id < begin + len) {
         const uint32_t i = (uint32_t)(id - begin), bit = 1u << (i & 31);
         if (atomicOr(&s.named[i >> 5], bit) & bit) f |= DSV41_STATUS_REPEATED;
       }
@@ -196,7 +197,7 @@ __global__ __launch_bounds__(NT, 8) void distill_kernel(Params p) {
     return flags == LIVE;
   };
   const State st = rows::scan<T, ONCE, false, true>(
-      x + begin, len, p.sc, nullptr, s.named, s.red, before, [](const float(&)[4]) {}, [](float) {});
+      x + begin, skew, len, p.sc, nullptr, s.named, s.red, before, [](const float(&)[4]) {}, [](float) {});
   if (p.slices == 1) {
     finish<T>(p, row, st, flags, mine, s.red);
   } else if (tid == 0) {
@@ -270,12 +271,12 @@ __global__ __launch_bounds__(NT) void distill_grad_kernel(GradParams p) {
   rows::map(x + begin, out, len, [&](float v) { return __builtin_fmaf(A, lift.exp2(v - base, p.sc.c), bad); });
   rows::own_stores_in_order();
   rows::lds_barrier();
-  rows::store_again(again, min(p.K, NT), out, len);
+  rows::store_again(again, min(p.K, NT), x + begin, out, len);
   for (int k = NT; k < p.K; k += NT) {
     rows::lds_barrier();
     again.at[tid] = k + tid < p.K ? entry(k + tid, again.v[tid]) : -1;
     rows::lds_barrier();
-    rows::store_again(again, min(p.K - k, NT), out, len);
+    rows::store_again(again, min(p.K - k, NT), x + begin, out, len);
   }
 }
 

@@ -38,7 +38,7 @@ using rows::WAVES;
 
 constexpr int MAX_K = 1024;
 constexpr int MAX_GROUPS = 5120;                  // of one slice
-constexpr int MAX_LEN = MAX_GROUPS * GROUP;       // elements of one slice
+constexpr int MAX_LEN = MAX_GROUPS * GROUP - rows::MOST_SKEW;  // elements of one slice
 constexpr int LIST = MAX_K + MAX_K / 4 + 64;      // groups that are read again
 constexpr int BATCH = 2048;                       // elements or keys that one step may add to the buffer
 constexpr int BUF = 2 * BATCH;
@@ -406,10 +406,10 @@ __device__ __forceinline__ int select_groups(Shared& s, int n, int K, float m, f
   return taken;
 }
 
-// s.buf = the first K elements of x[0, len) in order (or as many as are not masked); returns their
-// number.  `first`: the index of x[0] in its row.
+// s.buf = the first K elements of x[from, len) in order (or as many as are not masked); returns their
+// number.  `first`: the index of x[0] in its row (below 0 where x[from] is the row's first).
 template <typename T>
-__device__ __forceinline__ int top_of(Shared& s, const T* x, int len, int first, int K, float m) {
+__device__ __forceinline__ int top_of(Shared& s, const T* x, int from, int len, int first, int K, float m) {
   constexpr int VEC = Elem<T>::VEC, LANES = GROUP / VEC, AT_ONCE = BATCH / GROUP;
   float bound;
   const int n_groups = (len + GROUP - 1) / GROUP;
@@ -426,14 +426,14 @@ __device__ __forceinline__ int top_of(Shared& s, const T* x, int len, int first,
       for (int a = 0; a < AHEAD; ++a) {
         const int g = b + a * (NT / LANES) + (int)threadIdx.x / LANES;
         at[a] = g < groups ? (int)s.list[g] * LANES + lane : -1;
-        rows::load_some<false>(x, len, at[a], w[a]);
+        rows::load_some<false>(x, from, len, at[a], w[a]);
       }
 #pragma unroll
       for (int a = 0; a < AHEAD; ++a) f(w[a], at[a]);
     }
   };
   const auto element_key = [&](float v, int at, int j) { return key_of(v, (uint32_t)(first + at * VEC + j)); };
-  const auto gather = [&](float from) {
+  const auto gather = [&](float least) {
     each_chunk([&](const uint32_t(&w)[4], int at) {
       float v[VEC];
       Elem<T>::unpack(w, v);
@@ -442,7 +442,7 @@ __device__ __forceinline__ int top_of(Shared& s, const T* x, int len, int first,
       int total = 0;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        pass[j] = __ballot(v[j] >= from);
+        pass[j] = __ballot(v[j] >= least);
         total += __popcll(pass[j]);
       }
       if (total == 0) return;
@@ -452,7 +452,7 @@ __device__ __forceinline__ int top_of(Shared& s, const T* x, int len, int first,
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         const int mine = to + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(pass[j] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)pass[j], 0));
-        if (v[j] >= from && mine < BUF) s.buf[mine] = element_key(v[j], at, j);
+        if (v[j] >= least && mine < BUF) s.buf[mine] = element_key(v[j], at, j);
         to += __popcll(pass[j]);
       }
     });
@@ -499,7 +499,7 @@ __device__ __forceinline__ int top_of(Shared& s, const T* x, int len, int first,
         const int at = (int)s.list[g] * LANES + lane;
         uint32_t w[4];
         float v[VEC];
-        rows::load_some<false>(x, len, at, w);
+        rows::load_some<false>(x, from, len, at, w);
         Elem<T>::unpack(w, v);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
@@ -558,7 +558,7 @@ __global__ __launch_bounds__(NT, 8) void scores_kernel(Params p) {
   __shared__ Shared s;
   const int row = blockIdx.x / p.slices, slice = blockIdx.x % p.slices;
   const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.stride;
-  const int begin = slice * p.len, len = min(p.len, p.V - begin);
+  const int skew = rows::skew_of(x + slice * p.len), begin = slice * p.len - skew, len = min(p.len, p.V - slice * p.len) + skew;
   int64_t target = -1;
   float at_target = INFINITY;
   const auto before = [&](float& xt, int& t) {
@@ -584,7 +584,7 @@ __global__ __launch_bounds__(NT, 8) void scores_kernel(Params p) {
       if (p.K <= ALONE) search_alone(s, p.K, m);
   };
   const State st =
-      rows::scan<T, ONCE, TOP, false>(x + begin, len, p.sc, s.group_max, nullptr, s.red, before, met, found);
+      rows::scan<T, ONCE, TOP, false>(x + begin, skew, len, p.sc, s.group_max, nullptr, s.red, before, met, found);
   if constexpr (TOP)
     if (p.K > ALONE) search_shares(s, own, p.K, st.m);
   if (threadIdx.x == 0) {  // (registers that would be kept over the selection)
@@ -594,7 +594,7 @@ __global__ __launch_bounds__(NT, 8) void scores_kernel(Params p) {
   }
   int n = 0;
   if constexpr (TOP)
-    n = top_of(s, x + begin, len, begin, p.K, st.m);
+    n = top_of(s, x + begin, skew, len, begin, p.K, st.m);
   else
     __syncthreads();
   if (p.slices == 1) {
@@ -757,7 +757,7 @@ __global__ __launch_bounds__(NT, 8) void scores_grad_kernel(GradParams p) {
     rows::map(x + begin, out, len, dense);
     rows::own_stores_in_order();
     const int i = place(t);
-    if (i >= 0 && rows::wrote<T>(i, len) && (tid & 63) == 0) rows::store_one(out + i, value(t, g_lp));
+    if (i >= 0 && rows::wrote(x + begin, i, len) && (tid & 63) == 0) rows::store_one(out + i, value(t, g_lp));
     return;
   }
   // the alternatives, and the target where it is none of them
@@ -774,16 +774,16 @@ __global__ __launch_bounds__(NT, 8) void scores_grad_kernel(GradParams p) {
   rows::map(x + begin, out, len, dense);
   rows::own_stores_in_order();
   rows::lds_barrier();
-  rows::store_again(again, min(p.K, NT), out, len);
+  rows::store_again(again, min(p.K, NT), x + begin, out, len);
   for (int k = NT; k < p.K; k += NT) {
     rows::lds_barrier();
     entry(k + tid);
     rows::lds_barrier();
-    rows::store_again(again, min(p.K - k, NT), out, len);
+    rows::store_again(again, min(p.K - k, NT), x + begin, out, len);
   }
   listed = __syncthreads_or(listed);
   const int i = place(t);
-  if (!listed && i >= 0 && rows::wrote<T>(i, len) && (tid & 63) == 0) rows::store_one(out + i, value(t, g_lp));
+  if (!listed && i >= 0 && rows::wrote(x + begin, i, len) && (tid & 63) == 0) rows::store_one(out + i, value(t, g_lp));
 }
 
 // ---------------------------------------------------------------------------------------- host
