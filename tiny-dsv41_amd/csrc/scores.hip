@@ -15,7 +15,7 @@
 // A row of few is cut into slices, which leave their sums and their sorted lists in the workspace for a
 // second kernel.
 //
-// What bounds it.  4096 fp32 rows of 151936 with 64 alternatives take 381 us, 6.5 TB/s (7.0 is what
+// What bounds it.  4096 fp32 rows of 151936 with 64 alternatives take 379 us, 6.6 TB/s (7.0 is what
 // nontemporal reads reach): memory, and the selections, which fall together on the workgroups of a CU.
 // 1000 bf16 rows of 129280 with ranks take 50 us, 5.2 TB/s: 10.8 vector instructions an element, of which
 // the exponential counts twice.  A single row, 7.3 us and 4.6 to join, is a chain of latencies.
@@ -703,7 +703,7 @@ struct GradParams {
 // dx_i = (1 / T) (-(G + g_H (log p_i + H)) p_i + g_lp [i = t] + sum_k g_k [i = id_k]),  G = g_lp + sum_k g_k,
 // as e_i (A + B d_i) with e_i = 2^d_i and d_i = (x_i - m) c: one read and one write of the row.  The
 // tokens that have a gradient of their own are written again by the waves that wrote them.  Bound by memory:
-// 1000 bf16 rows of 151851 in 100-114 us, 5.3-6.0 TB/s of read and write.  The last rows come first: the
+// 1000 bf16 rows of 151851 in 95-107 us, 5.7-6.4 TB/s of read and write.  The last rows come first: the
 // forward read them last, and the caches may still hold them.
 template <typename T>
 __global__ __launch_bounds__(NT, 8) void scores_grad_kernel(GradParams p) {
