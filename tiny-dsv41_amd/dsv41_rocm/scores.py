@@ -118,29 +118,34 @@ def prepare(logits, targets, top_k, temperature):
     return logits, targets
 
 
-def forward(logits, targets, top_k, temperature, want_stats):
+def forward(logits, targets, top_k, temperature, want_stats, want_status=True):
     """One dsv41_scores_run; returns (log-probs, ranks, entropy, ids, log-probs, statuses, stats), None for
-    what is not asked for."""
+    what is not asked for.  Statuses that nobody looks at lie behind the workspace: an allocation less, 1.1 us of
+    a decoding call's 21."""
     rows, dev = logits.shape[0], logits.device
     f32, i64 = torch.float32, torch.int64
-    lp = rank = stats = ws = None
+    lp = rank = status = stats = ws = None
     if targets is not None:
         lp = torch.empty(rows, dtype=f32, device=dev)
         rank = torch.empty(rows, dtype=i64, device=dev)
     entropy = torch.empty(rows, dtype=f32, device=dev)
     top_ids = torch.empty(rows, top_k, dtype=i64, device=dev)
     top_lp = torch.empty(rows, top_k, dtype=f32, device=dev)
-    status = torch.empty(rows, dtype=torch.int32, device=dev)
+    if want_status:
+        status = torch.empty(rows, dtype=torch.int32, device=dev)
     if want_stats:
         stats = torch.empty(rows, 4, dtype=torch.float64, device=dev)
     if rows:
         d = _lib.ScoresDesc(*row_fields(_lib.ScoresDesc, logits), _ptr(targets), temperature, top_k, _ptr(lp), _ptr(rank),
                             entropy.data_ptr(), top_ids.data_ptr() if top_k else None, top_lp.data_ptr() if top_k else None,
-                            status.data_ptr(), _ptr(stats))
+                            entropy.data_ptr() if status is None else status.data_ptr(), _ptr(stats))
         lib = _lib.load()
         ref = ctypes.byref(d)
         size = lib.dsv41_scores_workspace_bytes(ref)
-        if size:
+        if status is None:  # (and not the entropies' place, which stood for it)
+            ws = torch.empty(size + 4 * rows, dtype=torch.uint8, device=dev)
+            d.out_status = ws.data_ptr() + size
+        elif size:
             ws = torch.empty(size, dtype=torch.uint8, device=dev)
         launch(lib.dsv41_scores_run, dev, ref, _ptr(ws), size)
     return lp, rank, entropy, top_ids, top_lp, status, stats
@@ -222,7 +227,7 @@ def logit_scores(
     if torch.is_grad_enabled() and logits.requires_grad:
         lp, rank, entropy, top_ids, top_lp, status = _LogitScores.apply(logits, targets, top_k, temperature)
     else:
-        lp, rank, entropy, top_ids, top_lp, status, _ = forward(logits, targets, top_k, temperature, False)
+        lp, rank, entropy, top_ids, top_lp, status, _ = forward(logits, targets, top_k, temperature, False, check)
     if check and any_set(status)[0]:
         _status_error(status)
     return LogitScores(lp, rank, entropy, top_ids, top_lp)
