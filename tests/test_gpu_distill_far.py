@@ -1,0 +1,132 @@
+"""distillation_loss where logits lie far apart: finite masks of any size beside normal logits, and logits whose
+product with the scale fp32 does not hold.
+
+The plain implementation is in 64 bits and in logarithms throughout.  Tolerances as in
+test_gpu_distill.py: a sum over exponentials is off by n 2^-24 relative, n = 32 + V / 512 + 16; the loss by that for
+Q log S and once more for the rest's logarithm, and by the rounding of the result.  Of the gradient outside
+the list, Q p_i takes two such sums and rest w_i (w: p outside the list by itself) one, each with
+the exponent's three roundings, 2^-24 of its size; the result is rounded once to the logits' dtype."""
+
+import math
+
+import pytest
+import torch
+
+from dsv41_rocm import distillation_loss
+
+pytestmark = pytest.mark.gpu
+
+DEV = torch.device("cuda:0")
+H = 2.0 ** -24
+
+
+def plain(x, ids, lq, T, tail):
+    """fp64 on the CPU: (loss, d loss / dx, what its tolerance counts)."""
+    # the call takes its temperature in fp32: 0.3 as 0.3 (1 + 4e-8), two thirds of the 2^-24 that a rounded -q / T may be off by
+    T = torch.tensor(T, dtype=torch.float32).item()
+    z, ids, lq = x.detach().cpu().double() / T, ids.cpu(), lq.cpu().double()
+    named = torch.zeros_like(z, dtype=torch.bool).scatter_(1, ids, True)
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    outside = z.masked_fill(named, -math.inf)
+    lse_out = torch.logsumexp(outside, 1, keepdim=True)
+    if tail == "renormalize":
+        lq = lq - torch.logsumexp(lq, 1, keepdim=True)
+    q = lq.exp()
+    loss = (q * (lq - (z - lse).gather(1, ids))).sum(1)
+    total = q.sum(1, keepdim=True)
+    rest = torch.zeros_like(total)
+    if tail == "rest":
+        rest = 1 - total
+        loss = loss + (rest * (rest.log() - (lse_out - lse)))[:, 0]
+        total = total + rest
+    p, w = (z - lse).exp(), (outside - lse_out).exp()
+    far = (outside - outside.amax(1, keepdim=True)).clamp(-800, 0).abs()
+    grad = (total * p - rest * w).scatter(1, ids, total * p.gather(1, ids) - q)
+    weight = 2 * total * p + rest * w
+    return loss, grad / T, weight * (1 + far) / T
+
+
+def compare(logits, ids, lq, T, tail, g=None):
+    print(f"case: distillation_loss {tuple(logits.shape)} {logits.dtype} T {T} {tail}", flush=True)
+    rows, V = logits.shape
+    g = torch.linspace(1, 2, rows) if g is None else g
+    leaf = logits.detach().requires_grad_()
+    loss = distillation_loss(leaf, ids, lq, temperature=T, tail=tail)
+    (grad,) = torch.autograd.grad(loss, leaf, g.to(DEV))
+    want, slope, weight = plain(logits.float(), ids, lq, T, tail)
+    n = 32 + V / 512 + 16
+    d = (loss.detach().cpu().double() - want).abs()
+    tol = H * (2.1 * n + 4 + 2 * want.abs())
+    assert bool((d <= tol).all()), (loss, want)
+    slope, weight = slope * g.double()[:, None], weight * g.double()[:, None]
+    bound = weight * H * (n + 20) + slope.abs() * torch.finfo(logits.dtype).eps / 2 * 1.01 + 1e-37
+    d = (grad.cpu().double() - slope).abs()
+    assert bool((d <= bound).all()), (d.max(), (d / bound).max())
+    assert torch.equal(distillation_loss(logits, ids, lq, temperature=T, tail=tail), loss.detach())
+
+
+def teacher(rows, V, k, seed):
+    g = torch.Generator().manual_seed(seed)
+    ids = torch.stack([torch.randperm(V, generator=g)[:k] for _ in range(rows)])
+    lq = torch.log_softmax(torch.randn(rows, k, generator=g), 1) + math.log(0.9)
+    return ids, lq.float()
+
+
+FILLS = [-1e4, -1e7, -2e7, -1e9, -1e10, -1e12, -1e20, -1e30, "lowest"]
+
+
+def value_of(fill, dtype):
+    return torch.finfo(dtype).min if fill == "lowest" else fill
+
+
+@pytest.mark.parametrize("tail", ["renormalize", "rest"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("fill", FILLS)
+@pytest.mark.parametrize("V", [9003, 40001])  # one slice a row, several
+def test_finite_masks_beside_normal_logits(V, fill, dtype, tail):
+    # nine tenths of the tokens are masked: whole runs of them at the row's begin and end and within, and others
+    # here and there; in some rows the list's tokens, too, but for one
+    rows, k = 4, 12
+    g = torch.Generator().manual_seed(V)
+    x = 3 * torch.randn(rows, V, generator=g)
+    gone = torch.rand(rows, V, generator=g) < 0.6
+    gone[:, :V // 2] = True
+    gone[:, V - V // 4:] = True
+    gone[1, :16] = False
+    ids, lq = teacher(rows, V, k, V + 1)
+    gone[:2].scatter_(1, ids[:2], False)
+    gone[2:].scatter_(1, ids[2:, :1], False)
+    # (masked tokens of the list are masked for the teacher, too)
+    lq[2:] = torch.where(gone[2:].gather(1, ids[2:]), torch.tensor(-1e38), lq[2:])
+    x = x.masked_fill(gone, value_of(fill, dtype)).to(dtype).to(DEV)
+    for T in (0.3, 0.5, 1.0, 2.0):
+        compare(x[:2], ids[:2].to(DEV), lq[:2].to(DEV), T, tail)
+    # a teacher's -1e38 has no probability: the entry counts for nothing but its place outside the rest
+    there = lq[2:] > -1e30
+    entries = lq[2:].masked_fill(~there, -math.inf).to(DEV)
+    for T in (0.3, 0.5, 1.0, 2.0):
+        loss = distillation_loss(x[2:], ids[2:].to(DEV), entries, temperature=T, tail=tail)
+        masked = x[2:].float().masked_fill(gone[2:].to(DEV), -math.inf)
+        want = distillation_loss(masked, ids[2:].to(DEV), entries, temperature=T, tail=tail)
+        # the masks' probabilities are zero in 64 bits, too, from -1e4 on
+        assert float((loss - want).abs().max()) <= H * (4.2 * (48 + V / 512) + 8 + 4 * float(want.abs().max()))
+
+
+def test_logits_beyond_what_a_product_with_the_scale_holds():
+    # the largest logits, of both signs, and a scale that takes their product out of fp32
+    V, k = 9003, 8
+    ids, lq = teacher(4, V, k, 9)
+    g = torch.Generator().manual_seed(6)
+    x = torch.randn(4, V, generator=g)
+    x[0] += 3e38 * (torch.rand(V, generator=g) < 0.5)
+    x[1] = 2e7 + 2 * torch.randint(-4, 5, (V,), generator=g)
+    x[2] = -2e7 + 2 * torch.randint(-4, 5, (V,), generator=g)
+    x[3, V // 2:] -= 1.1629e7  # (powers of two around -2^24)
+    for tail in ("renormalize", "rest"):
+        for T in (1.0, 0.7):
+            compare(x[1:].to(DEV), ids[1:].to(DEV), lq[1:].to(DEV), T, tail)
+    # (a row whose list lies 3e38 below its rest, or beside it)
+    for tail in ("renormalize", "rest"):
+        for T in (1.0, 1e30):
+            loss = distillation_loss(x[:1].to(DEV), ids[:1].to(DEV), lq[:1].to(DEV), temperature=T, tail=tail, check=False)
+            assert not bool(loss.isnan().any())

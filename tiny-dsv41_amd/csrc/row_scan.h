@@ -10,9 +10,10 @@
 // fp32, which puts the same relative error into every exponent; to first order it is made up for by
 // kappa U, kappa = ln 2 (c - fp32(c)) / fp32(c), which S takes in the end.
 //   For the mass outside a list, S = sum 2^(x c - r) alone: c as a sum of two and one multiply-add for
-// each, so there is nothing to make up for and r may be any number.  Where the largest x c leaves the
-// range that this is safe in (logits all at their type's lowest value, say), the sum is formed again as
-// 2^((x - m) c).
+// each, so there is nothing to make up for.  r is a rounded x c, and what is left of x c - r for that x itself
+// is up to half a step of r and what the second part of c adds: powers of two that the sums bear up to |r| =
+// FAR, and not beyond.  So r begins at -FAR: what lies further down, a mask of any finite size, adds
+// nothing, and where the largest x c is not within FAR, the sum is formed again as 2^((x - m) c).
 //   x = -inf is a masked token: it adds nothing to any sum.  A NaN or +inf makes S NaN.
 #pragma once
 
@@ -342,7 +343,9 @@ __device__ __forceinline__ float next_below(float x) {
   return __uint_as_float(x > 0.f ? b - 1u : b + 1u);
 }
 
-constexpr float SAFE = 1e30f;  // the largest |m c| that x c - r is formed with
+// The largest |r| that x c - r is formed with.  At 2^24, half a step is 1, and the second part of c, at most a step
+// of the first, adds 2: exponents up to 5, with the 2 that a logit may exceed its reference by.
+constexpr float FAR = 0x1p24f;
 
 // One pass over x[from, len) by the workgroup, whose threads take 16 bytes in turn; x is a line's begin, and
 // from below MOST_SKEW.
@@ -360,7 +363,7 @@ __device__ __forceinline__ State scan(const T* x, int from, int len, const Scale
   const int full = len / VEC, n = (len + VEC - 1) / VEC;
   const int tid = threadIdx.x;
   float own[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-  float r = LOWEST, S[2] = {0.f, 0.f}, Us[2] = {0.f, 0.f}, margin = NAMED ? 2.f : sc.margin;
+  float r = NAMED ? -FAR : LOWEST, S[2] = {0.f, 0.f}, Us[2] = {0.f, 0.f}, margin = NAMED ? 2.f : sc.margin;
   asm("" : "+v"(margin));  // (a scalar register short, the compiler would load it in every step)
   int ahead = 0, t = 0;  // (ahead: the wave's count)
   float xt = INFINITY;
@@ -483,7 +486,7 @@ __device__ __forceinline__ State scan(const T* x, int from, int len, const Scale
   met(own);
   s.m = block_max<true>(fmaxf(fmaxf(own[0], own[1]), fmaxf(own[2], own[3])), red);
   double sum[3] = {(double)S[0] + S[1], (double)Us[0] + Us[1], (tid & 63) == 0 ? (double)ahead : 0.0};
-  if (NAMED && fabsf(s.m * sc.c) > SAFE && s.m > -INFINITY) {
+  if (NAMED && fabsf(s.m * sc.c) > FAR && s.m > -INFINITY) {
     sum[0] = 0.0;
     for (int i = from + tid; i < len; i += NT)
       if (!(named[i >> 5] >> (i & 31) & 1)) sum[0] += exp2(((double)Elem<T>::one(x + i) - (double)s.m) * sc.cd);
