@@ -548,7 +548,8 @@ typedef struct dsv41_scores_grad_desc {
  *     temperature do as well); out_loss[r] = sum_k q_k (log q_k - log p_k).
  *   DSV41_TAIL_REST: q_k = exp(teacher_logprob), q_rest = 1 - sum q_k (below 2^-20: 0) and p_rest the
  *     student's mass outside the list; out_loss[r] = sum_k q_k (log q_k - log p_k)
- *     + q_rest (log q_rest - log p_rest).
+ *     + q_rest (log q_rest - log p_rest); p_rest is 0 where no logit outside the list is above the lowest
+ *     value of its type and one in the list is.
  * A row with an empty list: 0, whatever its logits.  An id at or above vocab, a token named
  * twice, teacher log-probs that are none: NaN and a status bit (BAD_TARGET, REPEATED, BAD_TEACHER).
  * A loss that is not finite: DSV41_STATUS_NONFINITE.

@@ -1,5 +1,5 @@
-"""distillation_loss where logits lie far apart: finite masks of any size beside normal logits, and logits whose
-product with the scale fp32 does not hold.
+"""distillation_loss where logits lie far apart: finite masks of any size beside normal logits, a rest of the
+vocabulary that consists of such masks, and a rest many hundreds of nats below the list.
 
 The plain implementation is in 64 bits and in logarithms throughout.  Tolerances as in
 test_gpu_distill.py: a sum over exponentials is off by n 2^-24 relative, n = 32 + V / 512 + 16; the loss by that for
@@ -26,21 +26,24 @@ def plain(x, ids, lq, T, tail):
     T = torch.tensor(T, dtype=torch.float32).item()
     z, ids, lq = x.detach().cpu().double() / T, ids.cpu(), lq.cpu().double()
     named = torch.zeros_like(z, dtype=torch.bool).scatter_(1, ids, True)
-    lse = torch.logsumexp(z, 1, keepdim=True)
+    # (differences first: logits of -1e12 in 64 bits have steps of 1e-4, which a logarithm added to them would drown in)
+    top = z.amax(1, keepdim=True)
+    logp, p = torch.log_softmax(z - top, 1), torch.softmax(z - top, 1)
     outside = z.masked_fill(named, -math.inf)
-    lse_out = torch.logsumexp(outside, 1, keepdim=True)
+    near = outside - outside.amax(1, keepdim=True)
+    w = torch.softmax(near, 1)
+    log_rest = (outside.amax(1, keepdim=True) - top) + torch.logsumexp(near, 1, keepdim=True) - torch.logsumexp(z - top, 1, keepdim=True)
     if tail == "renormalize":
         lq = lq - torch.logsumexp(lq, 1, keepdim=True)
     q = lq.exp()
-    loss = (q * (lq - (z - lse).gather(1, ids))).sum(1)
+    loss = (q * (lq - logp.gather(1, ids))).sum(1)
     total = q.sum(1, keepdim=True)
     rest = torch.zeros_like(total)
     if tail == "rest":
         rest = 1 - total
-        loss = loss + (rest * (rest.log() - (lse_out - lse)))[:, 0]
+        loss = loss + (rest * (rest.log() - log_rest))[:, 0]
         total = total + rest
-    p, w = (z - lse).exp(), (outside - lse_out).exp()
-    far = (outside - outside.amax(1, keepdim=True)).clamp(-800, 0).abs()
+    far = near.clamp(-800, 0).abs()
     grad = (total * p - rest * w).scatter(1, ids, total * p.gather(1, ids) - q)
     weight = 2 * total * p + rest * w
     return loss, grad / T, weight * (1 + far) / T
@@ -110,6 +113,50 @@ def test_finite_masks_beside_normal_logits(V, fill, dtype, tail):
         want = distillation_loss(masked, ids[2:].to(DEV), entries, temperature=T, tail=tail)
         # the masks' probabilities are zero in 64 bits, too, from -1e4 on
         assert float((loss - want).abs().max()) <= H * (4.2 * (48 + V / 512) + 8 + 4 * float(want.abs().max()))
+
+
+@pytest.mark.parametrize("tail", ["renormalize", "rest"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("fill", FILLS[:-1])
+@pytest.mark.parametrize("V", [9003, 40001])
+def test_a_rest_of_finite_masks(V, fill, dtype, tail):
+    # the student leaves the rest nothing but such masks: a divergence as large as their distance
+    rows, k = 3, 12
+    ids, lq = teacher(rows, V, k, V + 2)
+    x = torch.full((rows, V), value_of(fill, dtype))
+    x.scatter_(1, ids, torch.randn(rows, k, generator=torch.Generator().manual_seed(3)))
+    for T in (0.3, 0.5, 1.0, 2.0):
+        compare(x.to(dtype).to(DEV), ids.to(DEV), lq.to(DEV), T, tail)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_rest_at_the_lowest_value_is_masked(dtype):
+    # the lowest value of the logits' type is as good as -inf where all of the rest has it: no mass for the teacher's
+    V, k = 9003, 12
+    ids, lq = (t.to(DEV) for t in teacher(3, V, k, 5))
+    x = torch.full((3, V), torch.finfo(dtype).min, device=DEV)
+    x = x.scatter(1, ids, torch.randn(3, k, device=DEV)).to(dtype)
+    with pytest.raises(ValueError, match="non-finite"):
+        distillation_loss(x, ids, lq, tail="rest")
+    leaf = x.requires_grad_()
+    loss = distillation_loss(leaf, ids, lq, tail="rest", check=False)
+    (grad,) = torch.autograd.grad(loss.sum(), leaf)
+    assert bool((loss == math.inf).all()) and bool(grad.isfinite().all())
+    compare(x.detach(), ids, lq, 1.0, "renormalize")
+
+
+@pytest.mark.parametrize("tail", ["renormalize", "rest"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [3000, 40001])
+def test_a_rest_whose_mass_64_bits_do_not_hold(V, dtype, tail):
+    # 740, 800, 2000 and 20000 nats below the list at this temperature
+    T, k = 0.05, 6
+    ids, lq = teacher(4, V, k, V + 3)
+    g = torch.Generator().manual_seed(4)
+    x = 0.05 * torch.randn(4, V, generator=g)
+    x.scatter_(1, ids, torch.tensor([[37.0], [40.0], [100.0], [1000.0]]) + 0.05 * torch.randn(4, k, generator=g))
+    x = x.to(dtype)
+    compare(x.to(DEV), ids.to(DEV), lq.to(DEV), T, tail)
 
 
 def test_logits_beyond_what_a_product_with_the_scale_holds():

@@ -11,7 +11,8 @@
 // p_rest may be many orders below 1, so S_rest is summed by itself: the list's tokens are bits of a map
 // in LDS that the pass over the row treats as masked.  What is left of nearly cancelling terms, the
 // divergence, is formed in fp64 from the list's logits.  fp32 log-probs do not carry a rest mass below
-// 2^-20, which counts as none.
+// 2^-20, which counts as none.  Where no logit outside the list is above its type's lowest value and the list's
+// are, that value is a mask like -inf: the student has no mass for the teacher's rest.
 //
 // Forward: one read of the row, 4096 bf16 rows of 151936 with 64 entries (a tenth of them without) in
 // 201 us, 5.6 TB/s of what is read: vector instructions, 10 an element; 512 fp32 rows in 56 us, 5.5 TB/s.
@@ -61,6 +62,10 @@ struct Shared {
   double red[4 * WAVES];
   int flags;
 };
+template <typename T>
+constexpr float lowest() {
+  return sizeof(T) == 4 ? -0x1.fffffep127f : -0x1.fep127f;
+}
 constexpr int LIVE = 1 << 16;  // the list has an entry (above the status bits)
 
 // What the gradient needs of a row: p_k = exp((x_k - m) / T) / S in its list; p_i (Q - q_rest / p_rest) =
@@ -149,9 +154,10 @@ __device__ __forceinline__ void finish(const Params& p, int row, State st, int f
   if (p.rest) {
     rest = 1.0 - W;
     if (rest < REST_FLOOR) rest = 0.0;
-    // (the sum against its own largest logit, whose distance from m counts in full; a mass that fp64
-    // does not hold is none)
-    const double log_rest = S_rest > 0.0 ? log(st.S) + ((double)st.m - m) * p.sc.inv_t - ln_s : -(double)INFINITY;
+    // (the sum against its own largest logit, whose distance from m counts in full, also where fp64 does not
+    // hold the mass; a NaN is none above 0, and makes S one)
+    const bool masked = !(st.S > 0.0) || ((double)st.m == (double)lowest<T>() && m > (double)st.m);
+    const double log_rest = masked ? -(double)INFINITY : log(st.S) + ((double)st.m - m) * p.sc.inv_t - ln_s;
     loss = WL - WD + W * ln_s + (rest > 0.0 ? rest * (log(rest) - log_rest) : 0.0);
     Q = W + rest;
   } else {
