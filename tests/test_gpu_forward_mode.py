@@ -48,3 +48,15 @@ def test_a_teacher_with_a_tangent_is_constant():
         for leaf in (logits, logits.clone().requires_grad_()):
             loss = distillation_loss(leaf, ids, dual, tail="rest")
             assert torch.equal(loss.detach(), want) and fwad.unpack_dual(loss).tangent is None
+
+
+def test_upstream_gradients_with_a_tangent_are_refused():
+    logits, ids, lq = inputs()
+    leaf = logits.requires_grad_()
+    with fwad.dual_level():
+        weight = fwad.make_dual(torch.ones(3, device=DEV), torch.ones(3, device=DEV))
+        for out in (logit_scores(leaf, ids[:, 0]).log_probs, logit_scores(leaf).entropy, distillation_loss(leaf, ids, lq),
+                    torch.ops.dsv41_rocm.distillation_loss(leaf, ids, lq, 1.0, "rest")[0],
+                    torch.ops.dsv41_rocm.logit_scores(leaf, None, 2, 1.0)[4][:, 0]):
+            with pytest.raises(NotImplementedError, match="gradients carry a forward-mode"):
+                torch.autograd.grad(out, leaf, weight)

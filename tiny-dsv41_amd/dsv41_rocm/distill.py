@@ -15,7 +15,7 @@ import torch
 from . import _lib
 from ._check import any_set
 from .logprob import first_order
-from .scores import INTEGERS, fit_int32, launch, refuse_capture, row_fields, rows_of_logits, vector
+from .scores import INTEGERS, fit_int32, launch, refuse_capture, refuse_tangents, row_fields, rows_of_logits, vector
 
 STATS = 7  # fp64 values of a row that the backward needs of the forward
 _TAILS = {"renormalize": _lib.TAIL_RENORMALIZE, "rest": _lib.TAIL_REST}
@@ -37,7 +37,8 @@ def prepare(logits, teacher_ids, teacher_log_probs, temperature, tail):
     if teacher_ids.dtype not in INTEGERS:
         raise ValueError("teacher_ids must be integers")
     ids = vector(teacher_ids, torch.int64, shape, device)
-    lq = vector(teacher_log_probs.detach() if teacher_log_probs.requires_grad else teacher_log_probs, torch.float32, shape, device)
+    # (detached also where no gradient is required: a forward-mode tangent ends here too)
+    lq = vector(teacher_log_probs.detach(), torch.float32, shape, device)
     if shape[1] == 0:  # no row has an entry
         ids, lq = ids.new_full((rows, 1), -1), lq.new_zeros(rows, 1)
     return logits, ids, lq
@@ -62,6 +63,7 @@ def forward(logits, ids, lq, temperature, tail, want_stats):
 
 def distillation_backward(logits, ids, lq, temperature, stats, g_loss):
     """dL/dlogits of :func:`distillation_loss`, in the logits' dtype."""
+    refuse_tangents("gradients", g_loss)
     rows, vocab = logits.shape
     out = torch.empty(rows, vocab, dtype=logits.dtype, device=logits.device)
     if rows:
@@ -126,7 +128,8 @@ def distillation_loss(
     student's mass there counts however small it is, and is none where its logits are all -inf or all their
     dtype's lowest value, below the list's.
 
-    Differentiable in ``logits``, once (no second derivatives); the teacher's tensors are constants.
+    Differentiable in ``logits``, once (no second derivatives), and not in forward mode: logits that carry a
+    tangent are refused; the teacher's tensors are constants.
     The gradient is with respect to the logits before the division by ``temperature``; callers that
     keep gradients of several temperatures alike multiply the loss by its square.
 

@@ -15,6 +15,7 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _lib
 from ._check import any_set
@@ -46,11 +47,19 @@ def fit_int32(*sizes) -> None:
         raise NotImplementedError("sizes above 2^31 - 1 are not supported")
 
 
+def refuse_tangents(what, *tensors) -> None:
+    """The kernels would leave them out."""
+    for t in tensors:
+        if t is not None and unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what} carry a forward-mode tangent, for which there is no rule: detach them")
+
+
 def rows_of_logits(logits, temperature):
     """Validated fp32 or bf16 logits [rows, V] whose rows are contiguous."""
     validate_temperature(temperature)
     if not isinstance(logits, torch.Tensor) or logits.ndim != 2 or logits.shape[1] == 0:
         raise ValueError("logits must have shape [rows, vocabulary_size]")
+    refuse_tangents("logits", logits)
     if not logits.is_cuda:
         raise ValueError("logits must be on the GPU (libdsv41hip has no CPU path)")
     fit_int32(*logits.shape)
@@ -153,6 +162,7 @@ def forward(logits, targets, top_k, temperature, want_stats, want_status=True):
 
 def scores_backward(logits, targets, top_ids, temperature, stats, g_log_probs, g_entropy, g_top):
     """dL/dlogits of :func:`logit_scores`, in the logits' dtype; gradients that are None count as zero."""
+    refuse_tangents("gradients", g_log_probs, g_entropy, g_top)
     rows, vocab = logits.shape
     dev = logits.device
     out = torch.empty(rows, vocab, dtype=logits.dtype, device=dev)
@@ -216,7 +226,8 @@ def logit_scores(
     ``top_k`` is at most 1024 and V.
 
     Differentiable in ``logits``: log-probs, entropy and the alternatives' log-probs (with the
-    alternatives held fixed), once (no second derivatives).  A row whose upstream gradients are all zero
+    alternatives held fixed), once (no second derivatives), and not in forward mode: logits that carry a
+    tangent are refused.  A row whose upstream gradients are all zero
     gets zeros.
 
     With ``check`` the call synchronises and raises ``ValueError`` for a target outside the vocabulary,
