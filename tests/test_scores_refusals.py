@@ -1,4 +1,5 @@
-"""Refusals of the operators over rows of logits that need no GPU: forward-mode tangents."""
+"""Refusals of the operators over rows of logits that need no GPU: forward-mode tangents, and teacher lists of
+other than two dimensions."""
 
 import pytest
 import torch
@@ -40,3 +41,15 @@ def test_the_teachers_log_probs_lose_both_kinds_of_derivatives(monkeypatch):
         for t in (fwad.make_dual(lq, torch.ones_like(lq)), lq.clone().requires_grad_()):
             got = distill.prepare(x, ids, t, 1.0, "rest")[2]
             assert not got.requires_grad and fwad.unpack_dual(got).tangent is None
+
+
+def test_lists_of_other_dimensions_are_refused_by_name(monkeypatch):
+    monkeypatch.setattr(distill, "rows_of_logits", lambda logits, temperature: logits)
+    x, ids, lq = torch.zeros(2, 10), torch.zeros(2, 1, dtype=torch.int64), torch.zeros(2, 1)
+    for i, q in ((torch.tensor(3), lq), (ids, torch.tensor(0.5)), (torch.tensor(3), torch.tensor(0.5)), (ids[:, 0], lq[:, 0]),
+                 (ids[None], lq[None])):
+        with pytest.raises(ValueError, match="must have shape \\[rows, entries\\]"):
+            distill.prepare(x, i, q, 1.0, "rest")
+    # the sizes are checked behind the shapes
+    with pytest.raises(NotImplementedError, match="2\\^31"):
+        distill.prepare(x[:1], ids[:1].expand(1, 2 ** 31), lq[:1].expand(1, 2 ** 31), 1.0, "rest")

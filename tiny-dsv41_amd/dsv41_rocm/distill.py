@@ -28,10 +28,10 @@ def prepare(logits, teacher_ids, teacher_log_probs, temperature, tail):
     if tail not in _TAILS:
         raise ValueError("tail must be 'renormalize' or 'rest'")
     shape, device = teacher_ids.shape, logits.device
-    fit_int32(*shape)
     for t in (teacher_ids, teacher_log_probs):
         if t.ndim != 2 or t.shape[0] != rows:
             raise ValueError("teacher_ids and teacher_log_probs must have shape [rows, entries]")
+    fit_int32(*shape)
     if teacher_log_probs.shape != shape:
         raise ValueError("one teacher log probability is required per teacher ID")
     if teacher_ids.dtype not in INTEGERS:
