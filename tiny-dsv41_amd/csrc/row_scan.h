@@ -5,10 +5,14 @@
 // Sums.  With c = log2(e) / T and a reference that a thread raises when it meets a larger logit, a pass
 // keeps sums of exponentials in fp32 over the thread's few hundred elements; the threads' sums are
 // brought to the largest logit and added in fp64.
-//   For scores, S = sum 2^d and U = sum 2^d d with d = (x - r) c.  The difference is what keeps a row with
-// one likely token exact: that token's term is 1, and S - 1 has the others' precision.  c is rounded to
-// fp32, which puts the same relative error into every exponent; to first order it is made up for by
-// kappa U, kappa = ln 2 (c - fp32(c)) / fp32(c), which S takes in the end.
+//   For scores, S = sum 2^d and U = sum 2^d d with d = (x - r) c.  The difference is what lets a certain token
+// score 0: its term is 1 and S is 1, whatever its logit.  Beside a likely token's 1 a thread's two sums, of n / 1024
+// elements each in a row or slice of n, keep the other terms to half a step of 1, so S, and S - 1 with it, is off
+// by n / 1024 times 2^-24 at most: 9e-6 for an uncut row of 151936.  (One token 18 nats above all the others, at
+// -2.3e-3: 2.2e-6.  Sums that are emptied into fp64 ones every two steps have a tenth of that, and cost bf16
+// passes 3 to 4%: 4096 rows 210 us instead of 203.)  c is rounded to fp32, which puts the same relative error
+// into every exponent; to first order it is made up for by kappa U, kappa = ln 2 (c - fp32(c)) / fp32(c), which
+// S takes in the end.
 //   For the mass outside a list, S = sum 2^(x c - r) alone: c as a sum of two and one multiply-add for
 // each, so there is nothing to make up for.  r is a rounded x c, and what is left of x c - r for that x itself
 // is up to half a step of r and what the second part of c adds: powers of two that the sums bear up to |r| =
