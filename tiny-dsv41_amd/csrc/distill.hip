@@ -70,9 +70,10 @@ constexpr int LIVE = 1 << 16;  // the list has an entry (above the status bits)
 
 // What the gradient needs of a row: p_k = exp((x_k - m) / T) / S in its list; p_i (Q - q_rest / p_rest) =
 // others exp((x_i - base) / T) outside, with the largest of these logits as base, since p_rest may lie
-// below what fp32 holds; Q; q_k = exp(lq_k - log_z); whether there is anything to do.
+// below what fp32 holds; Q; q_k = share exp(lq_k - top), with the list's largest lq apart, to which the logarithm of
+// the list's sum may be too small to be added; share is 0 where there is nothing to do.
 struct Stats {
-  double m, S, base, others, Q, log_z, live;
+  double m, S, base, others, Q, top, share;
 };
 static_assert(sizeof(Stats) == STATS * sizeof(double), "the layout of out_stats");
 __device__ __forceinline__ void write_row(const Params& p, int row, float loss, int status, const Stats& st) {
@@ -150,7 +151,7 @@ __device__ __forceinline__ void finish(const Params& p, int row, State st, int f
     write_row(p, row, NAN, DSV41_STATUS_BAD_TEACHER, Stats{NAN, NAN, NAN, NAN, NAN, 0.0, 1.0});
     return;
   }
-  double loss, rest = 0.0, Q = 1.0, log_z = 0.0;
+  double loss, rest = 0.0, Q = 1.0, share = 1.0;
   if (p.rest) {
     rest = 1.0 - W;
     if (rest < REST_FLOOR) rest = 0.0;
@@ -161,11 +162,11 @@ __device__ __forceinline__ void finish(const Params& p, int row, State st, int f
     loss = WL - WD + W * ln_s + (rest > 0.0 ? rest * (log(rest) - log_rest) : 0.0);
     Q = W + rest;
   } else {
-    log_z = top + log(W);
+    share = 1.0 / W;
     loss = (WL - WD) / W - log(W) + ln_s;
   }
   const float l = nonfinite ? NAN : (float)loss;
-  Stats out{m, nonfinite ? (double)NAN : S, m, 0.0, Q, log_z, 1.0};
+  Stats out{m, nonfinite ? (double)NAN : S, m, 0.0, Q, top, share};
   if (st.S != 0.0) {
     out.base = st.m;
     out.others = Q * down / S - (rest > 0.0 ? rest / st.S : 0.0);
@@ -255,7 +256,7 @@ __global__ __launch_bounds__(NT) void distill_grad_kernel(GradParams p) {
   T* out = static_cast<T*>(p.out) + (int64_t)row * p.V + begin;
   const Stats st = reinterpret_cast<const Stats*>(p.stats)[row];
   const double g = (double)p.g[row] * p.sc.inv_t;
-  if (g == 0.0 || st.live == 0.0) {
+  if (g == 0.0 || st.share == 0.0) {
     rows::fill_zero(out, len);
     return;
   }
@@ -264,7 +265,7 @@ __global__ __launch_bounds__(NT) void distill_grad_kernel(GradParams p) {
     const int64_t id = p.ids[(int64_t)row * p.K + k], i = id - begin;
     if (id < 0 || i < 0 || i >= len) return -1;
     const double e = exp(((double)Elem<T>::one(x + id) - st.m) * p.sc.inv_t);
-    v = (float)(g * (st.Q * e / st.S - exp((double)p.lq[(int64_t)row * p.K + k] - st.log_z)));
+    v = (float)(g * (st.Q * e / st.S - st.share * exp((double)p.lq[(int64_t)row * p.K + k] - st.top)));
     return (int)i;
   };
   __shared__ rows::Again again;

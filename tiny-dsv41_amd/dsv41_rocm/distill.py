@@ -125,8 +125,8 @@ def distillation_loss(
     log-probs, so raw logits divided by the temperature do as well); ``"rest"`` takes ``q = exp`` of them
     and compares what is left of the teacher's mass, ``1 - sum q``, with the student's mass outside the
     list as one more outcome (a rest below 2^-20, which fp32 log-probs do not carry, counts as 0).  The
-    student's mass there counts however small it is, and is none where its logits are all -inf or all their
-    dtype's lowest value, below the list's.
+    student's mass there counts however small it is, and is none where its logits are all -inf or all the lowest
+    value of the dtype that the kernel reads (fp32 or bf16), below the list's.
 
     Differentiable in ``logits``, once (no second derivatives), and not in forward mode: logits that carry a
     tangent are refused; the teacher's tensors are constants.
