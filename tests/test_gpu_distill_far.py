@@ -177,3 +177,18 @@ def test_logits_beyond_what_a_product_with_the_scale_holds():
         for T in (1.0, 1e30):
             loss = distillation_loss(x[:1].to(DEV), ids[:1].to(DEV), lq[:1].to(DEV), temperature=T, tail=tail, check=False)
             assert not bool(loss.isnan().any())
+
+
+@pytest.mark.parametrize("tail", ["renormalize", "rest"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("base", [100.0, -5e3, -3e5, 3e5, 2e6, -5e6])
+@pytest.mark.parametrize("V", [9003, 40001])
+def test_logits_that_rise_far_from_zero(V, base, dtype, tail):
+    # every thread raises its reference again and again, where half a step of the reference is up to 1 / 2
+    rows, k = 3, 12
+    ids, lq = teacher(rows, V, k, V + 4)
+    step = 2.0 ** -6 if dtype == torch.float32 else abs(base) * 2.0 ** -8
+    x = torch.linspace(-8, 0, V).expand(rows, V) * max(1.0, 8 * step) + torch.randn(rows, V, generator=torch.Generator().manual_seed(8))
+    x = (x + base).to(dtype)
+    for T in (0.7, 1.0, 2.0):
+        compare(x.to(DEV), ids.to(DEV), lq.to(DEV), T * max(1.0, step), tail)

@@ -420,6 +420,9 @@ __device__ __forceinline__ State scan(const T* x, int from, int len, const Scale
       }
     }
     if constexpr (NAMED) {
+      // (the rounded product in both places: r - tm c in one step would bring the sums to another reference than the
+      // one that is kept, half a step of it apart)
+#pragma clang fp contract(off)
       const float mc = tm * sc.c;
       if (mc > r + margin) {
         const float f = __builtin_amdgcn_exp2f(r - mc);
