@@ -192,3 +192,48 @@ def test_logits_that_rise_far_from_zero(V, base, dtype, tail):
     x = (x + base).to(dtype)
     for T in (0.7, 1.0, 2.0):
         compare(x.to(DEV), ids.to(DEV), lq.to(DEV), T * max(1.0, step), tail)
+
+
+@pytest.mark.parametrize("tail", ["renormalize", "rest"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V,k", [(40, 12), (9003, 12), (9003, 600), (40001, 12), (40001, 700)])
+def test_rows_beyond_the_reference(V, k, dtype, tail):
+    # rows that lie beyond 2^24 powers of two, whose list is above, below and among the rest, and ties with it
+    ids, lq = teacher(6, V, k, V + 5)
+    g = torch.Generator().manual_seed(9)
+    unit = 2.0 if dtype == torch.float32 else 2.0 ** 17  # steps of the type there
+    x = torch.randint(-6, 1, (6, V), generator=g).float() * unit
+    x[1].scatter_(0, ids[1], unit * torch.randint(1, 4, (k,), generator=g).float())
+    x[2].scatter_(0, ids[2], -unit * torch.randint(7, 9, (k,), generator=g).float())
+    x[3].scatter_(0, ids[3], 0.0)
+    x[4, V // 3:] -= 2.0 ** 26  # parts of the row, and with it slices of it, far from the others
+    x[5, :V // 2] += 2.0 ** 26
+    for base in (2.0 ** 25, -(2.0 ** 25), -(2.0 ** 25) - 2.0 ** 30):
+        for T in (1.0, 2.0 * unit):
+            compare((x + base).to(dtype).to(DEV), ids.to(DEV), lq.to(DEV), T, tail)
+
+
+@pytest.mark.parametrize("tail", ["renormalize", "rest"])
+@pytest.mark.parametrize("V", [9003, 40001])
+@pytest.mark.parametrize("base", [-1e9, 3e7])
+def test_no_distribution_beyond_the_reference(V, base, tail):
+    # a NaN or +inf is found in a row whose rest lies there, and a row of masked tokens beside it
+    k = 12
+    ids, lq = teacher(5, V, k, V + 6)
+    x = torch.full((5, V), base)
+    x.scatter_(1, ids, torch.randn(5, k, generator=torch.Generator().manual_seed(3)))
+    spare = (~torch.zeros(5, V, dtype=torch.bool).scatter_(1, ids, True)).nonzero()
+    for row, value in ((1, math.nan), (2, math.inf)):
+        at = spare[spare[:, 0] == row][:, 1]
+        x[row, at[len(at) // 2]] = value
+    x[3] = -math.inf
+    ids, lq = ids.to(DEV), lq.to(DEV)
+    with pytest.raises(ValueError, match="non-finite"):
+        distillation_loss(x.to(DEV), ids, lq, tail=tail)
+    leaf = x.to(DEV).requires_grad_()
+    loss = distillation_loss(leaf, ids, lq, tail=tail, check=False)
+    (grad,) = torch.autograd.grad(loss.sum(), leaf)
+    assert loss.isfinite().tolist() == [True, False, False, False, True]
+    assert bool(loss[1:4].isnan().all()) and bool(grad[1:4].isnan().any(1).all()) and bool(grad[[0, 4]].isfinite().all())
+    keep = [0, 4]
+    compare(x[keep].to(DEV), ids[keep], lq[keep], 1.0, tail)

@@ -17,7 +17,7 @@
 // each, so there is nothing to make up for.  r is a rounded x c, and what is left of x c - r for that x itself
 // is up to half a step of r and what the second part of c adds: powers of two that the sums bear up to |r| =
 // FAR, and not beyond.  So r begins at -FAR: what lies further down, a mask of any finite size, adds
-// nothing, and where the largest x c is not within FAR, the sum is formed again as 2^((x - m) c).
+// nothing.  Where the largest x c is not within FAR, U says so, and S is no sum; below it, S is still NaN for a NaN.
 //   x = -inf is a masked token: it adds nothing to any sum.  A NaN or +inf makes S NaN.
 #pragma once
 
@@ -296,8 +296,8 @@ inline Scale scale_of(float temperature, bool split) {
 // Temperatures whose c or c_lo leave fp32's range are refused.
 inline bool scale_ok(float temperature) { return temperature >= 1e-30f && temperature <= 1e30f; }
 
-// What a slice of a row (or the whole row) adds up to: its largest logit, S and U against it, and how
-// many of its elements come before the target in (logit desc, index asc).
+// What a slice of a row (or the whole row) adds up to: its largest logit, S and U against it (outside a list, U
+// whether m c is beyond FAR), and how many of its elements come before the target in (logit desc, index asc).
 struct State {
   double S, U;
   float m;
@@ -493,11 +493,7 @@ __device__ __forceinline__ State scan(const T* x, int from, int len, const Scale
   met(own);
   s.m = block_max<true>(fmaxf(fmaxf(own[0], own[1]), fmaxf(own[2], own[3])), red);
   double sum[3] = {(double)S[0] + S[1], (double)Us[0] + Us[1], (tid & 63) == 0 ? (double)ahead : 0.0};
-  if (NAMED && fabsf(s.m * sc.c) > FAR && s.m > -INFINITY) {
-    sum[0] = 0.0;
-    for (int i = from + tid; i < len; i += NT)
-      if (!(named[i >> 5] >> (i & 31) & 1)) sum[0] += exp2(((double)Elem<T>::one(x + i) - (double)s.m) * sc.cd);
-  } else if (sum[0] == 0.0) {
+  if (sum[0] == 0.0) {
     sum[1] = 0.0;  // nothing met: its reference means nothing
   } else {
     // as rebase, with v_exp_f32: off by 2^-23 of the thread's share, and exact for the one that holds m
@@ -510,7 +506,7 @@ __device__ __forceinline__ State scan(const T* x, int from, int len, const Scale
   found(s.m);
   block_sums<true>(sum, red + WAVES);
   s.S = sum[0];
-  s.U = sum[1];
+  s.U = NAMED ? (fabsf(s.m * sc.c) > FAR && s.m > -INFINITY) : sum[1];
   s.before = (int32_t)sum[2];
   return s;
 }
