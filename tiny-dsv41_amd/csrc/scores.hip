@@ -15,7 +15,7 @@
 // A row of few is cut into slices, which leave their sums and their sorted lists in the workspace for a
 // second kernel.
 //
-// What bounds it.  4096 fp32 rows of 151936 with 64 alternatives take 379 us, 6.6 TB/s (7.0 is what
+// What bounds it.  4096 fp32 rows of 151936 with 64 alternatives take 379-383 us, 6.5 TB/s (7.0 is what
 // nontemporal reads reach): memory, and the selections, which fall together on the workgroups of a CU.
 // 1000 bf16 rows of 129280 with ranks take 50 us, 5.2 TB/s: 10.8 vector instructions an element, of which
 // the exponential counts twice.  A single row, 7.3 us and 4.6 to join, is a chain of latencies.
@@ -272,8 +272,8 @@ __device__ __forceinline__ void search(uint32_t& lo, uint32_t& hi, int& c, int K
 // largest of the shares' maxima is such a bound, and few more groups than K reach it where K is at most
 // half of the shares: in rows of no special order, 68 groups the 64th of 512, 710 the 512th of 1024.
 // Up to K = 256 one wave searches among the 512 threads' maxima by itself, without a barrier, while the
-// others join their sums (one row's top 5: 7.4 us instead of 8.7; 48 rows' top 20: 18.3 instead of 22.6);
-// above, all search among 1024 or 2048 (search_shares).
+// others join their sums (both launches of one row's top 5: 11.3 us instead of 13.9; of 48 rows' top 20: 15.9 instead
+// of 19.3; 4096 bf16 rows' top 64: 225 instead of 231); above, all search among 1024 or 2048 (search_shares).
 constexpr int ALONE = NT / 2;
 __device__ __forceinline__ void met_shares(Shared& s, const float (&own)[4], int K) {
   if (K <= ALONE) s.bucket[threadIdx.x] = __float_as_int(fmaxf(fmaxf(own[0], own[1]), fmaxf(own[2], own[3])));
