@@ -35,7 +35,10 @@
  *   dsv41_scores_run   <- an engine's logprobs output, of which rollout_manager/backends/
  *                         vllm_actor.py:260 takes the sampled token's: over rows of logits at hand,
  *                         with ranks, entropies and alternatives; dsv41_scores_grad_run is its gradient.
- * dsv41_distill_run and dsv41_distill_grad_run (divergence from a teacher's top tokens) replace nothing.
+ * dsv41_distill_run and dsv41_distill_grad_run (divergence from a teacher's top tokens) replace nothing,
+ * nor do dsv41_process_run (penalties, biases and token masks as rows of logits), dsv41_int_head_run (the
+ * head's product in 8-bit integers) and dsv41_embed_run (rows of a token table), with the gradients of the
+ * first and the last.
  */
 #ifndef DSV41_ROCM_H
 #define DSV41_ROCM_H
@@ -76,6 +79,12 @@ extern "C" {
 #define DSV41_STATUS_BAD_TEACHER 128 /* teacher log-probs NaN or +inf, or without mass  */
                                    /* to renormalize, or with more than 1.01 beside a   */
                                    /* rest (loss NaN)                                   */
+
+#define DSV41_STATUS_BAD_PENALTY 256 /* a row's repetition penalty is not finite and        */
+                                     /* positive, or another one not finite (row NaN)       */
+#define DSV41_STATUS_BAD_BIAS 512    /* a biased id was >= vocab (entry ignored)            */
+#define DSV41_STATUS_BAD_MASK 1024   /* mask_rows names no mask (row NaN)                   */
+#define DSV41_STATUS_NO_TOKEN 2048   /* the row's mask leaves no token                      */
 
 /*
  * Row sampler.  For each row r of logits[rows, vocab]:
@@ -593,6 +602,124 @@ typedef struct dsv41_distill_grad_desc {
   void* out;                 /* [rows, vocab], rows vocab elements apart */
 } dsv41_distill_grad_desc;
 
+/*
+ * Biases, penalties and token masks on rows of logits, the result as rows of logits again.  Element i of
+ * row r, in fp32 with every step rounded, as dsv41_sampler_run rounds its penalties:
+ *   x = float(logit);  x = x + bias  (for an id of the row's bias list; the last entry of an id counts);
+ *   for ids in the row's history (c = count, see history_prompt_lens of dsv41_sampler_desc):
+ *     x = x > 0 ? x / repetition_penalty : x * repetition_penalty;
+ *     x = x - frequency_penalty * c;  if (c > 0) x = x - presence_penalty;
+ *   x = fill where the row's mask holds a 0 bit; rounded to the logits' type.
+ * Knobs are those of the whole batch, or of each row where the arrays are given.  A row whose knobs are
+ * neutral does not read its history.  Negative ids, of the history or of a bias list, are no entries.
+ * Bit i % 32 of word i / 32 of a mask says whether token i is allowed; bits past the vocabulary are ignored.
+ * mask_rows[r] names the row's mask, a negative one none; without mask_rows there is one mask for all
+ * rows, or one per row.
+ * out == logits: in place; only biased, penalized and masked elements are written.
+ * dsv41_process_grad_run: out[r, i] = grad[r, i] times 0 where the mask holds a 0 bit, times
+ * (x + bias > 0 ? 1 / repetition_penalty : repetition_penalty) for ids of the history, or 1.  It reads
+ * logits only there, does not write in place and reports no status.
+ */
+typedef struct dsv41_process_desc {
+  uint32_t struct_size; /* = sizeof(dsv41_process_desc) */
+  int32_t rows;
+  int32_t vocab;             /* at most 2^21 */
+  int32_t logits_dtype;      /* DSV41_DTYPE_F32 or DSV41_DTYPE_BF16 */
+  int64_t logits_row_stride; /* in elements, >= vocab, or 0: every row the same */
+  const void* logits;        /* [rows, vocab] */
+  const int64_t* history;    /* [rows, history_row_stride] or NULL */
+  int64_t history_row_stride;
+  int32_t hist_len;            /* ids per row, at most 524287; with history_lens the most */
+  const int32_t* history_lens; /* [rows] or NULL; values outside [0, hist_len] are brought there */
+  const int32_t* history_prompt_lens; /* [rows] or NULL: leading history entries of the prompt */
+  float repetition_penalty;  /* finite, > 0; 1 = off */
+  float presence_penalty;    /* finite; 0 = off */
+  float frequency_penalty;   /* finite; 0 = off */
+  const float* repetition_penalties; /* [rows] or NULL */
+  const float* presence_penalties;   /* [rows] or NULL */
+  const float* frequency_penalties;  /* [rows] or NULL */
+  const int64_t* bias_ids;   /* [rows, bias_row_stride] or NULL */
+  const float* bias;         /* the same shape */
+  int64_t bias_row_stride;   /* in elements; 0: one list for all rows */
+  int32_t bias_len;          /* entries per row, at most 4095 */
+  int32_t masks;             /* rows of mask */
+  const int32_t* mask;       /* [masks, mask_row_stride] or NULL */
+  int64_t mask_row_stride;   /* in words */
+  const int32_t* mask_rows;  /* [rows] or NULL */
+  float fill;                /* not NaN */
+  void* out;                 /* [rows, vocab], in the logits' type */
+  int64_t out_row_stride;    /* in elements, >= vocab */
+  int32_t* out_status;       /* [rows] or NULL */
+  const void* grad;          /* dsv41_process_grad_run: [rows, vocab], in the logits' type */
+  int64_t grad_row_stride;   /* in elements, >= vocab, or 0 */
+} dsv41_process_desc;
+
+/*
+ * Logits of an 8-bit head.  A row x of hidden states becomes q_k = rint(127 x_k / a), a = max |x|, with the
+ * scale a / 127 in fp32, and
+ *   out[n, v] = (sum_k q[n, k] w[v, k]) * scale of row n * scales[v],
+ * the sum exact in integers, the products in fp32, rounded to out's type.  A row with a NaN or an infinity
+ * gives NaN and DSV41_STATUS_NONFINITE.
+ */
+typedef struct dsv41_int_head_desc {
+  uint32_t struct_size; /* = sizeof(dsv41_int_head_desc) */
+  int32_t n_tokens;
+  int32_t hidden;         /* at most 133120 */
+  int32_t vocab;
+  const void* x;          /* bf16 [n_tokens, hidden] */
+  int64_t x_row_stride;   /* in elements */
+  const int8_t* w;        /* [vocab, w_row_stride], as dsv41_quantize_rows_run leaves rows: 16-byte aligned;
+                             the columns from hidden to the next multiple of 128 are read, whatever they hold */
+  int64_t w_row_stride;   /* in elements, a multiple of 128 */
+  const float* scales;    /* [vocab], 16-byte aligned */
+  void* out;              /* [n_tokens, vocab] */
+  int64_t out_row_stride; /* in elements; rows that begin at multiples of 4 elements are written faster */
+  int32_t out_dtype;      /* DSV41_DTYPE_F32 or DSV41_DTYPE_BF16 */
+  int32_t* out_status;    /* [n_tokens] or NULL */
+} dsv41_int_head_desc;
+
+/*
+ * Rows of a token table: out[n, :] = scale * weight[ids[n], :], the product in fp32, rounded to the table's
+ * type.  A negative id is padding: zeros.  An id at or above vocab: NaN and DSV41_STATUS_BAD_TARGET.
+ */
+typedef struct dsv41_embed_desc {
+  uint32_t struct_size; /* = sizeof(dsv41_embed_desc) */
+  int32_t n_tokens;
+  int32_t hidden;
+  int32_t vocab;
+  const void* weight;        /* [vocab, hidden] */
+  int64_t weight_row_stride; /* in elements */
+  const int64_t* ids;        /* [n_tokens] */
+  float scale;
+  int32_t dtype;             /* DSV41_DTYPE_F32 or DSV41_DTYPE_BF16, of weight and out */
+  void* out;                 /* [n_tokens, hidden] */
+  int64_t out_row_stride;    /* in elements */
+  int32_t* out_status;       /* [n_tokens] or NULL */
+} dsv41_embed_desc;
+
+/*
+ * Gradient of dsv41_embed_run with respect to the table: out[v, :] = scale * sum of grad[n, :] over the n with
+ * ids[n] == v, summed in fp32, rounded once; zeros where there is none.  accumulate != 0: that is added to
+ * what out holds (in fp32, rounded once), and rows of tokens that do not occur are neither read nor
+ * written.  Ids outside [0, vocab) take no part.  The result does not depend on the order in which
+ * workgroups run.
+ */
+typedef struct dsv41_embed_grad_desc {
+  uint32_t struct_size; /* = sizeof(dsv41_embed_grad_desc) */
+  int32_t n_tokens;
+  int32_t hidden;
+  int32_t vocab;
+  const int64_t* ids;      /* [n_tokens] */
+  const void* grad;        /* [n_tokens, hidden] */
+  int64_t grad_row_stride; /* in elements, >= hidden, or 0: every row the same */
+  int32_t grad_dtype;
+  float scale;
+  void* out;               /* [vocab, hidden] */
+  int64_t out_row_stride;  /* in elements */
+  int32_t out_dtype;
+  int32_t accumulate;
+} dsv41_embed_grad_desc;
+
 /* ABI identity. */
 int dsv41_abi_version(void);
 size_t dsv41_sampler_desc_size(void);
@@ -610,6 +737,10 @@ size_t dsv41_scores_desc_size(void);
 size_t dsv41_scores_grad_desc_size(void);
 size_t dsv41_distill_desc_size(void);
 size_t dsv41_distill_grad_desc_size(void);
+size_t dsv41_process_desc_size(void);
+size_t dsv41_int_head_desc_size(void);
+size_t dsv41_embed_desc_size(void);
+size_t dsv41_embed_grad_desc_size(void);
 const char* dsv41_last_error(void);
 
 /* Sampler: replaces rollout.py:144-150 for a [rows, vocab] batch.
@@ -711,6 +842,30 @@ size_t dsv41_distill_workspace_bytes(const dsv41_distill_desc* desc);
 int dsv41_distill_run(const dsv41_distill_desc* desc, void* workspace, size_t workspace_bytes,
                       void* stream /* hipStream_t */);
 int dsv41_distill_grad_run(const dsv41_distill_grad_desc* desc, void* stream /* hipStream_t */);
+
+/* Biases, penalties and token masks on rows of logits, and the gradient (no workspace). */
+int dsv41_process_run(const dsv41_process_desc* desc, void* stream /* hipStream_t */);
+int dsv41_process_grad_run(const dsv41_process_desc* desc, void* stream /* hipStream_t */);
+
+/* Rows of bf16 as 8-bit integers with a scale each, as dsv41_int_head_desc says (weights are laid out
+ * with it once): q [rows, qs], 16-byte aligned, qs a multiple of 16 that holds the columns padded to a
+ * multiple of 128, the padding zeros; strides in elements.  A row with a NaN or an infinity: zeros, the scale NaN and
+ * DSV41_STATUS_NONFINITE in status (which may be NULL). */
+int dsv41_quantize_rows_run(const void* x, int64_t xs, int rows, int cols, int8_t* q, int64_t qs, float* scales,
+                            int32_t* status, void* stream /* hipStream_t */);
+
+/* Logits of an 8-bit head.  Workspace (16-byte aligned, contents need no initialisation): the quantized
+ * hidden states, n_tokens rounded up to 16 times hidden rounded up to 128 bytes, and their scales. */
+size_t dsv41_int_head_workspace_bytes(const dsv41_int_head_desc* desc);
+int dsv41_int_head_run(const dsv41_int_head_desc* desc, void* workspace, size_t workspace_bytes,
+                       void* stream /* hipStream_t */);
+
+/* Rows of a token table, and the table's gradient.  Workspace of the gradient (16-byte aligned, contents need
+ * no initialisation): the sorted tokens, and two rows of fp32 sums per 32 tokens. */
+int dsv41_embed_run(const dsv41_embed_desc* desc, void* stream /* hipStream_t */);
+size_t dsv41_embed_grad_workspace_bytes(const dsv41_embed_grad_desc* desc);
+int dsv41_embed_grad_run(const dsv41_embed_grad_desc* desc, void* workspace, size_t workspace_bytes,
+                         void* stream /* hipStream_t */);
 
 /* What a checked call asks after its launches: returns 1 when some of the n statuses is
  * nonzero, plus 2 when some of the n_ids ids lies outside [0, limit) (0: neither), or a negative

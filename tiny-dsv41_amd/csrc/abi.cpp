@@ -28,4 +28,8 @@ extern "C" size_t dsv41_scores_desc_size(void) { return sizeof(dsv41_scores_desc
 extern "C" size_t dsv41_scores_grad_desc_size(void) { return sizeof(dsv41_scores_grad_desc); }
 extern "C" size_t dsv41_distill_desc_size(void) { return sizeof(dsv41_distill_desc); }
 extern "C" size_t dsv41_distill_grad_desc_size(void) { return sizeof(dsv41_distill_grad_desc); }
+extern "C" size_t dsv41_process_desc_size(void) { return sizeof(dsv41_process_desc); }
+extern "C" size_t dsv41_int_head_desc_size(void) { return sizeof(dsv41_int_head_desc); }
+extern "C" size_t dsv41_embed_desc_size(void) { return sizeof(dsv41_embed_desc); }
+extern "C" size_t dsv41_embed_grad_desc_size(void) { return sizeof(dsv41_embed_grad_desc); }
 extern "C" const char* dsv41_last_error(void) { return dsv41::g_last_error.c_str(); }

@@ -1,0 +1,434 @@
+// embed.hip — rows of a table by token ids, scaled, and the gradient of the table.
+//
+//   out[n, :] = scale w[ids[n], :]                        (fp32 product, rounded once)
+//   dw[v, :]  = scale sum over n with ids[n] = v of g[n, :]   (fp32 sums in the order of the batch)
+//
+// Negative ids are padding: rows of zeros, and no part in the gradient.
+//
+// The gradient in three kernels, none of which adds into memory that another writes, so its bits do not
+// depend on the order in which workgroups run:
+//   sort_kernel   the batch's positions ordered by (id, position).  A workgroup owns RANGE ids and reads all
+//                 ids of the batch (from its L2): it counts its own, wave by wave, and how many lie below
+//                 its range, so it knows where its part of the sorted list begins without hearing from the
+//                 others; then each wave places its tokens in their order.
+//   sum_kernel    a chunk of CHUNK positions of the sorted list at a time, a strip of the columns: rows of
+//                 g summed while the id stays the same.  An id whose tokens all lie within the chunk is
+//                 finished there; one that reaches over its ends leaves a partial row.  Other workgroups
+//                 of the same launch write zeros where no token is.
+//   join_kernel   the partial rows of an id that reaches over chunks, in their order.
+
+#include <math.h>
+
+#include <algorithm>
+
+#include "row_scan.h"
+
+namespace dsv41 {
+namespace embed {
+
+using rows::bf16_t;
+using rows::Elem;
+
+constexpr int COPY_NT = 256;
+constexpr int SORT_NT = 1024, SORT_WAVES = SORT_NT / 64;
+constexpr int RANGE = 512;    // ids of a sorting workgroup
+constexpr int SUM_NT = 128;
+constexpr int CHUNK = 32;     // sorted positions of a summing workgroup
+constexpr int ZERO_ROWS = 8;  // rows of the table that a zeroing workgroup looks at
+constexpr int64_t MAX_GRID = 1 << 22;
+
+template <typename T>
+__device__ __forceinline__ void load_group(const T* p, int n, float (&v)[Elem<T>::VEC]) {
+  constexpr int G = Elem<T>::VEC;
+  uint32_t w[4] = {0, 0, 0, 0};
+  if (n >= G) {
+    rows::load16<false>(p, w);
+  } else {
+#pragma unroll
+    for (int j = 0; j < G; ++j)
+      if (j < n) Elem<T>::put(w, j, p[j]);
+  }
+  Elem<T>::unpack(w, v);
+}
+
+struct CopyParams {
+  const void* w;
+  int64_t ws;
+  const int64_t* ids;
+  int n, H, V;
+  float scale;
+  void* out;
+  int64_t os;
+  int32_t* status;
+  int lanes;  // threads of a row, a power of two
+};
+
+template <typename T>
+__global__ __launch_bounds__(COPY_NT) void copy_kernel(CopyParams p) {
+  constexpr int G = Elem<T>::VEC;
+  const int per = COPY_NT / p.lanes, lane = threadIdx.x % p.lanes;
+  const int64_t n = (int64_t)blockIdx.x * per + threadIdx.x / p.lanes;
+  if (n >= p.n) return;
+  const int64_t id = p.ids[n];
+  const bool bad = id >= p.V;
+  if (p.status && lane == 0) p.status[n] = bad ? DSV41_STATUS_BAD_TARGET : 0;
+  const float instead = bad ? __builtin_nanf("") : 0.f;
+  const bool some = id >= 0 && !bad;
+  const T* w = static_cast<const T*>(p.w) + (some ? id * p.ws : 0);
+  T* out = static_cast<T*>(p.out) + n * p.os;
+  for (int i = lane * G; i < p.H; i += p.lanes * G) {
+    float v[G];
+    if (some) load_group(w + i, p.H - i, v);
+#pragma unroll
+    for (int j = 0; j < G; ++j) v[j] = some ? v[j] * p.scale : instead;
+    if (p.H - i >= G) {
+      rows::store_full(out + i, 0, v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < G; ++j)
+        if (i + j < p.H) rows::store_one(out + i + j, v[j]);
+    }
+  }
+}
+
+struct GradParams {
+  const int64_t* ids;
+  int n, H, V;
+  const void* g;
+  int64_t gs;
+  float scale;
+  void* out;
+  int64_t os;
+  int ranges, chunks, strips, zeros;
+  int32_t* total;     // [1] tokens with a row
+  int32_t* place;     // [n] positions sorted by (id, position)
+  int32_t* name;      // [n] their ids
+  uint32_t* present;  // [(V + 31) / 32] ids that some token has
+  float* part;        // [chunks, 2, H]: of the id that reaches into the chunk, and of the one that reaches beyond
+};
+
+__global__ __launch_bounds__(SORT_NT) void sort_kernel(GradParams p) {
+  __shared__ uint32_t hist[SORT_WAVES][RANGE];
+  __shared__ uint32_t sums[SORT_WAVES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t r0 = (int64_t)blockIdx.x * RANGE;
+  const uint64_t width = (uint64_t)min((int64_t)RANGE, p.V - r0);
+  const int per = ((p.n + SORT_WAVES - 1) / SORT_WAVES + 63) / 64 * 64;
+  const int from = min(p.n, wave * per), to = min(p.n, from + per);
+  for (int i = tid; i < SORT_WAVES * RANGE; i += SORT_NT) (&hist[0][0])[i] = 0;
+  __syncthreads();
+  uint32_t below = 0;
+  for (int i = from + lane; i < to; i += 64) {
+    const int64_t id = p.ids[i];
+    const uint64_t at = (uint64_t)(id - r0);
+    if (id >= 0 && id < r0) ++below;
+    if (id >= 0 && at < width) atomicAdd(&hist[wave][at], 1u);
+  }
+  below = (uint32_t)wave_sum_i((int)below);
+  if (lane == 0) sums[wave] = below;
+  __syncthreads();
+  uint32_t base = 0;
+  for (int w = 0; w < SORT_WAVES; ++w) base += sums[w];
+  __syncthreads();
+  // starts: exclusive over (id, wave)
+  uint32_t mine = 0;
+  if (tid < RANGE)
+    for (int w = 0; w < SORT_WAVES; ++w) mine += hist[w][tid];
+  const uint32_t upto = wave_incl_scan_u32(mine);
+  if (lane == 63) sums[wave] = upto;
+  __syncthreads();
+  uint32_t start = base + upto - mine;
+  for (int w = 0; w < wave; ++w) start += sums[w];
+  if (tid < RANGE) {
+    uint32_t s = start;
+    for (int w = 0; w < SORT_WAVES; ++w) {
+      const uint32_t c = hist[w][tid];
+      hist[w][tid] = s;
+      s += c;
+    }
+    const uint64_t some = __ballot(mine != 0);
+    const int word = (int)(r0 / 32) + tid / 32;
+    if ((tid & 31) == 0 && word < (p.V + 31) / 32) p.present[word] = (uint32_t)(some >> (tid & 32));
+    if (tid == RANGE - 1 && blockIdx.x == gridDim.x - 1) *p.total = (int32_t)s;
+  }
+  __syncthreads();
+  for (int b = from; b < to; b += 64) {
+    const int i = b + lane;
+    const int64_t id = i < to ? p.ids[i] : -1;
+    const uint64_t at = (uint64_t)(id - r0);
+    const bool in = id >= 0 && at < width;
+    uint64_t left = __ballot(in);
+    while (left) {
+      // the tokens of this batch of 64 that share the first one's id take consecutive places
+      const int first = __builtin_ctzll(left);
+      const uint32_t which = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)at, first);
+      const uint64_t same = __ballot(in && (uint32_t)at == which) & left;
+      uint32_t s = 0;
+      if (lane == first) s = atomicAdd(&hist[wave][which], (uint32_t)__popcll(same));
+      s = (uint32_t)__builtin_amdgcn_readlane((int)s, first);
+      if (same >> lane & 1) {
+        const uint32_t to_place = s + (uint32_t)__popcll(same & ((1ull << lane) - 1));
+        p.place[to_place] = i;
+        p.name[to_place] = (int32_t)id;
+      }
+      left &= ~same;
+    }
+  }
+}
+
+// G columns of a finished row, of which the first n exist
+template <typename T, bool ONTO, int G>
+__device__ __forceinline__ void finish(T* out, int n, const float (&s)[G], float scale) {
+  constexpr int GO = Elem<T>::VEC;
+  n = min(n, G);
+#pragma unroll
+  for (int b = 0; b < G; b += GO) {
+    float v[GO];
+    if (ONTO) load_group(out + b, n - b, v);
+#pragma unroll
+    for (int j = 0; j < GO; ++j) {
+      const float sum = b + j < G ? s[b + j < G ? b + j : 0] * scale : 0.f;
+      v[j] = ONTO ? v[j] + sum : sum;
+    }
+    if (n - b >= GO) {
+      rows::store_full(out + b, 0, v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < GO; ++j)
+        if (b + j < n) rows::store_one(out + b + j, v[j]);
+    }
+  }
+}
+
+template <typename TG, typename TO, bool ONTO>
+__global__ __launch_bounds__(SUM_NT) void sum_kernel(GradParams p) {
+  constexpr int G = Elem<TG>::VEC;
+  const int tid = threadIdx.x;
+  TO* out = static_cast<TO*>(p.out);
+  const int64_t sums = (int64_t)p.chunks * p.strips;
+  if ((int64_t)blockIdx.x >= sums) {
+    // rows that no token has
+    const int64_t v0 = ((int64_t)blockIdx.x - sums) * ZERO_ROWS;
+    constexpr int GO = Elem<TO>::VEC;
+    float zero[GO];
+#pragma unroll
+    for (int j = 0; j < GO; ++j) zero[j] = 0.f;
+    for (int k = 0; k < ZERO_ROWS; ++k) {
+      const int64_t v = v0 + k;
+      if (v >= p.V || p.present[v >> 5] >> (v & 31) & 1) continue;
+      TO* row = out + v * p.os;
+      for (int i = tid * GO; i < p.H; i += SUM_NT * GO) {
+        if (p.H - i >= GO) {
+          rows::store_full(row + i, 0, zero);
+        } else {
+          for (int j = 0; i + j < p.H; ++j) rows::store_one(row + i + j, 0.f);
+        }
+      }
+    }
+    return;
+  }
+  const int total = *p.total;
+  const int chunk = (int)(blockIdx.x / p.strips), strip = (int)(blockIdx.x % p.strips);
+  const int c0 = chunk * CHUNK, c1 = min(c0 + CHUNK, total);
+  const int col = (strip * SUM_NT + tid) * G;
+  if (c0 >= total || col >= p.H) return;
+  const int n = p.H - col;
+  const TG* g = static_cast<const TG*>(p.g) + col;
+  float s[G];
+#pragma unroll
+  for (int j = 0; j < G; ++j) s[j] = 0.f;
+  bool reaches_in = c0 > 0 && p.name[c0 - 1] == p.name[c0];
+  constexpr int U = 8;
+  for (int c = c0; c < c1; c += U) {
+    float v[U][G];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (c + u < c1) load_group(g + p.place[c + u] * p.gs, n, v[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = c + u;
+      if (at >= c1) break;
+#pragma unroll
+      for (int j = 0; j < G; ++j) s[j] += v[u][j];
+      const int id = p.name[at];
+      const bool more = at + 1 < total && p.name[at + 1] == id;
+      if (more && at + 1 < c1) continue;
+      if (reaches_in || more) {
+        float* part = p.part + ((int64_t)chunk * 2 + (reaches_in ? 0 : 1)) * p.H + col;
+#pragma unroll
+        for (int j = 0; j < G; ++j)
+          if (j < n) part[j] = s[j];
+      } else {
+        finish<TO, ONTO, G>(out + id * p.os + col, n, s, p.scale);
+      }
+      reaches_in = false;
+#pragma unroll
+      for (int j = 0; j < G; ++j) s[j] = 0.f;
+    }
+  }
+}
+
+template <typename TO, bool ONTO>
+__global__ __launch_bounds__(SUM_NT) void join_kernel(GradParams p) {
+  constexpr int G = 4;
+  const int total = *p.total;
+  const int chunk = (int)(blockIdx.x / p.strips), strip = (int)(blockIdx.x % p.strips);
+  const int c1 = (chunk + 1) * CHUNK;
+  if (c1 >= total) return;
+  const int id = p.name[c1];
+  if (p.name[c1 - 1] != id) return;                                   // nothing reaches beyond this chunk,
+  if (chunk > 0 && p.name[chunk * CHUNK] == id && p.name[chunk * CHUNK - 1] == id) return;  // or not from here
+  const int col = (strip * SUM_NT + threadIdx.x) * G;
+  if (col >= p.H) return;
+  const int n = min(G, p.H - col);
+  float s[G] = {0.f, 0.f, 0.f, 0.f};
+  const float* part = p.part + ((int64_t)chunk * 2 + 1) * p.H + col;
+  for (int j = 0; j < n; ++j) s[j] = part[j];
+  for (int c = chunk + 1; c * CHUNK < total && p.name[c * CHUNK] == id; ++c) {
+    part = p.part + (int64_t)c * 2 * p.H + col;
+    for (int j = 0; j < n; ++j) s[j] += part[j];
+  }
+  TO* out = static_cast<TO*>(p.out) + id * p.os + col;
+  for (int j = 0; j < n; ++j) rows::store_one(out + j, ONTO ? Elem<TO>::one(out + j) + s[j] * p.scale : s[j] * p.scale);
+}
+
+int check_sizes(int dtype, int n, int h, int v) {
+  if (n < 0 || h <= 0 || v <= 0) return fail(DSV41_E_INVALID, "the table must have shape [vocabulary_size, hidden]");
+  if (dtype != DSV41_DTYPE_F32 && dtype != DSV41_DTYPE_BF16) return fail(DSV41_E_INVALID, "the table must be fp32 or bf16");
+  return DSV41_OK;
+}
+
+struct Plan {
+  int64_t ranges, chunks, strips, join_strips, zeros;
+  size_t place, name, present, part, bytes;  // offsets into the workspace (the total is at its begin)
+};
+
+Plan plan(const dsv41_embed_grad_desc* d) {
+  Plan q{};
+  const int g = d->grad_dtype == DSV41_DTYPE_F32 ? 4 : 8;
+  q.ranges = ((int64_t)d->vocab + RANGE - 1) / RANGE;
+  q.chunks = ((int64_t)d->n_tokens + CHUNK - 1) / CHUNK;
+  q.strips = ((int64_t)d->hidden + SUM_NT * g - 1) / (SUM_NT * g);
+  q.join_strips = ((int64_t)d->hidden + SUM_NT * 4 - 1) / (SUM_NT * 4);
+  q.zeros = d->accumulate ? 0 : ((int64_t)d->vocab + ZERO_ROWS - 1) / ZERO_ROWS;
+  auto up = [](size_t b) { return (b + 255) / 256 * 256; };
+  q.place = 256;
+  q.name = q.place + up((size_t)d->n_tokens * 4);
+  q.present = q.name + up((size_t)d->n_tokens * 4);
+  q.part = q.present + up((size_t)(d->vocab + 31) / 32 * 4);
+  q.bytes = q.part + (size_t)q.chunks * 2 * d->hidden * 4;
+  return q;
+}
+
+int check_grad(const dsv41_embed_grad_desc* d) {
+  if (!d) return fail(DSV41_E_INVALID, "embedding gradient descriptor is NULL");
+  if (d->struct_size != sizeof(dsv41_embed_grad_desc))
+    return fail(DSV41_E_ABI, "dsv41_embed_grad_desc size mismatch (rebuild the binding)");
+  if (int rc = check_sizes(d->out_dtype, d->n_tokens, d->hidden, d->vocab)) return rc;
+  if (int rc = check_sizes(d->grad_dtype, d->n_tokens, d->hidden, d->vocab)) return rc;
+  if (!d->out || (d->n_tokens > 0 && (!d->ids || !d->grad))) return fail(DSV41_E_INVALID, "ids, grad and out are required");
+  if (d->out_row_stride < d->hidden || (d->grad_row_stride != 0 && d->grad_row_stride < d->hidden))
+    return fail(DSV41_E_INVALID, "embedding gradient: row strides must cover the rows");
+  if ((uintptr_t)d->grad % (d->grad_dtype == DSV41_DTYPE_F32 ? 4 : 2) || (uintptr_t)d->out % (d->out_dtype == DSV41_DTYPE_F32 ? 4 : 2))
+    return fail(DSV41_E_INVALID, "embedding gradient: operands are not aligned to their type");
+  const Plan q = plan(d);
+  if (q.chunks * q.join_strips + q.zeros > MAX_GRID || q.chunks * q.strips + q.zeros > MAX_GRID || q.ranges >= MAX_GRID)
+    return fail(DSV41_E_UNSUPPORTED, "embedding gradient: the batch is too large for one call");
+  return DSV41_OK;
+}
+
+template <typename TG, typename TO, bool ONTO>
+void launch(GradParams p, const Plan& q, hipStream_t s) {
+  hipLaunchKernelGGL((sum_kernel<TG, TO, ONTO>), dim3((unsigned)(q.chunks * q.strips + q.zeros)), dim3(SUM_NT), 0, s, p);
+  if (q.chunks > 1) {
+    p.strips = (int)q.join_strips;
+    hipLaunchKernelGGL((join_kernel<TO, ONTO>), dim3((unsigned)((q.chunks - 1) * q.join_strips)), dim3(SUM_NT), 0, s, p);
+  }
+}
+template <typename TG, typename TO>
+void launch(const GradParams& p, const Plan& q, bool onto, hipStream_t s) {
+  onto ? launch<TG, TO, true>(p, q, s) : launch<TG, TO, false>(p, q, s);
+}
+
+}  // namespace embed
+}  // namespace dsv41
+
+using namespace dsv41;
+using namespace dsv41::embed;
+
+extern "C" int dsv41_embed_run(const dsv41_embed_desc* d, void* stream) {
+  if (!d) return fail(DSV41_E_INVALID, "embedding descriptor is NULL");
+  if (d->struct_size != sizeof(dsv41_embed_desc))
+    return fail(DSV41_E_ABI, "dsv41_embed_desc size mismatch (rebuild the binding)");
+  if (int rc = check_sizes(d->dtype, d->n_tokens, d->hidden, d->vocab)) return rc;
+  const bool f32 = d->dtype == DSV41_DTYPE_F32;
+  const int unit = f32 ? 4 : 2;
+  if (!d->weight || (d->n_tokens > 0 && (!d->ids || !d->out))) return fail(DSV41_E_INVALID, "weight, ids and out are required");
+  if (d->weight_row_stride < d->hidden || d->out_row_stride < d->hidden)
+    return fail(DSV41_E_INVALID, "embedding: row strides must cover the rows");
+  if ((uintptr_t)d->weight % unit || (uintptr_t)d->out % unit)
+    return fail(DSV41_E_INVALID, "embedding: operands are not aligned to their type");
+  if (d->n_tokens == 0) return DSV41_OK;
+  CopyParams p{};
+  p.w = d->weight;
+  p.ws = d->weight_row_stride;
+  p.ids = d->ids;
+  p.n = d->n_tokens;
+  p.H = d->hidden;
+  p.V = d->vocab;
+  p.scale = d->scale;
+  p.out = d->out;
+  p.os = d->out_row_stride;
+  p.status = d->out_status;
+  p.lanes = 1;
+  while (p.lanes < COPY_NT && p.lanes * (16 / unit) < p.H) p.lanes *= 2;
+  const int64_t grid = ((int64_t)p.n * p.lanes + COPY_NT - 1) / COPY_NT;
+  if (grid > MAX_GRID * 2) return fail(DSV41_E_UNSUPPORTED, "embedding: the batch is too large for one call");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (f32) hipLaunchKernelGGL(copy_kernel<float>, dim3((unsigned)grid), dim3(COPY_NT), 0, s, p);
+  else hipLaunchKernelGGL(copy_kernel<rows::bf16_t>, dim3((unsigned)grid), dim3(COPY_NT), 0, s, p);
+  DSV41_HIP_CHECK(hipGetLastError());
+  return DSV41_OK;
+}
+
+extern "C" size_t dsv41_embed_grad_workspace_bytes(const dsv41_embed_grad_desc* d) {
+  return check_grad(d) ? 0 : plan(d).bytes;
+}
+
+extern "C" int dsv41_embed_grad_run(const dsv41_embed_grad_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_grad(d)) return rc;
+  const Plan q = plan(d);
+  if (!workspace || workspace_bytes < q.bytes || (uintptr_t)workspace % 16)
+    return fail(DSV41_E_WORKSPACE, "embedding gradient workspace is missing, too small or not 16-byte aligned");
+  char* ws = static_cast<char*>(workspace);
+  GradParams p{};
+  p.ids = d->ids;
+  p.n = d->n_tokens;
+  p.H = d->hidden;
+  p.V = d->vocab;
+  p.g = d->grad;
+  p.gs = d->grad_row_stride;
+  p.scale = d->scale;
+  p.out = d->out;
+  p.os = d->out_row_stride;
+  p.ranges = (int)q.ranges;
+  p.chunks = (int)q.chunks;
+  p.strips = (int)q.strips;
+  p.zeros = (int)q.zeros;
+  p.total = reinterpret_cast<int32_t*>(ws);
+  p.place = reinterpret_cast<int32_t*>(ws + q.place);
+  p.name = reinterpret_cast<int32_t*>(ws + q.name);
+  p.present = reinterpret_cast<uint32_t*>(ws + q.present);
+  p.part = reinterpret_cast<float*>(ws + q.part);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(sort_kernel, dim3((unsigned)q.ranges), dim3(SORT_NT), 0, s, p);
+  const bool gf = d->grad_dtype == DSV41_DTYPE_F32, of = d->out_dtype == DSV41_DTYPE_F32, onto = d->accumulate != 0;
+  if (q.chunks * q.strips + q.zeros > 0) {
+    if (gf && of) launch<float, float>(p, q, onto, s);
+    else if (gf) launch<float, rows::bf16_t>(p, q, onto, s);
+    else if (of) launch<rows::bf16_t, float>(p, q, onto, s);
+    else launch<rows::bf16_t, rows::bf16_t>(p, q, onto, s);
+  }
+  DSV41_HIP_CHECK(hipGetLastError());
+  return DSV41_OK;
+}

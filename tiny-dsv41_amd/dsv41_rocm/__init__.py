@@ -17,9 +17,14 @@ from .rollout import generate_group_responses, generate_response  # noqa: F401
 from .tis import decoupled_token_tis_loss, grpo_loss  # noqa: F401
 from .scores import LogitScores, logit_scores  # noqa: F401
 from .distill import distillation_loss  # noqa: F401
+from .process import process_logits  # noqa: F401
+from .inthead import Int8Head, head_logits, quantize_head  # noqa: F401
+from .embedding import token_embedding, token_embedding_backward  # noqa: F401
 
 __all__ = ["SampleResult", "sample", "sample_next", "validate_temperature", "load_library",
            "ShardCandidates", "sample_shard", "merge_shards", "replay_log_probs",
            "full_shard_states", "full_shard_masses", "full_shard_draw", "full_shard_finish",
            "selected_log_probs", "score_targets", "token_log_probs", "shard_states", "combine_states", "sample_rows", "selected_log_probs_op",
-           "decoupled_token_tis_loss", "grpo_loss", "LogitScores", "logit_scores", "distillation_loss", "generate_response", "generate_group_responses"]
+           "decoupled_token_tis_loss", "grpo_loss", "LogitScores", "logit_scores", "distillation_loss",
+           "process_logits", "Int8Head", "quantize_head", "head_logits", "token_embedding", "token_embedding_backward",
+           "generate_response", "generate_group_responses"]

@@ -35,6 +35,10 @@ STATUS_BAD_TARGET = 16
 STATUS_BAD_SLICES = 32
 STATUS_REPEATED = 64
 STATUS_BAD_TEACHER = 128
+STATUS_BAD_PENALTY = 256
+STATUS_BAD_BIAS = 512
+STATUS_BAD_MASK = 1024
+STATUS_NO_TOKEN = 2048
 
 TAIL_RENORMALIZE = 0
 TAIL_REST = 1
@@ -351,6 +355,97 @@ class DistillGradDesc(ctypes.Structure):
     ]
 
 
+class ProcessDesc(ctypes.Structure):
+    """Mirror of dsv41_process_desc."""
+
+    _fields_ = _ROW_FIELDS + [
+        ("history", ctypes.c_void_p),
+        ("history_row_stride", ctypes.c_int64),
+        ("hist_len", ctypes.c_int32),
+        ("history_lens", ctypes.c_void_p),
+        ("history_prompt_lens", ctypes.c_void_p),
+        ("repetition_penalty", ctypes.c_float),
+        ("presence_penalty", ctypes.c_float),
+        ("frequency_penalty", ctypes.c_float),
+        ("repetition_penalties", ctypes.c_void_p),
+        ("presence_penalties", ctypes.c_void_p),
+        ("frequency_penalties", ctypes.c_void_p),
+        ("bias_ids", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("bias_row_stride", ctypes.c_int64),
+        ("bias_len", ctypes.c_int32),
+        ("masks", ctypes.c_int32),
+        ("mask", ctypes.c_void_p),
+        ("mask_row_stride", ctypes.c_int64),
+        ("mask_rows", ctypes.c_void_p),
+        ("fill", ctypes.c_float),
+        ("out", ctypes.c_void_p),
+        ("out_row_stride", ctypes.c_int64),
+        ("out_status", ctypes.c_void_p),
+        ("grad", ctypes.c_void_p),
+        ("grad_row_stride", ctypes.c_int64),
+    ]
+
+
+class IntHeadDesc(ctypes.Structure):
+    """Mirror of dsv41_int_head_desc."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("n_tokens", ctypes.c_int32),
+        ("hidden", ctypes.c_int32),
+        ("vocab", ctypes.c_int32),
+        ("x", ctypes.c_void_p),
+        ("x_row_stride", ctypes.c_int64),
+        ("w", ctypes.c_void_p),
+        ("w_row_stride", ctypes.c_int64),
+        ("scales", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("out_row_stride", ctypes.c_int64),
+        ("out_dtype", ctypes.c_int32),
+        ("out_status", ctypes.c_void_p),
+    ]
+
+
+class EmbedDesc(ctypes.Structure):
+    """Mirror of dsv41_embed_desc."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("n_tokens", ctypes.c_int32),
+        ("hidden", ctypes.c_int32),
+        ("vocab", ctypes.c_int32),
+        ("weight", ctypes.c_void_p),
+        ("weight_row_stride", ctypes.c_int64),
+        ("ids", ctypes.c_void_p),
+        ("scale", ctypes.c_float),
+        ("dtype", ctypes.c_int32),
+        ("out", ctypes.c_void_p),
+        ("out_row_stride", ctypes.c_int64),
+        ("out_status", ctypes.c_void_p),
+    ]
+
+
+class EmbedGradDesc(ctypes.Structure):
+    """Mirror of dsv41_embed_grad_desc."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("n_tokens", ctypes.c_int32),
+        ("hidden", ctypes.c_int32),
+        ("vocab", ctypes.c_int32),
+        ("ids", ctypes.c_void_p),
+        ("grad", ctypes.c_void_p),
+        ("grad_row_stride", ctypes.c_int64),
+        ("grad_dtype", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("out", ctypes.c_void_p),
+        ("out_row_stride", ctypes.c_int64),
+        ("out_dtype", ctypes.c_int32),
+        ("accumulate", ctypes.c_int32),
+    ]
+
+
 FULL_DRAW_CDF = 0
 FULL_DRAW_RACE = 1
 FULL_DRAW_GREEDY = 2
@@ -376,6 +471,10 @@ EXPORTS = (
     "dsv41_scores_grad_desc_size",
     "dsv41_distill_desc_size",
     "dsv41_distill_grad_desc_size",
+    "dsv41_process_desc_size",
+    "dsv41_int_head_desc_size",
+    "dsv41_embed_desc_size",
+    "dsv41_embed_grad_desc_size",
     "dsv41_last_error",
     "dsv41_sampler_workspace_bytes",
     "dsv41_sampler_run",
@@ -406,6 +505,14 @@ EXPORTS = (
     "dsv41_distill_workspace_bytes",
     "dsv41_distill_run",
     "dsv41_distill_grad_run",
+    "dsv41_process_run",
+    "dsv41_process_grad_run",
+    "dsv41_quantize_rows_run",
+    "dsv41_int_head_workspace_bytes",
+    "dsv41_int_head_run",
+    "dsv41_embed_run",
+    "dsv41_embed_grad_workspace_bytes",
+    "dsv41_embed_grad_run",
 )
 
 _lock = threading.Lock()
@@ -484,6 +591,20 @@ def _bind(lib: ctypes.CDLL) -> ctypes.CDLL:
         run.argtypes = [ctypes.POINTER(forward), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
         grad = getattr(lib, f"dsv41_{name}_grad_run")
         grad.restype, grad.argtypes = ctypes.c_int, [ctypes.POINTER(backward), ctypes.c_void_p]
+    for name in ("process", "int_head", "embed", "embed_grad"):
+        getattr(lib, f"dsv41_{name}_desc_size").restype = ctypes.c_size_t
+    for name, cls in (("process", ProcessDesc), ("process_grad", ProcessDesc), ("embed", EmbedDesc)):
+        run = getattr(lib, f"dsv41_{name}_run")
+        run.restype, run.argtypes = ctypes.c_int, [ctypes.POINTER(cls), ctypes.c_void_p]
+    for name, cls in (("int_head", IntHeadDesc), ("embed_grad", EmbedGradDesc)):
+        size = getattr(lib, f"dsv41_{name}_workspace_bytes")
+        size.restype, size.argtypes = ctypes.c_size_t, [ctypes.POINTER(cls)]
+        run = getattr(lib, f"dsv41_{name}_run")
+        run.restype = ctypes.c_int
+        run.argtypes = [ctypes.POINTER(cls), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+    lib.dsv41_quantize_rows_run.restype = ctypes.c_int
+    lib.dsv41_quantize_rows_run.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+                                            ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
     lib.dsv41_check_wait.restype = ctypes.c_int
     lib.dsv41_check_wait.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
                                     ctypes.c_void_p, ctypes.c_void_p]
@@ -530,7 +651,8 @@ def load() -> ctypes.CDLL:
         if lib.dsv41_sampler_full_finish_desc_size() != ctypes.sizeof(SamplerFullFinishDesc):
             raise RuntimeError("dsv41_sampler_full_finish_desc layout differs between library and binding")
         for name, cls in (("scores", ScoresDesc), ("scores_grad", ScoresGradDesc), ("distill", DistillDesc),
-                          ("distill_grad", DistillGradDesc)):
+                          ("distill_grad", DistillGradDesc), ("process", ProcessDesc), ("int_head", IntHeadDesc),
+                          ("embed", EmbedDesc), ("embed_grad", EmbedGradDesc)):
             if getattr(lib, f"dsv41_{name}_desc_size")() != ctypes.sizeof(cls):
                 raise RuntimeError(f"dsv41_{name}_desc layout differs between library and binding")
         _lib = lib

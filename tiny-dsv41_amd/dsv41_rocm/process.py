@@ -1,0 +1,296 @@
+"""Processed rows of logits on MI355X: biases, penalties for repeated tokens and token masks, with knobs
+for each row, differentiable in the logits.
+
+Reference (paths relative to the Tiny-DSV41 tree): ``rollout_manager/backends/vllm_actor.py:178-185`` names
+the penalties among an engine's SamplingParams and ``:260`` takes log-probs under the processed
+distribution.  ``sample`` applies one batch's penalties inside its draw; here they, and what engines apply
+beside them, come as rows of logits that ``sample``, ``logit_scores`` and ``distillation_loss`` take.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Union
+
+import torch
+
+from . import _lib
+from ._check import any_set
+from .logprob import first_order
+from .scores import INTEGERS, launch, refuse_capture, refuse_tangents, row_fields, rows_of_logits, vector, written
+
+Knob = Union[float, torch.Tensor]
+
+
+def _knob(value, name, rows, device):
+    """(the scalar of the descriptor, the per-row fp32 tensor or None)"""
+    if isinstance(value, torch.Tensor):
+        if value.shape != (rows,):
+            raise ValueError(f"{name} must be a number or have one value per row")
+        if value.requires_grad and torch.is_grad_enabled():
+            raise NotImplementedError(f"{name} has no gradient: detach it")
+        refuse_tangents(name, value)
+        return (1.0 if name == "repetition_penalty" else 0.0), vector(value, torch.float32, (rows,), device)
+    value = float(value)
+    if name == "repetition_penalty":
+        if not math.isfinite(value) or value <= 0:
+            raise ValueError("repetition_penalty must be finite and positive")
+    elif not math.isfinite(value):
+        raise ValueError("presence_penalty and frequency_penalty must be finite")
+    return value, None
+
+
+def _integers(t, name, dtype, device):
+    if not isinstance(t, torch.Tensor) or t.dtype not in INTEGERS:
+        raise ValueError(f"{name} must be integers")
+    return t if t.dtype == dtype and t.device == device else t.to(device=device, dtype=dtype)
+
+
+def _rows_of(t):
+    """A matrix whose rows are contiguous, at any row stride that is not negative."""
+    return t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
+
+
+def _list_stride(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+class _Arguments:
+    """Validated arguments in kernel form: the descriptor's fields, and the tensors that they point to."""
+
+    def __init__(self, logits, history, history_lens, history_prompt_lens, repetition_penalty, presence_penalty,
+                 frequency_penalty, bias_ids, bias, token_mask, mask_rows, fill):
+        rows, vocab = logits.shape
+        dev = logits.device
+        fields = {}
+        keep = []
+
+        def point(name, t):
+            fields[name] = t.data_ptr()
+            keep.append(t)
+
+        knobs = (("repetition_penalty", repetition_penalty, "repetition_penalties"),
+                 ("presence_penalty", presence_penalty, "presence_penalties"),
+                 ("frequency_penalty", frequency_penalty, "frequency_penalties"))
+        for name, value, array in knobs:
+            fields[name], t = _knob(value, name, rows, dev)
+            if t is not None:
+                point(array, t)
+        if history is None and (history_lens is not None or history_prompt_lens is not None):
+            raise ValueError("history_lens and history_prompt_lens require a history")
+        if history is not None:
+            if history.ndim != 2 or history.shape[0] != rows:
+                raise ValueError("history must have shape [rows, history_length]")
+            history = _rows_of(_integers(history, "history", torch.int64, dev))
+            for name, t in (("history_lens", history_lens), ("history_prompt_lens", history_prompt_lens)):
+                if t is not None:
+                    t = _integers(torch.as_tensor(t), name, torch.int32, dev)
+                    if t.shape != (rows,):
+                        raise ValueError(f"{name} must have one length per row")
+                    if history.shape[1]:
+                        point(name, t.contiguous())
+            if history.shape[1]:
+                point("history", history)
+                fields["history_row_stride"], fields["hist_len"] = _list_stride(history), history.shape[1]
+        if (bias_ids is None) != (bias is None):
+            raise ValueError("bias_ids and bias are given together")
+        if bias is not None:
+            if bias.requires_grad and torch.is_grad_enabled():
+                raise NotImplementedError("bias has no gradient: detach it")
+            refuse_tangents("biases", bias)
+            if not bias.is_floating_point() or bias.shape != bias_ids.shape or bias.ndim not in (1, 2) or \
+                    bias.ndim == 2 and bias.shape[0] != rows:
+                raise ValueError("bias_ids and bias must have shape [rows, entries] or [entries]")
+            bias_ids = _integers(bias_ids, "bias_ids", torch.int64, dev).contiguous()
+            bias = bias.to(device=dev, dtype=torch.float32).contiguous()
+            if bias.numel():
+                point("bias_ids", bias_ids)
+                point("bias", bias)
+                fields["bias_len"] = bias.shape[-1]
+                fields["bias_row_stride"] = bias.shape[-1] if bias.ndim == 2 else 0
+        if mask_rows is not None and token_mask is None:
+            raise ValueError("mask_rows requires a token_mask")
+        if token_mask is not None:
+            words = (vocab + 31) // 32
+            if not isinstance(token_mask, torch.Tensor) or token_mask.dtype != torch.int32 or \
+                    token_mask.ndim not in (1, 2) or token_mask.shape[-1] < words:
+                raise ValueError("token_mask must be int32 words, one bit per token: [masks, ceil(vocabulary_size / 32)]")
+            if token_mask.ndim == 1:
+                token_mask = token_mask[None]
+            token_mask = _rows_of(token_mask.to(dev))
+            if mask_rows is not None:
+                mask_rows = _integers(mask_rows, "mask_rows", torch.int32, dev).contiguous()
+                if mask_rows.shape != (rows,):
+                    raise ValueError("mask_rows must have one mask per row")
+                point("mask_rows", mask_rows)
+            elif token_mask.shape[0] not in (1, rows):
+                raise ValueError("without mask_rows there is one token_mask, or one per row")
+            if token_mask.shape[0]:
+                point("mask", token_mask)
+                fields["masks"], fields["mask_row_stride"] = token_mask.shape[0], _list_stride(token_mask)
+            elif rows:
+                raise ValueError("token_mask holds no mask")
+        fill = float(fill)
+        if math.isnan(fill):
+            raise ValueError("fill must be a number")
+        fields["fill"] = fill
+        self.fields, self.keep = fields, keep
+
+
+def _desc(logits, fields) -> _lib.ProcessDesc:
+    d = _lib.ProcessDesc(*row_fields(_lib.ProcessDesc, logits))
+    for name, value in fields.items():
+        setattr(d, name, value)
+    return d
+
+
+def forward(logits, fields, out, want_status):
+    """One dsv41_process_run into ``out``; returns the statuses or None."""
+    rows, vocab = logits.shape
+    status = torch.empty(rows, dtype=torch.int32, device=logits.device) if want_status else None
+    if rows:
+        d = _desc(logits, fields)
+        d.out, d.out_row_stride = out.data_ptr(), out.stride(0) if rows > 1 else vocab
+        if status is not None:
+            d.out_status = status.data_ptr()
+        launch(_lib.load().dsv41_process_run, logits.device, ctypes.byref(d))
+    return status
+
+
+def process_backward(logits, fields, grad):
+    """dL/dlogits of :func:`process_logits` from dL/dresult, in the logits' dtype."""
+    refuse_tangents("gradients", grad)
+    rows, vocab = logits.shape
+    out = torch.empty(rows, vocab, dtype=logits.dtype, device=logits.device)
+    if rows:
+        grad = grad.to(logits.dtype)
+        if grad.stride(1) != 1 and vocab > 1 or rows > 1 and 0 < grad.stride(0) < vocab:
+            grad = grad.contiguous()
+        d = _desc(logits, fields)
+        d.grad, d.grad_row_stride = grad.data_ptr(), grad.stride(0) if rows > 1 else vocab
+        d.out, d.out_row_stride = out.data_ptr(), vocab
+        launch(_lib.load().dsv41_process_grad_run, logits.device, ctypes.byref(d))
+    return out
+
+
+class _Process(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, fields, want_status, *lists):
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        status = forward(logits, fields, out, want_status)
+        ctx.fields = fields
+        ctx.save_for_backward(logits, *lists)
+        ctx.set_materialize_grads(False)
+        if status is not None:
+            ctx.mark_non_differentiable(status)
+        return out, status
+
+    @staticmethod
+    def backward(ctx, grad, g_status):
+        logits, *_ = ctx.saved_tensors  # (the lists too: one that was written since is refused here)
+        if grad is None:
+            return (None,) * len(ctx.needs_input_grad)
+        dx = process_backward(logits, ctx.fields, grad)
+        return (first_order(dx, logits, grad),) + (None,) * (len(ctx.needs_input_grad) - 1)
+
+
+def _status_error(status: torch.Tensor) -> None:
+    bits = 0
+    for v in status.unique().tolist():
+        bits |= int(v)
+    if bits & _lib.STATUS_BAD_PENALTY:
+        raise ValueError("repetition penalties must be finite and positive, the other penalties finite")
+    if bits & _lib.STATUS_BAD_MASK:
+        raise ValueError("mask_rows names a mask that there is not")
+    if bits & _lib.STATUS_BAD_HISTORY:
+        raise ValueError("history token ID is outside the model vocabulary")
+    if bits & _lib.STATUS_BAD_BIAS:
+        raise ValueError("biased token ID is outside the model vocabulary")
+    if bits & _lib.STATUS_NO_TOKEN:
+        raise ValueError("token mask leaves a row without tokens")
+
+
+def _extent(t):
+    """[first, past the last) byte that the matrix touches."""
+    size = t.element_size()
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * size
+
+
+def _output(out, logits):
+    """A validated ``out``: the logits' own tensor, or one that does not touch their memory."""
+    if not isinstance(out, torch.Tensor) or out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
+        raise ValueError("out must have the shape, dtype and device of the logits")
+    rows, vocab = out.shape
+    if vocab > 1 and out.stride(1) != 1 or rows > 1 and out.stride(0) < vocab:
+        raise ValueError("out must have contiguous rows that do not overlap")
+    if rows and not (out.data_ptr() == logits.data_ptr() and (rows == 1 or out.stride(0) == logits.stride(0))):
+        a, b = _extent(out), _extent(logits)
+        if a[0] < b[1] and b[0] < a[1]:
+            raise ValueError("out overlaps the logits without being them")
+    return out
+
+
+def process_logits(
+    logits: torch.Tensor,
+    *,
+    history: Optional[torch.Tensor] = None,
+    history_lens: Optional[torch.Tensor] = None,
+    history_prompt_lens: Optional[torch.Tensor] = None,
+    repetition_penalty: Knob = 1.0,
+    presence_penalty: Knob = 0.0,
+    frequency_penalty: Knob = 0.0,
+    bias_ids: Optional[torch.Tensor] = None,
+    bias: Optional[torch.Tensor] = None,
+    token_mask: Optional[torch.Tensor] = None,
+    mask_rows: Optional[torch.Tensor] = None,
+    fill: float = -math.inf,
+    out: Optional[torch.Tensor] = None,
+    check: bool = True,
+) -> torch.Tensor:
+    """Rows of logits with biases added, penalties applied and masked tokens filled, in that order.
+
+    ``logits [rows, V]`` are fp32 or bf16 on the GPU (other dtypes are converted to fp32), rows at any
+    stride; arithmetic is fp32 and the result has their dtype.
+
+    * ``bias_ids``, ``bias`` (``[rows, entries]``, or ``[entries]`` for every row): logits of these tokens
+      are raised by these values; of a token named twice the last entry counts, as in a dictionary.  Up to 4095 entries.
+    * ``history``, ``history_lens``, ``history_prompt_lens`` and the penalties are those of :func:`sample`,
+      bit for bit, with each penalty a number or a tensor of one value per row.  A row with
+      neutral penalties does not read its history.
+    * ``token_mask`` (int32 words ``[masks, ceil(V / 32)]`` or one mask): token ``i`` is allowed where bit
+      ``i % 32`` of word ``i // 32`` is set; others become ``fill``.  ``mask_rows [rows]`` names each row's
+      mask, -1 for none; without it there is one mask, or one per row.
+
+    Negative ids are padding.  ``logit_scores`` and ``distillation_loss`` take ``-inf`` for masked tokens;
+    ``sample`` takes finite logits only, so masks for it come with a finite ``fill`` that is far below any
+    logit times the temperature (-8192, or less for logits in the thousands).
+
+    ``out`` takes the result; it may be ``logits`` itself, in which case only what changes is written.  A call
+    with ``out`` has no gradient.  Otherwise the result is differentiable in ``logits``, once, in backward
+    mode: masked tokens get 0, tokens of the history their repetition penalty's factor.
+
+    With ``check`` the call synchronises and raises ``ValueError`` for ids outside the vocabulary, invalid
+    penalties, a mask that there is not, or one that leaves a row no token; without, such ids
+    are ignored, and rows of such penalties and masks hold NaN.
+    """
+    logits = rows_of_logits(logits, 1.0)
+    a = _Arguments(logits, history, history_lens, history_prompt_lens, repetition_penalty, presence_penalty,
+                   frequency_penalty, bias_ids, bias, token_mask, mask_rows, fill)
+    refuse_capture(check)
+    tracked = torch.is_grad_enabled() and logits.requires_grad
+    if out is not None:
+        if tracked or torch.is_grad_enabled() and out.requires_grad:
+            raise ValueError("a call with out has no gradient: leave it out, or call under no_grad")
+        out = _output(out, logits)
+        status = forward(logits, a.fields, out, check)
+        written(out)
+    elif tracked:
+        out, status = _Process.apply(logits, a.fields, check, *a.keep)
+    else:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        status = forward(logits, a.fields, out, check)
+    if check and any_set(status)[0]:
+        _status_error(status)
+    return out

@@ -97,6 +97,12 @@ def launch(call, device, *args) -> None:
         _lib.check(rc)
 
 
+def written(t) -> None:
+    """A kernel wrote ``t``, which was there before: autograd learns of it as of any operation in place."""
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
 def vector(t, dtype, shape, device):
     """A contiguous tensor of that dtype and shape on the device, ``t`` itself where it is one."""
     if t.dtype != dtype or t.device != device:
