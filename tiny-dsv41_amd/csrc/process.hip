@@ -33,7 +33,6 @@ constexpr int COUNT_BITS = 19;
 constexpr uint32_t COUNT = (1u << COUNT_BITS) - 1, SEEN = 1u << COUNT_BITS;
 constexpr int ENTRY_SHIFT = COUNT_BITS + 1;
 constexpr int MAX_BIAS = (1 << (32 - ENTRY_SHIFT)) - 1;  // entries of a row's list
-static_assert(SLICE % 32 == 0, "a slice begins at a word of a mask");
 
 constexpr int COPY = 0, INPLACE = 1, GRAD = 2;
 
@@ -78,42 +77,92 @@ struct Knobs {
     }
     return x;
   }
-  // the gradient's factor is 1 / rp or rp
+  // the gradient's factor is 1 / rp or rp, of ids that are not only biased
   __device__ __forceinline__ float slope(float g, float x, uint32_t word, const float* bias) const {
+    if (!(word & (SEEN | COUNT))) return g;
     if (word >> ENTRY_SHIFT) x = x + bias[(word >> ENTRY_SHIFT) - 1];
     return x > 0.0f ? g / rp : g * rp;
   }
 };
 
-// G elements from p of which the first n exist (the others come as 0)
+// A group of 16 bytes, kept as they are in memory: most groups go out as they came.
+struct Group {
+  uint32_t w[4];
+};
 template <typename T>
-__device__ __forceinline__ void load_group(const T* p, int n, float (&v)[Elem<T>::VEC]) {
-  constexpr int G = Elem<T>::VEC;
-  uint32_t w[4] = {0, 0, 0, 0};
-  if (n >= G) {
-    rows::load16<false>(p, w);
+constexpr uint32_t ALL = (1u << Elem<T>::VEC) - 1;
+// The elements j with bit j of `there`, from p (the others come as 0), and to it.
+template <typename T>
+__device__ __forceinline__ void load_group(const T* p, uint32_t there, Group& g) {
+  if (there == ALL<T>) {
+    rows::load16<false>(p, g.w);
   } else {
 #pragma unroll
-    for (int j = 0; j < G; ++j)
-      if (j < n) Elem<T>::put(w, j, p[j]);
+    for (int i = 0; i < 4; ++i) g.w[i] = 0;
+#pragma unroll
+    for (int j = 0; j < Elem<T>::VEC; ++j)
+      if (there >> j & 1) Elem<T>::put(g.w, j, p[j]);
   }
-  Elem<T>::unpack(w, v);
+}
+__device__ __forceinline__ void store_element(float* p, const Group& g, int j) { *p = __uint_as_float(g.w[j]); }
+__device__ __forceinline__ void store_element(bf16_t* p, const Group& g, int j) {
+  p->v = (uint16_t)(g.w[j >> 1] >> (16 * (j & 1)));
 }
 template <typename T>
-__device__ __forceinline__ void store_group(T* p, int n, const float (&v)[Elem<T>::VEC]) {
-  constexpr int G = Elem<T>::VEC;
-  if (n >= G) {
-    rows::store_full(p, 0, v);
+__device__ __forceinline__ void store_group(T* p, uint32_t there, const Group& g) {
+  if (there == ALL<T>) {
+    typename Elem<T>::Raw r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = g.w[i];
+    *reinterpret_cast<typename Elem<T>::Raw*>(p) = r;
   } else {
 #pragma unroll
-    for (int j = 0; j < G; ++j)
-      if (j < n) rows::store_one(p + j, v[j]);
+    for (int j = 0; j < Elem<T>::VEC; ++j)
+      if (there >> j & 1) store_element(p + j, g, j);
   }
+}
+// Element j, which differs from lane to lane (selections: registers have no addresses).
+__device__ __forceinline__ uint32_t pick(const Group& g, int i) {
+  const uint32_t lo = i & 1 ? g.w[1] : g.w[0], hi = i & 1 ? g.w[3] : g.w[2];
+  return i & 2 ? hi : lo;
+}
+__device__ __forceinline__ void place(Group& g, int i, uint32_t w) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) g.w[k] = i == k ? w : g.w[k];
+}
+__device__ __forceinline__ float get(const Group& g, int j, float) { return __uint_as_float(pick(g, j)); }
+__device__ __forceinline__ float get(const Group& g, int j, bf16_t) {
+  const uint32_t w = pick(g, j >> 1);
+  return j & 1 ? bf16_hi(w) : bf16_lo(w);
+}
+__device__ __forceinline__ void set(Group& g, int j, float v, float) { place(g, j, __float_as_uint(v)); }
+__device__ __forceinline__ void set(Group& g, int j, float v, bf16_t) {
+  const uint32_t w = pick(g, j >> 1), b = pack_bf16(v, v);
+  place(g, j >> 1, j & 1 ? (w & 0xFFFFu) | (b & 0xFFFF0000u) : (w & 0xFFFF0000u) | (b & 0xFFFFu));
+}
+// `instead` (of every element, in the type) where bit j of `allowed` is 0
+__device__ __forceinline__ void drop(Group& g, uint32_t allowed, uint32_t instead, float) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) g.w[k] = allowed >> k & 1 ? g.w[k] : instead;
+}
+__device__ __forceinline__ void drop(Group& g, uint32_t allowed, uint32_t instead, bf16_t) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t lo = (uint32_t)((int)(allowed << (31 - 2 * k)) >> 31), hi = (uint32_t)((int)(allowed << (30 - 2 * k)) >> 31);
+    const uint32_t keep = (lo & 0xFFFFu) | (hi & 0xFFFF0000u);
+    g.w[k] = (g.w[k] & keep) | (instead & ~keep);
+  }
+}
+// The word of element `at` of a slice: a thread's group of 8 bf16 elements lies in two planes, so that either
+// half of it is read without bank conflicts.
+template <typename T>
+__device__ __forceinline__ int word_at(int at) {
+  return Elem<T>::VEC == 4 ? at : ((at >> 2 & 1) * (SLICE / 2)) + (at >> 3 << 2) + (at & 3);
 }
 
 template <typename T, bool LISTS, bool MASK, int MODE>
-__global__ __launch_bounds__(NT) void process_kernel(Params p) {
-  constexpr int G = Elem<T>::VEC, U = SLICE / (NT * G);
+__global__ __launch_bounds__(NT, 8) void process_kernel(Params p) {
+  constexpr int G = Elem<T>::VEC, U = SLICE / (NT * G), AHEAD = 8;
   extern __shared__ uint32_t words[];  // SLICE words, then the row's biases
   float* biases = reinterpret_cast<float*>(words + SLICE);
   const int tid = threadIdx.x;
@@ -122,63 +171,16 @@ __global__ __launch_bounds__(NT) void process_kernel(Params p) {
   const int64_t item = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if ((int64_t)(blockIdx.x >> 3) >= per || item >= items) return;
   const int row = (int)(item / p.slices), slice = (int)(item % p.slices);
-  const int s0 = slice * SLICE, n = min(SLICE, p.V - s0);
-  const T* x = static_cast<const T*>(p.x) + row * p.xs + s0;
-  T* out = static_cast<T*>(p.out) + row * p.os + s0;
-
-  float v[U][G];
-  if constexpr (MODE != INPLACE) {
-    const T* from = MODE == GRAD ? static_cast<const T*>(p.grad) + row * p.gs + s0 : x;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = (u * NT + tid) * G;
-      if (i < n) load_group(from + i, n - i, v[u]);
-    }
-  }
+  const T* x = static_cast<const T*>(p.x) + row * p.xs;
+  T* out = static_cast<T*>(p.out) + row * p.os;
+  // slices begin at memory lines of the result
+  const int begin = slice * SLICE - rows::skew_of(out);
+  if (begin >= p.V) return;
+  const T* from = MODE == GRAD ? static_cast<const T*>(p.grad) + row * p.gs : x;
 
   Knobs knobs{1.f, 0.f, 0.f};
   bool bad = false;
   int bits = 0;  // status bits that this thread met
-  if constexpr (LISTS) {
-    knobs.rp = p.rps ? p.rps[row] : p.rp;
-    knobs.pres = p.press ? p.press[row] : p.pres;
-    knobs.freq = p.freqs ? p.freqs[row] : p.freq;
-    if (!(isfinite(knobs.rp) && knobs.rp > 0.f) || !isfinite(knobs.pres) || !isfinite(knobs.freq)) {
-      bad = true;
-      bits |= DSV41_STATUS_BAD_PENALTY;
-    }
-    uint4* w4 = reinterpret_cast<uint4*>(words);
-#pragma unroll
-    for (int i = 0; i < SLICE / 4 / NT; ++i) w4[i * NT + tid] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-    if (p.n_bias) {
-      const int64_t* ids = p.bias_ids + row * p.bs;
-      const float* b = p.bias + row * p.bs;
-      for (int e = tid; e < p.n_bias; e += NT) {
-        const int64_t id = ids[e];
-        biases[e] = b[e];
-        const uint64_t at = (uint64_t)(id - s0);
-        if (id >= 0 && at < (uint64_t)n) atomicMax(&words[at], (uint32_t)(e + 1) << ENTRY_SHIFT);
-        if (id >= p.V) bits |= DSV41_STATUS_BAD_BIAS;
-      }
-      __syncthreads();
-    }
-    if (p.history && !(knobs.rp == 1.f && knobs.pres == 0.f && knobs.freq == 0.f)) {
-      const int64_t* h = p.history + row * p.hs;
-      const int len = p.lens ? min(max(p.lens[row], 0), p.hist_len) : p.hist_len;
-      const int prompt = p.prompt_lens ? p.prompt_lens[row] : 0;
-      for (int j = tid; j < len; j += NT) {
-        const int64_t id = h[j];
-        const uint64_t at = (uint64_t)(id - s0);
-        if (id >= 0 && at < (uint64_t)n) {
-          if (j < prompt) atomicOr(&words[at], SEEN);
-          else atomicAdd(&words[at], 1u);
-        }
-        if (id >= p.V) bits |= DSV41_STATUS_BAD_HISTORY;
-      }
-    }
-    __syncthreads();
-  }
   const uint32_t* mask = nullptr;
   if constexpr (MASK) {
     const int m = p.mask_rows ? p.mask_rows[row] : p.masks == 1 ? 0 : row;
@@ -189,50 +191,143 @@ __global__ __launch_bounds__(NT) void process_kernel(Params p) {
       mask = p.mask + m * p.ms;
     }
   }
+  bool listed = false;
+  int len = 0, prompt = 0;
+  const int64_t* h = nullptr;
+  if constexpr (LISTS) {
+    knobs.rp = p.rps ? p.rps[row] : p.rp;
+    knobs.pres = p.press ? p.press[row] : p.pres;
+    knobs.freq = p.freqs ? p.freqs[row] : p.freq;
+    if (!(isfinite(knobs.rp) && knobs.rp > 0.f) || !isfinite(knobs.pres) || !isfinite(knobs.freq)) {
+      bad = true;
+      bits |= DSV41_STATUS_BAD_PENALTY;
+    }
+    // (a gradient asks for the repetition penalty alone)
+    if (p.history && !(knobs.rp == 1.f && (MODE == GRAD || (knobs.pres == 0.f && knobs.freq == 0.f)))) {
+      h = p.history + row * p.hs;
+      len = p.lens ? min(max(p.lens[row], 0), p.hist_len) : p.hist_len;
+      prompt = p.prompt_lens ? p.prompt_lens[row] : 0;
+    }
+    listed = len > 0 || (p.n_bias > 0 && (MODE != GRAD || h));
+  }
 
-  const float nan = __builtin_nanf("");
+  // the history's first entries, ahead of the slice itself: loads come back in order
+  uint2 ahead[AHEAD];
+  const uint2* h2 = reinterpret_cast<const uint2*>(h);
+  if (LISTS) {
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (tid + k * NT < len) ahead[k] = h2[tid + k * NT];
+  }
+  // which elements of the thread's groups there are, and which of them the mask allows
+  const bool inside = begin >= 0 && begin + SLICE <= p.V;  // (all of them)
+  uint32_t there[U], allowed[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int i = (u * NT + tid) * G;
-    if (i >= n) continue;
-    uint32_t w[G];
-#pragma unroll
-    for (int j = 0; j < G; ++j) w[j] = LISTS ? words[i + j] : 0;
-    uint32_t allowed = (1u << G) - 1;
-    if (MASK && mask) allowed &= mask[(s0 + i) >> 5] >> ((s0 + i) & 31);
-    if constexpr (MODE == INPLACE) {
-      bool all = true;
-      float o[G];
-#pragma unroll
-      for (int j = 0; j < G; ++j) {
-        o[j] = bad ? nan : p.fill;
-        all = all && (bad || !(allowed >> j & 1));
-      }
-      if (all) {
-        store_group(out + i, n - i, o);
-      } else {
-#pragma unroll
-        for (int j = 0; j < G; ++j) {
-          if (i + j >= n) continue;
-          if (!(allowed >> j & 1)) rows::store_one(out + i + j, p.fill);
-          else if (w[j]) rows::store_one(out + i + j, knobs.apply(Elem<T>::one(x + i + j), w[j], biases));
-        }
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < G; ++j) {
-        if (MODE == GRAD) {
-          if (w[j] & (SEEN | COUNT) && knobs.rp != 1.f && i + j < n)
-            v[u][j] = knobs.slope(v[u][j], Elem<T>::one(x + i + j), w[j], biases);
-          if (!(allowed >> j & 1)) v[u][j] = 0.f;
-        } else {
-          if (w[j]) v[u][j] = knobs.apply(v[u][j], w[j], biases);
-          if (!(allowed >> j & 1)) v[u][j] = p.fill;
-        }
-        if (bad) v[u][j] = nan;
-      }
-      store_group(out + i, n - i, v[u]);
+    const int i = begin + (u * NT + tid) * G;
+    there[u] = ALL<T>;
+    if (!inside) {
+      const int lo = max(-i, 0), hi = min(p.V - i, G);  // elements [lo, hi)
+      there[u] = lo < hi ? (ALL<T> << lo) & (ALL<T> >> (G - hi)) : 0u;
     }
+    allowed[u] = bad ? 0u : there[u];
+    if (MASK && mask && there[u]) {
+      const int k = max(i, 0) >> 5, last = (p.V - 1) >> 5;
+      const uint64_t both = (uint64_t)mask[min(k + 1, last)] << 32 | mask[k];
+      allowed[u] &= i >= 0 ? (uint32_t)(both >> (i & 31)) : (uint32_t)(both << -i);
+    }
+  }
+  if (LISTS && listed) {
+    uint4* w4 = reinterpret_cast<uint4*>(words);
+#pragma unroll
+    for (int i = 0; i < SLICE / 4 / NT; ++i) w4[i * NT + tid] = make_uint4(0, 0, 0, 0);
+    rows::lds_barrier();
+  }
+  // what is read: the groups with an allowed element
+  Group v[U];
+  if constexpr (MODE != INPLACE) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (allowed[u]) load_group(from + begin + (u * NT + tid) * G, there[u], v[u]);
+  }
+
+  if constexpr (LISTS) {
+    if (listed) {
+      // ids in [max(begin, 0), begin + SLICE) and below V, as unsigned offsets of the slice
+      const uint32_t first = (uint32_t)max(-begin, 0), count = (uint32_t)min(SLICE, p.V - begin) - first;
+      const bool report = MODE != GRAD && p.status && slice == 0;
+      if (p.n_bias) {
+        const uint2* ids = reinterpret_cast<const uint2*>(p.bias_ids + row * p.bs);
+        const float* b = p.bias + row * p.bs;
+        for (int e = tid; e < p.n_bias; e += NT) {
+          const uint2 id = ids[e];
+          biases[e] = b[e];
+          const uint32_t at = id.x - (uint32_t)begin;
+          if (id.y == 0 && at - first < count) atomicMax(&words[word_at<T>(at)], (uint32_t)(e + 1) << ENTRY_SHIFT);
+          if (report && (int)id.y >= 0 && (id.y > 0 || id.x >= (uint32_t)p.V)) bits |= DSV41_STATUS_BAD_BIAS;
+        }
+        rows::lds_barrier();
+      }
+      auto mark = [&](int j, uint2 id) {
+        const uint32_t at = id.x - (uint32_t)begin;
+        if (id.y == 0 && at - first < count) {
+          if (j < prompt) atomicOr(&words[word_at<T>(at)], SEEN);
+          else atomicAdd(&words[word_at<T>(at)], 1u);
+        }
+        if (report && (int)id.y >= 0 && (id.y > 0 || id.x >= (uint32_t)p.V)) bits |= DSV41_STATUS_BAD_HISTORY;
+      };
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+        if (tid + k * NT < len) mark(tid + k * NT, ahead[k]);
+      for (int j0 = AHEAD * NT; j0 < len; j0 += AHEAD * NT) {
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+          if (j0 + tid + k * NT < len) ahead[k] = h2[j0 + tid + k * NT];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+          if (j0 + tid + k * NT < len) mark(j0 + tid + k * NT, ahead[k]);
+      }
+      rows::lds_barrier();
+    }
+  }
+
+  const float value = bad ? __builtin_nanf("") : MODE == GRAD ? 0.f : p.fill;
+  const uint32_t instead = sizeof(T) == 4 ? __float_as_uint(value) : pack_bf16(value, value);
+  uint32_t marked[U];  // elements whose word is not 0
+  Group xs[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    marked[u] = 0;
+    const int at = (u * NT + tid) * G;
+    if (LISTS && listed) {
+#pragma unroll
+      for (int q = 0; q < G; q += 4) {
+        const uint4 w = *reinterpret_cast<const uint4*>(words + word_at<T>(at + q));
+        marked[u] |= (min(w.x, 1u) | min(w.y, 1u) << 1 | min(w.z, 1u) << 2 | min(w.w, 1u) << 3) << q;
+      }
+      marked[u] &= allowed[u];
+    }
+    // in place, groups that stay as they are are neither read nor written; of a gradient, the logits are
+    // read where a sign is asked for
+    if (MODE == INPLACE && allowed[u] && (marked[u] || allowed[u] != there[u])) load_group(x + begin + at, there[u], v[u]);
+    if (MODE == GRAD && marked[u]) load_group(x + begin + at, there[u], xs[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int at = (u * NT + tid) * G;
+    if (MODE == INPLACE && !marked[u] && allowed[u] == there[u]) continue;
+    if (LISTS) {
+      // (few: a wave takes as many turns as its lane with the most of them)
+      for (uint32_t m = marked[u]; m; m &= m - 1) {
+        const int j = __builtin_ctz(m);
+        const uint32_t word = words[word_at<T>(at + j)];
+        const float y = MODE == GRAD ? knobs.slope(get(v[u], j, T{}), get(xs[u], j, T{}), word, biases)
+                                     : knobs.apply(get(v[u], j, T{}), word, biases);
+        set(v[u], j, y, T{});
+      }
+    }
+    if (allowed[u] != there[u]) drop(v[u], allowed[u], instead, T{});
+    if (there[u]) store_group(out + begin + at, there[u], v[u]);
   }
 
   // the first slice reports for its row
@@ -267,6 +362,9 @@ void launch(const Params& p, hipStream_t s) {
 }
 
 constexpr int64_t MAX_GRID = (1 << 22) - 8;  // workgroups of 512 threads: HIP's grids stop short of 2^32 threads
+
+// (the last slice of a row that begins at a memory line may have nothing)
+int slices_of(int V) { return (V + rows::MOST_SKEW - 1 + SLICE - 1) / SLICE; }
 
 int check_desc(const dsv41_process_desc* d, bool grad) {
   if (!d) return fail(DSV41_E_INVALID, "process descriptor is NULL");
@@ -303,7 +401,7 @@ int check_desc(const dsv41_process_desc* d, bool grad) {
     if (d->mask_row_stride < 0) return fail(DSV41_E_INVALID, "mask row stride is negative");
   }
   if (isnan(d->fill)) return fail(DSV41_E_INVALID, "fill must be a number");
-  if ((int64_t)d->rows * ((d->vocab + SLICE - 1) / SLICE) > MAX_GRID)
+  if ((int64_t)d->rows * slices_of(d->vocab) > MAX_GRID)
     return fail(DSV41_E_UNSUPPORTED, "more than 2^22 row slices are not supported");
   return DSV41_OK;
 }
@@ -319,7 +417,7 @@ int run(const dsv41_process_desc* d, bool grad, void* stream) {
   p.gs = d->grad_row_stride;
   p.rows = d->rows;
   p.V = d->vocab;
-  p.slices = (d->vocab + SLICE - 1) / SLICE;
+  p.slices = slices_of(d->vocab);
   const bool neutral = !d->repetition_penalties && !d->presence_penalties && !d->frequency_penalties &&
                        d->repetition_penalty == 1.f && d->presence_penalty == 0.f && d->frequency_penalty == 0.f;
   if (d->hist_len > 0 && !neutral) {
