@@ -668,12 +668,10 @@ typedef struct dsv41_int_head_desc {
   int32_t vocab;
   const void* x;          /* bf16 [n_tokens, hidden] */
   int64_t x_row_stride;   /* in elements */
-  const int8_t* w;        /* [vocab, w_row_stride], as dsv41_quantize_rows_run leaves rows: 16-byte aligned;
-                             the columns from hidden to the next multiple of 128 are read, whatever they hold */
-  int64_t w_row_stride;   /* in elements, a multiple of 128 */
+  const int8_t* w;        /* the head's tiles, as dsv41_quantize_rows_run leaves them, 16-byte aligned */
   const float* scales;    /* [vocab], 16-byte aligned */
   void* out;              /* [n_tokens, vocab] */
-  int64_t out_row_stride; /* in elements; rows that begin at multiples of 4 elements are written faster */
+  int64_t out_row_stride; /* in elements; rows that begin at multiples of 16 bytes are written faster */
   int32_t out_dtype;      /* DSV41_DTYPE_F32 or DSV41_DTYPE_BF16 */
   int32_t* out_status;    /* [n_tokens] or NULL */
 } dsv41_int_head_desc;
@@ -847,12 +845,15 @@ int dsv41_distill_grad_run(const dsv41_distill_grad_desc* desc, void* stream /* 
 int dsv41_process_run(const dsv41_process_desc* desc, void* stream /* hipStream_t */);
 int dsv41_process_grad_run(const dsv41_process_desc* desc, void* stream /* hipStream_t */);
 
-/* Rows of bf16 as 8-bit integers with a scale each, as dsv41_int_head_desc says (weights are laid out
- * with it once): q [rows, qs], 16-byte aligned, qs a multiple of 16 that holds the columns padded to a
- * multiple of 128, the padding zeros; strides in elements.  A row with a NaN or an infinity: zeros, the scale NaN and
- * DSV41_STATUS_NONFINITE in status (which may be NULL). */
-int dsv41_quantize_rows_run(const void* x, int64_t xs, int rows, int cols, int8_t* q, int64_t qs, float* scales,
-                            int32_t* status, void* stream /* hipStream_t */);
+/* The rows of a head (bf16, stride in elements) as 8-bit integers with a scale each, as dsv41_int_head_desc
+ * says, laid out once for dsv41_int_head_run: rows rounded up to 64 times columns rounded up to 128 bytes, 16-byte
+ * aligned, in tiles of 16 rows x 64 columns.  Row v, column c lies at byte
+ *   ((m / 16) * (columns / 64) + c / 64) * 1024 + (c / 16 % 4) * 256 + (m % 16) * 16 + c % 16  with
+ *   m = v - v % 64 + (v % 16) / 4 * 16 + (v % 64) / 16 * 4 + v % 4,
+ * columns being the rounded number; those past cols are zeros, rows past the last are not written.  A row with a
+ * NaN or an infinity: zeros, the scale NaN and DSV41_STATUS_NONFINITE in status (which may be NULL). */
+int dsv41_quantize_rows_run(const void* x, int64_t xs, int rows, int cols, int8_t* q, float* scales, int32_t* status,
+                            void* stream /* hipStream_t */);
 
 /* Logits of an 8-bit head.  Workspace (16-byte aligned, contents need no initialisation): the quantized
  * hidden states, n_tokens rounded up to 16 times hidden rounded up to 128 bytes, and their scales. */

@@ -46,7 +46,9 @@ def test_exact(n, h, v, dtype):
     x, w = _inputs(n, h, v)
     head = quantize_head(w.to(DEV))
     q, t = _quantized(w)
-    assert torch.equal(head.weight.cpu().double(), q) and torch.equal(head.scales.cpu(), t)
+    assert torch.equal(head.integers().cpu().double(), q) and torch.equal(head.scales.cpu(), t)
+    again = Int8Head.from_quantized(head.integers(), head.scales)
+    assert torch.equal(again.tiles, head.tiles) and (again.vocab, again.hidden) == (v, h)
     want = _want(x, q, t, dtype)
     got = head_logits(x.to(DEV), head, dtype=dtype)
     assert got.dtype == dtype and got.shape == (n, v)
@@ -196,9 +198,9 @@ def test_refusals_on_the_gpu():
     with pytest.raises(NotImplementedError, match="no gradient"):
         quantize_head(w.to(DEV).requires_grad_())
     with pytest.raises(ValueError, match="layout"):
-        head_logits(d, Int8Head(head.weight.contiguous(), head.scales))
+        head_logits(d, Int8Head(head.tiles[:-1], head.scales, 50, 200))
     with pytest.raises(ValueError, match="layout"):
-        head_logits(d, Int8Head(head.weight, head.scales.double()))
+        head_logits(d, Int8Head(head.tiles, head.scales.double(), 50, 200))
     with pytest.raises(ValueError, match="out must"):
         head_logits(d, head, out=torch.empty(3, 51, device=DEV))
     with pytest.raises(ValueError, match="do not overlap"):

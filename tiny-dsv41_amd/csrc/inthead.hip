@@ -32,61 +32,106 @@ constexpr int LINE = ROWB;            // columns are padded to whole lines
 constexpr int MAX_COLUMNS = 133120;   // 2^31 / 127^2 = 133152, in whole lines
 constexpr int QUANT_NT = 256;
 constexpr int FEW = 64;               // tokens of head_kernel
-constexpr int HEAD_ROWS = 64;         // rows of w of its workgroup
 
 typedef int intx4 __attribute__((ext_vector_type(4)));
 
+// ------------------------------------------------------------------------------------ layout
+// Tiles of 16 rows x 64 columns, in the order of a fragment's lanes: 16 columns of each row, row after row, four
+// times.  The tiles of 16 rows follow one another along the columns.
+constexpr int TILE = 1024;
+constexpr int GROUP = 64;  // rows of a head that share four tiles' rows
+// Row m of a head's tile i is row 16 (m / 4) + 4 i + m % 4 of its group of 64: a lane, which holds sums of four rows of
+// a tile, holds 16 neighbouring logits of four tiles.
+__device__ __forceinline__ int64_t head_row(int64_t v) {  // -> the row's place among the tiles' rows
+  const int r = (int)(v % GROUP);
+  return v - r + (r >> 2 & 3) * 16 + (r >> 4) * 4 + (r & 3);
+}
+// Byte of column c (a multiple of 8) of the row at place m.
+__device__ __forceinline__ int64_t byte_of(int64_t m, int c, int padded) {
+  return (m / 16 * (padded / 64) + c / 64) * TILE + (c / 16 % 4) * 256 + m % 16 * 16 + c % 16;
+}
+
 // ------------------------------------------------------------------------------- quantization
-__global__ __launch_bounds__(QUANT_NT) void quantize_kernel(const bf16_t* x, int64_t xs, int cols, int8_t* q, int64_t qs,
-                                                            int padded, float* scales, int32_t* status) {
-  constexpr int G = 8;
-  __shared__ float tops[QUANT_NT / 64];
+// One workgroup a row; the first KEPT chunks of a thread stay in registers between the two passes.
+constexpr int KEPT = 4;
+
+// 8 elements of x[0, cols) from i on, zeros where it ends
+__device__ __forceinline__ void load_chunk(const bf16_t* x, int cols, int i, uint32_t (&w)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = 0;
+  if (i + 8 <= cols) {
+    rows::load16<false>(x + i, w);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i + j < cols) rows::Elem<bf16_t>::put(w, j, x[i + j]);
+  }
+}
+// The largest magnitude's bits, of which those of infinities and NaNs are the largest.
+__device__ __forceinline__ uint32_t top_of(const uint32_t (&w)[4], uint32_t top) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) top = max(top, max((w[j] << 16) & 0x7FFF0000u, w[j] & 0x7FFF0000u));
+  return top;
+}
+__device__ __forceinline__ uint2 quantize(const uint32_t (&w)[4], float lift, float top) {
+  uint32_t o[2] = {0, 0};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float v = j & 1 ? bf16_hi(w[j >> 1]) : bf16_lo(w[j >> 1]);
+    o[j >> 2] |= (uint32_t)((int)rintf(127.f * (v * lift) / top) & 0xFF) << (8 * (j & 3));
+  }
+  return make_uint2(o[0], o[1]);
+}
+
+template <bool HEAD>
+__global__ __launch_bounds__(QUANT_NT) void quantize_kernel(const bf16_t* x, int64_t xs, int cols, int8_t* q, int padded,
+                                                            float* scales, int32_t* status) {
+  constexpr int STEP = QUANT_NT * 8;
+  __shared__ uint32_t tops[QUANT_NT / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   x += (int64_t)blockIdx.x * xs;
-  q += (int64_t)blockIdx.x * qs;
-  float top = 0.f;
-  int odd = 0;  // a NaN or an infinity
-  for (int i = tid * G; i < cols; i += QUANT_NT * G) {
-    uint32_t w[4];
-    rows::load_some<false>(x, 0, cols, i / G, w);
+  const int64_t place = HEAD ? head_row(blockIdx.x) : blockIdx.x;
+  uint32_t kept[KEPT][4], top = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float lo = bf16_lo(w[j]), hi = bf16_hi(w[j]);
-      if (i + 2 * j < cols) odd |= !isfinite(lo), top = fmaxf(top, fabsf(lo));
-      if (i + 2 * j + 1 < cols) odd |= !isfinite(hi), top = fmaxf(top, fabsf(hi));
-    }
+  for (int c = 0; c < KEPT; ++c) load_chunk(x, cols, c * STEP + tid * 8, kept[c]);
+#pragma unroll
+  for (int c = 0; c < KEPT; ++c) top = top_of(kept[c], top);
+  for (int i = KEPT * STEP + tid * 8; i < cols; i += STEP) {
+    uint32_t w[4];
+    load_chunk(x, cols, i, w);
+    top = top_of(w, top);
   }
-  top = wave_max(top);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
   if (lane == 0) tops[wave] = top;
-  odd = __syncthreads_or(odd);
-  for (int w = 0; w < QUANT_NT / 64; ++w) top = fmaxf(top, tops[w]);
+  __syncthreads();
+  for (int w = 0; w < QUANT_NT / 64; ++w) top = max(top, tops[w]);
+  const bool odd = top >= 0x7F800000u;
+  float most = __uint_as_float(top);
   if (tid == 0) {
-    scales[blockIdx.x] = odd ? __builtin_nanf("") : top / 127.f;
+    scales[blockIdx.x] = odd ? __builtin_nanf("") : most / 127.f;
     if (status) status[blockIdx.x] = odd ? DSV41_STATUS_NONFINITE : 0;
   }
-  const bool none = odd || top == 0.f;
-  const float lift = top > 1e30f ? 0x1p-64f : 1.f;  // (127 x is finite; what it takes from small x is far below a half)
-  top *= lift;
-  for (int i = tid * G; i < padded; i += QUANT_NT * G) {
-    uint32_t w[4];
-    rows::load_some<false>(x, 0, cols, i / G, w);
-    uint32_t o[2] = {0, 0};
+  const bool none = odd || top == 0;
+  const float lift = most > 1e30f ? 0x1p-64f : 1.f;  // (127 x is finite; what it takes from small x is far below a half)
+  most *= lift;
 #pragma unroll
-    for (int j = 0; j < G; ++j) {
-      const float v = j & 1 ? bf16_hi(w[j >> 1]) : bf16_lo(w[j >> 1]);
-      const int k = none || i + j >= cols ? 0 : (int)rintf(127.f * (v * lift) / top);
-      o[j >> 2] |= (uint32_t)(k & 0xFF) << (8 * (j & 3));
-    }
-    *reinterpret_cast<uint2*>(q + i) = make_uint2(o[0], o[1]);
+  for (int c = 0; c < KEPT; ++c) {
+    const int i = c * STEP + tid * 8;
+    if (i < padded) *reinterpret_cast<uint2*>(q + byte_of(place, i, padded)) = none ? make_uint2(0, 0) : quantize(kept[c], lift, most);
+  }
+  for (int i = KEPT * STEP + tid * 8; i < padded; i += STEP) {
+    uint32_t w[4];
+    load_chunk(x, cols, i, w);
+    *reinterpret_cast<uint2*>(q + byte_of(place, i, padded)) = none ? make_uint2(0, 0) : quantize(w, lift, most);
   }
 }
 
 // -------------------------------------------------------------------------------- few tokens
 struct Params {
-  const int8_t* w;
-  int64_t ws;
-  const float* ts;  // scales of w's rows
-  const int8_t* q;  // [N rounded up to 16, K] (the rows past N are read, and their sums left out)
+  const int8_t* w;  // tiles of the head
+  const float* ts;  // scales of its rows
+  const int8_t* q;  // tiles of the tokens (rows past N are read, and their sums left out)
   const float* ss;
   int N, V, K;      // K: a multiple of 128
   void* out;
@@ -99,51 +144,104 @@ __device__ __forceinline__ float logit(int sum, float s, float t) {
   return (float)sum * s * t;
 }
 
-template <typename T, int NB>  // NB blocks of 16 tokens
-__global__ __launch_bounds__(NT) void head_kernel(Params p) {
-  __shared__ int sums[NB * 16][HEAD_ROWS + 4];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, quad = lane >> 4;
-  const int v0 = blockIdx.x * HEAD_ROWS;
-  for (int i = tid; i < NB * 16 * (HEAD_ROWS + 4); i += NT) (&sums[0][0])[i] = 0;
-  __syncthreads();
+// 16 neighbouring logits of a token, of which `left` exist; `wide`: its row begins at a multiple of 16 bytes.
+template <typename T>
+__device__ __forceinline__ void store_logits(T* o, int left, bool wide, const intx4& c0, const intx4& c1, const intx4& c2,
+                                             const intx4& c3, float s, const float* ts) {
+  const intx4 c[4] = {c0, c1, c2, c3};
+  if (wide && left >= 16) {
+    float r[16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 t = *reinterpret_cast<const float4*>(ts + 4 * i);
+      r[4 * i] = logit<T>(c[i][0], s, t.x), r[4 * i + 1] = logit<T>(c[i][1], s, t.y);
+      r[4 * i + 2] = logit<T>(c[i][2], s, t.z), r[4 * i + 3] = logit<T>(c[i][3], s, t.w);
+    }
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        reinterpret_cast<float4*>(o)[i] = make_float4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        reinterpret_cast<uint4*>(o)[i] = make_uint4(pack_bf16(r[8 * i], r[8 * i + 1]), pack_bf16(r[8 * i + 2], r[8 * i + 3]),
+                                                    pack_bf16(r[8 * i + 4], r[8 * i + 5]), pack_bf16(r[8 * i + 6], r[8 * i + 7]));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (i < left) rows::store_one(o + i, logit<T>(c[i / 4][i % 4], s, ts[i]));
+  }
+}
+
+// A line of a group of 64 rows and of NB blocks of 16 tokens: the fragments of two k-steps.
+template <int NB>
+struct Line {
+  intx4 a[4][2], b[NB][2];
+};
+
+template <typename T, int NB, int SPLIT>  // SPLIT waves share the columns
+__global__ __launch_bounds__(64 * SPLIT) void head_kernel(Params p, bool wide) {
+  __shared__ intx4 parts[SPLIT][4 * NB][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, quad = lane >> 4;
+  const int v0 = blockIdx.x * GROUP, lines = p.K / LINE;
+  const int8_t* w = p.w + (int64_t)v0 * p.K + lane * 16;
+  const int8_t* q = p.q + lane * 16;
   intx4 acc[4][NB];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int b = 0; b < NB; ++b) acc[i][b] = intx4{0, 0, 0, 0};
-  const int8_t* w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = p.w + (int64_t)min(v0 + 16 * i + r16, p.V - 1) * p.ws + 16 * quad;
-  const int8_t* q = p.q + (int64_t)r16 * p.K + 16 * quad;
-  for (int k = wave * LINE; k < p.K; k += NWAVES * LINE) {
-    intx4 a[4][2], b[NB][2];
+    for (int j = 0; j < NB; ++j) acc[i][j] = intx4{0, 0, 0, 0};
+  auto load = [&](int line, Line<NB>& f) {
+    if (line >= lines) return;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a[i][h] = *reinterpret_cast<const intx4*>(w[i] + k + 64 * h);
+      for (int i = 0; i < 4; ++i)
+        f.a[i][h] = __builtin_nontemporal_load(reinterpret_cast<const intx4*>(w + (int64_t)i * 16 * p.K + (2 * line + h) * TILE));
 #pragma unroll
-      for (int i = 0; i < NB; ++i) b[i][h] = *reinterpret_cast<const intx4*>(q + (int64_t)16 * i * p.K + k + 64 * h);
+      for (int j = 0; j < NB; ++j)
+        f.b[j][h] = *reinterpret_cast<const intx4*>(q + (int64_t)j * 16 * p.K + (2 * line + h) * TILE);
     }
+  };
+  auto multiply = [&](int line, const Line<NB>& f) {
+    if (line >= lines) return;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < NB; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i][h], b[j][h], acc[i][j], 0, 0, 0);
+        for (int j = 0; j < NB; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f.a[i][h], f.b[j][h], acc[i][j], 0, 0, 0);
+  };
+  Line<NB> f0, f1;
+  load(wave, f0);
+  for (int line = wave; line < lines; line += 2 * SPLIT) {
+    load(line + SPLIT, f1);
+    multiply(line, f0);
+    load(line + 2 * SPLIT, f0);
+    multiply(line + SPLIT, f1);
   }
-  // lane: rows 4 quad .. + 3 of w, token r16
+  // token block j of the waves' sums is wave j % SPLIT's to finish
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int j = 0; j < NB; ++j)
+    if (j % SPLIT != wave) {
 #pragma unroll
-    for (int j = 0; j < NB; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) atomicAdd(&sums[16 * j + r16][16 * i + 4 * quad + r], acc[i][j][r]);
+      for (int i = 0; i < 4; ++i) parts[wave][4 * j + i][lane] = acc[i][j];
+    }
   __syncthreads();
   T* out = static_cast<T*>(p.out);
-  for (int i = tid; i < NB * 16 * HEAD_ROWS; i += NT) {
-    const int n = i / HEAD_ROWS, v = i % HEAD_ROWS;
-    if (n < p.N && v0 + v < p.V)
-      rows::store_one(out + n * p.os + v0 + v, logit<T>(sums[n][v], p.ss[n], p.ts[v0 + v]));
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    if (j % SPLIT != wave) continue;
+#pragma unroll
+    for (int s = 0; s < SPLIT; ++s)
+      if (s != wave) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i][j] += parts[s][4 * j + i][lane];
+      }
+    const int n = 16 * j + r16, v = v0 + 16 * quad;
+    if (n < p.N && v < p.V)
+      store_logits(out + n * p.os + v, p.V - v, wide, acc[0][j], acc[1][j], acc[2][j], acc[3][j], p.ss[n], p.ts + v);
   }
 }
 
@@ -161,27 +259,19 @@ __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) v
   const int t0 = tb * BN;
 
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds;
-  uint32_t wvo[2], xvo[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = wid * 16 + 8 * i + (lane >> 3), c = (lane & 7) ^ swz(r);
-    wvo[i] = (uint32_t)(r * p.ws) + 16 * c;
-    xvo[i] = (uint32_t)(r * p.K) + 16 * c;
-  }
-  const uint32_t whalf = (uint32_t)(128 * p.ws), xhalf = (uint32_t)(128 * p.K);
+  const int bytes = 16 * p.K;  // of 16 rows
+  const uint32_t mine = (uint32_t)(wid * bytes + lane * 16), half = (uint32_t)(8 * bytes);
   int ld = 0, ld_k = 0, ld_m = mb0 * BM;  // the stage being loaded
-  auto rows_of_w = [&](int r0) { return rsrc(p.w + (int64_t)r0 * p.ws, (uint32_t)(min(BM, p.V - r0) * p.ws)); };
+  auto rows_of_w = [&](int r0) {
+    return rsrc(p.w + (int64_t)r0 * p.K, (uint32_t)((min(BM, p.V - r0) + GROUP - 1) / GROUP * GROUP * p.K));
+  };
   v4i wrs = rows_of_w(ld_m);
-  const v4i xrs = rsrc(p.q + (int64_t)t0 * p.K, (uint32_t)(min(BN, p.N - t0) * p.K));
+  const v4i xrs = rsrc(p.q + (int64_t)t0 * p.K, (uint32_t)((min(BN, p.N - t0) + 15) / 16 * bytes));
   auto load_region = [&](int reg) {
-    const uint32_t dst = lds0 + (uint32_t)((ld & 1) * TL::STAGE + reg * TL::REGION_W + wid * 2048);
-    const uint32_t past = ld >= total ? 1u << 31 : 0u;
-    const uint32_t off = (uint32_t)(ld_k * LINE) + (reg & 1) * (reg < B0 ? whalf : xhalf) + past;
+    const uint32_t dst = lds0 + (uint32_t)((ld & 1) * TL::STAGE + reg * TL::REGION_W + wid * 2 * TILE);
+    const uint32_t off = mine + (uint32_t)(ld_k * 2 * TILE) + (reg & 1) * half + (ld >= total ? 1u << 31 : 0u);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (reg < B0) load_lds(wrs, wvo[i] + off, dst + i * 1024);
-      else load_lds(xrs, xvo[i] + off, dst + i * 1024);
-    }
+    for (int i = 0; i < 2; ++i) load_lds(reg < B0 ? wrs : xrs, off + i * TILE, dst + i * TILE);
   };
   auto next_load_stage = [&]() {
     ++ld;
@@ -193,12 +283,8 @@ __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) v
   };
 
   const int r16 = lane & 15, quad = lane >> 4;
-  uint32_t ra[KS], rb[KS];
-#pragma unroll
-  for (int i = 0; i < KS; ++i) {
-    ra[i] = (uint32_t)((wv * 64 + r16) * ROWB + (((4 * i + quad) ^ swz(r16)) << 4));
-    rb[i] = 2 * TL::REGION_W + (uint32_t)((wt * 32 + r16) * ROWB + (((4 * i + quad) ^ swz(r16)) << 4));
-  }
+  // a region's tiles: those of a row block's two k-steps side by side
+  uint32_t ra = (uint32_t)(wv * 8 * TILE + lane * 16), rb = 2 * TL::REGION_W + (uint32_t)(wt * 4 * TILE + lane * 16);
   intx4 acc[WV][WT];
   intx4 fa[4][KS], fb0[2][KS], fb1[2][KS];
   auto frag = [&](uint32_t off) { return *reinterpret_cast<const intx4*>(lds + off); };
@@ -206,11 +292,11 @@ __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) v
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) fa[i][ks] = frag(ra[ks] + h * TL::REGION_W + i * 16 * ROWB);
+      for (int i = 0; i < 4; ++i) fa[i][ks] = frag(ra + h * TL::REGION_W + (2 * i + ks) * TILE);
   };
   auto read_x = [&](intx4 (&fb)[2][KS], int ks, int h) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) fb[i][ks] = frag(rb[ks] + h * TL::REGION_X + i * 16 * ROWB);
+    for (int i = 0; i < 2; ++i) fb[i][ks] = frag(rb + h * TL::REGION_X + (2 * i + ks) * TILE);
   };
   auto multiply = [&](auto first, int h, int j, const intx4 (&fb)[2][KS], auto&& after) {
     __builtin_amdgcn_s_setprio(1);
@@ -254,12 +340,9 @@ __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) v
     multiply(first, 1, 1, fb1, nothing);
     barrier();
 
-#pragma unroll
-    for (int i = 0; i < KS; ++i) {
-      ra[i] ^= TL::STAGE;
-      rb[i] ^= TL::STAGE;
-      asm volatile("" : "+v"(ra[i]), "+v"(rb[i]));  // here, not among the multiplies
-    }
+    ra ^= TL::STAGE;
+    rb ^= TL::STAGE;
+    asm volatile("" : "+v"(ra), "+v"(rb));  // here, not among the multiplies
     load_region(A0);
     wait_loads<TL::AHEAD>();
     barrier();
@@ -286,7 +369,7 @@ __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) v
       barrier();
       stage(std::false_type{});
     }
-    // lane: four consecutive rows of w and one token of each block
+    // lane: 16 neighbouring logits of one token of each block, in either half of the rows
 #pragma unroll
     for (int j = 0; j < WT; ++j) {
       int n = t0 + wt * 32 + col_off<TL>(j) + r16;
@@ -294,22 +377,10 @@ __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) v
       if (n >= p.N) continue;
       const float s = p.ss[n];
 #pragma unroll
-      for (int i = 0; i < WV; ++i) {
-        const int m = mb * BM + wv * 64 + row_off<TL>(i, 0) + 4 * quad;
-        const intx4 c = acc[i][j];
-        T* o = out + (int64_t)n * p.os + m;
-        if (WIDE && m + 4 <= p.V) {
-          const float4 t = *reinterpret_cast<const float4*>(p.ts + m);
-          const float r[4] = {logit<T>(c[0], s, t.x), logit<T>(c[1], s, t.y), logit<T>(c[2], s, t.z), logit<T>(c[3], s, t.w)};
-          if constexpr (sizeof(T) == 4)
-            *reinterpret_cast<float4*>(o) = make_float4(r[0], r[1], r[2], r[3]);
-          else
-            *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16(r[0], r[1]), pack_bf16(r[2], r[3]));
-        } else {
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (m + r < p.V) rows::store_one(o + r, logit<T>(c[r], s, p.ts[m + r]));
-        }
+      for (int i = 0; i < WV; i += 4) {
+        const int m = mb * BM + wv * 64 + row_off<TL>(i, 0) + 16 * quad;
+        if (m < p.V)
+          store_logits(out + (int64_t)n * p.os + m, p.V - m, WIDE, acc[i][j], acc[i + 1][j], acc[i + 2][j], acc[i + 3][j], s, p.ts + m);
       }
     }
     barrier();
@@ -339,27 +410,30 @@ int check_head(const dsv41_int_head_desc* d) {
   if (d->out_dtype != DSV41_DTYPE_F32 && d->out_dtype != DSV41_DTYPE_BF16) return fail(DSV41_E_INVALID, "logits must be fp32 or bf16");
   if (d->x_row_stride < d->hidden || d->out_row_stride < d->vocab)
     return fail(DSV41_E_INVALID, "8-bit head: row strides must cover the rows");
-  if (d->w_row_stride < padded_of(d->hidden) || d->w_row_stride % LINE || (uintptr_t)d->w % 16)
-    return fail(DSV41_E_INVALID, "8-bit head: rows of w are 16-byte aligned, and padded to a multiple of 128 columns");
+  if ((uintptr_t)d->w % 16) return fail(DSV41_E_INVALID, "8-bit head: the tiles must be 16-byte aligned");
   if ((uintptr_t)d->x % 2 || (uintptr_t)d->scales % 16 || (uintptr_t)d->out % (d->out_dtype == DSV41_DTYPE_F32 ? 4 : 2))
     return fail(DSV41_E_INVALID, "8-bit head: operands are not aligned to their type, or the scales not to 16 bytes");
-  if (256 * d->w_row_stride >= (1ll << 31)) return fail(DSV41_E_UNSUPPORTED, "row stride too large for 32-bit block offsets");
   if ((int64_t)d->n_tokens > MAX_GRID) return fail(DSV41_E_UNSUPPORTED, "8-bit head: the batch is too large for one call");
   return DSV41_OK;
 }
 
 size_t scales_at(const dsv41_int_head_desc* d) { return (size_t)((d->n_tokens + 15) / 16 * 16) * padded_of(d->hidden); }
 
+template <typename T, int NB>
+void launch_few(const Params& p, bool wide, hipStream_t s) {
+  const dim3 grid((p.V + GROUP - 1) / GROUP);
+  if (p.K >= 32 * LINE) hipLaunchKernelGGL((head_kernel<T, NB, 8>), grid, dim3(512), 0, s, p, wide);
+  else hipLaunchKernelGGL((head_kernel<T, NB, 4>), grid, dim3(256), 0, s, p, wide);
+}
 template <typename T>
 void launch(const Params& p, hipStream_t s) {
-  const dim3 few((p.V + HEAD_ROWS - 1) / HEAD_ROWS);
-  if (p.N <= 16) hipLaunchKernelGGL((head_kernel<T, 1>), few, dim3(NT), 0, s, p);
-  else if (p.N <= 32) hipLaunchKernelGGL((head_kernel<T, 2>), few, dim3(NT), 0, s, p);
-  else if (p.N <= 48) hipLaunchKernelGGL((head_kernel<T, 3>), few, dim3(NT), 0, s, p);
-  else if (p.N <= FEW) hipLaunchKernelGGL((head_kernel<T, 4>), few, dim3(NT), 0, s, p);
+  const bool wide = p.os * sizeof(T) % 16 == 0 && (uintptr_t)p.out % 16 == 0;
+  if (p.N <= 16) launch_few<T, 1>(p, wide, s);
+  else if (p.N <= 32) launch_few<T, 2>(p, wide, s);
+  else if (p.N <= 48) launch_few<T, 3>(p, wide, s);
+  else if (p.N <= FEW) launch_few<T, 4>(p, wide, s);
   else {
     const dim3 grid((p.n_tb * p.ranges + 7) / 8 * 8);
-    const bool wide = p.os % 4 == 0 && (uintptr_t)p.out % (4 * sizeof(T)) == 0;
     if (wide) hipLaunchKernelGGL((gemm_kernel<T, true>), grid, dim3(NT), 0, s, p);
     else hipLaunchKernelGGL((gemm_kernel<T, false>), grid, dim3(NT), 0, s, p);
   }
@@ -371,18 +445,17 @@ void launch(const Params& p, hipStream_t s) {
 using namespace dsv41;
 using namespace dsv41::inthead;
 
-extern "C" int dsv41_quantize_rows_run(const void* x, int64_t xs, int rows, int cols, int8_t* q, int64_t qs, float* scales,
-                                       int32_t* status, void* stream) {
+extern "C" int dsv41_quantize_rows_run(const void* x, int64_t xs, int rows, int cols, int8_t* q, float* scales, int32_t* status,
+                                       void* stream) {
   if (int rc = check_cols(cols)) return rc;
-  if (rows < 0 || xs < cols || qs < padded_of(cols) || qs % 16)
-    return fail(DSV41_E_INVALID, "quantize: row strides must cover the rows, padded to a multiple of 128 columns");
+  if (rows < 0 || xs < cols) return fail(DSV41_E_INVALID, "quantize: the row stride must cover the rows");
   if (rows > 0 && (!x || !q || !scales)) return fail(DSV41_E_INVALID, "quantize: x, q and scales are required");
   if ((uintptr_t)x % 2 || (uintptr_t)q % 16 || (uintptr_t)scales % 4)
     return fail(DSV41_E_INVALID, "quantize: operands are not aligned");
   if (rows > MAX_GRID) return fail(DSV41_E_UNSUPPORTED, "quantize: too many rows for one call");
   if (rows == 0) return DSV41_OK;
-  hipLaunchKernelGGL(quantize_kernel, dim3(rows), dim3(QUANT_NT), 0, static_cast<hipStream_t>(stream),
-                     static_cast<const bf16_t*>(x), xs, cols, q, qs, padded_of(cols), scales, status);
+  hipLaunchKernelGGL(quantize_kernel<true>, dim3(rows), dim3(QUANT_NT), 0, static_cast<hipStream_t>(stream),
+                     static_cast<const bf16_t*>(x), xs, cols, q, padded_of(cols), scales, status);
   DSV41_HIP_CHECK(hipGetLastError());
   return DSV41_OK;
 }
@@ -401,11 +474,10 @@ extern "C" int dsv41_int_head_run(const dsv41_int_head_desc* d, void* workspace,
   float* ss = reinterpret_cast<float*>(q + at);
   const int K = padded_of(d->hidden);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(quantize_kernel, dim3(d->n_tokens), dim3(QUANT_NT), 0, s, static_cast<const bf16_t*>(d->x),
-                     d->x_row_stride, d->hidden, q, (int64_t)K, K, ss, d->out_status);
+  hipLaunchKernelGGL(quantize_kernel<false>, dim3(d->n_tokens), dim3(QUANT_NT), 0, s, static_cast<const bf16_t*>(d->x),
+                     d->x_row_stride, d->hidden, q, K, ss, d->out_status);
   Params p{};
   p.w = d->w;
-  p.ws = d->w_row_stride;
   p.ts = d->scales;
   p.q = q;
   p.ss = ss;

@@ -398,7 +398,6 @@ class IntHeadDesc(ctypes.Structure):
         ("x", ctypes.c_void_p),
         ("x_row_stride", ctypes.c_int64),
         ("w", ctypes.c_void_p),
-        ("w_row_stride", ctypes.c_int64),
         ("scales", ctypes.c_void_p),
         ("out", ctypes.c_void_p),
         ("out_row_stride", ctypes.c_int64),
@@ -604,7 +603,7 @@ def _bind(lib: ctypes.CDLL) -> ctypes.CDLL:
         run.argtypes = [ctypes.POINTER(cls), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
     lib.dsv41_quantize_rows_run.restype = ctypes.c_int
     lib.dsv41_quantize_rows_run.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
-                                            ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
+                                            ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
     lib.dsv41_check_wait.restype = ctypes.c_int
     lib.dsv41_check_wait.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
                                     ctypes.c_void_p, ctypes.c_void_p]

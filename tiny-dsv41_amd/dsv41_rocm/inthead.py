@@ -19,18 +19,20 @@ from . import _lib
 from ._check import any_set
 from .scores import fit_int32, launch, refuse_capture, refuse_tangents, written
 
-LINE = 128  # columns are padded to whole cache lines
+LINE, GROUP = 128, 64  # columns and rows are rounded up to these
 
 _OUT_DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 
 
 @dataclass(frozen=True)
 class Int8Head:
-    """A head ``[vocab, hidden]`` whose row ``v`` is ``scales[v] * weight[v]``: int8 ``weight``, a view of rows that
-    are padded to a multiple of 128 columns, and fp32 ``scales``."""
+    """A head ``[vocab, hidden]`` whose row ``v`` is ``scales[v]`` times int8 integers: ``tiles`` holds them in the
+    order in which the kernels read them, ``scales`` is fp32.  :meth:`integers` gives them back as rows."""
 
-    weight: torch.Tensor
+    tiles: torch.Tensor
     scales: torch.Tensor
+    vocab: int
+    hidden: int
 
     @staticmethod
     def from_quantized(weight: torch.Tensor, scales: torch.Tensor) -> "Int8Head":
@@ -42,17 +44,21 @@ class Int8Head:
         if scales.shape != weight.shape[:1] or not scales.is_floating_point():
             raise ValueError("scales must have one value per row of weight")
         v, h = weight.shape
-        rows = _padded(v, h, weight.device)
-        rows[:, :h] = weight
-        return Int8Head(rows[:, :h], scales.detach().to(device=weight.device, dtype=torch.float32, copy=True).contiguous())
+        tiles = torch.zeros(_rounded(v, GROUP), _rounded(h, LINE), dtype=torch.int8, device=weight.device)
+        tiles[:v, :h] = weight
+        # group, (tile, row in four) of a group, four in a tile; column tile, 16 columns of it
+        tiles = tiles.view(-1, 4, 4, 4, tiles.shape[1] // 64, 4, 16).permute(0, 2, 4, 5, 1, 3, 6).contiguous()
+        scales = scales.detach().to(device=weight.device, dtype=torch.float32, copy=True).contiguous()
+        return Int8Head(tiles.view(-1), scales, v, h)
+
+    def integers(self) -> torch.Tensor:
+        """The int8 rows ``[vocab, hidden]`` (a copy)."""
+        t = self.tiles.view(-1, 4, _rounded(self.hidden, LINE) // 64, 4, 4, 4, 16).permute(0, 4, 1, 5, 2, 3, 6)
+        return t.reshape(_rounded(self.vocab, GROUP), -1)[:self.vocab, :self.hidden].contiguous()
 
 
-def _padded(rows, columns, device):
-    width = (columns + LINE - 1) // LINE * LINE
-    out = torch.empty(rows, width, dtype=torch.int8, device=device)
-    if width != columns:
-        out[:, columns:].zero_()
-    return out
+def _rounded(n, unit):
+    return (n + unit - 1) // unit * unit
 
 
 def _rows(x, name):
@@ -85,14 +91,14 @@ def quantize_head(weight: torch.Tensor, *, check: bool = True) -> Int8Head:
     if v == 0 or h == 0:
         raise ValueError("weight must be [vocab, hidden]")
     refuse_capture(check)
-    rows = _padded(v, h, w.device)
+    tiles = torch.zeros(_rounded(v, GROUP) * _rounded(h, LINE), dtype=torch.int8, device=w.device)
     scales = torch.empty(v, dtype=torch.float32, device=w.device)
     status = torch.empty(v, dtype=torch.int32, device=w.device) if check else None
     launch(_lib.load().dsv41_quantize_rows_run, w.device, w.data_ptr(), w.stride(0) if v > 1 else h, v, h,
-           rows.data_ptr(), rows.stride(0), scales.data_ptr(), None if status is None else status.data_ptr())
+           tiles.data_ptr(), scales.data_ptr(), None if status is None else status.data_ptr())
     if check and any_set(status)[0]:
         raise ValueError("weight contains non-finite values")
-    return Int8Head(rows[:, :h], scales)
+    return Int8Head(tiles, scales, v, h)
 
 
 def head_logits(
@@ -118,15 +124,14 @@ def head_logits(
     infinity; without, their rows are NaN.
     """
     x = _rows(hidden, "hidden")
-    w, scales = head.weight, head.scales
-    v, h = w.shape
+    w, scales, v, h = head.tiles, head.scales, head.vocab, head.hidden
     n = x.shape[0]
     if x.shape[1] != h:
         raise ValueError("hidden must be [tokens, hidden] and the head [vocab, hidden]")
-    if w.device != x.device:
+    if w.device != x.device or scales.device != x.device:
         raise ValueError("hidden and the head must be on the same GPU")
-    if w.dtype != torch.int8 or w.stride(1) != 1 or w.stride(0) % LINE or w.stride(0) < h or scales.dtype != torch.float32 or \
-            scales.shape != (v,) or not scales.is_contiguous():
+    if w.dtype != torch.int8 or not w.is_contiguous() or w.numel() != _rounded(v, GROUP) * _rounded(h, LINE) or \
+            scales.dtype != torch.float32 or scales.shape != (v,) or not scales.is_contiguous():
         raise ValueError("the head is not in the kernels' layout: make it with quantize_head or Int8Head.from_quantized")
     given = out
     if out is not None:
@@ -144,7 +149,7 @@ def head_logits(
     status = torch.empty(n, dtype=torch.int32, device=x.device) if check else None
     if n:
         d = _lib.IntHeadDesc(ctypes.sizeof(_lib.IntHeadDesc), n, h, v, x.data_ptr(), x.stride(0) if n > 1 else h,
-                             w.data_ptr(), w.stride(0), scales.data_ptr(), out.data_ptr(), out.stride(0) if n > 1 else max(v, out.stride(0)),
+                             w.data_ptr(), scales.data_ptr(), out.data_ptr(), out.stride(0) if n > 1 else max(v, out.stride(0)),
                              _OUT_DTYPES[out.dtype], None if status is None else status.data_ptr())
         lib = _lib.load()
         ref = ctypes.byref(d)
