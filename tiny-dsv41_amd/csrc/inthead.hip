@@ -144,111 +144,160 @@ __device__ __forceinline__ float logit(int sum, float s, float t) {
   return (float)sum * s * t;
 }
 
-// 16 neighbouring logits of a token, of which `left` exist; `wide`: its row begins at a multiple of 16 bytes.
+// The four rows of 16 lanes of b and a's, transposed as 2 x 2 blocks: a keeps its even rows and takes b's even rows for its
+// odd ones (permlane16), its lower half and b's lower half for its upper one (permlane32).
+__device__ __forceinline__ void swap_rows(uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+  a = r[0], b = r[1];
+}
+__device__ __forceinline__ void swap_halves(uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  a = r[0], b = r[1];
+}
+// 64 neighbouring logits, from column v on, of each of 16 tokens: lane (quad, token) has columns 16 quad .. + 15 in
+// c0 .. c3.  The quads exchange theirs, so that a store of 16 bytes a lane writes 64 neighbouring bytes of a token's row
+// (4096 tokens, 2048 -> 151936: fp32 1573 us without, bf16 1133).  All lanes take part; those of tokens that do not
+// exist (there == false) store nothing.  `wide`: rows begin at multiples of 16 bytes.
 template <typename T>
-__device__ __forceinline__ void store_logits(T* o, int left, bool wide, const intx4& c0, const intx4& c1, const intx4& c2,
-                                             const intx4& c3, float s, const float* ts) {
+__device__ __forceinline__ void store_logits(T* row, int v, int V, bool there, bool wide, const intx4& c0, const intx4& c1,
+                                             const intx4& c2, const intx4& c3, float s, const float* ts) {
   const intx4 c[4] = {c0, c1, c2, c3};
-  if (wide && left >= 16) {
-    float r[16];
+  const int quad = (threadIdx.x & 63) >> 4;
+  constexpr int E = 16 / sizeof(T), PARTS = 16 / E;  // elements of a store, stores
+  uint32_t w[PARTS][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float4 t = *reinterpret_cast<const float4*>(ts + 4 * i);
-      r[4 * i] = logit<T>(c[i][0], s, t.x), r[4 * i + 1] = logit<T>(c[i][1], s, t.y);
-      r[4 * i + 2] = logit<T>(c[i][2], s, t.z), r[4 * i + 3] = logit<T>(c[i][3], s, t.w);
-    }
+  for (int i = 0; i < 4; ++i) {
+    const float4 t = *reinterpret_cast<const float4*>(ts + 4 * i);
+    const float r0 = logit<T>(c[i][0], s, t.x), r1 = logit<T>(c[i][1], s, t.y);
+    const float r2 = logit<T>(c[i][2], s, t.z), r3 = logit<T>(c[i][3], s, t.w);
     if constexpr (sizeof(T) == 4) {
+      w[i][0] = __float_as_uint(r0), w[i][1] = __float_as_uint(r1), w[i][2] = __float_as_uint(r2), w[i][3] = __float_as_uint(r3);
+    } else {
+      w[i / 2][i % 2 * 2] = pack_bf16(r0, r1), w[i / 2][i % 2 * 2 + 1] = pack_bf16(r2, r3);
+    }
+  }
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        reinterpret_cast<float4*>(o)[i] = make_float4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+  for (int k = 0; k < 4; ++k) {
+#pragma unroll
+    for (int i = 0; i < PARTS; i += 2) swap_rows(w[i][k], w[i + 1][k]);
+    if constexpr (PARTS == 4) {
+      swap_halves(w[0][k], w[2][k]);
+      swap_halves(w[1][k], w[3][k]);
+    } else {
+      swap_halves(w[0][k], w[1][k]);
+    }
+  }
+  if (!there) return;
+#pragma unroll
+  for (int i = 0; i < PARTS; ++i) {
+    const int at = v + (4 * i + quad) * E, left = V - at;
+    if (wide && left >= E) {
+      *reinterpret_cast<uint4*>(row + at) = make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]);
     } else {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        reinterpret_cast<uint4*>(o)[i] = make_uint4(pack_bf16(r[8 * i], r[8 * i + 1]), pack_bf16(r[8 * i + 2], r[8 * i + 3]),
-                                                    pack_bf16(r[8 * i + 4], r[8 * i + 5]), pack_bf16(r[8 * i + 6], r[8 * i + 7]));
+      for (int j = 0; j < E; ++j)
+        if (j < left) {
+          if constexpr (sizeof(T) == 4) row[at + j] = __uint_as_float(w[i][j]);
+          else row[at + j].v = (uint16_t)(w[i][j / 2] >> (16 * (j % 2)));
+        }
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (i < left) rows::store_one(o + i, logit<T>(c[i / 4][i % 4], s, ts[i]));
   }
 }
 
-// A line of a group of 64 rows and of NB blocks of 16 tokens: the fragments of two k-steps.
+// The fragments of one k-step: of a group of 64 rows and of NB blocks of 16 tokens.
 template <int NB>
-struct Line {
-  intx4 a[4][2], b[NB][2];
+struct Step {
+  intx4 a[4], b[NB];
 };
 
-template <typename T, int NB, int SPLIT>  // SPLIT waves share the columns
-__global__ __launch_bounds__(64 * SPLIT) void head_kernel(Params p, bool wide) {
+// SPLIT waves share the columns of a group, every SPLIT-th k-step each; a workgroup takes group after group, with
+// DEPTH - 1 steps of each wave on their way from memory throughout.
+template <typename T, int NB, int SPLIT, int DEPTH, int PER_CU>
+__global__ __launch_bounds__(64 * SPLIT, SPLIT * PER_CU / 4) void head_kernel(Params p, bool wide) {
   __shared__ intx4 parts[SPLIT][4 * NB][64];
+  __shared__ float scales[SPLIT][GROUP];  // each wave's copy of the group's
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, quad = lane >> 4;
-  const int v0 = blockIdx.x * GROUP, lines = p.K / LINE;
-  const int8_t* w = p.w + (int64_t)v0 * p.K + lane * 16;
-  const int8_t* q = p.q + lane * 16;
-  intx4 acc[4][NB];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < NB; ++j) acc[i][j] = intx4{0, 0, 0, 0};
-  auto load = [&](int line, Line<NB>& f) {
-    if (line >= lines) return;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        f.a[i][h] = __builtin_nontemporal_load(reinterpret_cast<const intx4*>(w + (int64_t)i * 16 * p.K + (2 * line + h) * TILE));
-#pragma unroll
-      for (int j = 0; j < NB; ++j)
-        f.b[j][h] = *reinterpret_cast<const intx4*>(q + (int64_t)j * 16 * p.K + (2 * line + h) * TILE);
-    }
-  };
-  auto multiply = [&](int line, const Line<NB>& f) {
-    if (line >= lines) return;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < NB; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f.a[i][h], f.b[j][h], acc[i][j], 0, 0, 0);
-  };
-  Line<NB> f0, f1;
-  load(wave, f0);
-  for (int line = wave; line < lines; line += 2 * SPLIT) {
-    load(line + SPLIT, f1);
-    multiply(line, f0);
-    load(line + 2 * SPLIT, f0);
-    multiply(line + SPLIT, f1);
-  }
-  // token block j of the waves' sums is wave j % SPLIT's to finish
-#pragma unroll
-  for (int j = 0; j < NB; ++j)
-    if (j % SPLIT != wave) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) parts[wave][4 * j + i][lane] = acc[i][j];
-    }
-  __syncthreads();
+  const int steps = p.K / 64, turns = (steps + SPLIT * DEPTH - 1) / (SPLIT * DEPTH) * DEPTH, groups = (p.V + GROUP - 1) / GROUP;
   T* out = static_cast<T*>(p.out);
+  intx4 acc[4][NB];
+  auto clear = [&]() {
 #pragma unroll
-  for (int j = 0; j < NB; ++j) {
-    if (j % SPLIT != wave) continue;
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int s = 0; s < SPLIT; ++s)
-      if (s != wave) {
+      for (int j = 0; j < NB; ++j) acc[i][j] = intx4{0, 0, 0, 0};
+  };
+  clear();
+  Step<NB> f[DEPTH];
+  int at = wave, left = turns, ahead = blockIdx.x;  // the step to load, those left of its group, the group
+  const int8_t* w = p.w + (int64_t)ahead * GROUP * p.K;  // (the same in all lanes, which add theirs in 32 bits)
+  // (a step that is none reads the first bytes of q, which all caches hold: loads under a condition cost registers)
+  auto load = [&](Step<NB>& s) {
+    const bool some = ahead < groups && at < steps;
+    const int8_t *wa = some ? w + at * TILE : p.q, *qa = p.q + (some ? at * TILE : 0);
+    const int64_t wide_step = some ? (int64_t)16 * p.K : 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i][j] += parts[s][4 * j + i][lane];
+    for (int i = 0; i < 4; ++i) s.a[i] = __builtin_nontemporal_load(reinterpret_cast<const intx4*>(wa + i * wide_step) + lane);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) s.b[j] = reinterpret_cast<const intx4*>(qa + j * wide_step)[lane];
+    at += SPLIT;
+    if (--left == 0) {
+      at = wave, left = turns, ahead += gridDim.x;
+      w += (int64_t)gridDim.x * GROUP * p.K;
+    }
+  };
+#pragma unroll
+  for (int d = 0; d < DEPTH - 1; ++d) load(f[d]);
+  float ss[NB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) ss[j] = p.ss[min(16 * j + r16, p.N - 1)];
+  for (int group = blockIdx.x; group < groups; group += gridDim.x) {
+    // (read at the end, it would have the wave wait for all steps on their way)
+    const float t = p.ts[min(group * GROUP + lane, p.V - 1)];
+    for (int turn = 0; turn < turns; turn += DEPTH) {
+#pragma unroll
+      for (int d = 0; d < DEPTH; ++d) {
+        load(f[(d + DEPTH - 1) % DEPTH]);
+        if (wave + (turn + d) * SPLIT < steps) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[d].a[i], f[d].b[j], acc[i][j], 0, 0, 0);
+        }
       }
-    const int n = 16 * j + r16, v = v0 + 16 * quad;
-    if (n < p.N && v < p.V)
-      store_logits(out + n * p.os + v, p.V - v, wide, acc[0][j], acc[1][j], acc[2][j], acc[3][j], p.ss[n], p.ts + v);
+    }
+    // the waves' sums meet: token block j is wave j % SPLIT's to finish
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      if (j % SPLIT != wave) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) parts[wave][4 * j + i][lane] = acc[i][j];
+      }
+    scales[wave][lane] = t;
+    rows::lds_barrier();
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      if (j % SPLIT != wave) continue;
+#pragma unroll
+      for (int s = 0; s < SPLIT; ++s)
+        if (s != wave) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[i][j] += parts[s][4 * j + i][lane];
+        }
+      const int n = 16 * j + r16;
+      store_logits(out + n * p.os, group * GROUP, p.V, n < p.N, wide, acc[0][j], acc[1][j], acc[2][j], acc[3][j], ss[j],
+                   scales[wave] + 16 * quad);
+    }
+    rows::lds_barrier();
+    clear();
   }
 }
 
 // ------------------------------------------------------------------------------- many tokens
 template <typename T, bool WIDE>  // WIDE: rows of the output take 4 elements at once
 __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_kernel(Params p) {
-  __shared__ __align__(1024) unsigned char lds[2 * TL::STAGE];
+  // two stages, and for each wave the scales of the block's rows: read from memory between the multiplies, they would
+  // have the wave wait for its stores
+  __shared__ __align__(1024) unsigned char lds[2 * TL::STAGE + NWAVES * BM * 4];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wv = wid % SQUARE, wt = wid / SQUARE;
   int tb, range;
@@ -267,6 +316,11 @@ __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) v
   };
   v4i wrs = rows_of_w(ld_m);
   const v4i xrs = rsrc(p.q + (int64_t)t0 * p.K, (uint32_t)((min(BN, p.N - t0) + 15) / 16 * bytes));
+  const v4i srs = rsrc(p.ts, (uint32_t)p.V * 4);
+  float* scales = reinterpret_cast<float*>(lds + 2 * TL::STAGE) + wid * BM;
+  auto load_scales = [&](int mb) {
+    load_lds(srs, (uint32_t)(mb * BM * 4 + lane * 16), lds0 + (uint32_t)(2 * TL::STAGE + wid * BM * 4));
+  };
   auto load_region = [&](int reg) {
     const uint32_t dst = lds0 + (uint32_t)((ld & 1) * TL::STAGE + reg * TL::REGION_W + wid * 2 * TILE);
     const uint32_t off = mine + (uint32_t)(ld_k * 2 * TILE) + (reg & 1) * half + (ld >= total ? 1u << 31 : 0u);
@@ -349,6 +403,12 @@ __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) v
     multiply(first, 1, 0, fb0, [&](int ks) { read_x(fb0, ks, 0); });
   };
 
+  float ss[WT];  // scales of the lane's tokens
+#pragma unroll
+  for (int j = 0; j < WT; ++j) ss[j] = p.ss[min(t0 + wt * 32 + col_off<TL>(j) + r16, p.N - 1)];
+#pragma unroll
+  for (int j = 0; j < WT; ++j) asm volatile("" ::"v"(ss[j]));  // here, with no load behind them yet
+
   load_region(B0);
   load_region(A0);
   load_region(B1);
@@ -364,6 +424,7 @@ __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) v
 
   T* out = static_cast<T*>(p.out);
   for (int mb = mb0; mb < mb1; ++mb) {
+    load_scales(mb);  // here by the end of the next stage, whose loads are all younger
     stage(std::true_type{});
     for (int k = 1; k < nst; ++k) {
       barrier();
@@ -374,13 +435,11 @@ __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) v
     for (int j = 0; j < WT; ++j) {
       int n = t0 + wt * 32 + col_off<TL>(j) + r16;
       asm volatile("" : "+v"(n));  // addresses are formed here, not kept across the blocks
-      if (n >= p.N) continue;
-      const float s = p.ss[n];
 #pragma unroll
       for (int i = 0; i < WV; i += 4) {
-        const int m = mb * BM + wv * 64 + row_off<TL>(i, 0) + 16 * quad;
-        if (m < p.V)
-          store_logits(out + (int64_t)n * p.os + m, p.V - m, WIDE, acc[i][j], acc[i + 1][j], acc[i + 2][j], acc[i + 3][j], s, p.ts + m);
+        const int m = wv * 64 + row_off<TL>(i, 0);
+        store_logits(out + (int64_t)n * p.os, mb * BM + m, p.V, n < p.N, WIDE, acc[i][j], acc[i + 1][j], acc[i + 2][j],
+                     acc[i + 3][j], ss[j], scales + m + 16 * quad);
       }
     }
     barrier();
@@ -419,11 +478,15 @@ int check_head(const dsv41_int_head_desc* d) {
 
 size_t scales_at(const dsv41_int_head_desc* d) { return (size_t)((d->n_tokens + 15) / 16 * 16) * padded_of(d->hidden); }
 
+// As many workgroups as fit on the GPU together take the same number of groups each.  Four waves with three
+// steps ahead, two workgroups a CU: 2048 -> 151936, 1, 17, 48 and 64 tokens 52, 57, 64 and 68 us, 7168 -> 129280 151,
+// 164, 182 and 199.  Eight waves: 54, 59, 68, 72 and 155, 174, 193, 208; two (four workgroups): 57, 63, 70, 75 and 153,
+// 162, 177, 193; five steps ahead 60, 69, 77, 89 and 152, 167, 186, 222.
+constexpr int SPLIT = 4, DEPTH = 4, PER_CU = 2;
 template <typename T, int NB>
 void launch_few(const Params& p, bool wide, hipStream_t s) {
-  const dim3 grid((p.V + GROUP - 1) / GROUP);
-  if (p.K >= 32 * LINE) hipLaunchKernelGGL((head_kernel<T, NB, 8>), grid, dim3(512), 0, s, p, wide);
-  else hipLaunchKernelGGL((head_kernel<T, NB, 4>), grid, dim3(256), 0, s, p, wide);
+  const int groups = (p.V + GROUP - 1) / GROUP, slots = PER_CU * CU_COUNT, rounds = (groups + slots - 1) / slots;
+  hipLaunchKernelGGL((head_kernel<T, NB, SPLIT, DEPTH, PER_CU>), dim3((groups + rounds - 1) / rounds), dim3(64 * SPLIT), 0, s, p, wide);
 }
 template <typename T>
 void launch(const Params& p, hipStream_t s) {
