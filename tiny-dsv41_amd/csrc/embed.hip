@@ -7,14 +7,14 @@
 //
 // The gradient in three kernels, none of which adds into memory that another writes, so its bits do not
 // depend on the order in which workgroups run:
-//   sort_kernel   the batch's positions ordered by (id, position).  A workgroup owns RANGE ids and reads all
+//   sort_kernel   the batch's positions ordered by (id, position).  A workgroup owns `range` ids and reads all
 //                 ids of the batch (from its L2): it counts its own, wave by wave, and how many lie below
 //                 its range, so it knows where its part of the sorted list begins without hearing from the
 //                 others; then each wave places its tokens in their order.
-//   sum_kernel    a chunk of CHUNK positions of the sorted list at a time, a strip of the columns: rows of
+//   sum_kernel    a wave takes a chunk of CHUNK positions of the sorted list and a strip of the columns: rows of
 //                 g summed while the id stays the same.  An id whose tokens all lie within the chunk is
 //                 finished there; one that reaches over its ends leaves a partial row.  Other workgroups
-//                 of the same launch write zeros where no token is.
+//                 of the same launch write zeros where no token is, which is most of a dense gradient's time.
 //   join_kernel   the partial rows of an id that reaches over chunks, in their order.
 
 #include <math.h>
@@ -31,10 +31,11 @@ using rows::Elem;
 
 constexpr int COPY_NT = 256;
 constexpr int SORT_NT = 1024, SORT_WAVES = SORT_NT / 64;
-constexpr int RANGE = 512;    // ids of a sorting workgroup
-constexpr int SUM_NT = 128;
-constexpr int CHUNK = 32;     // sorted positions of a summing workgroup
-constexpr int ZERO_ROWS = 8;  // rows of the table that a zeroing workgroup looks at
+constexpr int RANGE = 512;    // ids of a sorting workgroup, at most
+constexpr int SUM_NT = 256, SUM_WAVES = SUM_NT / 64;
+constexpr int CHUNK = 32;     // sorted positions of a summing wave
+constexpr int ZERO_ROWS = 16; // rows of the table of a zeroing workgroup
+constexpr int JOIN_NT = 128;
 constexpr int64_t MAX_GRID = 1 << 22;
 
 template <typename T>
@@ -76,17 +77,27 @@ __global__ __launch_bounds__(COPY_NT) void copy_kernel(CopyParams p) {
   const bool some = id >= 0 && !bad;
   const T* w = static_cast<const T*>(p.w) + (some ? id * p.ws : 0);
   T* out = static_cast<T*>(p.out) + n * p.os;
-  for (int i = lane * G; i < p.H; i += p.lanes * G) {
-    float v[G];
-    if (some) load_group(w + i, p.H - i, v);
+  constexpr int U = 4;
+  for (int i0 = lane * G; i0 < p.H; i0 += U * p.lanes * G) {
+    float v[U][G];
 #pragma unroll
-    for (int j = 0; j < G; ++j) v[j] = some ? v[j] * p.scale : instead;
-    if (p.H - i >= G) {
-      rows::store_full(out + i, 0, v);
-    } else {
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * p.lanes * G;
+      if (some && i < p.H) load_group(w + i, p.H - i, v[u]);
+    }
 #pragma unroll
-      for (int j = 0; j < G; ++j)
-        if (i + j < p.H) rows::store_one(out + i + j, v[j]);
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * p.lanes * G;
+      if (i >= p.H) break;
+#pragma unroll
+      for (int j = 0; j < G; ++j) v[u][j] = some ? v[u][j] * p.scale : instead;
+      if (p.H - i >= G) {
+        rows::store_full(out + i, 0, v[u]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < G; ++j)
+          if (i + j < p.H) rows::store_one(out + i + j, v[u][j]);
+      }
     }
   }
 }
@@ -99,7 +110,7 @@ struct GradParams {
   float scale;
   void* out;
   int64_t os;
-  int ranges, chunks, strips, zeros;
+  int range, chunks, strips;
   int32_t* total;     // [1] tokens with a row
   int32_t* place;     // [n] positions sorted by (id, position)
   int32_t* name;      // [n] their ids
@@ -107,22 +118,41 @@ struct GradParams {
   float* part;        // [chunks, 2, H]: of the id that reaches into the chunk, and of the one that reaches beyond
 };
 
+// n elements from p on become 0: 16-byte stores from the first of their boundaries on, by the workgroup.
+template <typename T>
+__device__ __forceinline__ void clear_row(T* p, int64_t n) {
+  constexpr int G = 16 / sizeof(T);
+  const int tid = threadIdx.x, head = (int)min(n, (int64_t)((16 - ((uintptr_t)p & 15)) & 15) / (int)sizeof(T));
+  if (tid < head) rows::store_one(p + tid, 0.f);
+  uint4* q = reinterpret_cast<uint4*>(p + head);
+  const int64_t groups = (n - head) / G;
+  for (int64_t i = tid; i < groups; i += SUM_NT) q[i] = make_uint4(0, 0, 0, 0);
+  const int64_t tail = head + groups * G + tid;
+  if (tid < G && tail < n) rows::store_one(p + tail, 0.f);
+}
+
 __global__ __launch_bounds__(SORT_NT) void sort_kernel(GradParams p) {
   __shared__ uint32_t hist[SORT_WAVES][RANGE];
   __shared__ uint32_t sums[SORT_WAVES];
+  constexpr int AHEAD = 8;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t r0 = (int64_t)blockIdx.x * RANGE;
-  const uint64_t width = (uint64_t)min((int64_t)RANGE, p.V - r0);
+  const int64_t r0 = (int64_t)blockIdx.x * p.range;
+  const uint64_t width = (uint64_t)min((int64_t)p.range, p.V - r0);
   const int per = ((p.n + SORT_WAVES - 1) / SORT_WAVES + 63) / 64 * 64;
   const int from = min(p.n, wave * per), to = min(p.n, from + per);
   for (int i = tid; i < SORT_WAVES * RANGE; i += SORT_NT) (&hist[0][0])[i] = 0;
   __syncthreads();
   uint32_t below = 0;
-  for (int i = from + lane; i < to; i += 64) {
-    const int64_t id = p.ids[i];
-    const uint64_t at = (uint64_t)(id - r0);
-    if (id >= 0 && id < r0) ++below;
-    if (id >= 0 && at < width) atomicAdd(&hist[wave][at], 1u);
+  for (int b = from; b < to; b += AHEAD * 64) {
+    int64_t id[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) id[k] = b + k * 64 + lane < to ? p.ids[b + k * 64 + lane] : -1;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const uint64_t at = (uint64_t)(id[k] - r0);
+      if (id[k] >= 0 && id[k] < r0) ++below;
+      if (id[k] >= 0 && at < width) atomicAdd(&hist[wave][at], 1u);
+    }
   }
   below = (uint32_t)wave_sum_i((int)below);
   if (lane == 0) sums[wave] = below;
@@ -147,31 +177,36 @@ __global__ __launch_bounds__(SORT_NT) void sort_kernel(GradParams p) {
       s += c;
     }
     const uint64_t some = __ballot(mine != 0);
-    const int word = (int)(r0 / 32) + tid / 32;
-    if ((tid & 31) == 0 && word < (p.V + 31) / 32) p.present[word] = (uint32_t)(some >> (tid & 32));
+    const int64_t word = r0 / 32 + tid / 32;
+    if ((tid & 31) == 0 && tid < p.range && word < ((int64_t)p.V + 31) / 32) p.present[word] = (uint32_t)(some >> (tid & 32));
     if (tid == RANGE - 1 && blockIdx.x == gridDim.x - 1) *p.total = (int32_t)s;
   }
   __syncthreads();
-  for (int b = from; b < to; b += 64) {
-    const int i = b + lane;
-    const int64_t id = i < to ? p.ids[i] : -1;
-    const uint64_t at = (uint64_t)(id - r0);
-    const bool in = id >= 0 && at < width;
-    uint64_t left = __ballot(in);
-    while (left) {
-      // the tokens of this batch of 64 that share the first one's id take consecutive places
-      const int first = __builtin_ctzll(left);
-      const uint32_t which = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)at, first);
-      const uint64_t same = __ballot(in && (uint32_t)at == which) & left;
-      uint32_t s = 0;
-      if (lane == first) s = atomicAdd(&hist[wave][which], (uint32_t)__popcll(same));
-      s = (uint32_t)__builtin_amdgcn_readlane((int)s, first);
-      if (same >> lane & 1) {
-        const uint32_t to_place = s + (uint32_t)__popcll(same & ((1ull << lane) - 1));
-        p.place[to_place] = i;
-        p.name[to_place] = (int32_t)id;
+  for (int b0 = from; b0 < to; b0 += AHEAD * 64) {
+    int64_t ids[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) ids[k] = b0 + k * 64 + lane < to ? p.ids[b0 + k * 64 + lane] : -1;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int i = b0 + k * 64 + lane;
+      const uint64_t at = (uint64_t)(ids[k] - r0);
+      const bool in = ids[k] >= 0 && at < width;
+      uint64_t left = __ballot(in);
+      while (left) {
+        // the tokens of these 64 that share the first one's id take consecutive places
+        const int first = __builtin_ctzll(left);
+        const uint32_t which = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)at, first);
+        const uint64_t same = __ballot(in && (uint32_t)at == which) & left;
+        uint32_t s = 0;
+        if (lane == first) s = atomicAdd(&hist[wave][which], (uint32_t)__popcll(same));
+        s = (uint32_t)__builtin_amdgcn_readlane((int)s, first);
+        if (same >> lane & 1) {
+          const uint32_t to_place = s + (uint32_t)__popcll(same & ((1ull << lane) - 1));
+          p.place[to_place] = i;
+          p.name[to_place] = (int32_t)ids[k];
+        }
+        left &= ~same;
       }
-      left &= ~same;
     }
   }
 }
@@ -203,63 +238,64 @@ __device__ __forceinline__ void finish(T* out, int n, const float (&s)[G], float
 template <typename TG, typename TO, bool ONTO>
 __global__ __launch_bounds__(SUM_NT) void sum_kernel(GradParams p) {
   constexpr int G = Elem<TG>::VEC;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   TO* out = static_cast<TO*>(p.out);
-  const int64_t sums = (int64_t)p.chunks * p.strips;
+  const int64_t items = (int64_t)p.chunks * p.strips, sums = (items + SUM_WAVES - 1) / SUM_WAVES;
   if ((int64_t)blockIdx.x >= sums) {
-    // rows that no token has
     const int64_t v0 = ((int64_t)blockIdx.x - sums) * ZERO_ROWS;
-    constexpr int GO = Elem<TO>::VEC;
-    float zero[GO];
-#pragma unroll
-    for (int j = 0; j < GO; ++j) zero[j] = 0.f;
-    for (int k = 0; k < ZERO_ROWS; ++k) {
-      const int64_t v = v0 + k;
-      if (v >= p.V || p.present[v >> 5] >> (v & 31) & 1) continue;
-      TO* row = out + v * p.os;
-      for (int i = tid * GO; i < p.H; i += SUM_NT * GO) {
-        if (p.H - i >= GO) {
-          rows::store_full(row + i, 0, zero);
-        } else {
-          for (int j = 0; i + j < p.H; ++j) rows::store_one(row + i + j, 0.f);
-        }
-      }
+    const int rows_here = (int)min((int64_t)ZERO_ROWS, p.V - v0);
+    const uint32_t there = p.present[v0 >> 5] >> (v0 & 31) & ((1u << ZERO_ROWS) - 1);
+    if (there == 0 && p.os == p.H) {
+      clear_row(out + v0 * p.os, (int64_t)rows_here * p.H);
+    } else {
+      for (int r = 0; r < rows_here; ++r)
+        if (!(there >> r & 1)) clear_row(out + (v0 + r) * p.os, p.H);
     }
     return;
   }
+  const int64_t item = (int64_t)blockIdx.x * SUM_WAVES + wave;
   const int total = *p.total;
-  const int chunk = (int)(blockIdx.x / p.strips), strip = (int)(blockIdx.x % p.strips);
-  const int c0 = chunk * CHUNK, c1 = min(c0 + CHUNK, total);
-  const int col = (strip * SUM_NT + tid) * G;
-  if (c0 >= total || col >= p.H) return;
-  const int n = p.H - col;
+  const int chunk = (int)(item / p.strips), strip = (int)(item % p.strips);
+  const int c0 = chunk * CHUNK, count = min(CHUNK, total - c0);
+  if (item >= items || count <= 0) return;
+  // lane l: position and id of entry l; where its id ends, and whether the first one's began before
+  const int at = min(c0 + lane, total - 1);
+  const int place = p.place[at], name = p.name[at], after = p.name[min(at + 1, total - 1)];
+  const bool last = name != after || at + 1 == total;
+  const uint32_t ends = (uint32_t)__ballot(last);
+  bool reaches_in = c0 > 0 && p.name[max(c0 - 1, 0)] == __builtin_amdgcn_readfirstlane(name);
+  const int col = (strip * 64 + lane) * G, n = p.H - col;
   const TG* g = static_cast<const TG*>(p.g) + col;
   float s[G];
 #pragma unroll
   for (int j = 0; j < G; ++j) s[j] = 0.f;
-  bool reaches_in = c0 > 0 && p.name[c0 - 1] == p.name[c0];
-  constexpr int U = 8;
-  for (int c = c0; c < c1; c += U) {
-    float v[U][G];
+  constexpr int U = 16;  // rows in flight
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (c + u < c1) load_group(g + p.place[c + u] * p.gs, n, v[u]);
+  for (int c = 0; c < CHUNK; c += U) {
+    float v[U][G];
+    if (c >= count) break;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int at = c + u;
-      if (at >= c1) break;
+      const int64_t row = __builtin_amdgcn_readlane(place, min(c + u, count - 1));
+      if (n > 0) load_group(g + row * p.gs, n, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (c + u >= count) break;
 #pragma unroll
       for (int j = 0; j < G; ++j) s[j] += v[u][j];
-      const int id = p.name[at];
-      const bool more = at + 1 < total && p.name[at + 1] == id;
-      if (more && at + 1 < c1) continue;
-      if (reaches_in || more) {
-        float* part = p.part + ((int64_t)chunk * 2 + (reaches_in ? 0 : 1)) * p.H + col;
+      const bool done = ends >> (c + u) & 1;
+      if (!done && c + u + 1 < count) continue;
+      if (n > 0) {
+        if (reaches_in || !done) {
+          float* part = p.part + ((int64_t)chunk * 2 + (reaches_in ? 0 : 1)) * p.H + col;
 #pragma unroll
-        for (int j = 0; j < G; ++j)
-          if (j < n) part[j] = s[j];
-      } else {
-        finish<TO, ONTO, G>(out + id * p.os + col, n, s, p.scale);
+          for (int j = 0; j < G; ++j)
+            if (j < n) part[j] = s[j];
+        } else {
+          const int64_t id = __builtin_amdgcn_readlane(name, c + u);
+          finish<TO, ONTO, G>(out + id * p.os + col, n, s, p.scale);
+        }
       }
       reaches_in = false;
 #pragma unroll
@@ -269,7 +305,7 @@ __global__ __launch_bounds__(SUM_NT) void sum_kernel(GradParams p) {
 }
 
 template <typename TO, bool ONTO>
-__global__ __launch_bounds__(SUM_NT) void join_kernel(GradParams p) {
+__global__ __launch_bounds__(JOIN_NT) void join_kernel(GradParams p) {
   constexpr int G = 4;
   const int total = *p.total;
   const int chunk = (int)(blockIdx.x / p.strips), strip = (int)(blockIdx.x % p.strips);
@@ -278,18 +314,40 @@ __global__ __launch_bounds__(SUM_NT) void join_kernel(GradParams p) {
   const int id = p.name[c1];
   if (p.name[c1 - 1] != id) return;                                   // nothing reaches beyond this chunk,
   if (chunk > 0 && p.name[chunk * CHUNK] == id && p.name[chunk * CHUNK - 1] == id) return;  // or not from here
-  const int col = (strip * SUM_NT + threadIdx.x) * G;
+  const int col = (strip * JOIN_NT + threadIdx.x) * G;
   if (col >= p.H) return;
   const int n = min(G, p.H - col);
   float s[G] = {0.f, 0.f, 0.f, 0.f};
   const float* part = p.part + ((int64_t)chunk * 2 + 1) * p.H + col;
   for (int j = 0; j < n; ++j) s[j] = part[j];
-  for (int c = chunk + 1; c * CHUNK < total && p.name[c * CHUNK] == id; ++c) {
-    part = p.part + (int64_t)c * 2 * p.H + col;
-    for (int j = 0; j < n; ++j) s[j] += part[j];
+  // the chunks that the id reaches into: names and rows of U of them at a time
+  constexpr int U = 8;
+  for (int c = chunk + 1;; c += U) {
+    int more = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = (c + u) * CHUNK;
+      more += more == u && at < total && p.name[min(at, total - 1)] == id;
+    }
+    float v[U][G];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (u < more) {
+#pragma unroll
+        for (int j = 0; j < G; ++j) v[u][j] = j < n ? p.part[(int64_t)(c + u) * 2 * p.H + col + j] : 0.f;
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (u < more) {
+#pragma unroll
+        for (int j = 0; j < G; ++j) s[j] += v[u][j];
+      }
+    if (more < U) break;
   }
   TO* out = static_cast<TO*>(p.out) + id * p.os + col;
-  for (int j = 0; j < n; ++j) rows::store_one(out + j, ONTO ? Elem<TO>::one(out + j) + s[j] * p.scale : s[j] * p.scale);
+#pragma unroll
+  for (int j = 0; j < G; ++j)
+    if (j < n) rows::store_one(out + j, ONTO ? Elem<TO>::one(out + j) + s[j] * p.scale : s[j] * p.scale);
 }
 
 int check_sizes(int dtype, int n, int h, int v) {
@@ -299,23 +357,26 @@ int check_sizes(int dtype, int n, int h, int v) {
 }
 
 struct Plan {
-  int64_t ranges, chunks, strips, join_strips, zeros;
+  int64_t range, ranges, chunks, strips, join_strips, sum_grid;
   size_t place, name, present, part, bytes;  // offsets into the workspace (the total is at its begin)
 };
 
 Plan plan(const dsv41_embed_grad_desc* d) {
   Plan q{};
   const int g = d->grad_dtype == DSV41_DTYPE_F32 ? 4 : 8;
-  q.ranges = ((int64_t)d->vocab + RANGE - 1) / RANGE;
+  // a small vocabulary is cut finer, for as many workgroups as there are CUs
+  q.range = RANGE;
+  while (q.range > 32 && d->vocab < q.range * 256) q.range /= 2;
+  q.ranges = (d->vocab + q.range - 1) / q.range;
   q.chunks = ((int64_t)d->n_tokens + CHUNK - 1) / CHUNK;
-  q.strips = ((int64_t)d->hidden + SUM_NT * g - 1) / (SUM_NT * g);
-  q.join_strips = ((int64_t)d->hidden + SUM_NT * 4 - 1) / (SUM_NT * 4);
-  q.zeros = d->accumulate ? 0 : ((int64_t)d->vocab + ZERO_ROWS - 1) / ZERO_ROWS;
+  q.strips = ((int64_t)d->hidden + 64 * g - 1) / (64 * g);
+  q.join_strips = ((int64_t)d->hidden + JOIN_NT * 4 - 1) / (JOIN_NT * 4);
+  q.sum_grid = (q.chunks * q.strips + SUM_WAVES - 1) / SUM_WAVES + (d->accumulate ? 0 : ((int64_t)d->vocab + ZERO_ROWS - 1) / ZERO_ROWS);
   auto up = [](size_t b) { return (b + 255) / 256 * 256; };
   q.place = 256;
   q.name = q.place + up((size_t)d->n_tokens * 4);
   q.present = q.name + up((size_t)d->n_tokens * 4);
-  q.part = q.present + up((size_t)(d->vocab + 31) / 32 * 4);
+  q.part = q.present + up(((size_t)d->vocab + 31) / 32 * 4);
   q.bytes = q.part + (size_t)q.chunks * 2 * d->hidden * 4;
   return q;
 }
@@ -332,17 +393,17 @@ int check_grad(const dsv41_embed_grad_desc* d) {
   if ((uintptr_t)d->grad % (d->grad_dtype == DSV41_DTYPE_F32 ? 4 : 2) || (uintptr_t)d->out % (d->out_dtype == DSV41_DTYPE_F32 ? 4 : 2))
     return fail(DSV41_E_INVALID, "embedding gradient: operands are not aligned to their type");
   const Plan q = plan(d);
-  if (q.chunks * q.join_strips + q.zeros > MAX_GRID || q.chunks * q.strips + q.zeros > MAX_GRID || q.ranges >= MAX_GRID)
+  if (q.chunks * q.join_strips > MAX_GRID || q.sum_grid > MAX_GRID || q.ranges >= MAX_GRID)
     return fail(DSV41_E_UNSUPPORTED, "embedding gradient: the batch is too large for one call");
   return DSV41_OK;
 }
 
 template <typename TG, typename TO, bool ONTO>
 void launch(GradParams p, const Plan& q, hipStream_t s) {
-  hipLaunchKernelGGL((sum_kernel<TG, TO, ONTO>), dim3((unsigned)(q.chunks * q.strips + q.zeros)), dim3(SUM_NT), 0, s, p);
+  hipLaunchKernelGGL((sum_kernel<TG, TO, ONTO>), dim3((unsigned)q.sum_grid), dim3(SUM_NT), 0, s, p);
   if (q.chunks > 1) {
     p.strips = (int)q.join_strips;
-    hipLaunchKernelGGL((join_kernel<TO, ONTO>), dim3((unsigned)((q.chunks - 1) * q.join_strips)), dim3(SUM_NT), 0, s, p);
+    hipLaunchKernelGGL((join_kernel<TO, ONTO>), dim3((unsigned)((q.chunks - 1) * q.join_strips)), dim3(JOIN_NT), 0, s, p);
   }
 }
 template <typename TG, typename TO>
@@ -411,19 +472,18 @@ extern "C" int dsv41_embed_grad_run(const dsv41_embed_grad_desc* d, void* worksp
   p.scale = d->scale;
   p.out = d->out;
   p.os = d->out_row_stride;
-  p.ranges = (int)q.ranges;
+  p.range = (int)q.range;
   p.chunks = (int)q.chunks;
   p.strips = (int)q.strips;
-  p.zeros = (int)q.zeros;
   p.total = reinterpret_cast<int32_t*>(ws);
   p.place = reinterpret_cast<int32_t*>(ws + q.place);
   p.name = reinterpret_cast<int32_t*>(ws + q.name);
   p.present = reinterpret_cast<uint32_t*>(ws + q.present);
   p.part = reinterpret_cast<float*>(ws + q.part);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(sort_kernel, dim3((unsigned)q.ranges), dim3(SORT_NT), 0, s, p);
   const bool gf = d->grad_dtype == DSV41_DTYPE_F32, of = d->out_dtype == DSV41_DTYPE_F32, onto = d->accumulate != 0;
-  if (q.chunks * q.strips + q.zeros > 0) {
+  hipLaunchKernelGGL(sort_kernel, dim3((unsigned)q.ranges), dim3(SORT_NT), 0, s, p);
+  if (q.sum_grid > 0) {
     if (gf && of) launch<float, float>(p, q, onto, s);
     else if (gf) launch<float, rows::bf16_t>(p, q, onto, s);
     else if (of) launch<rows::bf16_t, float>(p, q, onto, s);

@@ -17,6 +17,7 @@
 // fragment (16 rows x 64) lies in a row's bytes exactly as a bf16 one (16 x 32).
 
 #include <algorithm>
+#include <iterator>
 #include <type_traits>
 
 #include "mfma_tile.h"
@@ -27,7 +28,7 @@ namespace inthead {
 
 using TL = Tile<SQUARE>;
 using rows::bf16_t;
-constexpr int BM = TL::BV, BN = TL::BT;
+constexpr int BM = TL::BV;
 constexpr int LINE = ROWB;            // columns are padded to whole lines
 constexpr int MAX_COLUMNS = 133120;   // 2^31 / 127^2 = 133152, in whole lines
 constexpr int QUANT_NT = 256;
@@ -136,7 +137,7 @@ struct Params {
   int N, V, K;      // K: a multiple of 128
   void* out;
   int64_t os;
-  int n_tb, ranges;
+  int n_tb, ranges, wide_tile;
 };
 
 template <typename T>
@@ -293,8 +294,10 @@ __global__ __launch_bounds__(64 * SPLIT, SPLIT * PER_CU / 4) void head_kernel(Pa
 }
 
 // ------------------------------------------------------------------------------- many tokens
-template <typename T, bool WIDE>  // WIDE: rows of the output take 4 elements at once
-__global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_kernel(Params p) {
+// W1: blocks of 16 tokens of a wave in the second half of its tokens: tiles of 256 tokens (2) or 192 (1).
+template <typename T, int W1>
+__global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_kernel(Params p, bool wide) {
+  constexpr int WT = 2 + W1, BN = 64 * WT, AHEAD = 6 + W1;  // loads of a wave's four regions
   // two stages, and for each wave the scales of the block's rows: read from memory between the multiplies, they would
   // have the wave wait for its stores
   __shared__ __align__(1024) unsigned char lds[2 * TL::STAGE + NWAVES * BM * 4];
@@ -324,6 +327,11 @@ __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) v
   auto load_region = [&](int reg) {
     const uint32_t dst = lds0 + (uint32_t)((ld & 1) * TL::STAGE + reg * TL::REGION_W + wid * 2 * TILE);
     const uint32_t off = mine + (uint32_t)(ld_k * 2 * TILE) + (reg & 1) * half + (ld >= total ? 1u << 31 : 0u);
+    if (W1 == 1 && reg == B1) {  // half a region: a tile a wave
+      const uint32_t some = (uint32_t)((8 + (wid >> 1)) * bytes + (wid & 1) * TILE + lane * 16);
+      load_lds(xrs, some + (uint32_t)(ld_k * 2 * TILE) + (ld >= total ? 1u << 31 : 0u), dst - wid * TILE);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i) load_lds(reg < B0 ? wrs : xrs, off + i * TILE, dst + i * TILE);
   };
@@ -339,8 +347,9 @@ __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) v
   const int r16 = lane & 15, quad = lane >> 4;
   // a region's tiles: those of a row block's two k-steps side by side
   uint32_t ra = (uint32_t)(wv * 8 * TILE + lane * 16), rb = 2 * TL::REGION_W + (uint32_t)(wt * 4 * TILE + lane * 16);
+  uint32_t rb1 = 2 * TL::REGION_W + TL::REGION_X + (uint32_t)(wt * 2 * W1 * TILE + lane * 16);
   intx4 acc[WV][WT];
-  intx4 fa[4][KS], fb0[2][KS], fb1[2][KS];
+  intx4 fa[4][KS], fb0[2][KS], fb1[W1][KS];
   auto frag = [&](uint32_t off) { return *reinterpret_cast<const intx4*>(lds + off); };
   auto read_w = [&](int h) {
 #pragma unroll
@@ -348,18 +357,18 @@ __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) v
 #pragma unroll
       for (int i = 0; i < 4; ++i) fa[i][ks] = frag(ra + h * TL::REGION_W + (2 * i + ks) * TILE);
   };
-  auto read_x = [&](intx4 (&fb)[2][KS], int ks, int h) {
+  auto read_x = [&](auto& fb, int ks, uint32_t r) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) fb[i][ks] = frag(rb + h * TL::REGION_X + (2 * i + ks) * TILE);
+    for (int i = 0; i < (int)std::size(fb); ++i) fb[i][ks] = frag(r + (2 * i + ks) * TILE);
   };
-  auto multiply = [&](auto first, int h, int j, const intx4 (&fb)[2][KS], auto&& after) {
+  auto multiply = [&](auto first, int h, int j, const auto& fb, auto&& after) {
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
+        for (int q = 0; q < (int)std::size(fb); ++q) {
           intx4& c = acc[4 * h + i][2 * j + q];
           const intx4 c0 = first && ks == 0 ? intx4{} : c;
           c = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[i][ks], fb[q][ks], c0, 0, 0, 0);
@@ -373,39 +382,41 @@ __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) v
   auto stage = [&](auto first) {
     read_w(0);
     load_region(B1);
-    wait_loads<TL::AHEAD>();
+    wait_loads<AHEAD>();
     barrier();
     multiply(first, 0, 0, fb0, nothing);
     barrier();
 
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) read_x(fb1, ks, 1);
+    for (int ks = 0; ks < KS; ++ks) read_x(fb1, ks, rb1);
     load_region(A1);
     next_load_stage();
-    wait_loads<TL::AHEAD>();
+    wait_loads<AHEAD>();
     barrier();
     multiply(first, 0, 1, fb1, nothing);
     barrier();
 
     read_w(1);
     load_region(B0);
-    wait_loads<TL::AHEAD>();
+    wait_loads<AHEAD>();
     barrier();
     multiply(first, 1, 1, fb1, nothing);
     barrier();
 
     ra ^= TL::STAGE;
     rb ^= TL::STAGE;
-    asm volatile("" : "+v"(ra), "+v"(rb));  // here, not among the multiplies
+    rb1 ^= TL::STAGE;
+    asm volatile("" : "+v"(ra), "+v"(rb), "+v"(rb1));  // here, not among the multiplies
     load_region(A0);
-    wait_loads<TL::AHEAD>();
+    wait_loads<AHEAD>();
     barrier();
-    multiply(first, 1, 0, fb0, [&](int ks) { read_x(fb0, ks, 0); });
+    multiply(first, 1, 0, fb0, [&](int ks) { read_x(fb0, ks, rb); });
   };
 
+  auto token_of = [&](int j) { return j < 2 ? wt * 32 + 16 * j : 128 + wt * 16 * W1 + 16 * (j - 2); };  // of block j, first
   float ss[WT];  // scales of the lane's tokens
 #pragma unroll
-  for (int j = 0; j < WT; ++j) ss[j] = p.ss[min(t0 + wt * 32 + col_off<TL>(j) + r16, p.N - 1)];
+  for (int j = 0; j < WT; ++j) ss[j] = p.ss[min(t0 + token_of(j) + r16, p.N - 1)];
 #pragma unroll
   for (int j = 0; j < WT; ++j) asm volatile("" ::"v"(ss[j]));  // here, with no load behind them yet
 
@@ -416,10 +427,10 @@ __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) v
   next_load_stage();
   load_region(B0);
   load_region(A0);
-  wait_loads<TL::AHEAD>();
+  wait_loads<AHEAD>();
   barrier();
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) read_x(fb0, ks, 0);
+  for (int ks = 0; ks < KS; ++ks) read_x(fb0, ks, rb);
   if (wid >= NWAVES / 2) barrier();
 
   T* out = static_cast<T*>(p.out);
@@ -433,12 +444,12 @@ __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) v
     // lane: 16 neighbouring logits of one token of each block, in either half of the rows
 #pragma unroll
     for (int j = 0; j < WT; ++j) {
-      int n = t0 + wt * 32 + col_off<TL>(j) + r16;
+      int n = t0 + token_of(j) + r16;
       asm volatile("" : "+v"(n));  // addresses are formed here, not kept across the blocks
 #pragma unroll
       for (int i = 0; i < WV; i += 4) {
         const int m = wv * 64 + row_off<TL>(i, 0);
-        store_logits(out + (int64_t)n * p.os, mb * BM + m, p.V, n < p.N, WIDE, acc[i][j], acc[i + 1][j], acc[i + 2][j],
+        store_logits(out + (int64_t)n * p.os, mb * BM + m, p.V, n < p.N, wide, acc[i][j], acc[i + 1][j], acc[i + 2][j],
                      acc[i + 3][j], ss[j], scales + m + 16 * quad);
       }
     }
@@ -478,6 +489,11 @@ int check_head(const dsv41_int_head_desc* d) {
 
 size_t scales_at(const dsv41_int_head_desc* d) { return (size_t)((d->n_tokens + 15) / 16 * 16) * padded_of(d->hidden); }
 
+// A block of rows against 192 tokens costs this of one against 256.  256 and 192 wide, us: 300 tokens of 7168 ->
+// 129280 (fp32) 370 and 322, of 2048 -> 151936 (bf16) 133 and 111, 576 tokens 195 and 167; but 256 tokens 99 and 110,
+// 1100 tokens 330 and 344, 4096 tokens 1136 and 1221.
+constexpr double NARROW_COST = 0.85;
+
 // As many workgroups as fit on the GPU together take the same number of groups each.  Four waves with three
 // steps ahead, two workgroups a CU: 2048 -> 151936, 1, 17, 48 and 64 tokens 52, 57, 64 and 68 us, 7168 -> 129280 151,
 // 164, 182 and 199.  Eight waves: 54, 59, 68, 72 and 155, 174, 193, 208; two (four workgroups): 57, 63, 70, 75 and 153,
@@ -497,8 +513,19 @@ void launch(const Params& p, hipStream_t s) {
   else if (p.N <= FEW) launch_few<T, 4>(p, wide, s);
   else {
     const dim3 grid((p.n_tb * p.ranges + 7) / 8 * 8);
-    if (wide) hipLaunchKernelGGL((gemm_kernel<T, true>), grid, dim3(NT), 0, s, p);
-    else hipLaunchKernelGGL((gemm_kernel<T, false>), grid, dim3(NT), 0, s, p);
+    if (p.wide_tile) hipLaunchKernelGGL((gemm_kernel<T, 2>), grid, dim3(NT), 0, s, p, wide);
+    else hipLaunchKernelGGL((gemm_kernel<T, 1>), grid, dim3(NT), 0, s, p, wide);
+  }
+}
+
+// The tile of the shorter estimate: rounds of workgroups, each of as many blocks of rows as the longest range has.
+void plan_tiles(Params& p) {
+  const int n_mb = (p.V + BM - 1) / BM;
+  double best = 1e300;
+  for (int w = 0; w < 2; ++w) {
+    const int bn = w ? 192 : 256, n_tb = (p.N + bn - 1) / bn, ranges = std::max(1, std::min(n_mb, CU_COUNT / n_tb));
+    const double cost = (double)((n_tb * ranges + CU_COUNT - 1) / CU_COUNT) * ((n_mb + ranges - 1) / ranges) * (w ? NARROW_COST : 1.0);
+    if (cost < best) best = cost, p.n_tb = n_tb, p.ranges = ranges, p.wide_tile = !w;
   }
 }
 
@@ -549,8 +576,7 @@ extern "C" int dsv41_int_head_run(const dsv41_int_head_desc* d, void* workspace,
   p.K = K;
   p.out = d->out;
   p.os = d->out_row_stride;
-  p.n_tb = (p.N + BN - 1) / BN;
-  p.ranges = std::max(1, std::min((p.V + BM - 1) / BM, CU_COUNT / p.n_tb));
+  plan_tiles(p);
   if (d->out_dtype == DSV41_DTYPE_F32) launch<float>(p, s);
   else launch<bf16_t>(p, s);
   DSV41_HIP_CHECK(hipGetLastError());
