@@ -34,21 +34,29 @@ constexpr int SORT_NT = 1024, SORT_WAVES = SORT_NT / 64;
 constexpr int RANGE = 512;    // ids of a sorting workgroup, at most
 constexpr int SUM_NT = 256, SUM_WAVES = SUM_NT / 64;
 constexpr int CHUNK = 32;     // sorted positions of a summing wave
-constexpr int ZERO_ROWS = 16; // rows of the table of a zeroing workgroup
+// A zeroing workgroup has about this many bytes, and those of an XCD a contiguous part of the table: 1.2 GB in 191 us,
+// 195 and 206 with spans of 8, 16 and 32 KB, 219, 212 and 231 where the XCDs take spans in turn, 232 and 219 at 1 MB.
+constexpr int ZERO_BYTES = 16384;
 constexpr int JOIN_NT = 128;
 constexpr int64_t MAX_GRID = 1 << 22;
 
+// 16 bytes of a row from p on, of which n elements exist (zeros beyond).
 template <typename T>
-__device__ __forceinline__ void load_group(const T* p, int n, float (&v)[Elem<T>::VEC]) {
-  constexpr int G = Elem<T>::VEC;
-  uint32_t w[4] = {0, 0, 0, 0};
-  if (n >= G) {
+__device__ __forceinline__ void load_raw(const T* p, int n, uint32_t (&w)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = 0;
+  if (n >= Elem<T>::VEC) {
     rows::load16<false>(p, w);
   } else {
 #pragma unroll
-    for (int j = 0; j < G; ++j)
+    for (int j = 0; j < Elem<T>::VEC; ++j)
       if (j < n) Elem<T>::put(w, j, p[j]);
   }
+}
+template <typename T>
+__device__ __forceinline__ void load_group(const T* p, int n, float (&v)[Elem<T>::VEC]) {
+  uint32_t w[4];
+  load_raw(p, n, w);
   Elem<T>::unpack(w, v);
 }
 
@@ -111,6 +119,8 @@ struct GradParams {
   void* out;
   int64_t os;
   int range, chunks, strips;
+  int zero_rows;      // rows of the table of a zeroing workgroup: 1 .. 16, a power of two
+  int64_t zero_grid;  // zeroing workgroups, a multiple of 8
   int32_t* total;     // [1] tokens with a row
   int32_t* place;     // [n] positions sorted by (id, position)
   int32_t* name;      // [n] their ids
@@ -126,6 +136,7 @@ __device__ __forceinline__ void clear_row(T* p, int64_t n) {
   if (tid < head) rows::store_one(p + tid, 0.f);
   uint4* q = reinterpret_cast<uint4*>(p + head);
   const int64_t groups = (n - head) / G;
+  
   for (int64_t i = tid; i < groups; i += SUM_NT) q[i] = make_uint4(0, 0, 0, 0);
   const int64_t tail = head + groups * G + tid;
   if (tid < G && tail < n) rows::store_one(p + tail, 0.f);
@@ -242,9 +253,10 @@ __global__ __launch_bounds__(SUM_NT) void sum_kernel(GradParams p) {
   TO* out = static_cast<TO*>(p.out);
   const int64_t items = (int64_t)p.chunks * p.strips, sums = (items + SUM_WAVES - 1) / SUM_WAVES;
   if ((int64_t)blockIdx.x >= sums) {
-    const int64_t v0 = ((int64_t)blockIdx.x - sums) * ZERO_ROWS;
-    const int rows_here = (int)min((int64_t)ZERO_ROWS, p.V - v0);
-    const uint32_t there = p.present[v0 >> 5] >> (v0 & 31) & ((1u << ZERO_ROWS) - 1);
+    const int64_t z = (int64_t)blockIdx.x - sums, v0 = ((z & 7) * (p.zero_grid / 8) + (z >> 3)) * p.zero_rows;
+    if (v0 >= p.V) return;
+    const int rows_here = (int)min((int64_t)p.zero_rows, p.V - v0);
+    const uint32_t there = p.present[v0 >> 5] >> (v0 & 31) & ((1u << p.zero_rows) - 1);
     if (there == 0 && p.os == p.H) {
       clear_row(out + v0 * p.os, (int64_t)rows_here * p.H);
     } else {
@@ -272,18 +284,20 @@ __global__ __launch_bounds__(SUM_NT) void sum_kernel(GradParams p) {
   constexpr int U = 16;  // rows in flight
 #pragma unroll
   for (int c = 0; c < CHUNK; c += U) {
-    float v[U][G];
+    uint32_t raw[U][4];
     if (c >= count) break;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t row = __builtin_amdgcn_readlane(place, min(c + u, count - 1));
-      if (n > 0) load_group(g + row * p.gs, n, v[u]);
+      if (n > 0) load_raw(g + row * p.gs, n, raw[u]);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (c + u >= count) break;
+      float v[G];
+      Elem<TG>::unpack(raw[u], v);
 #pragma unroll
-      for (int j = 0; j < G; ++j) s[j] += v[u][j];
+      for (int j = 0; j < G; ++j) s[j] += v[j];
       const bool done = ends >> (c + u) & 1;
       if (!done && c + u + 1 < count) continue;
       if (n > 0) {
@@ -357,7 +371,7 @@ int check_sizes(int dtype, int n, int h, int v) {
 }
 
 struct Plan {
-  int64_t range, ranges, chunks, strips, join_strips, sum_grid;
+  int64_t range, ranges, chunks, strips, join_strips, zero_rows, zero_grid, sum_grid;
   size_t place, name, present, part, bytes;  // offsets into the workspace (the total is at its begin)
 };
 
@@ -371,7 +385,11 @@ Plan plan(const dsv41_embed_grad_desc* d) {
   q.chunks = ((int64_t)d->n_tokens + CHUNK - 1) / CHUNK;
   q.strips = ((int64_t)d->hidden + 64 * g - 1) / (64 * g);
   q.join_strips = ((int64_t)d->hidden + JOIN_NT * 4 - 1) / (JOIN_NT * 4);
-  q.sum_grid = (q.chunks * q.strips + SUM_WAVES - 1) / SUM_WAVES + (d->accumulate ? 0 : ((int64_t)d->vocab + ZERO_ROWS - 1) / ZERO_ROWS);
+
+  q.zero_rows = 1;
+  while (q.zero_rows < 16 && q.zero_rows * 2 * d->hidden * (d->out_dtype == DSV41_DTYPE_F32 ? 4 : 2) <= ZERO_BYTES) q.zero_rows *= 2;
+  q.zero_grid = d->accumulate ? 0 : ((d->vocab + q.zero_rows - 1) / q.zero_rows + 7) / 8 * 8;
+  q.sum_grid = (q.chunks * q.strips + SUM_WAVES - 1) / SUM_WAVES + q.zero_grid;
   auto up = [](size_t b) { return (b + 255) / 256 * 256; };
   q.place = 256;
   q.name = q.place + up((size_t)d->n_tokens * 4);
@@ -475,6 +493,8 @@ extern "C" int dsv41_embed_grad_run(const dsv41_embed_grad_desc* d, void* worksp
   p.range = (int)q.range;
   p.chunks = (int)q.chunks;
   p.strips = (int)q.strips;
+  p.zero_rows = (int)q.zero_rows;
+  p.zero_grid = q.zero_grid;
   p.total = reinterpret_cast<int32_t*>(ws);
   p.place = reinterpret_cast<int32_t*>(ws + q.place);
   p.name = reinterpret_cast<int32_t*>(ws + q.name);
