@@ -24,7 +24,10 @@ _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 def _ids(ids, device):
     if not isinstance(ids, torch.Tensor) or ids.dtype not in INTEGERS:
         raise ValueError("ids must be integers")
-    ids = ids.to(device=device, dtype=torch.int64).reshape(-1)
+    if ids.dtype != torch.int64 or ids.device != device:
+        ids = ids.to(device=device, dtype=torch.int64)
+    if ids.ndim != 1:
+        ids = ids.reshape(-1)
     fit_int32(ids.numel())
     return ids if ids.is_contiguous() else ids.contiguous()
 
@@ -159,8 +162,8 @@ class _TokenEmbedding(torch.autograd.Function):
             return None, None, None, None
         (ids,) = ctx.saved_tensors
         refuse_tangents("gradients", grad)
-        with torch.no_grad():
-            dw = token_embedding_backward(grad, ids, ctx.vocab, scale=ctx.scale, dtype=ctx.dtype)
+        dw = torch.empty(ctx.vocab, grad.shape[1], dtype=ctx.dtype, device=grad.device)
+        _backward(ids, _matrix(grad, broadcast=True), ctx.scale, dw, False)
         return None, first_order(dw, grad), None, None
 
 
@@ -182,4 +185,4 @@ def token_embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1
         out, status = forward(flat, weight, scale, check)
     if check and any_set(status)[0]:
         raise ValueError("token ID is outside the model vocabulary")
-    return out.view(*ids.shape, weight.shape[1])
+    return out if ids.ndim == 1 else out.view(*ids.shape, weight.shape[1])

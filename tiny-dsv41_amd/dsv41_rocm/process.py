@@ -23,21 +23,21 @@ from .scores import INTEGERS, launch, refuse_capture, refuse_tangents, row_field
 Knob = Union[float, torch.Tensor]
 
 
-def _knob(value, name, rows, device):
-    """(the scalar of the descriptor, the per-row fp32 tensor or None)"""
+def _knob(value, name, neutral, rows, device, keep):
+    """(the descriptor's scalar, the pointer of its per-row values or None)"""
     if isinstance(value, torch.Tensor):
         if value.shape != (rows,):
             raise ValueError(f"{name} must be a number or have one value per row")
         if value.requires_grad and torch.is_grad_enabled():
             raise NotImplementedError(f"{name} has no gradient: detach it")
         refuse_tangents(name, value)
-        return (1.0 if name == "repetition_penalty" else 0.0), vector(value, torch.float32, (rows,), device)
+        value = vector(value, torch.float32, (rows,), device)
+        keep.append(value)
+        return neutral, value.data_ptr()
     value = float(value)
-    if name == "repetition_penalty":
-        if not math.isfinite(value) or value <= 0:
-            raise ValueError("repetition_penalty must be finite and positive")
-    elif not math.isfinite(value):
-        raise ValueError("presence_penalty and frequency_penalty must be finite")
+    if not math.isfinite(value) or neutral and value <= 0:
+        raise ValueError("repetition_penalty must be finite and positive" if neutral
+                         else "presence_penalty and frequency_penalty must be finite")
     return value, None
 
 
@@ -47,102 +47,95 @@ def _integers(t, name, dtype, device):
     return t if t.dtype == dtype and t.device == device else t.to(device=device, dtype=dtype)
 
 
+def _lengths(t, name, rows, device, keep):
+    t = _integers(torch.as_tensor(t), name, torch.int32, device)
+    if t.shape != (rows,):
+        raise ValueError(f"{name} must have one length per row")
+    t = t.contiguous()
+    keep.append(t)
+    return t.data_ptr()
+
+
 def _rows_of(t):
-    """A matrix whose rows are contiguous, at any row stride that is not negative."""
-    return t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
+    """(a matrix whose rows are contiguous, at any row stride that is not negative; that stride)"""
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        t = t.contiguous()
+    return t, t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _list_stride(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-class _Arguments:
-    """Validated arguments in kernel form: the descriptor's fields, and the tensors that they point to."""
-
-    def __init__(self, logits, history, history_lens, history_prompt_lens, repetition_penalty, presence_penalty,
-                 frequency_penalty, bias_ids, bias, token_mask, mask_rows, fill):
-        rows, vocab = logits.shape
-        dev = logits.device
-        fields = {}
-        keep = []
-
-        def point(name, t):
-            fields[name] = t.data_ptr()
-            keep.append(t)
-
-        knobs = (("repetition_penalty", repetition_penalty, "repetition_penalties"),
-                 ("presence_penalty", presence_penalty, "presence_penalties"),
-                 ("frequency_penalty", frequency_penalty, "frequency_penalties"))
-        for name, value, array in knobs:
-            fields[name], t = _knob(value, name, rows, dev)
-            if t is not None:
-                point(array, t)
-        if history is None and (history_lens is not None or history_prompt_lens is not None):
-            raise ValueError("history_lens and history_prompt_lens require a history")
-        if history is not None:
-            if history.ndim != 2 or history.shape[0] != rows:
-                raise ValueError("history must have shape [rows, history_length]")
-            history = _rows_of(_integers(history, "history", torch.int64, dev))
-            for name, t in (("history_lens", history_lens), ("history_prompt_lens", history_prompt_lens)):
-                if t is not None:
-                    t = _integers(torch.as_tensor(t), name, torch.int32, dev)
-                    if t.shape != (rows,):
-                        raise ValueError(f"{name} must have one length per row")
-                    if history.shape[1]:
-                        point(name, t.contiguous())
-            if history.shape[1]:
-                point("history", history)
-                fields["history_row_stride"], fields["hist_len"] = _list_stride(history), history.shape[1]
-        if (bias_ids is None) != (bias is None):
-            raise ValueError("bias_ids and bias are given together")
-        if bias is not None:
-            if bias.requires_grad and torch.is_grad_enabled():
-                raise NotImplementedError("bias has no gradient: detach it")
-            refuse_tangents("biases", bias)
-            if not bias.is_floating_point() or bias.shape != bias_ids.shape or bias.ndim not in (1, 2) or \
-                    bias.ndim == 2 and bias.shape[0] != rows:
-                raise ValueError("bias_ids and bias must have shape [rows, entries] or [entries]")
-            bias_ids = _integers(bias_ids, "bias_ids", torch.int64, dev).contiguous()
-            bias = bias.to(device=dev, dtype=torch.float32).contiguous()
-            if bias.numel():
-                point("bias_ids", bias_ids)
-                point("bias", bias)
-                fields["bias_len"] = bias.shape[-1]
-                fields["bias_row_stride"] = bias.shape[-1] if bias.ndim == 2 else 0
-        if mask_rows is not None and token_mask is None:
-            raise ValueError("mask_rows requires a token_mask")
-        if token_mask is not None:
-            words = (vocab + 31) // 32
-            if not isinstance(token_mask, torch.Tensor) or token_mask.dtype != torch.int32 or \
-                    token_mask.ndim not in (1, 2) or token_mask.shape[-1] < words:
-                raise ValueError("token_mask must be int32 words, one bit per token: [masks, ceil(vocabulary_size / 32)]")
-            if token_mask.ndim == 1:
-                token_mask = token_mask[None]
-            token_mask = _rows_of(token_mask.to(dev))
-            if mask_rows is not None:
-                mask_rows = _integers(mask_rows, "mask_rows", torch.int32, dev).contiguous()
-                if mask_rows.shape != (rows,):
-                    raise ValueError("mask_rows must have one mask per row")
-                point("mask_rows", mask_rows)
-            elif token_mask.shape[0] not in (1, rows):
-                raise ValueError("without mask_rows there is one token_mask, or one per row")
-            if token_mask.shape[0]:
-                point("mask", token_mask)
-                fields["masks"], fields["mask_row_stride"] = token_mask.shape[0], _list_stride(token_mask)
-            elif rows:
-                raise ValueError("token_mask holds no mask")
-        fill = float(fill)
-        if math.isnan(fill):
-            raise ValueError("fill must be a number")
-        fields["fill"] = fill
-        self.fields, self.keep = fields, keep
-
-
-def _desc(logits, fields) -> _lib.ProcessDesc:
-    d = _lib.ProcessDesc(*row_fields(_lib.ProcessDesc, logits))
-    for name, value in fields.items():
-        setattr(d, name, value)
-    return d
+def _arguments(logits, history, history_lens, history_prompt_lens, repetition_penalty, presence_penalty,
+               frequency_penalty, bias_ids, bias, token_mask, mask_rows, fill):
+    """Validated arguments in kernel form: the descriptor's values from history to fill, and the tensors that they
+    point to."""
+    rows, vocab = logits.shape
+    dev = logits.device
+    keep = []
+    rp, rps = _knob(repetition_penalty, "repetition_penalty", 1.0, rows, dev, keep)
+    pres, press = _knob(presence_penalty, "presence_penalty", 0.0, rows, dev, keep)
+    freq, freqs = _knob(frequency_penalty, "frequency_penalty", 0.0, rows, dev, keep)
+    hist = lens = prompts = None
+    hist_step = hist_len = 0
+    if history is not None:
+        if history.ndim != 2 or history.shape[0] != rows:
+            raise ValueError("history must have shape [rows, history_length]")
+        history, hist_step = _rows_of(_integers(history, "history", torch.int64, dev))
+        hist_len = history.shape[1]
+        if history_lens is not None:
+            lens = _lengths(history_lens, "history_lens", rows, dev, keep)
+        if history_prompt_lens is not None:
+            prompts = _lengths(history_prompt_lens, "history_prompt_lens", rows, dev, keep)
+        keep.append(history)
+        hist = history.data_ptr()
+    elif history_lens is not None or history_prompt_lens is not None:
+        raise ValueError("history_lens and history_prompt_lens require a history")
+    ids = values = None
+    bias_step = bias_len = 0
+    if bias is not None and bias_ids is not None:
+        if bias.requires_grad and torch.is_grad_enabled():
+            raise NotImplementedError("bias has no gradient: detach it")
+        refuse_tangents("biases", bias)
+        if not bias.is_floating_point() or bias.shape != bias_ids.shape or bias.ndim not in (1, 2) or \
+                bias.ndim == 2 and bias.shape[0] != rows:
+            raise ValueError("bias_ids and bias must have shape [rows, entries] or [entries]")
+        bias_ids = _integers(bias_ids, "bias_ids", torch.int64, dev).contiguous()
+        bias = vector(bias, torch.float32, bias.shape, dev)
+        bias_len = bias.shape[-1]
+        bias_step = bias_len if bias.ndim == 2 else 0
+        keep += (bias_ids, bias)
+        ids, values = bias_ids.data_ptr(), bias.data_ptr()
+    elif bias is not None or bias_ids is not None:
+        raise ValueError("bias_ids and bias are given together")
+    mask = which = None
+    masks = mask_step = 0
+    if token_mask is not None:
+        if not isinstance(token_mask, torch.Tensor) or token_mask.dtype != torch.int32 or \
+                token_mask.ndim not in (1, 2) or token_mask.shape[-1] < (vocab + 31) // 32:
+            raise ValueError("token_mask must be int32 words, one bit per token: [masks, ceil(vocabulary_size / 32)]")
+        if token_mask.ndim == 1:
+            token_mask = token_mask[None]
+        if token_mask.device != dev:
+            token_mask = token_mask.to(dev)
+        token_mask, mask_step = _rows_of(token_mask)
+        masks = token_mask.shape[0]
+        if mask_rows is not None:
+            mask_rows = _integers(mask_rows, "mask_rows", torch.int32, dev).contiguous()
+            if mask_rows.shape != (rows,):
+                raise ValueError("mask_rows must have one mask per row")
+            keep.append(mask_rows)
+            which = mask_rows.data_ptr()
+        elif masks != 1 and masks != rows:
+            raise ValueError("without mask_rows there is one token_mask, or one per row")
+        if masks == 0 and rows:
+            raise ValueError("token_mask holds no mask")
+        keep.append(token_mask)
+        mask = token_mask.data_ptr()
+    elif mask_rows is not None:
+        raise ValueError("mask_rows requires a token_mask")
+    fill = float(fill)
+    if math.isnan(fill):
+        raise ValueError("fill must be a number")
+    return (hist, hist_step, hist_len, lens, prompts, rp, pres, freq, rps, press, freqs, ids, values, bias_step, bias_len,
+            masks, mask, mask_step, which, fill), keep
 
 
 def forward(logits, fields, out, want_status):
@@ -150,10 +143,8 @@ def forward(logits, fields, out, want_status):
     rows, vocab = logits.shape
     status = torch.empty(rows, dtype=torch.int32, device=logits.device) if want_status else None
     if rows:
-        d = _desc(logits, fields)
-        d.out, d.out_row_stride = out.data_ptr(), out.stride(0) if rows > 1 else vocab
-        if status is not None:
-            d.out_status = status.data_ptr()
+        d = _lib.ProcessDesc(*row_fields(_lib.ProcessDesc, logits), *fields, out.data_ptr(), out.stride(0) if rows > 1 else vocab,
+                             None if status is None else status.data_ptr(), None, 0)
         launch(_lib.load().dsv41_process_run, logits.device, ctypes.byref(d))
     return status
 
@@ -165,11 +156,12 @@ def process_backward(logits, fields, grad):
     out = torch.empty(rows, vocab, dtype=logits.dtype, device=logits.device)
     if rows:
         grad = grad.to(logits.dtype)
-        if grad.stride(1) != 1 and vocab > 1 or rows > 1 and 0 < grad.stride(0) < vocab:
+        step, unit = grad.stride()
+        if unit != 1 and vocab > 1 or rows > 1 and 0 < step < vocab:
             grad = grad.contiguous()
-        d = _desc(logits, fields)
-        d.grad, d.grad_row_stride = grad.data_ptr(), grad.stride(0) if rows > 1 else vocab
-        d.out, d.out_row_stride = out.data_ptr(), vocab
+            step = vocab
+        d = _lib.ProcessDesc(*row_fields(_lib.ProcessDesc, logits), *fields, out.data_ptr(), vocab, None, grad.data_ptr(),
+                             step if rows > 1 else vocab)
         launch(_lib.load().dsv41_process_grad_run, logits.device, ctypes.byref(d))
     return out
 
@@ -188,11 +180,11 @@ class _Process(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad, g_status):
-        logits, *_ = ctx.saved_tensors  # (the lists too: one that was written since is refused here)
+        logits, *lists = ctx.saved_tensors  # (the lists too: one that was written since is refused here)
+        nothing = (None,) * (2 + len(lists))
         if grad is None:
-            return (None,) * len(ctx.needs_input_grad)
-        dx = process_backward(logits, ctx.fields, grad)
-        return (first_order(dx, logits, grad),) + (None,) * (len(ctx.needs_input_grad) - 1)
+            return None, *nothing
+        return first_order(process_backward(logits, ctx.fields, grad), logits, grad), *nothing
 
 
 def _status_error(status: torch.Tensor) -> None:
@@ -225,7 +217,7 @@ def _output(out, logits):
     rows, vocab = out.shape
     if vocab > 1 and out.stride(1) != 1 or rows > 1 and out.stride(0) < vocab:
         raise ValueError("out must have contiguous rows that do not overlap")
-    if rows and not (out.data_ptr() == logits.data_ptr() and (rows == 1 or out.stride(0) == logits.stride(0))):
+    if out is not logits and rows and not (out.data_ptr() == logits.data_ptr() and (rows == 1 or out.stride(0) == logits.stride(0))):
         a, b = _extent(out), _extent(logits)
         if a[0] < b[1] and b[0] < a[1]:
             raise ValueError("out overlaps the logits without being them")
@@ -276,21 +268,21 @@ def process_logits(
     are ignored, and rows of such penalties and masks hold NaN.
     """
     logits = rows_of_logits(logits, 1.0)
-    a = _Arguments(logits, history, history_lens, history_prompt_lens, repetition_penalty, presence_penalty,
-                   frequency_penalty, bias_ids, bias, token_mask, mask_rows, fill)
+    fields, keep = _arguments(logits, history, history_lens, history_prompt_lens, repetition_penalty, presence_penalty,
+                              frequency_penalty, bias_ids, bias, token_mask, mask_rows, fill)
     refuse_capture(check)
     tracked = torch.is_grad_enabled() and logits.requires_grad
     if out is not None:
         if tracked or torch.is_grad_enabled() and out.requires_grad:
             raise ValueError("a call with out has no gradient: leave it out, or call under no_grad")
         out = _output(out, logits)
-        status = forward(logits, a.fields, out, check)
+        status = forward(logits, fields, out, check)
         written(out)
     elif tracked:
-        out, status = _Process.apply(logits, a.fields, check, *a.keep)
+        out, status = _Process.apply(logits, fields, check, *keep)
     else:
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        status = forward(logits, a.fields, out, check)
+        status = forward(logits, fields, out, check)
     if check and any_set(status)[0]:
         _status_error(status)
     return out

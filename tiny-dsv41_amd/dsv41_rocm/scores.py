@@ -15,7 +15,7 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
-from torch.autograd.forward_ad import unpack_dual
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._check import any_set
@@ -49,8 +49,10 @@ def fit_int32(*sizes) -> None:
 
 def refuse_tangents(what, *tensors) -> None:
     """The kernels would leave them out."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # no level is open, so nothing carries one (1 us a tensor)
+        return
     for t in tensors:
-        if t is not None and unpack_dual(t).tangent is not None:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
             raise NotImplementedError(f"{what} carry a forward-mode tangent, for which there is no rule: detach them")
 
 
