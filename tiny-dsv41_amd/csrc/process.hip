@@ -91,7 +91,17 @@ struct Group {
 };
 template <typename T>
 constexpr uint32_t ALL = (1u << Elem<T>::VEC) - 1;
-// The elements j with bit j of `there`, from p (the others come as 0), and to it.
+// Element j, which differs from lane to lane (selections: registers have no addresses).
+__device__ __forceinline__ uint32_t pick(const Group& g, int i) {
+  const uint32_t lo = i & 1 ? g.w[1] : g.w[0], hi = i & 1 ? g.w[3] : g.w[2];
+  return i & 2 ? hi : lo;
+}
+__device__ __forceinline__ void place(Group& g, int i, uint32_t w) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) g.w[k] = i == k ? w : g.w[k];
+}
+// The elements j with bit j of `there`, from p (the others come as 0), and to it.  (Straight code: around a loop the
+// compiler waits for all loads in flight.)
 template <typename T>
 __device__ __forceinline__ void load_group(const T* p, uint32_t there, Group& g) {
   if (there == ALL<T>) {
@@ -120,15 +130,6 @@ __device__ __forceinline__ void store_group(T* p, uint32_t there, const Group& g
     for (int j = 0; j < Elem<T>::VEC; ++j)
       if (there >> j & 1) store_element(p + j, g, j);
   }
-}
-// Element j, which differs from lane to lane (selections: registers have no addresses).
-__device__ __forceinline__ uint32_t pick(const Group& g, int i) {
-  const uint32_t lo = i & 1 ? g.w[1] : g.w[0], hi = i & 1 ? g.w[3] : g.w[2];
-  return i & 2 ? hi : lo;
-}
-__device__ __forceinline__ void place(Group& g, int i, uint32_t w) {
-#pragma unroll
-  for (int k = 0; k < 4; ++k) g.w[k] = i == k ? w : g.w[k];
 }
 __device__ __forceinline__ float get(const Group& g, int j, float) { return __uint_as_float(pick(g, j)); }
 __device__ __forceinline__ float get(const Group& g, int j, bf16_t) {
@@ -167,10 +168,9 @@ __global__ __launch_bounds__(NT, 8) void process_kernel(Params p) {
   float* biases = reinterpret_cast<float*>(words + SLICE);
   const int tid = threadIdx.x;
   // a row's slices one after another on one XCD (workgroups go round-robin over the eight)
-  const int64_t items = (int64_t)p.rows * p.slices, per = (items + 7) / 8;
-  const int64_t item = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if ((int64_t)(blockIdx.x >> 3) >= per || item >= items) return;
-  const int row = (int)(item / p.slices), slice = (int)(item % p.slices);
+  const uint32_t item = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  const int row = (int)(item / (uint32_t)p.slices), slice = (int)(item % (uint32_t)p.slices);
+  if (row >= p.rows) return;
   const T* x = static_cast<const T*>(p.x) + row * p.xs;
   T* out = static_cast<T*>(p.out) + row * p.os;
   // slices begin at memory lines of the result
@@ -178,26 +178,30 @@ __global__ __launch_bounds__(NT, 8) void process_kernel(Params p) {
   if (begin >= p.V) return;
   const T* from = MODE == GRAD ? static_cast<const T*>(p.grad) + row * p.gs : x;
 
+  // the row's own values, all on their way at once: arrays that are not given are read at the arguments' begin
+  typedef const __attribute__((address_space(4))) int32_t* constant_t;
+  const uintptr_t nowhere = (uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
+  auto value_of = [&](const void* a) { return *(constant_t)(a ? (uintptr_t)a + 4 * (int64_t)row : nowhere); };
+  const int m_row = MASK ? value_of(p.mask_rows) : 0;
+  const int rp_row = LISTS ? value_of(p.rps) : 0, pres_row = LISTS ? value_of(p.press) : 0, freq_row = LISTS ? value_of(p.freqs) : 0;
+  const int len_row = LISTS ? value_of(p.lens) : 0, prompt_row = LISTS ? value_of(p.prompt_lens) : 0;
   Knobs knobs{1.f, 0.f, 0.f};
   bool bad = false;
   int bits = 0;  // status bits that this thread met
   const uint32_t* mask = nullptr;
   if constexpr (MASK) {
-    const int m = p.mask_rows ? p.mask_rows[row] : p.masks == 1 ? 0 : row;
-    if (m >= p.masks) {
-      bad = true;
-      bits |= DSV41_STATUS_BAD_MASK;
-    } else if (m >= 0) {
-      mask = p.mask + m * p.ms;
-    }
+    const int m = p.mask_rows ? m_row : p.masks == 1 ? 0 : row;
+    bad = m >= p.masks;
+    if (bad) bits |= DSV41_STATUS_BAD_MASK;
+    mask = m >= 0 && !bad ? p.mask + m * p.ms : nullptr;
   }
   bool listed = false;
   int len = 0, prompt = 0;
   const int64_t* h = nullptr;
   if constexpr (LISTS) {
-    knobs.rp = p.rps ? p.rps[row] : p.rp;
-    knobs.pres = p.press ? p.press[row] : p.pres;
-    knobs.freq = p.freqs ? p.freqs[row] : p.freq;
+    knobs.rp = p.rps ? __int_as_float(rp_row) : p.rp;
+    knobs.pres = p.press ? __int_as_float(pres_row) : p.pres;
+    knobs.freq = p.freqs ? __int_as_float(freq_row) : p.freq;
     if (!(isfinite(knobs.rp) && knobs.rp > 0.f) || !isfinite(knobs.pres) || !isfinite(knobs.freq)) {
       bad = true;
       bits |= DSV41_STATUS_BAD_PENALTY;
@@ -205,8 +209,8 @@ __global__ __launch_bounds__(NT, 8) void process_kernel(Params p) {
     // (a gradient asks for the repetition penalty alone)
     if (p.history && !(knobs.rp == 1.f && (MODE == GRAD || (knobs.pres == 0.f && knobs.freq == 0.f)))) {
       h = p.history + row * p.hs;
-      len = p.lens ? min(max(p.lens[row], 0), p.hist_len) : p.hist_len;
-      prompt = p.prompt_lens ? p.prompt_lens[row] : 0;
+      len = p.lens ? min(max(len_row, 0), p.hist_len) : p.hist_len;
+      prompt = p.prompt_lens ? prompt_row : 0;
     }
     listed = len > 0 || (p.n_bias > 0 && (MODE != GRAD || h));
   }
@@ -318,6 +322,7 @@ __global__ __launch_bounds__(NT, 8) void process_kernel(Params p) {
     if (MODE == INPLACE && !marked[u] && allowed[u] == there[u]) continue;
     if (LISTS) {
       // (few: a wave takes as many turns as its lane with the most of them)
+#pragma unroll 1
       for (uint32_t m = marked[u]; m; m &= m - 1) {
         const int j = __builtin_ctz(m);
         const uint32_t word = words[word_at<T>(at + j)];
