@@ -126,6 +126,8 @@ def _head(**kw):
     (dict(x=0x1001), _lib.E_INVALID, "aligned"),
     (dict(scales=0x3004), _lib.E_INVALID, "aligned"),
     (dict(out=0x4002), _lib.E_INVALID, "aligned"),
+    (dict(n_tokens=(1 << 22) + 1), _lib.E_UNSUPPORTED, "too large"),
+    (dict(vocab=(1 << 28) + 1, out_row_stride=1 << 29), _lib.E_UNSUPPORTED, "too large"),
 ])
 def test_head_refusals(kw, code, msg):
     lib = _lib.load()

@@ -483,7 +483,8 @@ int check_head(const dsv41_int_head_desc* d) {
   if ((uintptr_t)d->w % 16) return fail(DSV41_E_INVALID, "8-bit head: the tiles must be 16-byte aligned");
   if ((uintptr_t)d->x % 2 || (uintptr_t)d->scales % 16 || (uintptr_t)d->out % (d->out_dtype == DSV41_DTYPE_F32 ? 4 : 2))
     return fail(DSV41_E_INVALID, "8-bit head: operands are not aligned to their type, or the scales not to 16 bytes");
-  if ((int64_t)d->n_tokens > MAX_GRID) return fail(DSV41_E_UNSUPPORTED, "8-bit head: the batch is too large for one call");
+  if ((int64_t)d->n_tokens > MAX_GRID || d->vocab > 1 << 28)
+    return fail(DSV41_E_UNSUPPORTED, "8-bit head: the batch or the vocabulary is too large for one call");
   return DSV41_OK;
 }
 

@@ -8,7 +8,6 @@ onto the head's (``selected_log_probs_backward``): ``token_embedding_backward(..
 from __future__ import annotations
 
 import ctypes
-import math
 from typing import Optional
 
 import torch
@@ -16,7 +15,7 @@ import torch
 from . import _lib
 from ._check import any_set
 from .logprob import first_order
-from .scores import INTEGERS, fit_int32, launch, refuse_capture, refuse_tangents, written
+from .scores import INTEGERS, fit_int32, launch, overlap, refuse_capture, refuse_tangents, written
 
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 
@@ -34,7 +33,7 @@ def _ids(ids, device):
 
 def _scale(scale) -> float:
     scale = float(scale)
-    if not math.isfinite(scale):
+    if not abs(scale) <= torch.finfo(torch.float32).max:
         raise ValueError("scale must be finite")
     return scale
 
@@ -129,6 +128,8 @@ def token_embedding_backward(
             raise ValueError("out has another vocabulary_size or dtype")
         if h > 1 and out.stride(1) != 1 or out.shape[0] > 1 and out.stride(0) < h:
             raise ValueError("out must have contiguous rows that do not overlap")
+        if overlap(out, grad):
+            raise ValueError("out overlaps grad")
         fit_int32(*out.shape)
         if ids.numel():
             _backward(ids, grad, scale, out, True)

@@ -101,6 +101,40 @@ def quantize_head(weight: torch.Tensor, *, check: bool = True) -> Int8Head:
     return Int8Head(tiles, scales, v, h)
 
 
+def _check_head(head, x):
+    v, h = head.vocab, head.hidden
+    if x.shape[1] != h:
+        raise ValueError("hidden must be [tokens, hidden] and the head [vocab, hidden]")
+    if head.tiles.device != x.device or head.scales.device != x.device:
+        raise ValueError("hidden and the head must be on the same GPU")
+    if head.tiles.dtype != torch.int8 or not head.tiles.is_contiguous() or \
+            head.tiles.numel() != _rounded(v, GROUP) * _rounded(h, LINE) or \
+            head.scales.dtype != torch.float32 or head.scales.shape != (v,) or not head.scales.is_contiguous():
+        raise ValueError("the head is not in the kernels' layout: make it with quantize_head or Int8Head.from_quantized")
+
+
+def _forward(x, head, out, want_status):
+    """One dsv41_int_head_run into ``out``; returns the statuses or None."""
+    n, h, v = x.shape[0], head.hidden, head.vocab
+    status = torch.empty(n, dtype=torch.int32, device=x.device) if want_status else None
+    if n:
+        d = _lib.IntHeadDesc(ctypes.sizeof(_lib.IntHeadDesc), n, h, v, x.data_ptr(), x.stride(0) if n > 1 else h,
+                             head.tiles.data_ptr(), head.scales.data_ptr(), out.data_ptr(),
+                             out.stride(0) if n > 1 else max(v, out.stride(0)), _OUT_DTYPES[out.dtype],
+                             None if status is None else status.data_ptr())
+        lib = _lib.load()
+        ref = ctypes.byref(d)
+        size = lib.dsv41_int_head_workspace_bytes(ref)
+        ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+        launch(lib.dsv41_int_head_run, x.device, ref, ws.data_ptr(), size)
+    return status
+
+
+def _new_logits(n, v, dtype, device):
+    """Logits whose rows begin at multiples of 64 elements."""
+    return torch.empty(n, _rounded(v, 64), dtype=dtype, device=device)[:, :v]
+
+
 def head_logits(
     hidden: torch.Tensor,
     head: Int8Head,
@@ -124,15 +158,8 @@ def head_logits(
     infinity; without, their rows are NaN.
     """
     x = _rows(hidden, "hidden")
-    w, scales, v, h = head.tiles, head.scales, head.vocab, head.hidden
-    n = x.shape[0]
-    if x.shape[1] != h:
-        raise ValueError("hidden must be [tokens, hidden] and the head [vocab, hidden]")
-    if w.device != x.device or scales.device != x.device:
-        raise ValueError("hidden and the head must be on the same GPU")
-    if w.dtype != torch.int8 or not w.is_contiguous() or w.numel() != _rounded(v, GROUP) * _rounded(h, LINE) or \
-            scales.dtype != torch.float32 or scales.shape != (v,) or not scales.is_contiguous():
-        raise ValueError("the head is not in the kernels' layout: make it with quantize_head or Int8Head.from_quantized")
+    n, v = x.shape[0], head.vocab
+    _check_head(head, x)
     given = out
     if out is not None:
         if out.shape != (n, v) or out.dtype not in _OUT_DTYPES or out.device != x.device:
@@ -144,20 +171,11 @@ def head_logits(
     elif dtype not in _OUT_DTYPES:
         raise ValueError("logits are torch.float32 or torch.bfloat16")
     else:
-        out = torch.empty(n, (v + 63) // 64 * 64, dtype=dtype, device=x.device)[:, :v]
+        out = _new_logits(n, v, dtype, x.device)
     refuse_capture(check)
-    status = torch.empty(n, dtype=torch.int32, device=x.device) if check else None
-    if n:
-        d = _lib.IntHeadDesc(ctypes.sizeof(_lib.IntHeadDesc), n, h, v, x.data_ptr(), x.stride(0) if n > 1 else h,
-                             w.data_ptr(), scales.data_ptr(), out.data_ptr(), out.stride(0) if n > 1 else max(v, out.stride(0)),
-                             _OUT_DTYPES[out.dtype], None if status is None else status.data_ptr())
-        lib = _lib.load()
-        ref = ctypes.byref(d)
-        size = lib.dsv41_int_head_workspace_bytes(ref)
-        ws = torch.empty(size, dtype=torch.uint8, device=x.device)
-        launch(lib.dsv41_int_head_run, x.device, ref, ws.data_ptr(), size)
-        if given is not None:
-            written(given)
+    status = _forward(x, head, out, check)
+    if given is not None:
+        written(given)
     if check and any_set(status)[0]:
         raise ValueError("hidden states contain non-finite values")
     return out

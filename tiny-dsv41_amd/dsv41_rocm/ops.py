@@ -14,6 +14,11 @@
   the backward needs of the forward.
 * ``dsv41_rocm::distillation_loss`` — divergence from a teacher's top tokens; returns ``(loss,
   status, stats)``.  Differentiable in ``logits``.
+* ``dsv41_rocm::process_logits`` — biases, penalties (numbers, or a tensor of one value per row in their place) and
+  token masks; returns ``(logits, status)``.  Differentiable in ``logits``.
+* ``dsv41_rocm::head_logits`` — logits of an 8-bit head's ``tiles`` and ``scales``; returns ``(logits, status)``.
+* ``dsv41_rocm::token_embedding`` — rows of a token table; returns ``(rows, status)``.  Differentiable in
+  ``weight``.
 
 The ops only register a CUDA (HIP) kernel: called on CPU tensors they raise, as the library
 has no CPU path.  Status bits are returned, not raised, so the ops stay traceable; the
@@ -27,7 +32,10 @@ from typing import Optional
 import torch
 
 from . import distill as _distill
+from . import embedding as _embedding
+from . import inthead as _inthead
 from . import logprob as _logprob
+from . import process as _process
 from . import sampling as _sampling
 from . import scores as _scores
 
@@ -189,4 +197,114 @@ def _distillation_loss_backward(ctx, g_loss, g_status, g_stats):
 distillation_loss_op.register_autograd(_distillation_loss_backward, setup_context=_distillation_loss_setup)
 
 
-__all__ = ["sample_rows", "selected_log_probs_op", "logit_scores_op", "distillation_loss_op"]
+@torch.library.custom_op("dsv41_rocm::process_logits", mutates_args=(), device_types="cuda")
+def process_logits_op(
+    logits: torch.Tensor,
+    history: Optional[torch.Tensor],
+    history_lens: Optional[torch.Tensor],
+    history_prompt_lens: Optional[torch.Tensor],
+    repetition_penalty: float,
+    presence_penalty: float,
+    frequency_penalty: float,
+    repetition_penalties: Optional[torch.Tensor],
+    presence_penalties: Optional[torch.Tensor],
+    frequency_penalties: Optional[torch.Tensor],
+    bias_ids: Optional[torch.Tensor],
+    bias: Optional[torch.Tensor],
+    token_mask: Optional[torch.Tensor],
+    mask_rows: Optional[torch.Tensor],
+    fill: float,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    rows, numbers, tensors = _process_arguments(
+        logits, history, history_lens, history_prompt_lens, repetition_penalty, presence_penalty, frequency_penalty,
+        repetition_penalties, presence_penalties, frequency_penalties, bias_ids, bias, token_mask, mask_rows, fill)
+    out = torch.empty(rows.shape, dtype=rows.dtype, device=rows.device)
+    status = _process.forward(rows, numbers, tensors, out, True)
+    return out, status
+
+
+def _process_arguments(logits, history, history_lens, history_prompt_lens, repetition_penalty, presence_penalty,
+                       frequency_penalty, repetition_penalties, presence_penalties, frequency_penalties, bias_ids, bias,
+                       token_mask, mask_rows, fill):
+    either = lambda number, each: number if each is None else each
+    rows = _scores.rows_of_logits(logits, 1.0)
+    numbers, tensors = _process._arguments(
+        rows, history, history_lens, history_prompt_lens, either(repetition_penalty, repetition_penalties),
+        either(presence_penalty, presence_penalties), either(frequency_penalty, frequency_penalties), bias_ids, bias,
+        token_mask, mask_rows, fill)
+    return rows, numbers, tensors
+
+
+@process_logits_op.register_fake
+def _process_logits_fake(logits, *arguments):
+    dtype = logits.dtype if logits.dtype in (torch.float32, torch.bfloat16) else torch.float32
+    return (torch.empty(logits.shape, dtype=dtype, device=logits.device),
+            torch.empty(logits.shape[0], dtype=torch.int32, device=logits.device))
+
+
+def _process_logits_setup(ctx, inputs, output):
+    tensors = [t if isinstance(t, torch.Tensor) else None for t in inputs]
+    ctx.save_for_backward(*tensors)
+    ctx.numbers = [None if isinstance(t, torch.Tensor) else t for t in inputs]
+
+
+def _process_logits_backward(ctx, g_out, g_status):
+    inputs = [n if t is None else t for n, t in zip(ctx.numbers, ctx.saved_tensors)]
+    rows, numbers, tensors = _process_arguments(*inputs)
+    grad = _process.process_backward(rows, numbers, tensors, g_out).to(inputs[0].dtype)
+    return (_logprob.first_order(grad, inputs[0], g_out),) + (None,) * (len(inputs) - 1)
+
+
+process_logits_op.register_autograd(_process_logits_backward, setup_context=_process_logits_setup)
+
+
+@torch.library.custom_op("dsv41_rocm::head_logits", mutates_args=(), device_types="cuda")
+def head_logits_op(
+    hidden: torch.Tensor, tiles: torch.Tensor, scales: torch.Tensor, vocab: int, dtype: torch.dtype
+) -> tuple[torch.Tensor, torch.Tensor]:
+    x = _inthead._rows(hidden, "hidden")
+    head = _inthead.Int8Head(tiles, scales, vocab, hidden.shape[1])
+    _inthead._check_head(head, x)
+    if dtype not in _inthead._OUT_DTYPES:
+        raise ValueError("logits are torch.float32 or torch.bfloat16")
+    out = _inthead._new_logits(x.shape[0], vocab, dtype, x.device)
+    return out, _inthead._forward(x, head, out, True)
+
+
+@head_logits_op.register_fake
+def _head_logits_fake(hidden, tiles, scales, vocab, dtype):
+    n, dev = hidden.shape[0], hidden.device
+    return _inthead._new_logits(n, vocab, dtype, dev), torch.empty(n, dtype=torch.int32, device=dev)
+
+
+@torch.library.custom_op("dsv41_rocm::token_embedding", mutates_args=(), device_types="cuda")
+def token_embedding_op(ids: torch.Tensor, weight: torch.Tensor, scale: float) -> tuple[torch.Tensor, torch.Tensor]:
+    flat, weight, scale = _embedding.prepare(ids, weight, scale)
+    out, status = _embedding.forward(flat, weight, scale, True)
+    return out.view(*ids.shape, weight.shape[1]), status
+
+
+@token_embedding_op.register_fake
+def _token_embedding_fake(ids, weight, scale):
+    return (torch.empty(*ids.shape, weight.shape[1], dtype=weight.dtype, device=weight.device),
+            torch.empty(ids.numel(), dtype=torch.int32, device=weight.device))
+
+
+def _token_embedding_setup(ctx, inputs, output):
+    ids, weight, scale = inputs
+    ctx.vocab, ctx.dtype, ctx.scale = weight.shape[0], weight.dtype, scale
+    ctx.save_for_backward(ids)
+
+
+def _token_embedding_backward(ctx, g_rows, g_status):
+    (ids,) = ctx.saved_tensors
+    with torch.no_grad():
+        dw = _embedding.token_embedding_backward(g_rows, ids, ctx.vocab, scale=ctx.scale, dtype=ctx.dtype)
+    return None, _logprob.first_order(dw, g_rows), None
+
+
+token_embedding_op.register_autograd(_token_embedding_backward, setup_context=_token_embedding_setup)
+
+
+__all__ = ["sample_rows", "selected_log_probs_op", "logit_scores_op", "distillation_loss_op", "process_logits_op",
+           "head_logits_op", "token_embedding_op"]

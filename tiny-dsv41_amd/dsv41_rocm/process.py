@@ -18,22 +18,20 @@ import torch
 from . import _lib
 from ._check import any_set
 from .logprob import first_order
-from .scores import INTEGERS, launch, refuse_capture, refuse_tangents, row_fields, rows_of_logits, vector, written
+from .scores import INTEGERS, launch, overlap, refuse_capture, refuse_tangents, row_fields, rows_of_logits, vector, written
 
 Knob = Union[float, torch.Tensor]
 
 
-def _knob(value, name, neutral, rows, device, keep):
-    """(the descriptor's scalar, the pointer of its per-row values or None)"""
+def _knob(value, name, neutral, rows, device):
+    """(the scalar of all rows, a tensor of one value per row or None)"""
     if isinstance(value, torch.Tensor):
         if value.shape != (rows,):
             raise ValueError(f"{name} must be a number or have one value per row")
         if value.requires_grad and torch.is_grad_enabled():
             raise NotImplementedError(f"{name} has no gradient: detach it")
         refuse_tangents(name, value)
-        value = vector(value, torch.float32, (rows,), device)
-        keep.append(value)
-        return neutral, value.data_ptr()
+        return neutral, vector(value, torch.float32, (rows,), device)
     value = float(value)
     if not math.isfinite(value) or neutral and value <= 0:
         raise ValueError("repetition_penalty must be finite and positive" if neutral
@@ -44,52 +42,47 @@ def _knob(value, name, neutral, rows, device, keep):
 def _integers(t, name, dtype, device):
     if not isinstance(t, torch.Tensor) or t.dtype not in INTEGERS:
         raise ValueError(f"{name} must be integers")
-    return t if t.dtype == dtype and t.device == device else t.to(device=device, dtype=dtype)
+    if t.dtype != dtype or t.device != device:
+        if dtype == torch.int32 and t.dtype == torch.int64:  # (what 32 bits would wrap stays out of range)
+            t = t.clamp(-(1 << 31), (1 << 31) - 1)
+        t = t.to(device=device, dtype=dtype)
+    return t
 
 
-def _lengths(t, name, rows, device, keep):
+def _lengths(t, name, rows, device):
     t = _integers(torch.as_tensor(t), name, torch.int32, device)
     if t.shape != (rows,):
         raise ValueError(f"{name} must have one length per row")
-    t = t.contiguous()
-    keep.append(t)
-    return t.data_ptr()
+    return t.contiguous()
 
 
 def _rows_of(t):
-    """(a matrix whose rows are contiguous, at any row stride that is not negative; that stride)"""
-    if t.shape[1] > 1 and t.stride(1) != 1:
-        t = t.contiguous()
-    return t, t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    """A matrix whose rows are contiguous, at any row stride that is not negative."""
+    return t.contiguous() if t.shape[1] > 1 and t.stride(1) != 1 else t
+
+
+def _step(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def _arguments(logits, history, history_lens, history_prompt_lens, repetition_penalty, presence_penalty,
                frequency_penalty, bias_ids, bias, token_mask, mask_rows, fill):
-    """Validated arguments in kernel form: the descriptor's values from history to fill, and the tensors that they
-    point to."""
+    """Validated arguments in kernel form: the numbers, and the tensors (or None) that :func:`_fields` takes."""
     rows, vocab = logits.shape
     dev = logits.device
-    keep = []
-    rp, rps = _knob(repetition_penalty, "repetition_penalty", 1.0, rows, dev, keep)
-    pres, press = _knob(presence_penalty, "presence_penalty", 0.0, rows, dev, keep)
-    freq, freqs = _knob(frequency_penalty, "frequency_penalty", 0.0, rows, dev, keep)
-    hist = lens = prompts = None
-    hist_step = hist_len = 0
+    rp, rps = _knob(repetition_penalty, "repetition_penalty", 1.0, rows, dev)
+    pres, press = _knob(presence_penalty, "presence_penalty", 0.0, rows, dev)
+    freq, freqs = _knob(frequency_penalty, "frequency_penalty", 0.0, rows, dev)
     if history is not None:
         if history.ndim != 2 or history.shape[0] != rows:
             raise ValueError("history must have shape [rows, history_length]")
-        history, hist_step = _rows_of(_integers(history, "history", torch.int64, dev))
-        hist_len = history.shape[1]
+        history = _rows_of(_integers(history, "history", torch.int64, dev))
         if history_lens is not None:
-            lens = _lengths(history_lens, "history_lens", rows, dev, keep)
+            history_lens = _lengths(history_lens, "history_lens", rows, dev)
         if history_prompt_lens is not None:
-            prompts = _lengths(history_prompt_lens, "history_prompt_lens", rows, dev, keep)
-        keep.append(history)
-        hist = history.data_ptr()
+            history_prompt_lens = _lengths(history_prompt_lens, "history_prompt_lens", rows, dev)
     elif history_lens is not None or history_prompt_lens is not None:
         raise ValueError("history_lens and history_prompt_lens require a history")
-    ids = values = None
-    bias_step = bias_len = 0
     if bias is not None and bias_ids is not None:
         if bias.requires_grad and torch.is_grad_enabled():
             raise NotImplementedError("bias has no gradient: detach it")
@@ -99,14 +92,8 @@ def _arguments(logits, history, history_lens, history_prompt_lens, repetition_pe
             raise ValueError("bias_ids and bias must have shape [rows, entries] or [entries]")
         bias_ids = _integers(bias_ids, "bias_ids", torch.int64, dev).contiguous()
         bias = vector(bias, torch.float32, bias.shape, dev)
-        bias_len = bias.shape[-1]
-        bias_step = bias_len if bias.ndim == 2 else 0
-        keep += (bias_ids, bias)
-        ids, values = bias_ids.data_ptr(), bias.data_ptr()
     elif bias is not None or bias_ids is not None:
         raise ValueError("bias_ids and bias are given together")
-    mask = which = None
-    masks = mask_step = 0
     if token_mask is not None:
         if not isinstance(token_mask, torch.Tensor) or token_mask.dtype != torch.int32 or \
                 token_mask.ndim not in (1, 2) or token_mask.shape[-1] < (vocab + 31) // 32:
@@ -115,41 +102,52 @@ def _arguments(logits, history, history_lens, history_prompt_lens, repetition_pe
             token_mask = token_mask[None]
         if token_mask.device != dev:
             token_mask = token_mask.to(dev)
-        token_mask, mask_step = _rows_of(token_mask)
+        token_mask = _rows_of(token_mask)
         masks = token_mask.shape[0]
         if mask_rows is not None:
             mask_rows = _integers(mask_rows, "mask_rows", torch.int32, dev).contiguous()
             if mask_rows.shape != (rows,):
                 raise ValueError("mask_rows must have one mask per row")
-            keep.append(mask_rows)
-            which = mask_rows.data_ptr()
         elif masks != 1 and masks != rows:
             raise ValueError("without mask_rows there is one token_mask, or one per row")
         if masks == 0 and rows:
             raise ValueError("token_mask holds no mask")
-        keep.append(token_mask)
-        mask = token_mask.data_ptr()
     elif mask_rows is not None:
         raise ValueError("mask_rows requires a token_mask")
     fill = float(fill)
     if math.isnan(fill):
         raise ValueError("fill must be a number")
-    return (hist, hist_step, hist_len, lens, prompts, rp, pres, freq, rps, press, freqs, ids, values, bias_step, bias_len,
-            masks, mask, mask_step, which, fill), keep
+    return (rp, pres, freq, fill), (rps, press, freqs, history, history_lens, history_prompt_lens, bias_ids, bias,
+                                    token_mask, mask_rows)
 
 
-def forward(logits, fields, out, want_status):
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _fields(numbers, tensors):
+    """The descriptor's values from history to fill.  (Formed anew in the backward: what a graph saved may have been
+    moved, to the host and back, in between.)"""
+    rp, pres, freq, fill = numbers
+    rps, press, freqs, history, lens, prompts, ids, bias, mask, which = tensors
+    return (*((None, 0, 0) if history is None else (history.data_ptr(), _step(history), history.shape[1])), _ptr(lens),
+            _ptr(prompts), rp, pres, freq, _ptr(rps), _ptr(press), _ptr(freqs), _ptr(ids), _ptr(bias),
+            *((0, 0) if bias is None else (bias.shape[-1] if bias.ndim == 2 else 0, bias.shape[-1])),
+            *((0, None, 0) if mask is None else (mask.shape[0], mask.data_ptr(), _step(mask))), _ptr(which), fill)
+
+
+def forward(logits, numbers, tensors, out, want_status):
     """One dsv41_process_run into ``out``; returns the statuses or None."""
     rows, vocab = logits.shape
     status = torch.empty(rows, dtype=torch.int32, device=logits.device) if want_status else None
     if rows:
-        d = _lib.ProcessDesc(*row_fields(_lib.ProcessDesc, logits), *fields, out.data_ptr(), out.stride(0) if rows > 1 else vocab,
-                             None if status is None else status.data_ptr(), None, 0)
+        d = _lib.ProcessDesc(*row_fields(_lib.ProcessDesc, logits), *_fields(numbers, tensors), out.data_ptr(),
+                             out.stride(0) if rows > 1 else vocab, _ptr(status), None, 0)
         launch(_lib.load().dsv41_process_run, logits.device, ctypes.byref(d))
     return status
 
 
-def process_backward(logits, fields, grad):
+def process_backward(logits, numbers, tensors, grad):
     """dL/dlogits of :func:`process_logits` from dL/dresult, in the logits' dtype."""
     refuse_tangents("gradients", grad)
     rows, vocab = logits.shape
@@ -160,19 +158,19 @@ def process_backward(logits, fields, grad):
         if unit != 1 and vocab > 1 or rows > 1 and 0 < step < vocab:
             grad = grad.contiguous()
             step = vocab
-        d = _lib.ProcessDesc(*row_fields(_lib.ProcessDesc, logits), *fields, out.data_ptr(), vocab, None, grad.data_ptr(),
-                             step if rows > 1 else vocab)
+        d = _lib.ProcessDesc(*row_fields(_lib.ProcessDesc, logits), *_fields(numbers, tensors), out.data_ptr(), vocab, None,
+                             grad.data_ptr(), step if rows > 1 else vocab)
         launch(_lib.load().dsv41_process_grad_run, logits.device, ctypes.byref(d))
     return out
 
 
 class _Process(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, fields, want_status, *lists):
+    def forward(ctx, logits, numbers, want_status, *tensors):
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        status = forward(logits, fields, out, want_status)
-        ctx.fields = fields
-        ctx.save_for_backward(logits, *lists)
+        status = forward(logits, numbers, tensors, out, want_status)
+        ctx.numbers = numbers
+        ctx.save_for_backward(logits, *tensors)
         ctx.set_materialize_grads(False)
         if status is not None:
             ctx.mark_non_differentiable(status)
@@ -180,11 +178,11 @@ class _Process(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad, g_status):
-        logits, *lists = ctx.saved_tensors  # (the lists too: one that was written since is refused here)
-        nothing = (None,) * (2 + len(lists))
+        logits, *tensors = ctx.saved_tensors
+        nothing = (None,) * (2 + len(tensors))
         if grad is None:
             return None, *nothing
-        return first_order(process_backward(logits, ctx.fields, grad), logits, grad), *nothing
+        return first_order(process_backward(logits, ctx.numbers, tensors, grad), logits, grad), *nothing
 
 
 def _status_error(status: torch.Tensor) -> None:
@@ -203,13 +201,6 @@ def _status_error(status: torch.Tensor) -> None:
         raise ValueError("token mask leaves a row without tokens")
 
 
-def _extent(t):
-    """[first, past the last) byte that the matrix touches."""
-    size = t.element_size()
-    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + (last + 1) * size
-
-
 def _output(out, logits):
     """A validated ``out``: the logits' own tensor, or one that does not touch their memory."""
     if not isinstance(out, torch.Tensor) or out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
@@ -217,10 +208,9 @@ def _output(out, logits):
     rows, vocab = out.shape
     if vocab > 1 and out.stride(1) != 1 or rows > 1 and out.stride(0) < vocab:
         raise ValueError("out must have contiguous rows that do not overlap")
-    if out is not logits and rows and not (out.data_ptr() == logits.data_ptr() and (rows == 1 or out.stride(0) == logits.stride(0))):
-        a, b = _extent(out), _extent(logits)
-        if a[0] < b[1] and b[0] < a[1]:
-            raise ValueError("out overlaps the logits without being them")
+    same = out is logits or out.data_ptr() == logits.data_ptr() and (rows == 1 or out.stride(0) == logits.stride(0))
+    if not same and overlap(out, logits):
+        raise ValueError("out overlaps the logits without being them")
     return out
 
 
@@ -256,8 +246,8 @@ def process_logits(
       mask, -1 for none; without it there is one mask, or one per row.
 
     Negative ids are padding.  ``logit_scores`` and ``distillation_loss`` take ``-inf`` for masked tokens;
-    ``sample`` takes finite logits only, so masks for it come with a finite ``fill`` that is far below any
-    logit times the temperature (-8192, or less for logits in the thousands).
+    ``sample`` takes finite logits only, so masks for it come with a finite ``fill`` that stays finite in the logits' type
+    and when divided by the temperature, and is 40 temperatures or more below the logits (-8192, say).
 
     ``out`` takes the result; it may be ``logits`` itself, in which case only what changes is written.  A call
     with ``out`` has no gradient.  Otherwise the result is differentiable in ``logits``, once, in backward
@@ -268,21 +258,21 @@ def process_logits(
     are ignored, and rows of such penalties and masks hold NaN.
     """
     logits = rows_of_logits(logits, 1.0)
-    fields, keep = _arguments(logits, history, history_lens, history_prompt_lens, repetition_penalty, presence_penalty,
-                              frequency_penalty, bias_ids, bias, token_mask, mask_rows, fill)
+    numbers, tensors = _arguments(logits, history, history_lens, history_prompt_lens, repetition_penalty, presence_penalty,
+                                  frequency_penalty, bias_ids, bias, token_mask, mask_rows, fill)
     refuse_capture(check)
     tracked = torch.is_grad_enabled() and logits.requires_grad
     if out is not None:
         if tracked or torch.is_grad_enabled() and out.requires_grad:
             raise ValueError("a call with out has no gradient: leave it out, or call under no_grad")
         out = _output(out, logits)
-        status = forward(logits, fields, out, check)
+        status = forward(logits, numbers, tensors, out, check)
         written(out)
     elif tracked:
-        out, status = _Process.apply(logits, fields, check, *keep)
+        out, status = _Process.apply(logits, numbers, check, *tensors)
     else:
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        status = forward(logits, fields, out, check)
+        status = forward(logits, numbers, tensors, out, check)
     if check and any_set(status)[0]:
         _status_error(status)
     return out

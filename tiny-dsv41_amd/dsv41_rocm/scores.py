@@ -105,6 +105,18 @@ def written(t) -> None:
         torch.autograd.graph.increment_version(t)
 
 
+def overlap(a, b) -> bool:
+    """Whether the memory that two tensors of nonnegative strides reach over meets."""
+    def extent(t):
+        last = sum((n - 1) * step for n, step in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+    if a.numel() == 0 or b.numel() == 0 or a.device != b.device:
+        return False
+    (a0, a1), (b0, b1) = extent(a), extent(b)
+    return a0 < b1 and b0 < a1
+
+
 def vector(t, dtype, shape, device):
     """A contiguous tensor of that dtype and shape on the device, ``t`` itself where it is one."""
     if t.dtype != dtype or t.device != device:
