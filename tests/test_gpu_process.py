@@ -429,3 +429,53 @@ def test_refusals_on_the_gpu():
         process_logits(d, out=w)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+@pytest.mark.parametrize("rows,V,hist,bias,masks", [(1100, 300, 60, 9, 5), (530, 20001, 700, 64, 0), (1030, 16385, 16383, 0, 3),
+                                                    (1030, 5000, 16384, 3, 0), (1030, 5000, 40, 65, 2)])
+def test_many_bf16_rows_are_those_of_few(rows, V, hist, bias, masks):
+    # large batches of bf16 rows keep what the lists say in words of 16 bits, where those hold it; small ones in 32
+    x, a = _inputs(rows, V, torch.bfloat16, hist, bias, masks, pad=3)
+    a["history"][0] = V - 1  # one token as often as the list is long
+    a["history_prompt_lens"][0] = 0
+    a["history"][1] = 7
+    a["history_prompt_lens"][1] = hist
+    a, d = _to(a), x.to(DEV)
+    up = torch.randn(rows, V, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV).bfloat16()
+
+    def part(take):
+        return {k: v[take] if isinstance(v, torch.Tensor) and k != "token_mask" else v for k, v in a.items()}
+
+    def both(take):
+        leaf = d[take].detach().requires_grad_()
+        y = process_logits(leaf, **part(take))
+        own = d[take].clone()
+        process_logits(own, **part(take), out=own)
+        assert torch.equal(own, y)
+        return y.detach(), torch.autograd.grad(y, leaf, up[take])[0]
+
+    whole = both(slice(None))
+    for r in range(0, rows, 50):
+        take = slice(r, min(rows, r + 50))
+        for u, v in zip(whole, both(take)):
+            assert torch.equal(u[take], v)
+    few = [0, 1, 2, rows // 2, rows - 1]
+    small = {k: v[few].cpu() if isinstance(v, torch.Tensor) and k != "token_mask" else v.cpu() if isinstance(v, torch.Tensor) else v
+             for k, v in a.items()}
+    want, bound, grad, gbound = _plain(x[few], small, up[few].cpu())
+    _close(whole[0][few], want, bound)
+    _close(whole[1][few], grad, gbound)
+
+
+def test_longest_lists_of_bf16_rows():
+    V = 9000
+    x = torch.randn(1, V, device=DEV).bfloat16()
+    ids = torch.arange(4095, device=DEV) * 2
+    b = torch.randn(4095, device=DEV)
+    want = x.float()
+    want[0, ids] += b
+    assert torch.equal(process_logits(x, bias_ids=ids, bias=b), want.bfloat16())
+    h = torch.full((1, 524287), 8999, device=DEV)
+    want = x.float()
+    want[0, 8999] = want[0, 8999] - 524287.0
+    assert torch.equal(process_logits(x, history=h, frequency_penalty=1.0), want.bfloat16())

@@ -10,12 +10,21 @@
 // and, for a gradient g of the outputs: 0 where the mask leaves i out, g / rp or g rp in the history by the
 // sign of x + b_i, g elsewhere.
 //
-// One pass: a workgroup takes a slice of SLICE ids of a row.  What the lists say of the slice's ids goes into
-// one LDS word each, by integer atomics, so in any order to the same words: 12 bits the last bias entry that
-// names the id (+ 1), one bit "in the history", 19 bits its count.  The slice's elements are on their way
-// meanwhile, and most words are 0 then: such elements go out as they came.  Every slice reads all of its
-// row's lists, which therefore stay on one XCD (whose L2 serves all but the first).
-// In place nothing is read but what a list names, and nothing written but that and what is masked.
+// One pass: a workgroup takes a slice of 8192 ids of a row.  What the lists say of the slice's ids goes into
+// one LDS word each, by integer atomics, so in any order to the same words.  The slice's elements are on their way
+// meanwhile, and most words are 0 then: such groups of 16 bytes go out as they came.  Every slice reads all of its
+// row's lists, which therefore stay on one XCD (whose L2 serves all but the first).  A mask's words come before the
+// elements: groups without an allowed one are not read.
+// In place, nothing is read but groups that a list names or that are masked in part, and written but those and what is masked.
+// The gradient needs two bits an id: whether the history has it, and the sign of x + b, from single logits that are
+// read for the history's ids while the gradient's own are on their way.
+//
+// Slices begin at memory lines of the result, so rows of an odd vocabulary are written by whole lines: 500 bf16 rows of
+// 151851 copied in 51 us (5.9 TB/s of read and write), as many of 151936 in 53.  2048 fp32 rows: 445 us (5.6 TB/s),
+// with masks 471, with histories of 4096 500; bf16 210, 226 and 293.  256 to 1024 threads and slices of 8192 to 16384
+// ids: 512 and 8192 are the best or within 3% (1024 and 16384: 2048 fp32 rows with histories 506, 256 and 8192: 778).
+// What bounds it: memory, and beside long histories of bf16 rows the instructions of reading the lists, once a slice
+// (2048 ids cost 500 rows 12 us).
 
 #include <math.h>
 
@@ -28,13 +37,11 @@ using rows::bf16_t;
 using rows::Elem;
 
 constexpr int NT = 512;
-constexpr int SLICE = 8192;  // ids; 32 KB of words: four workgroups a CU
-constexpr int COUNT_BITS = 19;
-constexpr uint32_t COUNT = (1u << COUNT_BITS) - 1, SEEN = 1u << COUNT_BITS;
-constexpr int ENTRY_SHIFT = COUNT_BITS + 1;
-constexpr int MAX_BIAS = (1 << (32 - ENTRY_SHIFT)) - 1;  // entries of a row's list
-
-constexpr int COPY = 0, INPLACE = 1, GRAD = 2;
+// ids of a slice: 32 KB of words, four workgroups a CU
+constexpr int SLICE = 8192, SHORT_SLICE = 16384;
+constexpr int MAX_HISTORY = (1 << 19) - 1, MAX_BIAS = (1 << 12) - 1;  // entries of a row's lists
+constexpr int SHORT_HISTORY = (1 << 14) - 1, SHORT_BIAS = 64;         // those that words of 16 bits take
+constexpr int AHEAD = 8;                                              // history entries of a thread in flight
 
 struct Params {
   const void* x;
@@ -63,25 +70,80 @@ struct Params {
   int32_t* status;
 };
 
-// What the row's knobs and lists make of an element whose word is not 0.
+// What the lists say of an element: how often it was said, whether it is in the history at all, and its entry of the
+// bias list (-1: none).
+struct Said {
+  uint32_t count;
+  bool listed;
+  int entry;
+};
+
+// What the row's knobs make of it.
 struct Knobs {
   float rp, pres, freq;
-  __device__ __forceinline__ float apply(float x, uint32_t word, const float* bias) const {
-    if (word >> ENTRY_SHIFT) x = x + bias[(word >> ENTRY_SHIFT) - 1];
-    const uint32_t c = word & COUNT;
-    if (word & (SEEN | COUNT)) {
+  __device__ __forceinline__ float apply(float x, Said s, const float* bias) const {
+    if (s.entry >= 0) x = x + bias[s.entry];
+    if (s.listed) {
       x = x > 0.0f ? x / rp : x * rp;
-      const float f = freq * (float)c;
+      const float f = freq * (float)s.count;
       x = x - f;
-      if (c > 0) x = x - pres;
+      if (s.count > 0) x = x - pres;
     }
     return x;
   }
-  // the gradient's factor is 1 / rp or rp, of ids that are not only biased
-  __device__ __forceinline__ float slope(float g, float x, uint32_t word, const float* bias) const {
-    if (!(word & (SEEN | COUNT))) return g;
-    if (word >> ENTRY_SHIFT) x = x + bias[(word >> ENTRY_SHIFT) - 1];
-    return x > 0.0f ? g / rp : g * rp;
+};
+
+// The words of a slice.  Of 32 bits: count (19), in the history (1), bias entry + 1 (12).
+template <typename T, bool SHORT>
+struct Words {
+  static constexpr int IDS = SLICE, G = Elem<T>::VEC;
+  uint32_t* w;
+  // a thread's group of 8 bf16 elements lies in two planes, so that either half of it is read without bank conflicts
+  static __device__ __forceinline__ int place(int at) {
+    return G == 4 ? at : ((at >> 2 & 1) * (IDS / 2)) + (at >> 3 << 2) + (at & 3);
+  }
+  __device__ __forceinline__ void say(int at) const { atomicAdd(&w[place(at)], 1u); }
+  __device__ __forceinline__ void list(int at) const { atomicOr(&w[place(at)], 1u << 19); }
+  __device__ __forceinline__ void bias(int at, int entry) const { atomicMax(&w[place(at)], (uint32_t)(entry + 1) << 20); }
+  // the elements at .. at + G - 1 that anything is said of
+  __device__ __forceinline__ uint32_t marked(int at) const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int q = 0; q < G; q += 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(w + place(at + q));
+      m |= (min(v.x, 1u) | min(v.y, 1u) << 1 | min(v.z, 1u) << 2 | min(v.w, 1u) << 3) << q;
+    }
+    return m;
+  }
+  __device__ __forceinline__ Said read(int at, const int*, int) const {
+    const uint32_t v = w[place(at)];
+    return {v & MAX_HISTORY, (v & 0xFFFFF) != 0, (int)(v >> 20) - 1};
+  }
+};
+// Of 16 bits: count (14), in the history (1), biased (1), for slices twice as long, whose lists are read half as often;
+// a biased element looks for its entry among the list's places.
+template <typename T>
+struct Words<T, true> {
+  static constexpr int IDS = SHORT_SLICE, G = Elem<T>::VEC;
+  uint32_t* w;
+  __device__ __forceinline__ void say(int at) const { atomicAdd(&w[at >> 1], 1u << (16 * (at & 1))); }
+  __device__ __forceinline__ void list(int at) const { atomicOr(&w[at >> 1], 0x4000u << (16 * (at & 1))); }
+  __device__ __forceinline__ void bias(int at, int) const { atomicOr(&w[at >> 1], 0x8000u << (16 * (at & 1))); }
+  __device__ __forceinline__ uint32_t marked(int at) const {
+    static_assert(G == 8, "a group's words are 16 bytes");
+    const uint4 v = *reinterpret_cast<const uint4*>(w + (at >> 1));
+    const uint32_t d[4] = {v.x, v.y, v.z, v.w};
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m |= (min(d[i] & 0xFFFFu, 1u) | min(d[i] >> 16, 1u) << 1) << (2 * i);
+    return m;
+  }
+  __device__ __forceinline__ Said read(int at, const int* places, int n) const {
+    const uint32_t v = w[at >> 1] >> (16 * (at & 1)) & 0xFFFFu;
+    int entry = -1;
+    if (v & 0x8000u)
+      for (entry = n - 1; entry > 0 && places[entry] != at; --entry) {}
+    return {v & SHORT_HISTORY, (v & 0x7FFFu) != 0, entry};
   }
 };
 
@@ -154,222 +216,348 @@ __device__ __forceinline__ void drop(Group& g, uint32_t allowed, uint32_t instea
     g.w[k] = (g.w[k] & keep) | (instead & ~keep);
   }
 }
-// The word of element `at` of a slice: a thread's group of 8 bf16 elements lies in two planes, so that either
-// half of it is read without bank conflicts.
-template <typename T>
-__device__ __forceinline__ int word_at(int at) {
-  return Elem<T>::VEC == 4 ? at : ((at >> 2 & 1) * (SLICE / 2)) + (at >> 3 << 2) + (at & 3);
+// A workgroup's slice: ids [begin, begin + IDS) of a row, those of them that exist from `first` on, `count` of them.
+struct Slice {
+  int row, number, begin;
+  uint32_t first, count;
+  // the slice's place of an id (any 64 bits), where that is below `count` when `first` is taken off
+  __device__ __forceinline__ bool place_of(uint2 id, uint32_t& at) const {
+    at = id.x - (uint32_t)begin;
+    return id.y == 0 && at - first < count;
+  }
+};
+// false: none.  A row's slices go one after another to one XCD (workgroups go round-robin over the eight), and begin at
+// memory lines of the result.
+template <typename T, int IDS>
+__device__ __forceinline__ bool slice_of(const Params& p, Slice& s) {
+  const uint32_t item = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  s.row = (int)(item / (uint32_t)p.slices), s.number = (int)(item % (uint32_t)p.slices);
+  if (s.row >= p.rows) return false;
+  s.begin = s.number * IDS - rows::skew_of(static_cast<const T*>(p.out) + s.row * p.os);
+  if (s.begin >= p.V) return false;
+  s.first = (uint32_t)max(-s.begin, 0), s.count = (uint32_t)min(IDS, p.V - s.begin) - s.first;
+  return true;
 }
 
-template <typename T, bool LISTS, bool MASK, int MODE>
-__global__ __launch_bounds__(NT, 8) void process_kernel(Params p) {
-  constexpr int G = Elem<T>::VEC, U = SLICE / (NT * G), AHEAD = 8;
-  extern __shared__ uint32_t words[];  // SLICE words, then the row's biases
-  float* biases = reinterpret_cast<float*>(words + SLICE);
-  const int tid = threadIdx.x;
-  // a row's slices one after another on one XCD (workgroups go round-robin over the eight)
-  const uint32_t item = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
-  const int row = (int)(item / (uint32_t)p.slices), slice = (int)(item % (uint32_t)p.slices);
-  if (row >= p.rows) return;
-  const T* x = static_cast<const T*>(p.x) + row * p.xs;
-  T* out = static_cast<T*>(p.out) + row * p.os;
-  // slices begin at memory lines of the result
-  const int begin = slice * SLICE - rows::skew_of(out);
-  if (begin >= p.V) return;
-  const T* from = MODE == GRAD ? static_cast<const T*>(p.grad) + row * p.gs : x;
-
-  // the row's own values, all on their way at once: arrays that are not given are read at the arguments' begin
+// The row's own values.
+struct Row {
+  Knobs knobs{1.f, 0.f, 0.f};
+  bool bad = false;  // the row holds NaN
+  int bits = 0;      // the status bit that says why
+  const uint32_t* mask = nullptr;
+  const uint2* h = nullptr;  // the history, where the knobs ask for it
+  int len = 0, prompt = 0;
+};
+template <bool LISTS, bool MASK, bool GRADIENT>
+__device__ __forceinline__ Row row_of(const Params& p, int row) {
+  // all on their way at once: arrays that are not given are read at the arguments' begin
   typedef const __attribute__((address_space(4))) int32_t* constant_t;
   const uintptr_t nowhere = (uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
   auto value_of = [&](const void* a) { return *(constant_t)(a ? (uintptr_t)a + 4 * (int64_t)row : nowhere); };
   const int m_row = MASK ? value_of(p.mask_rows) : 0;
   const int rp_row = LISTS ? value_of(p.rps) : 0, pres_row = LISTS ? value_of(p.press) : 0, freq_row = LISTS ? value_of(p.freqs) : 0;
   const int len_row = LISTS ? value_of(p.lens) : 0, prompt_row = LISTS ? value_of(p.prompt_lens) : 0;
-  Knobs knobs{1.f, 0.f, 0.f};
-  bool bad = false;
-  int bits = 0;  // status bits that this thread met
-  const uint32_t* mask = nullptr;
+  Row r;
   if constexpr (MASK) {
     const int m = p.mask_rows ? m_row : p.masks == 1 ? 0 : row;
-    bad = m >= p.masks;
-    if (bad) bits |= DSV41_STATUS_BAD_MASK;
-    mask = m >= 0 && !bad ? p.mask + m * p.ms : nullptr;
+    r.bad = m >= p.masks;
+    if (r.bad) r.bits |= DSV41_STATUS_BAD_MASK;
+    r.mask = m >= 0 && !r.bad ? p.mask + m * p.ms : nullptr;
   }
-  bool listed = false;
-  int len = 0, prompt = 0;
-  const int64_t* h = nullptr;
   if constexpr (LISTS) {
-    knobs.rp = p.rps ? __int_as_float(rp_row) : p.rp;
-    knobs.pres = p.press ? __int_as_float(pres_row) : p.pres;
-    knobs.freq = p.freqs ? __int_as_float(freq_row) : p.freq;
-    if (!(isfinite(knobs.rp) && knobs.rp > 0.f) || !isfinite(knobs.pres) || !isfinite(knobs.freq)) {
-      bad = true;
-      bits |= DSV41_STATUS_BAD_PENALTY;
+    Knobs& k = r.knobs;
+    k.rp = p.rps ? __int_as_float(rp_row) : p.rp;
+    k.pres = p.press ? __int_as_float(pres_row) : p.pres;
+    k.freq = p.freqs ? __int_as_float(freq_row) : p.freq;
+    if (!(isfinite(k.rp) && k.rp > 0.f) || !isfinite(k.pres) || !isfinite(k.freq)) {
+      r.bad = true;
+      r.bits |= DSV41_STATUS_BAD_PENALTY;
     }
     // (a gradient asks for the repetition penalty alone)
-    if (p.history && !(knobs.rp == 1.f && (MODE == GRAD || (knobs.pres == 0.f && knobs.freq == 0.f)))) {
-      h = p.history + row * p.hs;
-      len = p.lens ? min(max(len_row, 0), p.hist_len) : p.hist_len;
-      prompt = p.prompt_lens ? prompt_row : 0;
+    if (p.history && !(k.rp == 1.f && (GRADIENT || (k.pres == 0.f && k.freq == 0.f)))) {
+      r.h = reinterpret_cast<const uint2*>(p.history + row * p.hs);
+      r.len = p.lens ? min(max(len_row, 0), p.hist_len) : p.hist_len;
+      r.prompt = p.prompt_lens ? prompt_row : 0;
     }
-    listed = len > 0 || (p.n_bias > 0 && (MODE != GRAD || h));
   }
+  return r;
+}
 
-  // the history's first entries, ahead of the slice itself: loads come back in order
-  uint2 ahead[AHEAD];
-  const uint2* h2 = reinterpret_cast<const uint2*>(h);
-  if (LISTS) {
-#pragma unroll
-    for (int k = 0; k < AHEAD; ++k)
-      if (tid + k * NT < len) ahead[k] = h2[tid + k * NT];
+// Which elements of a group at id i there are, and which of them the row's mask allows.
+template <typename T, bool MASK>
+__device__ __forceinline__ void group_at(const Params& p, const Row& r, int i, bool inside, uint32_t& there, uint32_t& allowed) {
+  constexpr int G = Elem<T>::VEC;
+  there = ALL<T>;
+  if (!inside) {
+    const int lo = max(-i, 0), hi = min(p.V - i, G);  // elements [lo, hi)
+    there = lo < hi ? (ALL<T> << lo) & (ALL<T> >> (G - hi)) : 0u;
   }
-  // which elements of the thread's groups there are, and which of them the mask allows
-  const bool inside = begin >= 0 && begin + SLICE <= p.V;  // (all of them)
+  allowed = r.bad ? 0u : there;
+  if (MASK && r.mask && there) {
+    const int k = max(i, 0) >> 5, last = (p.V - 1) >> 5;
+    const uint64_t both = (uint64_t)r.mask[min(k + 1, last)] << 32 | r.mask[k];
+    allowed &= i >= 0 ? (uint32_t)(both >> (i & 31)) : (uint32_t)(both << -i);
+  }
+}
+
+// `batch(first, ids)` for every AHEAD entries of a thread; the first ones were loaded ahead of the slice itself, as loads come back
+// in order.
+__device__ __forceinline__ void load_ahead(const Row& r, int j0, uint2 (&ids)[AHEAD]) {
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k)
+    if (j0 + k * NT < r.len) ids[k] = r.h[j0 + k * NT];
+}
+template <class F>
+__device__ __forceinline__ void for_history(const Row& r, uint2 (&ahead)[AHEAD], F batch) {
+  batch((int)threadIdx.x, ahead);
+  for (int j0 = AHEAD * NT; j0 < r.len; j0 += AHEAD * NT) {
+    load_ahead(r, j0 + (int)threadIdx.x, ahead);
+    batch(j0 + (int)threadIdx.x, ahead);
+  }
+}
+__device__ __forceinline__ bool past(uint2 id, int V) { return (int)id.y >= 0 && (id.y > 0 || id.x >= (uint32_t)V); }
+
+template <typename T, bool LISTS, bool MASK, bool INPLACE, bool SHORT>
+__global__ __launch_bounds__(NT, 8) void process_kernel(Params p) {
+  using W = Words<T, SHORT>;
+  constexpr int IDS = W::IDS, G = Elem<T>::VEC, U = IDS / (NT * G), DWORDS = IDS / (SHORT ? 2 : 1);
+  extern __shared__ uint32_t shared[];  // the words, then the row's biases and (short words) their places in the slice
+  const W words{shared};
+  float* biases = reinterpret_cast<float*>(shared + DWORDS);
+  int* places = reinterpret_cast<int*>(biases + p.n_bias);
+  const int tid = threadIdx.x;
+  Slice s;
+  if (!slice_of<T, IDS>(p, s)) return;
+  const Row r = row_of<LISTS, MASK, false>(p, s.row);
+  const T* x = static_cast<const T*>(p.x) + s.row * p.xs + s.begin;
+  T* out = static_cast<T*>(p.out) + s.row * p.os + s.begin;
+  const bool listed = LISTS && (r.len > 0 || p.n_bias > 0), inside = s.begin >= 0 && s.begin + IDS <= p.V;
+  int bits = r.bits;  // status bits that this thread met
+
+  uint2 ahead[AHEAD];
+  if (LISTS) load_ahead(r, tid, ahead);
   uint32_t there[U], allowed[U];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int i = begin + (u * NT + tid) * G;
-    there[u] = ALL<T>;
-    if (!inside) {
-      const int lo = max(-i, 0), hi = min(p.V - i, G);  // elements [lo, hi)
-      there[u] = lo < hi ? (ALL<T> << lo) & (ALL<T> >> (G - hi)) : 0u;
-    }
-    allowed[u] = bad ? 0u : there[u];
-    if (MASK && mask && there[u]) {
-      const int k = max(i, 0) >> 5, last = (p.V - 1) >> 5;
-      const uint64_t both = (uint64_t)mask[min(k + 1, last)] << 32 | mask[k];
-      allowed[u] &= i >= 0 ? (uint32_t)(both >> (i & 31)) : (uint32_t)(both << -i);
-    }
-  }
-  if (LISTS && listed) {
-    uint4* w4 = reinterpret_cast<uint4*>(words);
+  for (int u = 0; u < U; ++u) group_at<T, MASK>(p, r, s.begin + (u * NT + tid) * G, inside, there[u], allowed[u]);
+  if (listed) {
+    uint4* w4 = reinterpret_cast<uint4*>(shared);
 #pragma unroll
-    for (int i = 0; i < SLICE / 4 / NT; ++i) w4[i * NT + tid] = make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < DWORDS / 4 / NT; ++i) w4[i * NT + tid] = make_uint4(0, 0, 0, 0);
     rows::lds_barrier();
   }
   // what is read: the groups with an allowed element
   Group v[U];
-  if constexpr (MODE != INPLACE) {
+  if constexpr (!INPLACE) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (allowed[u]) load_group(from + begin + (u * NT + tid) * G, there[u], v[u]);
+      if (allowed[u]) load_group(x + (u * NT + tid) * G, there[u], v[u]);
   }
 
-  if constexpr (LISTS) {
-    if (listed) {
-      // ids in [max(begin, 0), begin + SLICE) and below V, as unsigned offsets of the slice
-      const uint32_t first = (uint32_t)max(-begin, 0), count = (uint32_t)min(SLICE, p.V - begin) - first;
-      const bool report = MODE != GRAD && p.status && slice == 0;
-      if (p.n_bias) {
-        const uint2* ids = reinterpret_cast<const uint2*>(p.bias_ids + row * p.bs);
-        const float* b = p.bias + row * p.bs;
-        for (int e = tid; e < p.n_bias; e += NT) {
-          const uint2 id = ids[e];
-          biases[e] = b[e];
-          const uint32_t at = id.x - (uint32_t)begin;
-          if (id.y == 0 && at - first < count) atomicMax(&words[word_at<T>(at)], (uint32_t)(e + 1) << ENTRY_SHIFT);
-          if (report && (int)id.y >= 0 && (id.y > 0 || id.x >= (uint32_t)p.V)) bits |= DSV41_STATUS_BAD_BIAS;
-        }
-        rows::lds_barrier();
-      }
-      auto mark = [&](int j, uint2 id) {
-        const uint32_t at = id.x - (uint32_t)begin;
-        if (id.y == 0 && at - first < count) {
-          if (j < prompt) atomicOr(&words[word_at<T>(at)], SEEN);
-          else atomicAdd(&words[word_at<T>(at)], 1u);
-        }
-        if (report && (int)id.y >= 0 && (id.y > 0 || id.x >= (uint32_t)p.V)) bits |= DSV41_STATUS_BAD_HISTORY;
-      };
-#pragma unroll
-      for (int k = 0; k < AHEAD; ++k)
-        if (tid + k * NT < len) mark(tid + k * NT, ahead[k]);
-      for (int j0 = AHEAD * NT; j0 < len; j0 += AHEAD * NT) {
-#pragma unroll
-        for (int k = 0; k < AHEAD; ++k)
-          if (j0 + tid + k * NT < len) ahead[k] = h2[j0 + tid + k * NT];
-#pragma unroll
-        for (int k = 0; k < AHEAD; ++k)
-          if (j0 + tid + k * NT < len) mark(j0 + tid + k * NT, ahead[k]);
+  if (listed) {
+    const bool report = p.status && s.number == 0;
+    if (p.n_bias) {
+      const uint2* ids = reinterpret_cast<const uint2*>(p.bias_ids + s.row * p.bs);
+      const float* b = p.bias + s.row * p.bs;
+      for (int e = tid; e < p.n_bias; e += NT) {
+        const uint2 id = ids[e];
+        biases[e] = b[e];
+        uint32_t at;
+        const bool here = s.place_of(id, at);
+        if (SHORT) places[e] = here ? (int)at : -1;
+        if (here) words.bias(at, e);
+        if (report && past(id, p.V)) bits |= DSV41_STATUS_BAD_BIAS;
       }
       rows::lds_barrier();
     }
+    for_history(r, ahead, [&](int j0, const uint2 (&ids)[AHEAD]) {
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int j = j0 + k * NT;
+        if (j >= r.len) continue;
+        uint32_t at;
+        if (s.place_of(ids[k], at)) {
+          if (j < r.prompt) words.list(at);
+          else words.say(at);
+        }
+        if (report && past(ids[k], p.V)) bits |= DSV41_STATUS_BAD_HISTORY;
+      }
+    });
+    rows::lds_barrier();
   }
 
-  const float value = bad ? __builtin_nanf("") : MODE == GRAD ? 0.f : p.fill;
+  const float value = r.bad ? __builtin_nanf("") : p.fill;
   const uint32_t instead = sizeof(T) == 4 ? __float_as_uint(value) : pack_bf16(value, value);
   uint32_t marked[U];  // elements whose word is not 0
-  Group xs[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    marked[u] = 0;
     const int at = (u * NT + tid) * G;
-    if (LISTS && listed) {
-#pragma unroll
-      for (int q = 0; q < G; q += 4) {
-        const uint4 w = *reinterpret_cast<const uint4*>(words + word_at<T>(at + q));
-        marked[u] |= (min(w.x, 1u) | min(w.y, 1u) << 1 | min(w.z, 1u) << 2 | min(w.w, 1u) << 3) << q;
-      }
-      marked[u] &= allowed[u];
-    }
-    // in place, groups that stay as they are are neither read nor written; of a gradient, the logits are
-    // read where a sign is asked for
-    if (MODE == INPLACE && allowed[u] && (marked[u] || allowed[u] != there[u])) load_group(x + begin + at, there[u], v[u]);
-    if (MODE == GRAD && marked[u]) load_group(x + begin + at, there[u], xs[u]);
+    marked[u] = listed ? words.marked(at) & allowed[u] : 0u;
+    // in place, groups that stay as they are are neither read nor written
+    if (INPLACE && allowed[u] && (marked[u] || allowed[u] != there[u])) load_group(x + at, there[u], v[u]);
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int at = (u * NT + tid) * G;
-    if (MODE == INPLACE && !marked[u] && allowed[u] == there[u]) continue;
+    if (INPLACE && !marked[u] && allowed[u] == there[u]) continue;
     if (LISTS) {
       // (few: a wave takes as many turns as its lane with the most of them)
 #pragma unroll 1
       for (uint32_t m = marked[u]; m; m &= m - 1) {
         const int j = __builtin_ctz(m);
-        const uint32_t word = words[word_at<T>(at + j)];
-        const float y = MODE == GRAD ? knobs.slope(get(v[u], j, T{}), get(xs[u], j, T{}), word, biases)
-                                     : knobs.apply(get(v[u], j, T{}), word, biases);
-        set(v[u], j, y, T{});
+        set(v[u], j, r.knobs.apply(get(v[u], j, T{}), words.read(at + j, places, p.n_bias), biases), T{});
       }
     }
     if (allowed[u] != there[u]) drop(v[u], allowed[u], instead, T{});
-    if (there[u]) store_group(out + begin + at, there[u], v[u]);
+    if (there[u]) store_group(out + at, there[u], v[u]);
   }
 
   // the first slice reports for its row
-  if (MODE != GRAD && p.status && slice == 0) {
+  if (p.status && s.number == 0) {
     bool some = true;
-    if (MASK && mask) {
+    if (MASK && r.mask) {
       some = false;
       const int full = p.V / 32;
-      for (int k = tid; k < full; k += NT) some = some || mask[k] != 0;
-      if (tid == 0 && p.V % 32) some = some || (mask[full] & ((1u << (p.V % 32)) - 1)) != 0;
+      for (int k = tid; k < full; k += NT) some = some || r.mask[k] != 0;
+      if (tid == 0 && p.V % 32) some = some || (r.mask[full] & ((1u << (p.V % 32)) - 1)) != 0;
     }
     if (!__syncthreads_or(some)) bits |= DSV41_STATUS_NO_TOKEN;
     if (__syncthreads_or(bits & DSV41_STATUS_BAD_HISTORY)) bits |= DSV41_STATUS_BAD_HISTORY;
     if (__syncthreads_or(bits & DSV41_STATUS_BAD_BIAS)) bits |= DSV41_STATUS_BAD_BIAS;
-    if (tid == 0) p.status[row] = bits;
+    if (tid == 0) p.status[s.row] = bits;
   }
 }
 
-template <typename T, bool LISTS, bool MASK, int MODE>
-void launch(const Params& p, hipStream_t s) {
-  const int64_t items = (int64_t)p.rows * p.slices;
-  const size_t lds = LISTS ? SLICE * sizeof(uint32_t) + p.n_bias * sizeof(float) : 0;
-  hipLaunchKernelGGL((process_kernel<T, LISTS, MASK, MODE>), dim3((unsigned)((items + 7) / 8 * 8)), dim3(NT), lds, s, p);
+template <typename T, bool LISTS, bool MASK>
+__global__ __launch_bounds__(NT, 8) void process_grad_kernel(Params p) {
+  constexpr int IDS = sizeof(T) == 4 ? SLICE : SHORT_SLICE, G = Elem<T>::VEC, U = IDS / (NT * G);
+  __shared__ uint32_t in_history[IDS / 32], positive[IDS / 32];  // of an id that is in the history: whether x + b > 0
+  extern __shared__ int places[];                                // the bias entries' places in the slice
+  const int tid = threadIdx.x;
+  Slice s;
+  if (!slice_of<T, IDS>(p, s)) return;
+  const Row r = row_of<LISTS, MASK, true>(p, s.row);
+  const T* x = static_cast<const T*>(p.x) + s.row * p.xs + s.begin;
+  const T* g = static_cast<const T*>(p.grad) + s.row * p.gs + s.begin;
+  T* out = static_cast<T*>(p.out) + s.row * p.os + s.begin;
+  const bool listed = LISTS && r.len > 0, inside = s.begin >= 0 && s.begin + IDS <= p.V;
+
+  uint2 ahead[AHEAD];
+  if (LISTS) load_ahead(r, tid, ahead);
+  uint32_t there[U], allowed[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) group_at<T, MASK>(p, r, s.begin + (u * NT + tid) * G, inside, there[u], allowed[u]);
+  if (listed) {
+    static_assert(IDS / 32 <= NT);
+    if (tid < IDS / 32) in_history[tid] = positive[tid] = 0;
+    rows::lds_barrier();
+  }
+  Group v[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (allowed[u]) load_group(g + (u * NT + tid) * G, there[u], v[u]);
+
+  if (listed) {
+    for_history(r, ahead, [&](int j0, const uint2 (&ids)[AHEAD]) {
+      float logit[AHEAD];
+      uint32_t at[AHEAD];
+      bool here[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        here[k] = j0 + k * NT < r.len && s.place_of(ids[k], at[k]);
+        if (here[k]) logit[k] = Elem<T>::one(x + at[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        if (!here[k]) continue;
+        atomicOr(&in_history[at[k] >> 5], 1u << (at[k] & 31));
+        if (logit[k] > 0.f) atomicOr(&positive[at[k] >> 5], 1u << (at[k] & 31));
+      }
+    });
+    if (p.n_bias) {
+      const uint2* ids = reinterpret_cast<const uint2*>(p.bias_ids + s.row * p.bs);
+      const float* b = p.bias + s.row * p.bs;
+      for (int e = tid; e < p.n_bias; e += NT) {
+        uint32_t at;
+        places[e] = s.place_of(ids[e], at) ? (int)at : -1;
+      }
+      rows::lds_barrier();
+      // the last entry of an id in the history says its sign anew
+      for (int e = tid; e < p.n_bias; e += NT) {
+        const int at = places[e];
+        if (at < 0 || !(in_history[at >> 5] >> (at & 31) & 1)) continue;
+        int later = e + 1;
+        while (later < p.n_bias && places[later] != at) ++later;
+        if (later < p.n_bias) continue;
+        const float sum = Elem<T>::one(x + at) + b[e];
+        if (sum > 0.f) atomicOr(&positive[at >> 5], 1u << (at & 31));
+        else atomicAnd(&positive[at >> 5], ~(1u << (at & 31)));
+      }
+    }
+    rows::lds_barrier();
+  }
+
+  const float value = r.bad ? __builtin_nanf("") : 0.f, rp = r.knobs.rp;
+  const uint32_t instead = sizeof(T) == 4 ? __float_as_uint(value) : pack_bf16(value, value);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int at = (u * NT + tid) * G;
+    if (listed) {
+      const uint32_t sign = positive[at >> 5] >> (at & 31);
+#pragma unroll 1
+      for (uint32_t m = in_history[at >> 5] >> (at & 31) & allowed[u]; m; m &= m - 1) {
+        const int j = __builtin_ctz(m);
+        const float y = get(v[u], j, T{});
+        set(v[u], j, sign >> j & 1 ? y / rp : y * rp, T{});
+      }
+    }
+    if (allowed[u] != there[u]) drop(v[u], allowed[u], instead, T{});
+    if (there[u]) store_group(out + at, there[u], v[u]);
+  }
 }
-template <typename T, int MODE>
+
+// ---------------------------------------------------------------------------------------- host
+// (the last slice of a row that begins at a memory line may have nothing)
+int slices_of(int V, int ids) { return (V + rows::MOST_SKEW - 1 + ids - 1) / ids; }
+dim3 grid_of(Params& p, int ids) {
+  p.slices = slices_of(p.V, ids);
+  return dim3((unsigned)(((int64_t)p.rows * p.slices + 7) / 8 * 8));
+}
+
+template <typename T, bool LISTS, bool MASK, bool INPLACE, bool SHORT>
+void launch(Params p, hipStream_t s) {
+  const dim3 grid = grid_of(p, Words<T, SHORT>::IDS);
+  const size_t lds = LISTS ? SLICE * sizeof(uint32_t) + (size_t)p.n_bias * (SHORT ? 8 : 4) : 0;
+  hipLaunchKernelGGL((process_kernel<T, LISTS, MASK, INPLACE, SHORT>), grid, dim3(NT), lds, s, p);
+}
+// Words of 16 bits take what they hold of bf16 rows' lists, in batches that fill the GPU with the longer slices too.  With
+// histories of 2048 and 4096 and in place with 2048, us, 32 and 16 bits: 2048 rows 289 and 266, 337 and 293, 280 and 230; 500
+// rows 76 and 72, 89 and 80, 60 and 51; 200 rows 28.7 and 28.3, 33.8 and 32.1, 27.4 and 24.5.
+template <typename T, bool MASK, bool INPLACE>
+void launch_lists(const Params& p, hipStream_t s) {
+  if constexpr (sizeof(T) == 2)
+    if (p.hist_len <= SHORT_HISTORY && p.n_bias <= SHORT_BIAS && (int64_t)p.rows * slices_of(p.V, SHORT_SLICE) >= 1024)
+      return launch<T, true, MASK, INPLACE, true>(p, s);
+  launch<T, true, MASK, INPLACE, false>(p, s);
+}
+template <typename T, bool INPLACE>
 void launch(const Params& p, hipStream_t s) {
   const bool lists = p.n_bias || p.history;
-  if (lists && p.mask) launch<T, true, true, MODE>(p, s);
-  else if (lists) launch<T, true, false, MODE>(p, s);
-  else if (p.mask) launch<T, false, true, MODE>(p, s);
-  else launch<T, false, false, MODE>(p, s);
+  if (lists && p.mask) launch_lists<T, true, INPLACE>(p, s);
+  else if (lists) launch_lists<T, false, INPLACE>(p, s);
+  else if (p.mask) launch<T, false, true, INPLACE, false>(p, s);
+  else launch<T, false, false, INPLACE, false>(p, s);
+}
+template <typename T>
+void launch_grad(Params p, hipStream_t s) {
+  const dim3 grid = grid_of(p, sizeof(T) == 4 ? SLICE : SHORT_SLICE);
+  const size_t lds = (size_t)p.n_bias * sizeof(int);
+  if (p.history && p.mask) hipLaunchKernelGGL((process_grad_kernel<T, true, true>), grid, dim3(NT), lds, s, p);
+  else if (p.history) hipLaunchKernelGGL((process_grad_kernel<T, true, false>), grid, dim3(NT), lds, s, p);
+  else if (p.mask) hipLaunchKernelGGL((process_grad_kernel<T, false, true>), grid, dim3(NT), lds, s, p);
+  else hipLaunchKernelGGL((process_grad_kernel<T, false, false>), grid, dim3(NT), lds, s, p);
 }
 
 constexpr int64_t MAX_GRID = (1 << 22) - 8;  // workgroups of 512 threads: HIP's grids stop short of 2^32 threads
-
-// (the last slice of a row that begins at a memory line may have nothing)
-int slices_of(int V) { return (V + rows::MOST_SKEW - 1 + SLICE - 1) / SLICE; }
 
 int check_desc(const dsv41_process_desc* d, bool grad) {
   if (!d) return fail(DSV41_E_INVALID, "process descriptor is NULL");
@@ -395,7 +583,7 @@ int check_desc(const dsv41_process_desc* d, bool grad) {
     return fail(DSV41_E_INVALID, "presence_penalty and frequency_penalty must be finite");
   if (d->hist_len < 0 || (d->hist_len > 0 && !d->history)) return fail(DSV41_E_INVALID, "hist_len needs a history");
   if (d->hist_len > 0 && d->history_row_stride < 0) return fail(DSV41_E_INVALID, "history row stride is negative");
-  if (d->hist_len > (int)COUNT) return fail(DSV41_E_UNSUPPORTED, "histories above 524287 tokens are not supported");
+  if (d->hist_len > MAX_HISTORY) return fail(DSV41_E_UNSUPPORTED, "histories above 524287 tokens are not supported");
   if (d->bias_len < 0 || (d->bias_len > 0 && (!d->bias_ids || !d->bias)))
     return fail(DSV41_E_INVALID, "bias_len needs bias_ids and bias");
   if (d->bias_len > 0 && d->bias_row_stride < 0) return fail(DSV41_E_INVALID, "bias row stride is negative");
@@ -406,7 +594,7 @@ int check_desc(const dsv41_process_desc* d, bool grad) {
     if (d->mask_row_stride < 0) return fail(DSV41_E_INVALID, "mask row stride is negative");
   }
   if (isnan(d->fill)) return fail(DSV41_E_INVALID, "fill must be a number");
-  if ((int64_t)d->rows * slices_of(d->vocab) > MAX_GRID)
+  if ((int64_t)d->rows * slices_of(d->vocab, SLICE) > MAX_GRID)
     return fail(DSV41_E_UNSUPPORTED, "more than 2^22 row slices are not supported");
   return DSV41_OK;
 }
@@ -422,7 +610,6 @@ int run(const dsv41_process_desc* d, bool grad, void* stream) {
   p.gs = d->grad_row_stride;
   p.rows = d->rows;
   p.V = d->vocab;
-  p.slices = slices_of(d->vocab);
   const bool neutral = !d->repetition_penalties && !d->presence_penalties && !d->frequency_penalties &&
                        d->repetition_penalty == 1.f && d->presence_penalty == 0.f && d->frequency_penalty == 0.f;
   if (d->hist_len > 0 && !neutral) {
@@ -455,9 +642,9 @@ int run(const dsv41_process_desc* d, bool grad, void* stream) {
   p.status = d->out_status;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool f32 = d->logits_dtype == DSV41_DTYPE_F32;
-  if (grad) f32 ? launch<float, GRAD>(p, s) : launch<bf16_t, GRAD>(p, s);
-  else if (d->out == d->logits) f32 ? launch<float, INPLACE>(p, s) : launch<bf16_t, INPLACE>(p, s);
-  else f32 ? launch<float, COPY>(p, s) : launch<bf16_t, COPY>(p, s);
+  if (grad) f32 ? launch_grad<float>(p, s) : launch_grad<bf16_t>(p, s);
+  else if (d->out == d->logits) f32 ? launch<float, true>(p, s) : launch<bf16_t, true>(p, s);
+  else f32 ? launch<float, false>(p, s) : launch<bf16_t, false>(p, s);
   DSV41_HIP_CHECK(hipGetLastError());
   return DSV41_OK;
 }
