@@ -16,6 +16,10 @@
 //                 finished there; one that reaches over its ends leaves a partial row.  Other workgroups
 //                 of the same launch write zeros where no token is, which is most of a dense gradient's time.
 //   join_kernel   the partial rows of an id that reaches over chunks, in their order.
+// Bound by memory: a gradient of 151851 x 2048 in fp32 from 1000 tokens takes 7 + 177 + 4 us, 7.0 TB/s of zeros
+// (by torch's fill 6.9); 129280 x 7168 in bf16 from 16384 tokens 14 + 339 + 14, 6.1 TB/s of zeros, gradients and partial
+// rows.  Rows of the table, 16384 x 7168 in bf16, take 64 us: 7.2 TB/s of result and rows, of which frequent tokens' come
+// from caches.
 
 #include <math.h>
 

@@ -2,19 +2,23 @@
 // rows on the integer matrix cores.
 //
 // A row x of bf16 becomes q_k = rint(127 x_k / a) with a = max |x| and the scale a / 127 (fp32); the
-// head's rows w are kept that way.  127 x_k and a have 15 and 8 bits, so their quotient is a half or at
-// least 2^-9 of its size away from one: the fp32 division decides as the exact one.  With s, t the scales,
+// head's rows w are kept that way.  x_k and a have 8 bits, so 127 x_k / a is a half or at least 2^-16 of its
+// size away from one (254 X - (2 k + 1) A 2^s is an integer): the fp32 division decides as the exact one.  With s, t the scales,
 //   out[n, v] = (sum_k q[n, k] w[v, k]) s[n] t[v],
-// the sum exact in 32-bit integers (up to 2^31 / 127^2 = 133152 columns), then two fp32 products.
+// the sum exact in 32-bit integers (up to 2^31 / 127^2 = 133144 columns), then two fp32 products.
 //
 // The columns are padded to a multiple of 128 (one cache line of a row), those of q with zeros.
 //
-// head_kernel, up to 64 tokens, is bound by reading w once.  A workgroup takes 64 rows of w, its eight waves
-// every eighth line of their columns; fragments go from memory to registers with no LDS between, and
-// the waves' integer sums meet in LDS (atomics whose order does not matter to integers).
-// gemm_kernel, above, has the schedule of the bf16 products (mfma_tile.h): 256 x 256 tiles, eight waves
-// whose pairs multiply and read in turns, stages of 128 bytes a row loaded straight to LDS.  An integer
-// fragment (16 rows x 64) lies in a row's bytes exactly as a bf16 one (16 x 32).
+// head_kernel, up to 64 tokens, is bound by reading w once: one token, 7168 -> 129280, 130 us (7.1 TB/s, what a
+// nontemporal read reaches); 48 tokens of 2048 -> 151936 55 us.  A workgroup takes 64 rows of w, its four
+// waves every fourth k-step of their columns; fragments go from memory to registers with no LDS between, so the rows lie
+// in memory as tiles of a fragment's lanes.  (Row-major, each load of a wave met 16 lines, and the loads' rate was the
+// bound: 203 us, and 316 with 48 tokens of 7168 -> 129280 where tiles take 182.)  The waves' integer sums meet in LDS.
+// What more tokens cost is their own tiles, read from L2 by every workgroup.
+// gemm_kernel, above, has the schedule of the bf16 products (mfma_tile.h): eight waves whose pairs multiply and read in
+// turns, stages of 128 columns loaded straight to LDS, tiles of 256 rows x 256 or 192 tokens.  4096 tokens of 7168 ->
+// 129280: 2.69 ms, 2.8 POP/s, the matrix cores busy 71% of the cycles at 1.75 GHz (power); of 2048 -> 151936 1.11 ms,
+// 2.3 POP/s: a tile there has 16 stages, and a fifth of its time is the conversion and stores of its logits.
 
 #include <algorithm>
 #include <iterator>
@@ -30,9 +34,10 @@ using TL = Tile<SQUARE>;
 using rows::bf16_t;
 constexpr int BM = TL::BV;
 constexpr int LINE = ROWB;            // columns are padded to whole lines
-constexpr int MAX_COLUMNS = 133120;   // 2^31 / 127^2 = 133152, in whole lines
+constexpr int MAX_COLUMNS = 133120;   // 2^31 / 127^2 = 133144, in whole lines
 constexpr int QUANT_NT = 256;
-constexpr int FEW = 64;               // tokens of head_kernel
+// Tokens of head_kernel.  64 and 65, the first of gemm_kernel: 2048 -> 151936 68 and 81 us, 7168 -> 129280 187 and 189.
+constexpr int FEW = 64;
 
 typedef int intx4 __attribute__((ext_vector_type(4)));
 
@@ -85,13 +90,17 @@ __device__ __forceinline__ uint2 quantize(const uint32_t (&w)[4], float lift, fl
 }
 
 template <bool HEAD>
-__global__ __launch_bounds__(QUANT_NT) void quantize_kernel(const bf16_t* x, int64_t xs, int cols, int8_t* q, int padded,
-                                                            float* scales, int32_t* status) {
+__global__ __launch_bounds__(QUANT_NT) void quantize_kernel(const bf16_t* x, int64_t xs, int rows, int cols, int8_t* q,
+                                                            int padded, float* scales, int32_t* status) {
   constexpr int STEP = QUANT_NT * 8;
   __shared__ uint32_t tops[QUANT_NT / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  x += (int64_t)blockIdx.x * xs;
-  const int64_t place = HEAD ? head_row(blockIdx.x) : blockIdx.x;
+  // the rows of a tile on one XCD, whose L2 puts their lines together (workgroups go round-robin over the eight): a head of
+  // 7168 x 129280 in 897 us, 1111 with rows in turn
+  const int64_t row = (int64_t)(blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  if (row >= rows) return;
+  x += row * xs;
+  const int64_t place = HEAD ? head_row(row) : row;
   uint32_t kept[KEPT][4], top = 0;
 #pragma unroll
   for (int c = 0; c < KEPT; ++c) load_chunk(x, cols, c * STEP + tid * 8, kept[c]);
@@ -110,8 +119,8 @@ __global__ __launch_bounds__(QUANT_NT) void quantize_kernel(const bf16_t* x, int
   const bool odd = top >= 0x7F800000u;
   float most = __uint_as_float(top);
   if (tid == 0) {
-    scales[blockIdx.x] = odd ? __builtin_nanf("") : most / 127.f;
-    if (status) status[blockIdx.x] = odd ? DSV41_STATUS_NONFINITE : 0;
+    scales[row] = odd ? __builtin_nanf("") : most / 127.f;
+    if (status) status[row] = odd ? DSV41_STATUS_NONFINITE : 0;
   }
   const bool none = odd || top == 0;
   const float lift = most > 1e30f ? 0x1p-64f : 1.f;  // (127 x is finite; what it takes from small x is far below a half)
@@ -464,6 +473,9 @@ constexpr int64_t MAX_GRID = 1 << 22;
 
 int padded_of(int cols) { return (cols + LINE - 1) / LINE * LINE; }
 
+// Workgroups of a quantization: eight XCDs' runs of whole groups of rows.
+dim3 quantize_grid(int rows) { return dim3((unsigned)(((int64_t)rows + 8 * GROUP - 1) / (8 * GROUP) * (8 * GROUP))); }
+
 int check_cols(int cols) {
   if (cols <= 0) return fail(DSV41_E_INVALID, "rows need columns");
   if (cols > MAX_COLUMNS) return fail(DSV41_E_UNSUPPORTED, "more than 133120 columns overflow a 32-bit sum");
@@ -545,8 +557,8 @@ extern "C" int dsv41_quantize_rows_run(const void* x, int64_t xs, int rows, int 
     return fail(DSV41_E_INVALID, "quantize: operands are not aligned");
   if (rows > MAX_GRID) return fail(DSV41_E_UNSUPPORTED, "quantize: too many rows for one call");
   if (rows == 0) return DSV41_OK;
-  hipLaunchKernelGGL(quantize_kernel<true>, dim3(rows), dim3(QUANT_NT), 0, static_cast<hipStream_t>(stream),
-                     static_cast<const bf16_t*>(x), xs, cols, q, padded_of(cols), scales, status);
+  hipLaunchKernelGGL(quantize_kernel<true>, quantize_grid(rows), dim3(QUANT_NT), 0, static_cast<hipStream_t>(stream),
+                     static_cast<const bf16_t*>(x), xs, rows, cols, q, padded_of(cols), scales, status);
   DSV41_HIP_CHECK(hipGetLastError());
   return DSV41_OK;
 }
@@ -565,8 +577,8 @@ extern "C" int dsv41_int_head_run(const dsv41_int_head_desc* d, void* workspace,
   float* ss = reinterpret_cast<float*>(q + at);
   const int K = padded_of(d->hidden);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(quantize_kernel<false>, dim3(d->n_tokens), dim3(QUANT_NT), 0, s, static_cast<const bf16_t*>(d->x),
-                     d->x_row_stride, d->hidden, q, K, ss, d->out_status);
+  hipLaunchKernelGGL(quantize_kernel<false>, quantize_grid(d->n_tokens), dim3(QUANT_NT), 0, s,
+                     static_cast<const bf16_t*>(d->x), d->x_row_stride, d->n_tokens, d->hidden, q, K, ss, d->out_status);
   Params p{};
   p.w = d->w;
   p.ts = d->scales;
