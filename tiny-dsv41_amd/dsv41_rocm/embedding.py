@@ -67,7 +67,7 @@ def prepare(ids, weight, scale):
 def forward(ids, weight, scale, want_status):
     """One dsv41_embed_run; returns (rows, statuses or None)."""
     n, (v, h) = ids.numel(), weight.shape
-    out = torch.empty(n, h, dtype=weight.dtype, device=weight.device)
+    out = weight.new_empty(n, h)
     status = torch.empty(n, dtype=torch.int32, device=weight.device) if want_status else None
     if n:
         d = _lib.EmbedDesc(ctypes.sizeof(_lib.EmbedDesc), n, h, v, weight.data_ptr(), _step(weight), ids.data_ptr(), scale,

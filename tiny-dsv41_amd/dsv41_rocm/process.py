@@ -23,9 +23,17 @@ from .scores import INTEGERS, launch, overlap, refuse_capture, refuse_tangents, 
 Knob = Union[float, torch.Tensor]
 
 
+def _ready(t, dtype, rows, device):
+    """Whether ``t`` is a vector of one value per row as the kernels take it."""
+    return t.dtype is dtype and t.shape == (rows,) and t.device == device and t.is_contiguous()
+
+
 def _knob(value, name, neutral, rows, device):
     """(the scalar of all rows, a tensor of one value per row or None)"""
     if isinstance(value, torch.Tensor):
+        if _ready(value, torch.float32, rows, device) and not value.requires_grad:
+            refuse_tangents(name, value)
+            return neutral, value
         if value.shape != (rows,):
             raise ValueError(f"{name} must be a number or have one value per row")
         if value.requires_grad and torch.is_grad_enabled():
@@ -50,6 +58,8 @@ def _integers(t, name, dtype, device):
 
 
 def _lengths(t, name, rows, device):
+    if isinstance(t, torch.Tensor) and _ready(t, torch.int32, rows, device):
+        return t
     t = _integers(torch.as_tensor(t), name, torch.int32, device)
     if t.shape != (rows,):
         raise ValueError(f"{name} must have one length per row")
@@ -105,9 +115,10 @@ def _arguments(logits, history, history_lens, history_prompt_lens, repetition_pe
         token_mask = _rows_of(token_mask)
         masks = token_mask.shape[0]
         if mask_rows is not None:
-            mask_rows = _integers(mask_rows, "mask_rows", torch.int32, dev).contiguous()
-            if mask_rows.shape != (rows,):
-                raise ValueError("mask_rows must have one mask per row")
+            if not (isinstance(mask_rows, torch.Tensor) and _ready(mask_rows, torch.int32, rows, dev)):
+                mask_rows = _integers(mask_rows, "mask_rows", torch.int32, dev).contiguous()
+                if mask_rows.shape != (rows,):
+                    raise ValueError("mask_rows must have one mask per row")
         elif masks != 1 and masks != rows:
             raise ValueError("without mask_rows there is one token_mask, or one per row")
         if masks == 0 and rows:
@@ -151,7 +162,7 @@ def process_backward(logits, numbers, tensors, grad):
     """dL/dlogits of :func:`process_logits` from dL/dresult, in the logits' dtype."""
     refuse_tangents("gradients", grad)
     rows, vocab = logits.shape
-    out = torch.empty(rows, vocab, dtype=logits.dtype, device=logits.device)
+    out = logits.new_empty(rows, vocab)
     if rows:
         grad = grad.to(logits.dtype)
         step, unit = grad.stride()
@@ -167,7 +178,7 @@ def process_backward(logits, numbers, tensors, grad):
 class _Process(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, numbers, want_status, *tensors):
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        out = logits.new_empty(logits.shape)
         status = forward(logits, numbers, tensors, out, want_status)
         ctx.numbers = numbers
         ctx.save_for_backward(logits, *tensors)
@@ -271,7 +282,7 @@ def process_logits(
     elif tracked:
         out, status = _Process.apply(logits, numbers, check, *tensors)
     else:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        out = logits.new_empty(logits.shape)  # (half of torch.empty's 2.2 us)
         status = forward(logits, numbers, tensors, out, check)
     if check and any_set(status)[0]:
         _status_error(status)
