@@ -65,6 +65,23 @@ def test_exact(n, h, v, dtype):
     assert torch.equal(head_logits(big[:, 1:h + 1], head, dtype=dtype).cpu(), want)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [33, 48, 49, 64])
+@pytest.mark.parametrize("h,v", [(4100, 32827), (4100, 65536), (4000, 32827), (4100, 32768)])
+def test_many_groups(n, h, v, dtype):
+    # groups of 64 rows by twos (an odd number of them, with a part of one at the end; an even one), and one by one
+    x = _inputs(n, h, 1)[0]
+    w = torch.randint(-127, 128, (v, h), generator=torch.Generator(DEV).manual_seed(n + h + v), dtype=torch.int8, device=DEV)
+    t = torch.rand(v, generator=torch.Generator(DEV).manual_seed(n), device=DEV)
+    q, s = _quantized(x)
+    sums = torch.cat([q.to(DEV) @ part.double().t() for part in w.split(8192)], 1)  # integers below 2^53
+    want = ((sums.float() * s.to(DEV)[:, None]) * t).to(dtype)
+    wide = torch.full((n, v + 16), 7.0, dtype=dtype, device=DEV)
+    head_logits(x.to(DEV), Int8Head.from_quantized(w, t), out=wide[:, 8:8 + v])
+    assert torch.equal(wide[:, 8:8 + v], want)
+    assert bool((wide[:, :8] == 7).all()) and bool((wide[:, 8 + v:] == 7).all())
+
+
 def test_ties_and_borders():
     # against a maximum of 254, odd numbers are ties, and go to the even integer
     x = torch.arange(-254.0, 255.0).bfloat16()[None]

@@ -140,7 +140,6 @@ __device__ __forceinline__ void clear_row(T* p, int64_t n) {
   if (tid < head) rows::store_one(p + tid, 0.f);
   uint4* q = reinterpret_cast<uint4*>(p + head);
   const int64_t groups = (n - head) / G;
-  
   for (int64_t i = tid; i < groups; i += SUM_NT) q[i] = make_uint4(0, 0, 0, 0);
   const int64_t tail = head + groups * G + tid;
   if (tid < G && tail < n) rows::store_one(p + tail, 0.f);
@@ -389,7 +388,6 @@ Plan plan(const dsv41_embed_grad_desc* d) {
   q.chunks = ((int64_t)d->n_tokens + CHUNK - 1) / CHUNK;
   q.strips = ((int64_t)d->hidden + 64 * g - 1) / (64 * g);
   q.join_strips = ((int64_t)d->hidden + JOIN_NT * 4 - 1) / (JOIN_NT * 4);
-
   q.zero_rows = 1;
   while (q.zero_rows < 16 && q.zero_rows * 2 * d->hidden * (d->out_dtype == DSV41_DTYPE_F32 ? 4 : 2) <= ZERO_BYTES) q.zero_rows *= 2;
   q.zero_grid = d->accumulate ? 0 : ((d->vocab + q.zero_rows - 1) / q.zero_rows + 7) / 8 * 8;

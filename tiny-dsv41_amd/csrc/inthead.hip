@@ -138,6 +138,8 @@ __global__ __launch_bounds__(QUANT_NT) void quantize_kernel(const bf16_t* x, int
 }
 
 // -------------------------------------------------------------------------------- few tokens
+constexpr int SPLIT = 4, PER_CU = 2;  // waves of a workgroup, workgroups of a CU
+
 struct Params {
   const int8_t* w;  // tiles of the head
   const float* ts;  // scales of its rows
@@ -214,90 +216,102 @@ __device__ __forceinline__ void store_logits(T* row, int v, int V, bool there, b
   }
 }
 
-// The fragments of one k-step: of a group of 64 rows and of NB blocks of 16 tokens.
-template <int NB>
+// The fragments of one k-step: of GB groups of 64 rows and of NB blocks of 16 tokens.
+template <int NB, int GB>
 struct Step {
-  intx4 a[4], b[NB];
+  intx4 a[4 * GB], b[NB];
 };
 
-// SPLIT waves share the columns of a group, every SPLIT-th k-step each; a workgroup takes group after group, with
+// SPLIT waves share the columns of GB groups, every SPLIT-th k-step each; a workgroup takes item after item of GB groups, with
 // DEPTH - 1 steps of each wave on their way from memory throughout.
-template <typename T, int NB, int SPLIT, int DEPTH, int PER_CU>
+template <typename T, int NB, int GB, int DEPTH>
 __global__ __launch_bounds__(64 * SPLIT, SPLIT * PER_CU / 4) void head_kernel(Params p, bool wide) {
   __shared__ intx4 parts[SPLIT][4 * NB][64];
-  __shared__ float scales[SPLIT][GROUP];  // each wave's copy of the group's
+  __shared__ float scales[SPLIT][GB * GROUP];  // each wave's copy of the groups'
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, quad = lane >> 4;
   const int steps = p.K / 64, turns = (steps + SPLIT * DEPTH - 1) / (SPLIT * DEPTH) * DEPTH, groups = (p.V + GROUP - 1) / GROUP;
+  const int items = (groups + GB - 1) / GB;
   T* out = static_cast<T*>(p.out);
-  intx4 acc[4][NB];
+  intx4 acc[4 * GB][NB];
   auto clear = [&]() {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4 * GB; ++i)
 #pragma unroll
       for (int j = 0; j < NB; ++j) acc[i][j] = intx4{0, 0, 0, 0};
   };
   clear();
-  Step<NB> f[DEPTH];
-  int at = wave, left = turns, ahead = blockIdx.x;  // the step to load, those left of its group, the group
-  const int8_t* w = p.w + (int64_t)ahead * GROUP * p.K;  // (the same in all lanes, which add theirs in 32 bits)
-  // (a step that is none reads the first bytes of q, which all caches hold: loads under a condition cost registers)
-  auto load = [&](Step<NB>& s) {
-    const bool some = ahead < groups && at < steps;
-    const int8_t *wa = some ? w + at * TILE : p.q, *qa = p.q + (some ? at * TILE : 0);
-    const int64_t wide_step = some ? (int64_t)16 * p.K : 0;
+  Step<NB, GB> f[DEPTH];
+  int at = wave, left = turns, ahead = blockIdx.x;  // the step to load, those left of its item, the item
+  // (addresses are the same in all lanes, which add theirs in 32 bits; a step that is none reads the first bytes of q, which
+  // all caches hold, as loads under a condition cost registers; a group past the last is the last one again)
+  auto load = [&](Step<NB, GB>& s) {
+    const bool some = ahead < items && at < steps;
+    const int8_t* qa = p.q + (some ? at * TILE : 0);
+    const int64_t tile_row = some ? (int64_t)16 * p.K : 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s.a[i] = __builtin_nontemporal_load(reinterpret_cast<const intx4*>(wa + i * wide_step) + lane);
+    for (int g = 0; g < GB; ++g) {
+      const int8_t* wa = some ? p.w + (int64_t)min(ahead * GB + g, groups - 1) * GROUP * p.K + at * TILE : p.q;
 #pragma unroll
-    for (int j = 0; j < NB; ++j) s.b[j] = reinterpret_cast<const intx4*>(qa + j * wide_step)[lane];
-    at += SPLIT;
-    if (--left == 0) {
-      at = wave, left = turns, ahead += gridDim.x;
-      w += (int64_t)gridDim.x * GROUP * p.K;
+      for (int i = 0; i < 4; ++i)
+        s.a[4 * g + i] = __builtin_nontemporal_load(reinterpret_cast<const intx4*>(wa + i * tile_row) + lane);
     }
+#pragma unroll
+    for (int j = 0; j < NB; ++j) s.b[j] = reinterpret_cast<const intx4*>(qa + j * tile_row)[lane];
+    at += SPLIT;
+    if (--left == 0) at = wave, left = turns, ahead += gridDim.x;
   };
 #pragma unroll
   for (int d = 0; d < DEPTH - 1; ++d) load(f[d]);
   float ss[NB];
 #pragma unroll
   for (int j = 0; j < NB; ++j) ss[j] = p.ss[min(16 * j + r16, p.N - 1)];
-  for (int group = blockIdx.x; group < groups; group += gridDim.x) {
-    // (read at the end, it would have the wave wait for all steps on their way)
-    const float t = p.ts[min(group * GROUP + lane, p.V - 1)];
+  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    // (read at the end, they would have the wave wait for all steps on their way)
+    float t[GB];
+#pragma unroll
+    for (int g = 0; g < GB; ++g) t[g] = p.ts[min((item * GB + g) * GROUP + lane, p.V - 1)];
     for (int turn = 0; turn < turns; turn += DEPTH) {
 #pragma unroll
       for (int d = 0; d < DEPTH; ++d) {
         load(f[(d + DEPTH - 1) % DEPTH]);
         if (wave + (turn + d) * SPLIT < steps) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < 4 * GB; ++i)
 #pragma unroll
             for (int j = 0; j < NB; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[d].a[i], f[d].b[j], acc[i][j], 0, 0, 0);
         }
       }
     }
-    // the waves' sums meet: token block j is wave j % SPLIT's to finish
+    // the waves' sums meet, a group at a time: token block j is wave j % SPLIT's to finish
 #pragma unroll
-    for (int j = 0; j < NB; ++j)
-      if (j % SPLIT != wave) {
+    for (int g = 0; g < GB; ++g) scales[wave][g * GROUP + lane] = t[g];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) parts[wave][4 * j + i][lane] = acc[i][j];
-      }
-    scales[wave][lane] = t;
-    rows::lds_barrier();
+    for (int g = 0; g < GB; ++g) {
 #pragma unroll
-    for (int j = 0; j < NB; ++j) {
-      if (j % SPLIT != wave) continue;
+      for (int j = 0; j < NB; ++j)
+        if (j % SPLIT != wave) {
 #pragma unroll
-      for (int s = 0; s < SPLIT; ++s)
-        if (s != wave) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[i][j] += parts[s][4 * j + i][lane];
+          for (int i = 0; i < 4; ++i) parts[wave][4 * j + i][lane] = acc[4 * g + i][j];
         }
-      const int n = 16 * j + r16;
-      store_logits(out + n * p.os, group * GROUP, p.V, n < p.N, wide, acc[0][j], acc[1][j], acc[2][j], acc[3][j], ss[j],
-                   scales[wave] + 16 * quad);
+      rows::lds_barrier();
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        if (j % SPLIT != wave) continue;
+        intx4 c[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[i] = acc[4 * g + i][j];
+#pragma unroll
+        for (int s = 0; s < SPLIT; ++s)
+          if (s != wave) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[i] += parts[s][4 * j + i][lane];
+          }
+        const int n = 16 * j + r16;
+        store_logits(out + n * p.os, (item * GB + g) * GROUP, p.V, n < p.N, wide, c[0], c[1], c[2], c[3], ss[j],
+                     scales[wave] + g * GROUP + 16 * quad);
+      }
+      rows::lds_barrier();
     }
-    rows::lds_barrier();
     clear();
   }
 }
@@ -511,19 +525,24 @@ constexpr double NARROW_COST = 0.85;
 // steps ahead, two workgroups a CU: 2048 -> 151936, 1, 17, 48 and 64 tokens 52, 57, 64 and 68 us, 7168 -> 129280 151,
 // 164, 182 and 199.  Eight waves: 54, 59, 68, 72 and 155, 174, 193, 208; two (four workgroups): 57, 63, 70, 75 and 153,
 // 162, 177, 193; five steps ahead 60, 69, 77, 89 and 152, 167, 186, 222.
-constexpr int SPLIT = 4, DEPTH = 4, PER_CU = 2;
-template <typename T, int NB>
+constexpr int rounds_of(int items) { return (items + PER_CU * CU_COUNT - 1) / (PER_CU * CU_COUNT); }
+template <typename T, int NB, int GB, int DEPTH>
 void launch_few(const Params& p, bool wide, hipStream_t s) {
-  const int groups = (p.V + GROUP - 1) / GROUP, slots = PER_CU * CU_COUNT, rounds = (groups + slots - 1) / slots;
-  hipLaunchKernelGGL((head_kernel<T, NB, SPLIT, DEPTH, PER_CU>), dim3((groups + rounds - 1) / rounds), dim3(64 * SPLIT), 0, s, p, wide);
+  const int items = ((p.V + GROUP - 1) / GROUP + GB - 1) / GB, rounds = rounds_of(items);
+  hipLaunchKernelGGL((head_kernel<T, NB, GB, DEPTH>), dim3((items + rounds - 1) / rounds), dim3(64 * SPLIT), 0, s, p, wide);
 }
 template <typename T>
 void launch(const Params& p, hipStream_t s) {
   const bool wide = p.os * sizeof(T) % 16 == 0 && (uintptr_t)p.out % 16 == 0;
-  if (p.N <= 16) launch_few<T, 1>(p, wide, s);
-  else if (p.N <= 32) launch_few<T, 2>(p, wide, s);
-  else if (p.N <= 48) launch_few<T, 3>(p, wide, s);
-  else if (p.N <= FEW) launch_few<T, 4>(p, wide, s);
+  const int groups = (p.V + GROUP - 1) / GROUP;
+  // Groups of 64 rows by twos read the tokens' tiles half as often, if no workgroup gets more of them by it: 7168 -> 129280,
+  // 48 tokens 181 -> 172 us, 64 tokens 205 -> 185 (bf16: 187 -> 171); 8192 -> 65536, 64 tokens 123 -> 110.  In short rows the
+  // meeting of the waves' sums, two groups' at once, costs more: 2048 -> 129280, 48 tokens 57 -> 61.
+  const bool pairs = p.K >= 4096 && 2 * rounds_of((groups + 1) / 2) <= rounds_of(groups);
+  if (p.N <= 16) launch_few<T, 1, 1, 4>(p, wide, s);
+  else if (p.N <= 32) launch_few<T, 2, 1, 4>(p, wide, s);
+  else if (p.N <= 48) pairs ? launch_few<T, 3, 2, 3>(p, wide, s) : launch_few<T, 3, 1, 4>(p, wide, s);
+  else if (p.N <= FEW) pairs ? launch_few<T, 4, 2, 2>(p, wide, s) : launch_few<T, 4, 1, 4>(p, wide, s);
   else {
     const dim3 grid((p.n_tb * p.ranges + 7) / 8 * 8);
     if (p.wide_tile) hipLaunchKernelGGL((gemm_kernel<T, 2>), grid, dim3(NT), 0, s, p, wide);
