@@ -220,6 +220,17 @@ def test_embed_grad_refusals(kw, code, msg):
     assert lib.dsv41_embed_grad_workspace_bytes(ctypes.byref(d)) == 0
 
 
+@pytest.mark.parametrize("hidden", [(1 << 24) + 1, 0x7FFFFFFF])
+def test_wide_tables_are_refused(hidden):
+    # 32-bit column counts would pass their range in the last step of a row
+    lib = _lib.load()
+    wide = dict(hidden=hidden, out_row_stride=hidden)
+    assert lib.dsv41_embed_run(ctypes.byref(_embed(weight_row_stride=hidden, **wide)), None) == _lib.E_UNSUPPORTED
+    grad = _embed_grad(n_tokens=1, grad_row_stride=hidden, **wide)
+    assert lib.dsv41_embed_grad_run(ctypes.byref(grad), 0x8000, 1 << 60, None) == _lib.E_UNSUPPORTED
+    assert "2^24" in _lib.last_error()
+
+
 def test_embed_grad_workspace():
     lib = _lib.load()
     d = _embed_grad()
@@ -228,6 +239,11 @@ def test_embed_grad_workspace():
     for ws, n in ((None, size), (0x8000, size - 1), (0x8004, size)):
         assert lib.dsv41_embed_grad_run(ctypes.byref(d), ws, n, None) == _lib.E_WORKSPACE
     assert lib.dsv41_embed_grad_run(None, None, 0, None) == _lib.E_INVALID
+
+
+def test_ids_that_are_no_tensor_are_refused():
+    with pytest.raises(ValueError, match="integers"):
+        token_embedding_backward(torch.zeros(2, 5), [1, 2], 5)
 
 
 def test_host_tensors_are_refused():

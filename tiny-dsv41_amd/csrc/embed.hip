@@ -43,6 +43,7 @@ constexpr int CHUNK = 32;     // sorted positions of a summing wave
 constexpr int ZERO_BYTES = 16384;
 constexpr int JOIN_NT = 128;
 constexpr int64_t MAX_GRID = 1 << 22;
+constexpr int MAX_HIDDEN = 1 << 24;  // columns are counted in 32 bits, steps beyond the last one included
 
 // 16 bytes of a row from p on, of which n elements exist (zeros beyond).
 template <typename T>
@@ -370,6 +371,7 @@ __global__ __launch_bounds__(JOIN_NT) void join_kernel(GradParams p) {
 int check_sizes(int dtype, int n, int h, int v) {
   if (n < 0 || h <= 0 || v <= 0) return fail(DSV41_E_INVALID, "the table must have shape [vocabulary_size, hidden]");
   if (dtype != DSV41_DTYPE_F32 && dtype != DSV41_DTYPE_BF16) return fail(DSV41_E_INVALID, "the table must be fp32 or bf16");
+  if (h > MAX_HIDDEN) return fail(DSV41_E_UNSUPPORTED, "hidden sizes above 2^24 are not supported");
   return DSV41_OK;
 }
 

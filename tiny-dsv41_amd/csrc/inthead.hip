@@ -536,7 +536,7 @@ void launch(const Params& p, hipStream_t s) {
   const bool wide = p.os * sizeof(T) % 16 == 0 && (uintptr_t)p.out % 16 == 0;
   const int groups = (p.V + GROUP - 1) / GROUP;
   // Groups of 64 rows by twos read the tokens' tiles half as often, if no workgroup gets more of them by it: 7168 -> 129280,
-  // 48 tokens 181 -> 172 us, 64 tokens 205 -> 185 (bf16: 187 -> 171); 8192 -> 65536, 64 tokens 123 -> 110.  In short rows the
+  // 48 tokens 198 -> 184 us, 64 tokens 210 -> 185 (bf16: 182 -> 173, 195 -> 177); 8192 -> 65536, 64 tokens 123 -> 110.  In short rows the
   // meeting of the waves' sums, two groups' at once, costs more: 2048 -> 129280, 48 tokens 57 -> 61.
   const bool pairs = p.K >= 4096 && 2 * rounds_of((groups + 1) / 2) <= rounds_of(groups);
   if (p.N <= 16) launch_few<T, 1, 1, 4>(p, wide, s);

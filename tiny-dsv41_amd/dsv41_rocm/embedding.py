@@ -107,6 +107,8 @@ def token_embedding_backward(
 
     Bit for bit the same for the same inputs.
     """
+    if not isinstance(ids, torch.Tensor):
+        raise ValueError("ids must be integers")
     if not isinstance(grad, torch.Tensor) or grad.ndim < 1 or grad.shape[-1] == 0 or grad.shape[:-1] != ids.shape:
         raise ValueError("grad must have the shape of ids and the hidden size")
     if not grad.is_cuda:
