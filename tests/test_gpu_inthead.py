@@ -70,6 +70,18 @@ def test_exact(n, h, v, dtype):
 @pytest.mark.parametrize("h,v", [(4100, 32827), (4100, 65536), (4000, 32827), (4100, 32768)])
 def test_many_groups(n, h, v, dtype):
     # groups of 64 rows by twos (an odd number of them, with a part of one at the end; an even one), and one by one
+    _many_rows(n, h, v, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,h,v", [(257, 128, 33000), (300, 129, 33000), (320, 300, 65536), (305, 513, 65537), (321, 257, 33000),
+                                   (640, 256, 32500), (590, 384, 40001)])
+def test_tiles_of_tokens(n, h, v, dtype):
+    # rows for many workgroups, where the widest tiles of tokens are taken: full and cut ones, one stage and several
+    _many_rows(n, h, v, dtype)
+
+
+def _many_rows(n, h, v, dtype):
     x = _inputs(n, h, 1)[0]
     w = torch.randint(-127, 128, (v, h), generator=torch.Generator(DEV).manual_seed(n + h + v), dtype=torch.int8, device=DEV)
     t = torch.rand(v, generator=torch.Generator(DEV).manual_seed(n), device=DEV)

@@ -148,7 +148,7 @@ struct Params {
   int N, V, K;      // K: a multiple of 128
   void* out;
   int64_t os;
-  int n_tb, ranges, wide_tile;
+  int n_tb, ranges, w1;  // gemm_kernel's blocks of tokens, the parts its rows are cut into, and its W1
 };
 
 template <typename T>
@@ -317,13 +317,14 @@ __global__ __launch_bounds__(64 * SPLIT, SPLIT * PER_CU / 4) void head_kernel(Pa
 }
 
 // ------------------------------------------------------------------------------- many tokens
-// W1: blocks of 16 tokens of a wave in the second half of its tokens: tiles of 256 tokens (2) or 192 (1).
+// W1: blocks of 16 tokens of a wave beyond its first two: tiles of 192 tokens (1), 256 (2) or 320 (3).
 template <typename T, int W1>
 __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_kernel(Params p, bool wide) {
   constexpr int WT = 2 + W1, BN = 64 * WT, AHEAD = 6 + W1;  // loads of a wave's four regions
+  constexpr int STAGE = 2 * TL::REGION_W + TL::REGION_X + W1 * 8 * TILE;
   // two stages, and for each wave the scales of the block's rows: read from memory between the multiplies, they would
   // have the wave wait for its stores
-  __shared__ __align__(1024) unsigned char lds[2 * TL::STAGE + NWAVES * BM * 4];
+  __shared__ __align__(1024) unsigned char lds[2 * STAGE + NWAVES * BM * 4];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wv = wid % SQUARE, wt = wid / SQUARE;
   int tb, range;
@@ -343,16 +344,20 @@ __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) v
   v4i wrs = rows_of_w(ld_m);
   const v4i xrs = rsrc(p.q + (int64_t)t0 * p.K, (uint32_t)((min(BN, p.N - t0) + 15) / 16 * bytes));
   const v4i srs = rsrc(p.ts, (uint32_t)p.V * 4);
-  float* scales = reinterpret_cast<float*>(lds + 2 * TL::STAGE) + wid * BM;
+  float* scales = reinterpret_cast<float*>(lds + 2 * STAGE) + wid * BM;
   auto load_scales = [&](int mb) {
-    load_lds(srs, (uint32_t)(mb * BM * 4 + lane * 16), lds0 + (uint32_t)(2 * TL::STAGE + wid * BM * 4));
+    load_lds(srs, (uint32_t)(mb * BM * 4 + lane * 16), lds0 + (uint32_t)(2 * STAGE + wid * BM * 4));
   };
   auto load_region = [&](int reg) {
-    const uint32_t dst = lds0 + (uint32_t)((ld & 1) * TL::STAGE + reg * TL::REGION_W + wid * 2 * TILE);
+    const uint32_t dst = lds0 + (uint32_t)((ld & 1) * STAGE + reg * TL::REGION_W + wid * 2 * TILE);
     const uint32_t off = mine + (uint32_t)(ld_k * 2 * TILE) + (reg & 1) * half + (ld >= total ? 1u << 31 : 0u);
-    if (W1 == 1 && reg == B1) {  // half a region: a tile a wave
-      const uint32_t some = (uint32_t)((8 + (wid >> 1)) * bytes + (wid & 1) * TILE + lane * 16);
-      load_lds(xrs, some + (uint32_t)(ld_k * 2 * TILE) + (ld >= total ? 1u << 31 : 0u), dst - wid * TILE);
+    if (W1 != 2 && reg == B1) {  // not two tiles a wave, a row block's, but one or three
+#pragma unroll
+      for (int i = 0; i < W1; ++i) {
+        const int tile = wid * W1 + i;
+        load_lds(xrs, (uint32_t)((8 + (tile >> 1)) * bytes + (tile & 1) * TILE + ld_k * 2 * TILE) + (ld >= total ? 1u << 31 : 0u) +
+                          (uint32_t)(lane * 16), dst + (tile - 2 * wid) * TILE);
+      }
       return;
     }
 #pragma unroll
@@ -371,6 +376,7 @@ __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) v
   // a region's tiles: those of a row block's two k-steps side by side
   uint32_t ra = (uint32_t)(wv * 8 * TILE + lane * 16), rb = 2 * TL::REGION_W + (uint32_t)(wt * 4 * TILE + lane * 16);
   uint32_t rb1 = 2 * TL::REGION_W + TL::REGION_X + (uint32_t)(wt * 2 * W1 * TILE + lane * 16);
+  int other = STAGE;  // from this stage's place to the other one's
   intx4 acc[WV][WT];
   intx4 fa[4][KS], fb0[2][KS], fb1[W1][KS];
   auto frag = [&](uint32_t off) { return *reinterpret_cast<const intx4*>(lds + off); };
@@ -426,9 +432,10 @@ __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) v
     multiply(first, 1, 1, fb1, nothing);
     barrier();
 
-    ra ^= TL::STAGE;
-    rb ^= TL::STAGE;
-    rb1 ^= TL::STAGE;
+    ra += other;
+    rb += other;
+    rb1 += other;
+    other = -other;
     asm volatile("" : "+v"(ra), "+v"(rb), "+v"(rb1));  // here, not among the multiplies
     load_region(A0);
     wait_loads<AHEAD>();
@@ -519,7 +526,7 @@ size_t scales_at(const dsv41_int_head_desc* d) { return (size_t)((d->n_tokens + 
 // A block of rows against 192 tokens costs this of one against 256.  256 and 192 wide, us: 300 tokens of 7168 ->
 // 129280 (fp32) 370 and 322, of 2048 -> 151936 (bf16) 133 and 111, 576 tokens 195 and 167; but 256 tokens 99 and 110,
 // 1100 tokens 330 and 344, 4096 tokens 1136 and 1221.
-constexpr double NARROW_COST = 0.85;
+constexpr double TILE_COST[4] = {0, 0.85, 1.0, 1.2};
 
 // As many workgroups as fit on the GPU together take the same number of groups each.  Four waves with three
 // steps ahead, two workgroups a CU: 2048 -> 151936, 1, 17, 48 and 64 tokens 52, 57, 64 and 68 us, 7168 -> 129280 151,
@@ -545,8 +552,9 @@ void launch(const Params& p, hipStream_t s) {
   else if (p.N <= FEW) pairs ? launch_few<T, 4, 2, 2>(p, wide, s) : launch_few<T, 4, 1, 4>(p, wide, s);
   else {
     const dim3 grid((p.n_tb * p.ranges + 7) / 8 * 8);
-    if (p.wide_tile) hipLaunchKernelGGL((gemm_kernel<T, 2>), grid, dim3(NT), 0, s, p, wide);
-    else hipLaunchKernelGGL((gemm_kernel<T, 1>), grid, dim3(NT), 0, s, p, wide);
+    if (p.w1 == 1) hipLaunchKernelGGL((gemm_kernel<T, 1>), grid, dim3(NT), 0, s, p, wide);
+    else if (p.w1 == 2) hipLaunchKernelGGL((gemm_kernel<T, 2>), grid, dim3(NT), 0, s, p, wide);
+    else hipLaunchKernelGGL((gemm_kernel<T, 3>), grid, dim3(NT), 0, s, p, wide);
   }
 }
 
@@ -554,10 +562,10 @@ void launch(const Params& p, hipStream_t s) {
 void plan_tiles(Params& p) {
   const int n_mb = (p.V + BM - 1) / BM;
   double best = 1e300;
-  for (int w = 0; w < 2; ++w) {
-    const int bn = w ? 192 : 256, n_tb = (p.N + bn - 1) / bn, ranges = std::max(1, std::min(n_mb, CU_COUNT / n_tb));
-    const double cost = (double)((n_tb * ranges + CU_COUNT - 1) / CU_COUNT) * ((n_mb + ranges - 1) / ranges) * (w ? NARROW_COST : 1.0);
-    if (cost < best) best = cost, p.n_tb = n_tb, p.ranges = ranges, p.wide_tile = !w;
+  for (int w1 : {2, 1, 3}) {
+    const int bn = 128 + 64 * w1, n_tb = (p.N + bn - 1) / bn, ranges = std::max(1, std::min(n_mb, CU_COUNT / n_tb));
+    const double cost = (double)((n_tb * ranges + CU_COUNT - 1) / CU_COUNT) * ((n_mb + ranges - 1) / ranges) * TILE_COST[w1];
+    if (cost < best) best = cost, p.n_tb = n_tb, p.ranges = ranges, p.w1 = w1;
   }
 }
 
