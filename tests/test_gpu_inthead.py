@@ -69,7 +69,7 @@ def test_exact(n, h, v, dtype):
 @pytest.mark.parametrize("n", [33, 48, 49, 64])
 @pytest.mark.parametrize("h,v", [(4100, 32827), (4100, 65536), (4000, 32827), (4100, 32768)])
 def test_many_groups(n, h, v, dtype):
-    # groups of 64 rows by twos (an odd number of them, with a part of one at the end; an even one), and one by one
+    # two groups of 64 rows a workgroup, three in one of them, or a part of one at the end
     _many_rows(n, h, v, dtype)
 
 
@@ -78,6 +78,14 @@ def test_many_groups(n, h, v, dtype):
                                    (640, 256, 32500), (590, 384, 40001)])
 def test_tiles_of_tokens(n, h, v, dtype):
     # rows for many workgroups, where the widest tiles of tokens are taken: full and cut ones, one stage and several
+    _many_rows(n, h, v, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,h,v", [(17, 100, 70001), (64, 128, 65600), (65, 128, 70001), (128, 129, 70001), (100, 300, 140000),
+                                   (40, 400, 140001), (128, 513, 20000), (70, 257, 64), (20, 130, 70)])
+def test_rings(n, h, v, dtype):
+    # runs of groups that make several blocks of rows, whole and not, of one stage, two and more
     _many_rows(n, h, v, dtype)
 
 

@@ -9,14 +9,16 @@
 //
 // The columns are padded to a multiple of 128 (one cache line of a row), those of q with zeros.
 //
-// head_kernel, up to 64 tokens, is bound by reading w once: one token, 7168 -> 129280, 130 us (7.1 TB/s, what a
-// nontemporal read reaches); 48 tokens of 2048 -> 151936 55 us.  A workgroup takes 64 rows of w, its four
-// waves every fourth k-step of their columns; fragments go from memory to registers with no LDS between, so the rows lie
-// in memory as tiles of a fragment's lanes.  (Row-major, each load of a wave met 16 lines, and the loads' rate was the
-// bound: 203 us, and 316 with 48 tokens of 7168 -> 129280 where tiles take 182.)  The waves' integer sums meet in LDS.
-// What more tokens cost is their own tiles, read from L2 by every workgroup.
+// head_kernel, up to 16 tokens, is bound by reading w once: one token, 7168 -> 129280, 130 us (7.1 TB/s, what a
+// nontemporal read reaches).  A workgroup takes 64 rows of w, its four waves every fourth k-step of their columns;
+// fragments go from memory to registers with no LDS between, so the rows lie in memory as tiles of a fragment's lanes.
+// (Row-major, each load of a wave met 16 lines, and the loads' rate was the bound: 203 us.)  The waves' integer sums
+// meet in LDS.
+// ring_kernel, up to 128 tokens, shares the tokens' tiles among up to 256 rows of w, by LDS: in head_kernel, whose
+// workgroups read them from L2 for every 64 rows, 64 tokens of 7168 -> 129280 took 205 us, and 170 here; of 2048 -> 151936
+// 73 and 69.
 // gemm_kernel, above, has the schedule of the bf16 products (mfma_tile.h): eight waves whose pairs multiply and read in
-// turns, stages of 128 columns loaded straight to LDS, tiles of 256 rows x 256 or 192 tokens.  4096 tokens of 7168 ->
+// turns, stages of 128 columns loaded straight to LDS, tiles of 256 rows x 192, 256 or 320 tokens.  4096 tokens of 7168 ->
 // 129280: 2.69 ms, 2.8 POP/s, the matrix cores busy 71% of the cycles at 1.75 GHz (power); of 2048 -> 151936 1.11 ms,
 // 2.3 POP/s: a tile there has 16 stages, and a fifth of its time is the conversion and stores of its logits.
 
@@ -36,8 +38,9 @@ constexpr int BM = TL::BV;
 constexpr int LINE = ROWB;            // columns are padded to whole lines
 constexpr int MAX_COLUMNS = 133120;   // 2^31 / 127^2 = 133144, in whole lines
 constexpr int QUANT_NT = 256;
-// Tokens of head_kernel.  64 and 65, the first of gemm_kernel: 2048 -> 151936 68 and 81 us, 7168 -> 129280 187 and 189.
-constexpr int FEW = 64;
+// Tokens of head_kernel, and of ring_kernel.  17 tokens of 7168 -> 129280 (fp32): 176 us by the first, 161 by the second; 16
+// tokens 159 and 159, one 152 and 155.  128 tokens: 188 by the second, 214 by gemm_kernel; of 2048 -> 151936 82 and 98.
+constexpr int FEW = 16, RING_TOKENS = 128;
 
 typedef int intx4 __attribute__((ext_vector_type(4)));
 
@@ -138,7 +141,9 @@ __global__ __launch_bounds__(QUANT_NT) void quantize_kernel(const bf16_t* x, int
 }
 
 // -------------------------------------------------------------------------------- few tokens
-constexpr int SPLIT = 4, PER_CU = 2;  // waves of a workgroup, workgroups of a CU
+// waves of a workgroup, steps of theirs in registers, workgroups of a CU: of one token, 2048 -> 151936 and 7168 -> 129280,
+// 52 and 151 us; eight waves 54 and 155, two (four workgroups) 57 and 153, five steps ahead 60 and 152.
+constexpr int SPLIT = 4, DEPTH = 4, PER_CU = 2;
 
 struct Params {
   const int8_t* w;  // tiles of the head
@@ -216,109 +221,186 @@ __device__ __forceinline__ void store_logits(T* row, int v, int V, bool there, b
   }
 }
 
-// The fragments of one k-step: of GB groups of 64 rows and of NB blocks of 16 tokens.
-template <int NB, int GB>
+// The fragments of one k-step: of a group of 64 rows and of the tokens.
 struct Step {
-  intx4 a[4 * GB], b[NB];
+  intx4 a[4], b;
 };
 
-// SPLIT waves share the columns of GB groups, every SPLIT-th k-step each; a workgroup takes item after item of GB groups, with
+// SPLIT waves share the columns of a group, every SPLIT-th k-step each; a workgroup takes group after group, with
 // DEPTH - 1 steps of each wave on their way from memory throughout.
-template <typename T, int NB, int GB, int DEPTH>
+template <typename T>
 __global__ __launch_bounds__(64 * SPLIT, SPLIT * PER_CU / 4) void head_kernel(Params p, bool wide) {
-  __shared__ intx4 parts[SPLIT][4 * NB][64];
-  __shared__ float scales[SPLIT][GB * GROUP];  // each wave's copy of the groups'
+  __shared__ intx4 parts[SPLIT - 1][4][64];
+  __shared__ float scales[GROUP];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, quad = lane >> 4;
   const int steps = p.K / 64, turns = (steps + SPLIT * DEPTH - 1) / (SPLIT * DEPTH) * DEPTH, groups = (p.V + GROUP - 1) / GROUP;
-  const int items = (groups + GB - 1) / GB;
-  T* out = static_cast<T*>(p.out);
-  intx4 acc[4 * GB][NB];
-  auto clear = [&]() {
-#pragma unroll
-    for (int i = 0; i < 4 * GB; ++i)
-#pragma unroll
-      for (int j = 0; j < NB; ++j) acc[i][j] = intx4{0, 0, 0, 0};
-  };
-  clear();
-  Step<NB, GB> f[DEPTH];
-  int at = wave, left = turns, ahead = blockIdx.x;  // the step to load, those left of its item, the item
-  // (addresses are the same in all lanes, which add theirs in 32 bits; a step that is none reads the first bytes of q, which
-  // all caches hold, as loads under a condition cost registers; a group past the last is the last one again)
-  auto load = [&](Step<NB, GB>& s) {
-    const bool some = ahead < items && at < steps;
-    const int8_t* qa = p.q + (some ? at * TILE : 0);
+  T* out = static_cast<T*>(p.out) + r16 * p.os;
+  intx4 acc[4] = {};
+  Step f[DEPTH];
+  int at = wave, left = turns, ahead = blockIdx.x;  // the step to load, those left of its group, the group
+  const int8_t* w = p.w + (int64_t)ahead * GROUP * p.K;  // (the same in all lanes, which add theirs in 32 bits)
+  // (a step that is none reads the first bytes of q, which all caches hold: loads under a condition cost registers)
+  auto load = [&](Step& s) {
+    const bool some = ahead < groups && at < steps;
+    const int8_t *wa = some ? w + at * TILE : p.q, *qa = p.q + (some ? at * TILE : 0);
     const int64_t tile_row = some ? (int64_t)16 * p.K : 0;
 #pragma unroll
-    for (int g = 0; g < GB; ++g) {
-      const int8_t* wa = some ? p.w + (int64_t)min(ahead * GB + g, groups - 1) * GROUP * p.K + at * TILE : p.q;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        s.a[4 * g + i] = __builtin_nontemporal_load(reinterpret_cast<const intx4*>(wa + i * tile_row) + lane);
-    }
-#pragma unroll
-    for (int j = 0; j < NB; ++j) s.b[j] = reinterpret_cast<const intx4*>(qa + j * tile_row)[lane];
+    for (int i = 0; i < 4; ++i) s.a[i] = __builtin_nontemporal_load(reinterpret_cast<const intx4*>(wa + i * tile_row) + lane);
+    s.b = reinterpret_cast<const intx4*>(qa)[lane];
     at += SPLIT;
-    if (--left == 0) at = wave, left = turns, ahead += gridDim.x;
+    if (--left == 0) {
+      at = wave, left = turns, ahead += gridDim.x;
+      w += (int64_t)gridDim.x * GROUP * p.K;
+    }
   };
 #pragma unroll
   for (int d = 0; d < DEPTH - 1; ++d) load(f[d]);
-  float ss[NB];
-#pragma unroll
-  for (int j = 0; j < NB; ++j) ss[j] = p.ss[min(16 * j + r16, p.N - 1)];
-  for (int item = blockIdx.x; item < items; item += gridDim.x) {
-    // (read at the end, they would have the wave wait for all steps on their way)
-    float t[GB];
-#pragma unroll
-    for (int g = 0; g < GB; ++g) t[g] = p.ts[min((item * GB + g) * GROUP + lane, p.V - 1)];
+  const float ss = p.ss[min(r16, p.N - 1)];
+  for (int group = blockIdx.x; group < groups; group += gridDim.x) {
+    // (read at the end, it would have the wave wait for all steps on their way)
+    const float t = p.ts[min(group * GROUP + lane, p.V - 1)];
     for (int turn = 0; turn < turns; turn += DEPTH) {
 #pragma unroll
       for (int d = 0; d < DEPTH; ++d) {
         load(f[(d + DEPTH - 1) % DEPTH]);
         if (wave + (turn + d) * SPLIT < steps) {
 #pragma unroll
-          for (int i = 0; i < 4 * GB; ++i)
-#pragma unroll
-            for (int j = 0; j < NB; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[d].a[i], f[d].b[j], acc[i][j], 0, 0, 0);
+          for (int i = 0; i < 4; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[d].a[i], f[d].b, acc[i], 0, 0, 0);
         }
       }
     }
-    // the waves' sums meet, a group at a time: token block j is wave j % SPLIT's to finish
+    // the waves' sums meet in the first one
+    if (wave > 0) {
 #pragma unroll
-    for (int g = 0; g < GB; ++g) scales[wave][g * GROUP + lane] = t[g];
-#pragma unroll
-    for (int g = 0; g < GB; ++g) {
-#pragma unroll
-      for (int j = 0; j < NB; ++j)
-        if (j % SPLIT != wave) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) parts[wave][4 * j + i][lane] = acc[4 * g + i][j];
-        }
-      rows::lds_barrier();
-#pragma unroll
-      for (int j = 0; j < NB; ++j) {
-        if (j % SPLIT != wave) continue;
-        intx4 c[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) c[i] = acc[4 * g + i][j];
-#pragma unroll
-        for (int s = 0; s < SPLIT; ++s)
-          if (s != wave) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) c[i] += parts[s][4 * j + i][lane];
-          }
-        const int n = 16 * j + r16;
-        store_logits(out + n * p.os, (item * GB + g) * GROUP, p.V, n < p.N, wide, c[0], c[1], c[2], c[3], ss[j],
-                     scales[wave] + g * GROUP + 16 * quad);
-      }
-      rows::lds_barrier();
+      for (int i = 0; i < 4; ++i) parts[wave - 1][i][lane] = acc[i];
+    } else {
+      scales[lane] = t;
     }
-    clear();
+    rows::lds_barrier();
+    if (wave == 0) {
+#pragma unroll
+      for (int s = 0; s < SPLIT - 1; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] += parts[s][i][lane];
+      store_logits(out, group * GROUP, p.V, r16 < p.N, wide, acc[0], acc[1], acc[2], acc[3], ss, scales + 16 * quad);
+    }
+    rows::lds_barrier();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = intx4{0, 0, 0, 0};
   }
 }
 
+// ---------------------------------------------------------------------------- up to 128 tokens
+// A workgroup takes a run of groups, up to four at a time, against all tokens, 32 NB at most: wave (wv, wt) group wv's 64 rows
+// and half of the tokens.  Stages of 128 columns go straight to a ring of RING in LDS, RING - 1 of them on their way from
+// memory throughout; one barrier a stage says that it has come and that the one before it is free.
+constexpr int RING = 3;  // (32 tokens a stage, and four stages: no faster)
+// load_lds of what is read once: 7168 -> 129280, 128 tokens 216 us without the hint, 197 with it
+__device__ __forceinline__ void load_lds_once(v4i rs, uint32_t voff, uint32_t lds_addr) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen nt lds" ::"v"(voff), "s"(rs),
+               "s"(lds_addr)
+               : "memory");
+}
+template <typename T, int NB>
+__global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) void ring_kernel(Params p, bool wide) {
+  constexpr int STAGE = (32 + 4 * NB) * TILE, LOADS = 4 + NB / 2;  // loads of a wave a stage
+  __shared__ __align__(1024) unsigned char lds[RING * STAGE + NWAVES * BM * 4];  // for each wave the block's scales, too
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, quad = lane >> 4;
+  const int wv = wid & 3, wt = wid >> 2;
+  const int groups = (p.V + GROUP - 1) / GROUP, nst = p.K / LINE;
+  const int g0 = (int)((int64_t)blockIdx.x * groups / p.ranges), g1 = (int)((int64_t)(blockIdx.x + 1) * groups / p.ranges);
+  const int blocks = (g1 - g0 + 3) / 4, total = blocks * nst;
+  auto first_of = [&](int b) { return g0 + (g1 - g0) * b / blocks; };
+
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds;
+  const uint32_t bytes = (uint32_t)(16 * p.K);  // of 16 rows
+  auto rows_of_w = [&](int b) {
+    const int g = first_of(b);
+    return rsrc(p.w + (int64_t)g * GROUP * p.K, (uint32_t)(first_of(b + 1) - g) * 4 * bytes);
+  };
+  v4i wrs = rows_of_w(0);
+  const v4i xrs = rsrc(p.q, (uint32_t)(p.N + 15) / 16 * bytes);
+  const v4i srs = rsrc(p.ts, (uint32_t)p.V * 4);
+  float* scales = reinterpret_cast<float*>(lds + RING * STAGE) + wid * BM;
+  int ld = 0, ld_k = 0, ld_b = 0;  // the stage being loaded
+  uint32_t ld_at = 0;
+  auto load_stage = [&]() {
+    const uint32_t off = (uint32_t)(lane * 16 + ld_k * 2 * TILE) + (ld >= total ? 1u << 31 : 0u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int m = 2 * wid + i / 2;
+      load_lds_once(wrs, off + m * bytes + (i & 1) * TILE, lds0 + ld_at + (2 * m + (i & 1)) * TILE);
+    }
+#pragma unroll
+    for (int i = 0; i < NB / 2; ++i) {
+      const int tile = wid * (NB / 2) + i;
+      load_lds(xrs, off + (tile >> 1) * bytes + (tile & 1) * TILE, lds0 + ld_at + (32 + tile) * TILE);
+    }
+    ++ld;
+    ld_at = ld_at == (RING - 1) * STAGE ? 0 : ld_at + STAGE;
+    if (++ld_k == nst) {
+      ld_k = 0;
+      ld_b = min(ld_b + 1, blocks - 1);  // (past the last stage nothing is read)
+      wrs = rows_of_w(ld_b);
+    }
+  };
+  float ss[NB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) ss[j] = p.ss[min((wt * NB + j) * 16 + r16, p.N - 1)];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) asm volatile("" ::"v"(ss[j]));  // here, with no load behind them yet
+#pragma unroll
+  for (int i = 0; i < RING - 1; ++i) load_stage();
+
+  T* out = static_cast<T*>(p.out);
+  uint32_t at = 0;
+  for (int b = 0; b < blocks; ++b) {
+    const int g = first_of(b);
+    const bool some = wv < first_of(b + 1) - g;
+    intx4 acc[4][NB];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) acc[i][j] = intx4{0, 0, 0, 0};
+    for (int k = 0; k < nst; ++k) {
+      wait_loads<(RING - 2) * LOADS>();
+      barrier();
+      if (k == 0) load_lds(srs, (uint32_t)(g * GROUP * 4 + lane * 16), lds0 + (uint32_t)(RING * STAGE + wid * BM * 4));
+      load_stage();
+      if (some) {
+        const unsigned char* from = lds + at + lane * 16;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          intx4 fa[4], fb[NB];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) fa[i] = *reinterpret_cast<const intx4*>(from + (2 * (4 * wv + i) + ks) * TILE);
+#pragma unroll
+          for (int j = 0; j < NB; ++j) fb[j] = *reinterpret_cast<const intx4*>(from + (32 + 2 * (NB * wt + j) + ks) * TILE);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[i], fb[j], acc[i][j], 0, 0, 0);
+        }
+      }
+      at = at == (RING - 1) * STAGE ? 0 : at + STAGE;
+    }
+    if (nst < RING) wait_loads<(RING - 1) * LOADS>();  // (longer rows have waited for the scales by now)
+    if (some) {
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        const int n = (wt * NB + j) * 16 + r16;
+        store_logits(out + (int64_t)n * p.os, (g + wv) * GROUP, p.V, n < p.N, wide, acc[0][j], acc[1][j], acc[2][j], acc[3][j],
+                     ss[j], scales + wv * GROUP + 16 * quad);
+      }
+    }
+  }
+  wait_loads<0>();  // no load to LDS outlives the loop
+}
+
 // ------------------------------------------------------------------------------- many tokens
-// W1: blocks of 16 tokens of a wave beyond its first two: tiles of 192 tokens (1), 256 (2) or 320 (3).
-template <typename T, int W1>
+// W1: blocks of 16 tokens of a wave beyond its first two: tiles of 192 tokens (1), 256 (2) or 320 (3).  ONCE: one tile has all
+// tokens, so that no other reads the weights again (256 tokens of 7168 -> 129280 256 us without the hint, 237 with it).
+template <typename T, int W1, bool ONCE>
 __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_kernel(Params p, bool wide) {
   constexpr int WT = 2 + W1, BN = 64 * WT, AHEAD = 6 + W1;  // loads of a wave's four regions
   constexpr int STAGE = 2 * TL::REGION_W + TL::REGION_X + W1 * 8 * TILE;
@@ -361,7 +443,10 @@ __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) v
       return;
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) load_lds(reg < B0 ? wrs : xrs, off + i * TILE, dst + i * TILE);
+    for (int i = 0; i < 2; ++i) {
+      if (ONCE && reg < B0) load_lds_once(wrs, off + i * TILE, dst + i * TILE);
+      else load_lds(reg < B0 ? wrs : xrs, off + i * TILE, dst + i * TILE);
+    }
   };
   auto next_load_stage = [&]() {
     ++ld;
@@ -523,38 +608,40 @@ int check_head(const dsv41_int_head_desc* d) {
 
 size_t scales_at(const dsv41_int_head_desc* d) { return (size_t)((d->n_tokens + 15) / 16 * 16) * padded_of(d->hidden); }
 
-// A block of rows against 192 tokens costs this of one against 256.  256 and 192 wide, us: 300 tokens of 7168 ->
-// 129280 (fp32) 370 and 322, of 2048 -> 151936 (bf16) 133 and 111, 576 tokens 195 and 167; but 256 tokens 99 and 110,
-// 1100 tokens 330 and 344, 4096 tokens 1136 and 1221.
+// What a block of rows costs against a tile of 128 + 64 W1 tokens, 256 tokens' being 1.  Tiles of 256 or 192 and of 320, us:
+// 300 tokens of 7168 -> 129280 (fp32) 337 and 281, of 2048 -> 151936 143 and 138, 600 tokens 553 and 500, 247 and 230; but
+// 4096 tokens of 7168 3026 and 3050.  Of 256 and 192: 576 tokens of 2048 -> 151936 (bf16) 195 and 167; but 256 tokens 99
+// and 110, 1100 tokens 330 and 344, 4096 tokens 1136 and 1221.
 constexpr double TILE_COST[4] = {0, 0.85, 1.0, 1.2};
 
-// As many workgroups as fit on the GPU together take the same number of groups each.  Four waves with three
-// steps ahead, two workgroups a CU: 2048 -> 151936, 1, 17, 48 and 64 tokens 52, 57, 64 and 68 us, 7168 -> 129280 151,
-// 164, 182 and 199.  Eight waves: 54, 59, 68, 72 and 155, 174, 193, 208; two (four workgroups): 57, 63, 70, 75 and 153,
-// 162, 177, 193; five steps ahead 60, 69, 77, 89 and 152, 167, 186, 222.
-constexpr int rounds_of(int items) { return (items + PER_CU * CU_COUNT - 1) / (PER_CU * CU_COUNT); }
-template <typename T, int NB, int GB, int DEPTH>
+// As many workgroups as fit on the GPU together take the same number of groups each.
+template <typename T>
 void launch_few(const Params& p, bool wide, hipStream_t s) {
-  const int items = ((p.V + GROUP - 1) / GROUP + GB - 1) / GB, rounds = rounds_of(items);
-  hipLaunchKernelGGL((head_kernel<T, NB, GB, DEPTH>), dim3((items + rounds - 1) / rounds), dim3(64 * SPLIT), 0, s, p, wide);
+  const int groups = (p.V + GROUP - 1) / GROUP, slots = PER_CU * CU_COUNT, rounds = (groups + slots - 1) / slots;
+  hipLaunchKernelGGL(head_kernel<T>, dim3((groups + rounds - 1) / rounds), dim3(64 * SPLIT), 0, s, p, wide);
+}
+template <typename T, int NB>
+void launch_ring(Params p, bool wide, hipStream_t s) {
+  p.ranges = std::min((p.V + GROUP - 1) / GROUP, CU_COUNT);
+  hipLaunchKernelGGL((ring_kernel<T, NB>), dim3(p.ranges), dim3(NT), 0, s, p, wide);
+}
+template <typename T, int W1>
+void launch_tiles(const Params& p, bool wide, hipStream_t s) {
+  const dim3 grid((p.n_tb * p.ranges + 7) / 8 * 8);
+  if (p.n_tb == 1) hipLaunchKernelGGL((gemm_kernel<T, W1, true>), grid, dim3(NT), 0, s, p, wide);
+  else hipLaunchKernelGGL((gemm_kernel<T, W1, false>), grid, dim3(NT), 0, s, p, wide);
 }
 template <typename T>
 void launch(const Params& p, hipStream_t s) {
   const bool wide = p.os * sizeof(T) % 16 == 0 && (uintptr_t)p.out % 16 == 0;
-  const int groups = (p.V + GROUP - 1) / GROUP;
-  // Groups of 64 rows by twos read the tokens' tiles half as often, if no workgroup gets more of them by it: 7168 -> 129280,
-  // 48 tokens 198 -> 184 us, 64 tokens 210 -> 185 (bf16: 182 -> 173, 195 -> 177); 8192 -> 65536, 64 tokens 123 -> 110.  In short rows the
-  // meeting of the waves' sums, two groups' at once, costs more: 2048 -> 129280, 48 tokens 57 -> 61.
-  const bool pairs = p.K >= 4096 && 2 * rounds_of((groups + 1) / 2) <= rounds_of(groups);
-  if (p.N <= 16) launch_few<T, 1, 1, 4>(p, wide, s);
-  else if (p.N <= 32) launch_few<T, 2, 1, 4>(p, wide, s);
-  else if (p.N <= 48) pairs ? launch_few<T, 3, 2, 3>(p, wide, s) : launch_few<T, 3, 1, 4>(p, wide, s);
-  else if (p.N <= FEW) pairs ? launch_few<T, 4, 2, 2>(p, wide, s) : launch_few<T, 4, 1, 4>(p, wide, s);
-  else {
-    const dim3 grid((p.n_tb * p.ranges + 7) / 8 * 8);
-    if (p.w1 == 1) hipLaunchKernelGGL((gemm_kernel<T, 1>), grid, dim3(NT), 0, s, p, wide);
-    else if (p.w1 == 2) hipLaunchKernelGGL((gemm_kernel<T, 2>), grid, dim3(NT), 0, s, p, wide);
-    else hipLaunchKernelGGL((gemm_kernel<T, 3>), grid, dim3(NT), 0, s, p, wide);
+  if (p.N <= FEW) {
+    launch_few<T>(p, wide, s);
+  } else if (p.N <= 64) {
+    launch_ring<T, 2>(p, wide, s);
+  } else if (p.N <= RING_TOKENS) {
+    launch_ring<T, 4>(p, wide, s);
+  } else {
+    p.w1 == 1 ? launch_tiles<T, 1>(p, wide, s) : p.w1 == 2 ? launch_tiles<T, 2>(p, wide, s) : launch_tiles<T, 3>(p, wide, s);
   }
 }
 
