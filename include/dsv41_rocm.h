@@ -4,7 +4,7 @@
  *
  * Plain C: pointers, sizes and PODs only. Every device pointer is a HIP device
  * address owned by the caller; the library never allocates or frees device
- * memory, never synchronises the stream (dsv41_check_wait alone does), and launches only on
+ * memory, never synchronises the stream (dsv41_check_wait and dsv41_embed_checked_run alone do), and launches only on
  * `stream`.
  *
  * Return codes: 0 on success, a negative DSV41_E_* code before any launch on a
@@ -864,6 +864,9 @@ int dsv41_int_head_run(const dsv41_int_head_desc* desc, void* workspace, size_t 
 /* Rows of a token table, and the table's gradient.  Workspace of the gradient (16-byte aligned, contents need
  * no initialisation): the sorted tokens, and two rows of fp32 sums per 32 tokens. */
 int dsv41_embed_run(const dsv41_embed_desc* desc, void* stream /* hipStream_t */);
+/* The same, with an answer: 1 when some id is at or above the vocabulary size, 0 when none is, or a negative error.  It
+ * waits until the ids have been looked at, not for the rows.  `flags` as for dsv41_check_wait. */
+int dsv41_embed_checked_run(const dsv41_embed_desc* desc, int32_t* flags, void* stream /* hipStream_t */);
 size_t dsv41_embed_grad_workspace_bytes(const dsv41_embed_grad_desc* desc);
 int dsv41_embed_grad_run(const dsv41_embed_grad_desc* desc, void* workspace, size_t workspace_bytes,
                          void* stream /* hipStream_t */);

@@ -134,6 +134,27 @@ def test_ids_outside_the_vocabulary():
     assert grad[:, 0].tolist() == [0, 0, 1, 0, 0, 0, 0, 0, 0, 1]
 
 
+@pytest.mark.parametrize("n", [1, 63, 1024, 1025, 5000, 300001])
+@pytest.mark.parametrize("train", [False, True])
+def test_one_id_outside_among_many(n, train):
+    # the check looks at every id, wherever it lies and however the ids are aligned; the next call is sound again
+    table = torch.randn(50, 4, device=DEV, requires_grad=train)
+    g = torch.Generator(DEV).manual_seed(n)
+    ids = torch.randint(-3, 50, (n + 1,), generator=g, device=DEV)
+    for shift in (0, 1):
+        mine = ids[shift:shift + n].clone() if shift == 0 else ids[shift:]
+        assert token_embedding(mine, table).shape == (n, 4)
+        for at in {0, n // 2, n - 1}:
+            good = int(mine[at])
+            for bad in (50, 1 << 40):
+                mine[at] = bad
+                with pytest.raises(ValueError, match="token ID is outside the model vocabulary"):
+                    token_embedding(mine, table)
+            mine[at] = good
+    want = torch.where((mine >= 0)[:, None], table.detach()[mine.clamp_min(0)], 0.0)
+    assert torch.equal(token_embedding(mine, table).detach(), want)
+
+
 def test_no_tokens():
     table = torch.randn(10, 16, device=DEV, requires_grad=True)
     ids = torch.zeros(3, 0, dtype=torch.int64, device=DEV)

@@ -203,6 +203,14 @@ def test_embed_refusals(kw, code, msg):
     assert _lib.load().dsv41_embed_run(ctypes.byref(_embed(n_tokens=0, ids=None, out=None)), None) == _lib.OK
 
 
+def test_checked_embed_refusals():
+    run = _lib.load().dsv41_embed_checked_run
+    assert run(ctypes.byref(_embed()), None, None) == _lib.E_INVALID and "flags" in _lib.last_error()
+    assert run(ctypes.byref(_embed(hidden=0)), 0x4000, None) == _lib.E_INVALID
+    assert run(None, 0x4000, None) == _lib.E_INVALID
+    assert run(ctypes.byref(_embed(n_tokens=0, ids=None, out=None)), 0x4000, None) == _lib.OK
+
+
 @pytest.mark.parametrize("kw,code,msg", TABLE + [
     (dict(grad=None), _lib.E_INVALID, "required"),
     (dict(grad=0x1002), _lib.E_INVALID, "aligned"),

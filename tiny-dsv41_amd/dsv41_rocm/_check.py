@@ -44,17 +44,22 @@ def any_set(status: Optional[torch.Tensor], ids: Optional[torch.Tensor] = None, 
         return False, False
     if max(n, n_ids) > MAX_VALUES:
         return n > 0 and bool((status != 0).any()), n_ids > 0 and bool(((ids < 0) | (ids >= limit)).any())
+    got = answer(_lib.load().dsv41_check_wait, t.device.index, status.data_ptr() if n else None, n,
+                 ids.data_ptr() if n_ids else None, n_ids, limit)
+    return bool(got & 1), bool(got & 2)
+
+
+def answer(call, index: int, *args) -> int:
+    """What ``call(*args, word, stream)`` answers on GPU ``index``'s current stream, with its error raised."""
     if _word.ptr is None:
         _word.make()
-    index = t.device.index
-    args = (status.data_ptr() if n else None, n, ids.data_ptr() if n_ids else None, n_ids, limit, _word.ptr)
     if torch.cuda.current_device() == index:
-        got = _lib.load().dsv41_check_wait(*args, _lib.stream(index))
+        got = call(*args, _word.ptr, _lib.stream(index))
     else:
         with torch.cuda.device(index):
-            got = _lib.load().dsv41_check_wait(*args, _lib.stream(index))
+            got = call(*args, _word.ptr, _lib.stream(index))
     if got < 0:
         _left.append(_word.host)
         _word.make()
         _lib.check(got)
-    return bool(got & 1), bool(got & 2)
+    return got

@@ -510,6 +510,7 @@ EXPORTS = (
     "dsv41_int_head_workspace_bytes",
     "dsv41_int_head_run",
     "dsv41_embed_run",
+    "dsv41_embed_checked_run",
     "dsv41_embed_grad_workspace_bytes",
     "dsv41_embed_grad_run",
 )
@@ -595,6 +596,8 @@ def _bind(lib: ctypes.CDLL) -> ctypes.CDLL:
     for name, cls in (("process", ProcessDesc), ("process_grad", ProcessDesc), ("embed", EmbedDesc)):
         run = getattr(lib, f"dsv41_{name}_run")
         run.restype, run.argtypes = ctypes.c_int, [ctypes.POINTER(cls), ctypes.c_void_p]
+    lib.dsv41_embed_checked_run.restype = ctypes.c_int
+    lib.dsv41_embed_checked_run.argtypes = [ctypes.POINTER(EmbedDesc), ctypes.c_void_p, ctypes.c_void_p]
     for name, cls in (("int_head", IntHeadDesc), ("embed_grad", EmbedGradDesc)):
         size = getattr(lib, f"dsv41_{name}_workspace_bytes")
         size.restype, size.argtypes = ctypes.c_size_t, [ctypes.POINTER(cls)]

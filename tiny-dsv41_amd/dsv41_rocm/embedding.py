@@ -13,7 +13,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._check import any_set
+from ._check import answer
 from .logprob import first_order
 from .scores import INTEGERS, fit_int32, launch, overlap, refuse_capture, refuse_tangents, written
 
@@ -64,16 +64,18 @@ def prepare(ids, weight, scale):
     return _ids(ids, weight.device), _matrix(weight), _scale(scale)
 
 
-def forward(ids, weight, scale, want_status):
-    """One dsv41_embed_run; returns (rows, statuses or None)."""
+def forward(ids, weight, scale, status=None, check=False):
+    """One dsv41_embed_run, with every id's status if asked for; with ``check`` one that raises."""
     n, (v, h) = ids.numel(), weight.shape
     out = weight.new_empty(n, h)
-    status = torch.empty(n, dtype=torch.int32, device=weight.device) if want_status else None
     if n:
         d = _lib.EmbedDesc(ctypes.sizeof(_lib.EmbedDesc), n, h, v, weight.data_ptr(), _step(weight), ids.data_ptr(), scale,
                            _DTYPES[weight.dtype], out.data_ptr(), h, None if status is None else status.data_ptr())
-        launch(_lib.load().dsv41_embed_run, weight.device, ctypes.byref(d))
-    return out, status
+        if not check:
+            launch(_lib.load().dsv41_embed_run, weight.device, ctypes.byref(d))
+        elif answer(_lib.load().dsv41_embed_checked_run, weight.device.index, ctypes.byref(d)):
+            raise ValueError("token ID is outside the model vocabulary")
+    return out
 
 
 def _backward(ids, grad, scale, out, accumulate):
@@ -150,17 +152,15 @@ def token_embedding_backward(
 
 class _TokenEmbedding(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, ids, weight, scale, want_status):
-        out, status = forward(ids, weight, scale, want_status)
+    def forward(ctx, ids, weight, scale, check):
+        out = forward(ids, weight, scale, check=check)
         ctx.save_for_backward(ids)
         ctx.vocab, ctx.dtype, ctx.scale = weight.shape[0], weight.dtype, scale
         ctx.set_materialize_grads(False)
-        if status is not None:
-            ctx.mark_non_differentiable(status)
-        return out, status
+        return out
 
     @staticmethod
-    def backward(ctx, grad, g_status):
+    def backward(ctx, grad):
         if grad is None:
             return None, None, None, None
         (ids,) = ctx.saved_tensors
@@ -177,15 +177,13 @@ def token_embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1
     Negative ids are padding: rows of zeros, which take no part in the gradient.  Differentiable in
     ``weight`` (a dense gradient, see :func:`token_embedding_backward`), once, in backward mode.
 
-    With ``check`` the call synchronises and raises ``ValueError`` for an id at or above the vocabulary size;
-    without, such a token's row is NaN.
+    With ``check`` the call waits until the GPU has looked at the ids and raises ``ValueError`` for one at or above the
+    vocabulary size; without, such a token's row is NaN.
     """
     flat, weight, scale = prepare(ids, weight, scale)
     refuse_capture(check)
     if torch.is_grad_enabled() and weight.requires_grad:
-        out, status = _TokenEmbedding.apply(flat, weight, scale, check)
+        out = _TokenEmbedding.apply(flat, weight, scale, check)
     else:
-        out, status = forward(flat, weight, scale, check)
-    if check and any_set(status)[0]:
-        raise ValueError("token ID is outside the model vocabulary")
+        out = forward(flat, weight, scale, check=check)
     return out if ids.ndim == 1 else out.view(*ids.shape, weight.shape[1])

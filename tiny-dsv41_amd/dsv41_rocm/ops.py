@@ -280,7 +280,8 @@ def _head_logits_fake(hidden, tiles, scales, vocab, dtype):
 @torch.library.custom_op("dsv41_rocm::token_embedding", mutates_args=(), device_types="cuda")
 def token_embedding_op(ids: torch.Tensor, weight: torch.Tensor, scale: float) -> tuple[torch.Tensor, torch.Tensor]:
     flat, weight, scale = _embedding.prepare(ids, weight, scale)
-    out, status = _embedding.forward(flat, weight, scale, True)
+    status = torch.empty(flat.numel(), dtype=torch.int32, device=weight.device)
+    out = _embedding.forward(flat, weight, scale, status)
     return out.view(*ids.shape, weight.shape[1]), status
 
 
