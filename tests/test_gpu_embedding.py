@@ -155,6 +155,31 @@ def test_one_id_outside_among_many(n, train):
     assert torch.equal(token_embedding(mine, table).detach(), want)
 
 
+def test_checked_behind_work_that_takes_long():
+    # the answer comes long after the host begins to look for it, on a stream of its own too
+    table = torch.randn(60, 32, device=DEV, requires_grad=True)
+    ids = torch.randint(0, 60, (100,), device=DEV)
+    bad = ids.clone()
+    bad[57] = 60
+    a = torch.rand(4096, 4096, device=DEV)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for stream in (torch.cuda.current_stream(), side):
+        with torch.cuda.stream(stream):
+            for _ in range(8):
+                b = a @ a
+            rows = token_embedding(ids, table)
+            for _ in range(8):
+                b = a @ a
+            with pytest.raises(ValueError, match="token ID is outside the model vocabulary"):
+                token_embedding(bad, table)
+            (grad,) = torch.autograd.grad(rows.sum(), table)
+        torch.cuda.synchronize()
+        assert torch.equal(rows.detach(), table.detach()[ids])
+        assert torch.equal(grad, torch.bincount(ids, minlength=60).float()[:, None].expand(60, 32))
+        del b
+
+
 def test_no_tokens():
     table = torch.randn(10, 16, device=DEV, requires_grad=True)
     ids = torch.zeros(3, 0, dtype=torch.int64, device=DEV)
