@@ -89,6 +89,14 @@ def test_rings(n, h, v, dtype):
     _many_rows(n, h, v, dtype)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,h", [(1, 1), (1, 8), (2, 136), (3, 2040), (4, 2048), (5, 2048), (4, 2047), (4, 2056), (2, 7168), (1, 16385),
+                                 (3, 700), (16, 2048), (4, 128)])
+def test_tokens_quantized_by_the_product(n, h, dtype):
+    # few short tokens are quantized in the product's own launch: full ones, cut ones, one too many, too long, of odd lengths
+    _many_rows(n, h, 33000 + n, dtype)
+
+
 def _many_rows(n, h, v, dtype):
     x = _inputs(n, h, 1)[0]
     w = torch.randint(-127, 128, (v, h), generator=torch.Generator(DEV).manual_seed(n + h + v), dtype=torch.int8, device=DEV)
@@ -109,6 +117,24 @@ def test_ties_and_borders():
     got = head_logits(x.to(DEV), head)[0].cpu()
     want = torch.round(x[0].double() / 2).float() * (torch.tensor(254.0) / 127)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("scale", [2.0**-133, 2.0**-126, 2.0**-101, 2.0**-100, 2.0**-99, 2.0**-7, 2.0**92, 2.0**93, 2.0**120])
+def test_every_quotient(scale):
+    # every mantissa of the largest against every mantissa, at every exponent that is not far below a half of a step
+    a = torch.arange(128, 256, dtype=torch.float64)
+    x = torch.cat([a * 2.0**-s for s in range(10)] + [torch.zeros(1, dtype=torch.float64)])
+    rows = torch.where(x[None, :] <= a[:, None], x[None, :], 0.0).repeat(1, 2)
+    rows[:, x.numel():] *= -1
+    rows[:, x.numel() - 1] = a
+    rows = (rows * scale).bfloat16()  # (exact but for the subnormal ones, which are rounded before both sides see them)
+    q, s = _quantized(rows)
+    head = quantize_head(rows.to(DEV))
+    assert torch.equal(head.integers().cpu().double(), q) and torch.equal(head.scales.cpu(), s)
+    eye = Int8Head.from_quantized(torch.eye(rows.shape[1], dtype=torch.int8, device=DEV), torch.ones(rows.shape[1], device=DEV))
+    want = q.float() * s[:, None]
+    for n in (2, 16, 128):  # quantized by the product, and before it
+        assert torch.equal(torch.cat([head_logits(part, eye) for part in rows.to(DEV).split(n)]).cpu(), want)
 
 
 @pytest.mark.parametrize("n", [3, 70])

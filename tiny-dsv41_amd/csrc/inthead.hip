@@ -3,7 +3,7 @@
 //
 // A row x of bf16 becomes q_k = rint(127 x_k / a) with a = max |x| and the scale a / 127 (fp32); the
 // head's rows w are kept that way.  x_k and a have 8 bits, so 127 x_k / a is a half or at least 2^-16 of its
-// size away from one (254 X - (2 k + 1) A 2^s is an integer): the fp32 division decides as the exact one.  With s, t the scales,
+// size away from one (254 X - (2 k + 1) A 2^s is an integer): a quotient good to a last place decides as the exact one.  With s, t the scales,
 //   out[n, v] = (sum_k q[n, k] w[v, k]) s[n] t[v],
 // the sum exact in 32-bit integers (up to 2^31 / 127^2 = 133144 columns), then two fp32 products.
 //
@@ -76,18 +76,56 @@ __device__ __forceinline__ void load_chunk(const bf16_t* x, int cols, int i, uin
       if (i + j < cols) rows::Elem<bf16_t>::put(w, j, x[i + j]);
   }
 }
+// Chunks of x[0, cols), c STEP + i for c < C: those of rows of whole chunks are on their way together (a condition around
+// a load has the wave wait for it); ones past the end hold anything until cut() makes them zeros.
+template <int C, int STEP>
+__device__ __forceinline__ void load_chunks(const bf16_t* x, int cols, int i, uint32_t (&w)[C][4]) {
+  if (cols % 8 == 0) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) rows::load16<false>(x + min(c * STEP + i, cols - 8), w[c]);
+  } else {
+#pragma unroll
+    for (int c = 0; c < C; ++c) load_chunk(x, cols, c * STEP + i, w[c]);
+  }
+}
+__device__ __forceinline__ void cut(uint32_t (&w)[4], bool there) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = there ? w[j] : 0;
+}
 // The largest magnitude's bits, of which those of infinities and NaNs are the largest.
 __device__ __forceinline__ uint32_t top_of(const uint32_t (&w)[4], uint32_t top) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) top = max(top, max((w[j] << 16) & 0x7FFF0000u, w[j] & 0x7FFF0000u));
   return top;
 }
-__device__ __forceinline__ uint2 quantize(const uint32_t (&w)[4], float lift, float top) {
+// What the largest magnitude of a row makes of it.
+struct Span {
+  bool odd, none;
+  float lift, most, over, scale;  // over: about 1 / most
+};
+__device__ __forceinline__ Span span_of(uint32_t top) {
+  const float most = __uint_as_float(top);
+  Span r;
+  r.odd = top >= 0x7F800000u, r.none = r.odd || top == 0;
+  r.scale = r.odd ? __builtin_nanf("") : most / 127.f;
+  // (127 x and 1 / most are finite and normal; what it takes from small x is far below a half)
+  r.lift = most > 1e30f ? 0x1p-64f : most < 1e-30f ? 0x1p64f : 1.f;
+  r.most = most * r.lift;
+  r.over = __builtin_amdgcn_rcpf(r.most);
+  return r;
+}
+// The quotient's first guess is off by a few last places at most, so what is left of the dividend (of 15 bits, where guess
+// times divisor has 32) is exact, and one step with it (Markstein's) gives a half or an integer exactly and others to a
+// last place, far nearer than 2^-16.
+__device__ __forceinline__ uint2 quantize(const uint32_t (&w)[4], const Span& r) {
   uint32_t o[2] = {0, 0};
+  if (r.none) return make_uint2(0, 0);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float v = j & 1 ? bf16_hi(w[j >> 1]) : bf16_lo(w[j >> 1]);
-    o[j >> 2] |= (uint32_t)((int)rintf(127.f * (v * lift) / top) & 0xFF) << (8 * (j & 3));
+    const float x = 127.f * (v * r.lift), guess = x * r.over;
+    const float q = __builtin_fmaf(__builtin_fmaf(-guess, r.most, x), r.over, guess);
+    o[j >> 2] |= (uint32_t)((int)rintf(q) & 0xFF) << (8 * (j & 3));
   }
   return make_uint2(o[0], o[1]);
 }
@@ -105,10 +143,12 @@ __global__ __launch_bounds__(QUANT_NT) void quantize_kernel(const bf16_t* x, int
   x += row * xs;
   const int64_t place = HEAD ? head_row(row) : row;
   uint32_t kept[KEPT][4], top = 0;
+  load_chunks<KEPT, STEP>(x, cols, tid * 8, kept);
 #pragma unroll
-  for (int c = 0; c < KEPT; ++c) load_chunk(x, cols, c * STEP + tid * 8, kept[c]);
-#pragma unroll
-  for (int c = 0; c < KEPT; ++c) top = top_of(kept[c], top);
+  for (int c = 0; c < KEPT; ++c) {
+    cut(kept[c], c * STEP + tid * 8 < cols);
+    top = top_of(kept[c], top);
+  }
   for (int i = KEPT * STEP + tid * 8; i < cols; i += STEP) {
     uint32_t w[4];
     load_chunk(x, cols, i, w);
@@ -119,24 +159,20 @@ __global__ __launch_bounds__(QUANT_NT) void quantize_kernel(const bf16_t* x, int
   if (lane == 0) tops[wave] = top;
   __syncthreads();
   for (int w = 0; w < QUANT_NT / 64; ++w) top = max(top, tops[w]);
-  const bool odd = top >= 0x7F800000u;
-  float most = __uint_as_float(top);
+  const Span span = span_of(top);
   if (tid == 0) {
-    scales[row] = odd ? __builtin_nanf("") : most / 127.f;
-    if (status) status[row] = odd ? DSV41_STATUS_NONFINITE : 0;
+    scales[row] = span.scale;
+    if (status) status[row] = span.odd ? DSV41_STATUS_NONFINITE : 0;
   }
-  const bool none = odd || top == 0;
-  const float lift = most > 1e30f ? 0x1p-64f : 1.f;  // (127 x is finite; what it takes from small x is far below a half)
-  most *= lift;
 #pragma unroll
   for (int c = 0; c < KEPT; ++c) {
     const int i = c * STEP + tid * 8;
-    if (i < padded) *reinterpret_cast<uint2*>(q + byte_of(place, i, padded)) = none ? make_uint2(0, 0) : quantize(kept[c], lift, most);
+    if (i < padded) *reinterpret_cast<uint2*>(q + byte_of(place, i, padded)) = quantize(kept[c], span);
   }
   for (int i = KEPT * STEP + tid * 8; i < padded; i += STEP) {
     uint32_t w[4];
     load_chunk(x, cols, i, w);
-    *reinterpret_cast<uint2*>(q + byte_of(place, i, padded)) = none ? make_uint2(0, 0) : quantize(w, lift, most);
+    *reinterpret_cast<uint2*>(q + byte_of(place, i, padded)) = quantize(w, span);
   }
 }
 
@@ -144,6 +180,8 @@ __global__ __launch_bounds__(QUANT_NT) void quantize_kernel(const bf16_t* x, int
 // waves of a workgroup, steps of theirs in registers, workgroups of a CU: of one token, 2048 -> 151936 and 7168 -> 129280,
 // 52 and 151 us; eight waves 54 and 155, two (four workgroups) 57 and 153, five steps ahead 60 and 152.
 constexpr int SPLIT = 4, DEPTH = 4, PER_CU = 2;
+// tokens that head_kernel quantizes itself (of eight: one token 48.9 us for 47.7), their columns, LDS bytes that shift banks
+constexpr int OWN = 4, OWN_COLUMNS = 64 * SPLIT * 8, OWN_PAD = 64;
 
 struct Params {
   const int8_t* w;  // tiles of the head
@@ -153,6 +191,10 @@ struct Params {
   int N, V, K;      // K: a multiple of 128
   void* out;
   int64_t os;
+  const bf16_t* x;  // the tokens themselves, which head_kernel quantizes where they are few
+  int64_t xs;
+  int cols;
+  int32_t* status;
   int n_tb, ranges, w1;  // gemm_kernel's blocks of tokens, the parts its rows are cut into, and its W1
 };
 
@@ -228,10 +270,14 @@ struct Step {
 
 // SPLIT waves share the columns of a group, every SPLIT-th k-step each; a workgroup takes group after group, with
 // DEPTH - 1 steps of each wave on their way from memory throughout.
-template <typename T>
+// SELF: every workgroup quantizes the tokens itself, into LDS, while its first weights are on their way.
+template <typename T, bool SELF>
 __global__ __launch_bounds__(64 * SPLIT, SPLIT * PER_CU / 4) void head_kernel(Params p, bool wide) {
   __shared__ intx4 parts[SPLIT - 1][4][64];
   __shared__ float scales[GROUP];
+  __shared__ __align__(16) int8_t own[SELF ? OWN * (OWN_COLUMNS + OWN_PAD) : 16];
+  __shared__ uint32_t tops[OWN][SPLIT];
+  __shared__ float own_scales[OWN];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, quad = lane >> 4;
   const int steps = p.K / 64, turns = (steps + SPLIT * DEPTH - 1) / (SPLIT * DEPTH) * DEPTH, groups = (p.V + GROUP - 1) / GROUP;
   T* out = static_cast<T*>(p.out) + r16 * p.os;
@@ -239,23 +285,57 @@ __global__ __launch_bounds__(64 * SPLIT, SPLIT * PER_CU / 4) void head_kernel(Pa
   Step f[DEPTH];
   int at = wave, left = turns, ahead = blockIdx.x;  // the step to load, those left of its group, the group
   const int8_t* w = p.w + (int64_t)ahead * GROUP * p.K;  // (the same in all lanes, which add theirs in 32 bits)
-  // (a step that is none reads the first bytes of q, which all caches hold: loads under a condition cost registers)
+  // (a step that is none reads the first bytes of w, which caches hold: loads under a condition cost registers)
   auto load = [&](Step& s) {
     const bool some = ahead < groups && at < steps;
-    const int8_t *wa = some ? w + at * TILE : p.q, *qa = p.q + (some ? at * TILE : 0);
+    const int8_t* wa = some ? w + at * TILE : p.w;
     const int64_t tile_row = some ? (int64_t)16 * p.K : 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) s.a[i] = __builtin_nontemporal_load(reinterpret_cast<const intx4*>(wa + i * tile_row) + lane);
-    s.b = reinterpret_cast<const intx4*>(qa)[lane];
+    if (!SELF) s.b = reinterpret_cast<const intx4*>(p.q + (some ? at * TILE : 0))[lane];
     at += SPLIT;
     if (--left == 0) {
       at = wave, left = turns, ahead += gridDim.x;
       w += (int64_t)gridDim.x * GROUP * p.K;
     }
   };
+  // a thread has 8 columns of each token (those past the last token are its again)
+  const int token = min(r16, p.N - 1);
+  uint32_t kept[OWN][4];
+  if (SELF) {
+#pragma unroll
+    for (int n = 0; n < OWN; ++n) rows::load16<false>(p.x + min(n, p.N - 1) * p.xs + min(tid * 8, p.cols - 8), kept[n]);
+  }
 #pragma unroll
   for (int d = 0; d < DEPTH - 1; ++d) load(f[d]);
-  const float ss = p.ss[min(r16, p.N - 1)];
+  if (SELF) {
+    uint32_t top[OWN];
+#pragma unroll
+    for (int n = 0; n < OWN; ++n) {
+      cut(kept[n], tid * 8 < p.cols);
+      top[n] = top_of(kept[n], 0);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+#pragma unroll
+      for (int n = 0; n < OWN; ++n) top[n] = max(top[n], (uint32_t)__shfl_xor((int)top[n], o));
+    if (lane == 0) {
+#pragma unroll
+      for (int n = 0; n < OWN; ++n) tops[n][wave] = top[n];
+    }
+    rows::lds_barrier();
+#pragma unroll
+    for (int n = 0; n < OWN; ++n) {
+      const Span span = span_of(max(max(tops[n][0], tops[n][1]), max(tops[n][2], tops[n][3])));
+      if (tid * 8 < p.K) *reinterpret_cast<uint2*>(own + n * (OWN_COLUMNS + OWN_PAD) + tid * 8) = quantize(kept[n], span);
+      if (tid == 0) {
+        own_scales[n] = span.scale;
+        if (p.status && blockIdx.x == 0 && n < p.N) p.status[n] = span.odd ? DSV41_STATUS_NONFINITE : 0;
+      }
+    }
+    rows::lds_barrier();
+  }
+  const float ss = SELF ? own_scales[token] : p.ss[token];
   for (int group = blockIdx.x; group < groups; group += gridDim.x) {
     // (read at the end, it would have the wave wait for all steps on their way)
     const float t = p.ts[min(group * GROUP + lane, p.V - 1)];
@@ -263,9 +343,11 @@ __global__ __launch_bounds__(64 * SPLIT, SPLIT * PER_CU / 4) void head_kernel(Pa
 #pragma unroll
       for (int d = 0; d < DEPTH; ++d) {
         load(f[(d + DEPTH - 1) % DEPTH]);
-        if (wave + (turn + d) * SPLIT < steps) {
+        const int step = wave + (turn + d) * SPLIT;
+        if (step < steps) {
+          const intx4 b = SELF ? *reinterpret_cast<const intx4*>(own + token * (OWN_COLUMNS + OWN_PAD) + step * 64 + quad * 16) : f[d].b;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[d].a[i], f[d].b, acc[i], 0, 0, 0);
+          for (int i = 0; i < 4; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[d].a[i], b, acc[i], 0, 0, 0);
         }
       }
     }
@@ -614,11 +696,17 @@ size_t scales_at(const dsv41_int_head_desc* d) { return (size_t)((d->n_tokens + 
 // and 110, 1100 tokens 330 and 344, 4096 tokens 1136 and 1221.
 constexpr double TILE_COST[4] = {0, 0.85, 1.0, 1.2};
 
+// Whether head_kernel quantizes the tokens: 2048 -> 151936, one and four tokens 47.7 and 48.8 us, 50.4 and 51.7 by a launch
+// before it; of 7168 -> 129280 one token, whose parts a thread would hold together, 136.4 and 134.9.
+bool own_quantization(int n, int cols) { return n <= OWN && cols <= OWN_COLUMNS && cols % 8 == 0; }
+
 // As many workgroups as fit on the GPU together take the same number of groups each.
 template <typename T>
 void launch_few(const Params& p, bool wide, hipStream_t s) {
   const int groups = (p.V + GROUP - 1) / GROUP, slots = PER_CU * CU_COUNT, rounds = (groups + slots - 1) / slots;
-  hipLaunchKernelGGL(head_kernel<T>, dim3((groups + rounds - 1) / rounds), dim3(64 * SPLIT), 0, s, p, wide);
+  const dim3 grid((groups + rounds - 1) / rounds);
+  if (own_quantization(p.N, p.cols)) hipLaunchKernelGGL((head_kernel<T, true>), grid, dim3(64 * SPLIT), 0, s, p, wide);
+  else hipLaunchKernelGGL((head_kernel<T, false>), grid, dim3(64 * SPLIT), 0, s, p, wide);
 }
 template <typename T, int NB>
 void launch_ring(Params p, bool wide, hipStream_t s) {
@@ -691,13 +779,18 @@ extern "C" int dsv41_int_head_run(const dsv41_int_head_desc* d, void* workspace,
   float* ss = reinterpret_cast<float*>(q + at);
   const int K = padded_of(d->hidden);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(quantize_kernel<false>, quantize_grid(d->n_tokens), dim3(QUANT_NT), 0, s,
-                     static_cast<const bf16_t*>(d->x), d->x_row_stride, d->n_tokens, d->hidden, q, K, ss, d->out_status);
+  if (!own_quantization(d->n_tokens, d->hidden))
+    hipLaunchKernelGGL(quantize_kernel<false>, quantize_grid(d->n_tokens), dim3(QUANT_NT), 0, s,
+                       static_cast<const bf16_t*>(d->x), d->x_row_stride, d->n_tokens, d->hidden, q, K, ss, d->out_status);
   Params p{};
   p.w = d->w;
   p.ts = d->scales;
   p.q = q;
   p.ss = ss;
+  p.x = static_cast<const bf16_t*>(d->x);
+  p.xs = d->x_row_stride;
+  p.cols = d->hidden;
+  p.status = d->out_status;
   p.N = d->n_tokens;
   p.V = d->vocab;
   p.K = K;
