@@ -92,6 +92,23 @@ __global__ __launch_bounds__(COPY_NT) void copy_kernel(CopyParams p) {
   const T* w = static_cast<const T*>(p.w) + (some ? id * p.ws : 0);
   T* out = static_cast<T*>(p.out) + n * p.os;
   constexpr int U = 4;
+  if (p.H % G == 0) {  // U loads on their way together: a condition around a load has the wave wait for it
+    for (int i0 = lane * G; i0 < p.H; i0 += U * p.lanes * G) {
+      uint32_t raw[U][4];
+#pragma unroll
+      for (int u = 0; u < U; ++u) rows::load16<false>(w + min(i0 + u * p.lanes * G, p.H - G), raw[u]);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * p.lanes * G;
+        float v[G];
+        Elem<T>::unpack(raw[u], v);
+#pragma unroll
+        for (int j = 0; j < G; ++j) v[j] = some ? v[j] * p.scale : instead;
+        if (i < p.H) rows::store_full(out + i, 0, v);
+      }
+    }
+    return;
+  }
   for (int i0 = lane * G; i0 < p.H; i0 += U * p.lanes * G) {
     float v[U][G];
 #pragma unroll
