@@ -74,6 +74,25 @@ def test_gradient(n, h, V, kind, tg, to):
     assert torch.equal(onto.cpu()[:, 0], base[:, 0]) and torch.equal(onto.cpu()[:, h + 1:], base[:, h + 1:])
 
 
+@pytest.mark.parametrize("n,h,V", [(4000, 9, 140000), (2500, 20, 131072), (6000, 8, 70000), (5000, 4, 300)])
+@pytest.mark.parametrize("kind", ["zipf", "few", "two"])
+def test_gradient_of_ids_close_together(n, h, V, kind):
+    # most of the batch in one range of ids: many of them among 64 neighbours, few, and two in turn; integers, so exact
+    g = torch.Generator().manual_seed(n)
+    if kind == "zipf":
+        ids = _ids("zipf", n, V, g)
+    elif kind == "few":
+        ids = torch.randint(0, 5, (n,), generator=g) * 7 + V - 40
+    else:
+        ids = torch.arange(n) % 2 * 3 + 100
+    grad = torch.randint(-8, 9, (n, h), generator=g).float()
+    want = torch.zeros(V, h).index_add_(0, ids.clamp_min(0), torch.where((ids >= 0)[:, None], grad, 0.0))
+    assert torch.equal(token_embedding_backward(grad.to(DEV), ids.to(DEV), V).cpu(), want)
+    onto = torch.ones(V, h, dtype=torch.float32, device=DEV)
+    token_embedding_backward(grad.to(DEV), ids.to(DEV), out=onto)
+    assert torch.equal(onto.cpu(), want + 1)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("n,h,V", CASES)
 def test_rows(n, h, V, dtype):

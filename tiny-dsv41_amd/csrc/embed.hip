@@ -17,13 +17,14 @@
 //                 of the same launch write zeros where no token is, which is most of a dense gradient's time.
 //   join_kernel   the partial rows of an id that reaches over chunks, in their order.
 // Bound by memory: a gradient of 151851 x 2048 in fp32 from 1000 tokens takes 7 + 177 + 4 us, 7.0 TB/s of zeros
-// (by torch's fill 6.9); 129280 x 7168 in bf16 from 16384 tokens 14 + 339 + 14, 6.1 TB/s of zeros, gradients and partial
-// rows.  Rows of the table, 16384 x 7168 in bf16, take 64 us: 7.2 TB/s of result and rows, of which frequent tokens' come
+// (by torch's fill 6.9); 129280 x 7168 in bf16 from 16384 tokens 14 + 342 + 11, 6.0 TB/s of zeros, gradients and partial
+// rows.  Rows of the table, 16384 x 7168 in bf16, take 59 us: 7.9 TB/s of result and rows, of which frequent tokens' come
 // from caches.
 
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "row_scan.h"
 #include "status.h"
@@ -36,7 +37,8 @@ using rows::Elem;
 
 constexpr int COPY_NT = 256;
 constexpr int SORT_NT = 1024, SORT_WAVES = SORT_NT / 64;
-constexpr int RANGE = 512;    // ids of a sorting workgroup, at most
+constexpr int RANGE_BITS = 9, RANGE = 1 << RANGE_BITS;  // ids of a sorting workgroup, at most
+constexpr int ONE_BY_ONE = 3;  // of the ids among 64 tokens, of which few are the range's
 constexpr int SUM_NT = 256, SUM_WAVES = SUM_NT / 64;
 constexpr int CHUNK = 32;     // sorted positions of a summing wave
 // A zeroing workgroup has about this many bytes, and those of an XCD a contiguous part of the table: 1.2 GB in 191 us,
@@ -231,8 +233,10 @@ __global__ __launch_bounds__(SORT_NT) void sort_kernel(GradParams p) {
       const uint64_t at = (uint64_t)(ids[k] - r0);
       const bool in = ids[k] >= 0 && at < width;
       uint64_t left = __ballot(in);
-      while (left) {
-        // the tokens of these 64 that share the first one's id take consecutive places
+      // the tokens of these 64 that share an id take consecutive places: the first few ids one by one, as most ranges have
+      // few tokens, or many of one
+      const int turns = __popcll(left) > 16 ? 1 : ONE_BY_ONE;
+      for (int t = 0; t < turns && left; ++t) {
         const int first = __builtin_ctzll(left);
         const uint32_t which = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)at, first);
         const uint64_t same = __ballot(in && (uint32_t)at == which) & left;
@@ -246,19 +250,39 @@ __global__ __launch_bounds__(SORT_NT) void sort_kernel(GradParams p) {
         }
         left &= ~same;
       }
+      if (left == 0) continue;
+      // the others at once, found bit by bit of their id's place: a range of frequent tokens' ids, which often are the lowest,
+      // has half of a batch (16384 tokens, ids log-uniform below 129280: 84 us one by one, about 20 so; alike in all ranges
+      // 14, and 20 without any one by one)
+      const bool mine = left >> lane & 1;
+      uint64_t same = left;
+#pragma unroll
+      for (int bit = 0; bit < RANGE_BITS; ++bit) {
+        const uint64_t set = __ballot(mine && (at >> bit & 1));
+        same &= at >> bit & 1 ? set : ~set;
+      }
+      const int rank = __popcll(same & ((1ull << lane) - 1)), first = mine ? __builtin_ctzll(same) : lane;
+      uint32_t s = 0;
+      if (mine && rank == 0) s = atomicAdd(&hist[wave][at], (uint32_t)__popcll(same));
+      s = (uint32_t)__shfl((int)s, first);
+      if (mine) {
+        p.place[s + rank] = i;
+        p.name[s + rank] = (int32_t)ids[k];
+      }
     }
   }
 }
 
-// G columns of a finished row, of which the first n exist
-template <typename T, bool ONTO, int G>
-__device__ __forceinline__ void finish(T* out, int n, const float (&s)[G], float scale) {
+// G columns of a finished row, of which the first n exist; EARLY: `old` holds what was there.
+template <typename T, bool ONTO, bool EARLY, int G>
+__device__ __forceinline__ void finish(T* out, int n, const float (&s)[G], float scale, const uint32_t (&old)[4]) {
   constexpr int GO = Elem<T>::VEC;
   n = min(n, G);
 #pragma unroll
   for (int b = 0; b < G; b += GO) {
     float v[GO];
-    if (ONTO) load_group(out + b, n - b, v);
+    if (EARLY) Elem<T>::unpack(old, v);
+    else if (ONTO) load_group(out + b, n - b, v);
 #pragma unroll
     for (int j = 0; j < GO; ++j) {
       const float sum = b + j < G ? s[b + j < G ? b + j : 0] * scale : 0.f;
@@ -310,14 +334,25 @@ __global__ __launch_bounds__(SUM_NT) void sum_kernel(GradParams p) {
 #pragma unroll
   for (int j = 0; j < G; ++j) s[j] = 0.f;
   constexpr int U = 16;  // rows in flight
+  // Onto a gradient of the same type, finished ids' rows are read beside them: 16384 bf16 rows of 7168 take 172 us,
+  // 185 where each waits for its own.
+  constexpr bool EARLY = ONTO && std::is_same<TG, TO>::value;
 #pragma unroll
   for (int c = 0; c < CHUNK; c += U) {
-    uint32_t raw[U][4];
+    uint32_t raw[U][4], old[EARLY ? U : 1][4];
     if (c >= count) break;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t row = __builtin_amdgcn_readlane(place, min(c + u, count - 1));
       if (n > 0) load_raw(g + row * p.gs, n, raw[u]);
+    }
+    if constexpr (EARLY) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (c + u < count && (ends >> (c + u) & 1)) {
+          const int64_t id = __builtin_amdgcn_readlane(name, c + u);
+          if (n > 0) load_raw(out + id * p.os + col, n, old[u]);
+        }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -336,7 +371,7 @@ __global__ __launch_bounds__(SUM_NT) void sum_kernel(GradParams p) {
             if (j < n) part[j] = s[j];
         } else {
           const int64_t id = __builtin_amdgcn_readlane(name, c + u);
-          finish<TO, ONTO, G>(out + id * p.os + col, n, s, p.scale);
+          finish<TO, ONTO, EARLY>(out + id * p.os + col, n, s, p.scale, old[EARLY ? u : 0]);
         }
       }
       reaches_in = false;
@@ -359,25 +394,32 @@ __global__ __launch_bounds__(JOIN_NT) void join_kernel(GradParams p) {
   const int col = (strip * JOIN_NT + threadIdx.x) * G;
   if (col >= p.H) return;
   const int n = min(G, p.H - col);
-  float s[G] = {0.f, 0.f, 0.f, 0.f};
-  const float* part = p.part + ((int64_t)chunk * 2 + 1) * p.H + col;
-  for (int j = 0; j < n; ++j) s[j] = part[j];
-  // the chunks that the id reaches into: names and rows of U of them at a time
-  constexpr int U = 8;
-  for (int c = chunk + 1;; c += U) {
-    int more = 0;
+  const bool whole = p.H % G == 0;  // groups of 16 bytes, all of them
+  auto row = [&](int64_t r, float (&v)[G]) {
+    const float* part = p.part + r * p.H + col;
+    if (whole) {
+      const float4 w = *reinterpret_cast<const float4*>(part);
+      v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
+    } else {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int at = (c + u) * CHUNK;
-      more += more == u && at < total && p.name[min(at, total - 1)] == id;
+      for (int j = 0; j < G; ++j) v[j] = part[min(j, n - 1)];
     }
+  };
+  float s[G];
+  row((int64_t)chunk * 2 + 1, s);
+  // the chunks that the id reaches into: names and rows of U of them at a time
+  constexpr int U = 16;
+  for (int c = chunk + 1;; c += U) {
+    int name[U], more = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) name[u] = p.name[min((c + u) * CHUNK, total - 1)];
+#pragma unroll
+    for (int u = 0; u < U; ++u) more += more == u && (c + u) * CHUNK < total && name[u] == id;
     float v[U][G];
+    // (most ids reach into few)
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (u < more) {
-#pragma unroll
-        for (int j = 0; j < G; ++j) v[u][j] = j < n ? p.part[(int64_t)(c + u) * 2 * p.H + col + j] : 0.f;
-      }
+      if (u < more) row((int64_t)(c + u) * 2, v[u]);
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (u < more) {
