@@ -21,8 +21,8 @@
 //
 // Slices begin at memory lines of the result, so rows of an odd vocabulary are written by whole lines: 500 bf16 rows of
 // 151851 copied in 51 us (5.9 TB/s of read and write), as many of 151936 in 53.  2048 fp32 rows: 445 us (5.6 TB/s),
-// with masks 471, with histories of 4096 500; bf16 210, 226 and 293.  256 to 1024 threads and slices of 8192 to 16384
-// ids: 512 and 8192 are the best or within 3% (1024 and 16384: 2048 fp32 rows with histories 506, 256 and 8192: 778).
+// with histories of 4096 452.  256 to 1024 threads and slices of 8192 to 16384 ids, before the loads of a slice went
+// together: 512 and 8192 the best or within 3% (2048 fp32 rows with histories 477; 1024 and 16384: 506, 256 and 8192: 778).
 // What bounds it: memory, and beside long histories of bf16 rows the instructions of reading the lists, once a slice
 // (2048 ids cost 500 rows 12 us).
 
@@ -285,13 +285,10 @@ __device__ __forceinline__ Row row_of(const Params& p, int row) {
 
 // Which elements of a group at id i there are, and which of them the row's mask allows.
 template <typename T, bool MASK>
-__device__ __forceinline__ void group_at(const Params& p, const Row& r, int i, bool inside, uint32_t& there, uint32_t& allowed) {
+__device__ __forceinline__ void group_at(const Params& p, const Row& r, int i, uint32_t& there, uint32_t& allowed) {
   constexpr int G = Elem<T>::VEC;
-  there = ALL<T>;
-  if (!inside) {
-    const int lo = max(-i, 0), hi = min(p.V - i, G);  // elements [lo, hi)
-    there = lo < hi ? (ALL<T> << lo) & (ALL<T> >> (G - hi)) : 0u;
-  }
+  const int lo = max(-i, 0), hi = min(p.V - i, G);  // elements [lo, hi)
+  there = lo < hi ? (ALL<T> << lo) & (ALL<T> >> (G - hi)) : 0u;
   allowed = r.bad ? 0u : there;
   if (MASK && r.mask && there) {
     const int k = max(i, 0) >> 5, last = (p.V - 1) >> 5;
@@ -299,19 +296,60 @@ __device__ __forceinline__ void group_at(const Params& p, const Row& r, int i, b
     allowed &= i >= 0 ? (uint32_t)(both >> (i & 31)) : (uint32_t)(both << -i);
   }
 }
+// The same for a thread's groups from id i on.  `inside`: all of the slice's ids exist.  Its loads go together then, here and in
+// load_groups: a condition that differs from lane to lane has the wave wait for the loads under it.
+template <typename T, bool MASK, int U>
+__device__ __forceinline__ void groups_at(const Params& p, const Row& r, int i, bool inside, uint32_t (&there)[U], uint32_t (&allowed)[U]) {
+  constexpr int STEP = NT * Elem<T>::VEC;
+  if (!inside) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) group_at<T, MASK>(p, r, i + u * STEP, there[u], allowed[u]);
+    return;
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) there[u] = ALL<T>, allowed[u] = r.bad ? 0u : ALL<T>;
+  if (MASK && r.mask) {
+    uint32_t lo[U], hi[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = (i + u * STEP) >> 5;
+      lo[u] = r.mask[k], hi[u] = r.mask[min(k + 1, (p.V - 1) >> 5)];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) allowed[u] &= (uint32_t)(((uint64_t)hi[u] << 32 | lo[u]) >> ((i + u * STEP) & 31));
+  }
+}
+// A thread's groups that are wanted, from x at the slice's begin (others hold anything).
+template <typename T, int U>
+__device__ __forceinline__ void load_groups(const T* x, bool inside, const uint32_t (&there)[U], const uint32_t (&want)[U], Group (&v)[U]) {
+  constexpr int G = Elem<T>::VEC;
+  if (inside) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) rows::load16<false>(x + (want[u] ? (u * NT + (int)threadIdx.x) * G : 0), v[u].w);
+  } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (want[u]) load_group(x + (u * NT + (int)threadIdx.x) * G, there[u], v[u]);
+  }
+}
 
 // `batch(first, ids)` for every AHEAD entries of a thread; the first ones were loaded ahead of the slice itself, as loads come back
 // in order.
+// (EACH: loads that wait for one another.  In the gradient and with short words they are better so, 500 bf16 rows by 2 us
+// each; 2048 fp32 rows take 459 us that way and 452 with all of them together.)
+template <bool EACH>
 __device__ __forceinline__ void load_ahead(const Row& r, int j0, uint2 (&ids)[AHEAD]) {
 #pragma unroll
-  for (int k = 0; k < AHEAD; ++k)
-    if (j0 + k * NT < r.len) ids[k] = r.h[j0 + k * NT];
+  for (int k = 0; k < AHEAD; ++k) {
+    const int j = j0 + k * NT + (int)threadIdx.x;
+    if (EACH ? j < r.len : j0 + k * NT < r.len) ids[k] = r.h[min(j, r.len - 1)];
+  }
 }
-template <class F>
+template <bool EACH, class F>
 __device__ __forceinline__ void for_history(const Row& r, uint2 (&ahead)[AHEAD], F batch) {
   batch((int)threadIdx.x, ahead);
   for (int j0 = AHEAD * NT; j0 < r.len; j0 += AHEAD * NT) {
-    load_ahead(r, j0 + (int)threadIdx.x, ahead);
+    load_ahead<EACH>(r, j0, ahead);
     batch(j0 + (int)threadIdx.x, ahead);
   }
 }
@@ -335,10 +373,9 @@ __global__ __launch_bounds__(NT, 8) void process_kernel(Params p) {
   int bits = r.bits;  // status bits that this thread met
 
   uint2 ahead[AHEAD];
-  if (LISTS) load_ahead(r, tid, ahead);
+  if (LISTS) load_ahead<SHORT>(r, 0, ahead);
   uint32_t there[U], allowed[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) group_at<T, MASK>(p, r, s.begin + (u * NT + tid) * G, inside, there[u], allowed[u]);
+  groups_at<T, MASK, U>(p, r, s.begin + tid * G, inside, there, allowed);
   if (listed) {
     uint4* w4 = reinterpret_cast<uint4*>(shared);
 #pragma unroll
@@ -347,11 +384,7 @@ __global__ __launch_bounds__(NT, 8) void process_kernel(Params p) {
   }
   // what is read: the groups with an allowed element
   Group v[U];
-  if constexpr (!INPLACE) {
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (allowed[u]) load_group(x + (u * NT + tid) * G, there[u], v[u]);
-  }
+  if constexpr (!INPLACE) load_groups<T, U>(x, inside, there, allowed, v);
 
   if (listed) {
     const bool report = p.status && s.number == 0;
@@ -369,7 +402,7 @@ __global__ __launch_bounds__(NT, 8) void process_kernel(Params p) {
       }
       rows::lds_barrier();
     }
-    for_history(r, ahead, [&](int j0, const uint2 (&ids)[AHEAD]) {
+    for_history<SHORT>(r, ahead, [&](int j0, const uint2 (&ids)[AHEAD]) {
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
         const int j = j0 + k * NT;
@@ -442,22 +475,19 @@ __global__ __launch_bounds__(NT, 8) void process_grad_kernel(Params p) {
   const bool listed = LISTS && r.len > 0, inside = s.begin >= 0 && s.begin + IDS <= p.V;
 
   uint2 ahead[AHEAD];
-  if (LISTS) load_ahead(r, tid, ahead);
+  if (LISTS) load_ahead<true>(r, 0, ahead);
   uint32_t there[U], allowed[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) group_at<T, MASK>(p, r, s.begin + (u * NT + tid) * G, inside, there[u], allowed[u]);
+  groups_at<T, MASK, U>(p, r, s.begin + tid * G, inside, there, allowed);
   if (listed) {
     static_assert(IDS / 32 <= NT);
     if (tid < IDS / 32) in_history[tid] = positive[tid] = 0;
     rows::lds_barrier();
   }
   Group v[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-    if (allowed[u]) load_group(g + (u * NT + tid) * G, there[u], v[u]);
+  load_groups<T, U>(g, inside, there, allowed, v);
 
   if (listed) {
-    for_history(r, ahead, [&](int j0, const uint2 (&ids)[AHEAD]) {
+    for_history<true>(r, ahead, [&](int j0, const uint2 (&ids)[AHEAD]) {
       float logit[AHEAD];
       uint32_t at[AHEAD];
       bool here[AHEAD];
