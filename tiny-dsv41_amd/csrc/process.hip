@@ -20,8 +20,8 @@
 // read for the history's ids while the gradient's own are on their way.
 //
 // Slices begin at memory lines of the result, so rows of an odd vocabulary are written by whole lines: 500 bf16 rows of
-// 151851 copied in 51 us (5.9 TB/s of read and write), as many of 151936 in 53.  2048 fp32 rows: 445 us (5.6 TB/s),
-// with histories of 4096 452.  256 to 1024 threads and slices of 8192 to 16384 ids, before the loads of a slice went
+// 151851 copied in 51 us (5.9 TB/s of read and write), as many of 151936 in 53.  2048 fp32 rows: 434 us (5.7 TB/s),
+// with masks 443, with histories of 4096 464; bf16 214, 219 and 262.  256 to 1024 threads and slices of 8192 to 16384 ids, before the loads of a slice went
 // together: 512 and 8192 the best or within 3% (2048 fp32 rows with histories 477; 1024 and 16384: 506, 256 and 8192: 778).
 // What bounds it: memory, and beside long histories of bf16 rows the instructions of reading the lists, once a slice
 // (2048 ids cost 500 rows 12 us).
@@ -560,8 +560,8 @@ void launch(Params p, hipStream_t s) {
   hipLaunchKernelGGL((process_kernel<T, LISTS, MASK, INPLACE, SHORT>), grid, dim3(NT), lds, s, p);
 }
 // Words of 16 bits take what they hold of bf16 rows' lists, in batches that fill the GPU with the longer slices too.  With
-// histories of 2048 and 4096 and in place with 2048, us, 32 and 16 bits: 2048 rows 289 and 266, 337 and 293, 280 and 230; 500
-// rows 76 and 72, 89 and 80, 60 and 51; 200 rows 28.7 and 28.3, 33.8 and 32.1, 27.4 and 24.5.
+// histories of 2048 and 4096 and in place with 2048, us, 32 and 16 bits: 2048 rows 244 and 236, 286 and 262, 257 and 226; 500
+// rows 66 and 64, 78 and 71, 57 and 50; 200 rows 27.7 and 27.6, 32.4 and 30.7, 27.2 and 24.8.
 template <typename T, bool MASK, bool INPLACE>
 void launch_lists(const Params& p, hipStream_t s) {
   if constexpr (sizeof(T) == 2)
