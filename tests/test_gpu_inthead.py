@@ -97,6 +97,28 @@ def test_tokens_quantized_by_the_product(n, h, dtype):
     _many_rows(n, h, 33000 + n, dtype)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,h,v", [(17, 64, 70001), (40, 128, 70001), (64, 100, 200), (65, 128, 70001), (128, 127, 140001)])
+def test_scales_that_come_from_memory(n, h, v, dtype):
+    # rows of one stage: the call before leaves another head's scales where this one's come to, and they come late, as no
+    # cache holds them
+    g = torch.Generator(DEV).manual_seed(n + h + v)
+    x = _inputs(n, h, 1)[0]
+    q, s = _quantized(x)
+    w = torch.randint(-127, 128, (v, h), generator=g, dtype=torch.int8, device=DEV)
+    sums = torch.cat([q.to(DEV) @ part.double().t() for part in w.split(8192)], 1).float() * s.to(DEV)[:, None]
+    scales = [torch.rand(v, generator=g, device=DEV) + k for k in (1, 100)]
+    heads = [Int8Head.from_quantized(w, t) for t in scales]
+    x = x.to(DEV)
+    junk = torch.empty(1 << 30, dtype=torch.int8, device=DEV)
+    outs = []
+    for k in (0, 1, 0):
+        junk.fill_(k)
+        outs.append((k, head_logits(x, heads[k], dtype=dtype, check=False)))
+    for k, got in outs:
+        assert torch.equal(got, (sums * scales[k]).to(dtype))
+
+
 def _many_rows(n, h, v, dtype):
     x = _inputs(n, h, 1)[0]
     w = torch.randint(-127, 128, (v, h), generator=torch.Generator(DEV).manual_seed(n + h + v), dtype=torch.int8, device=DEV)

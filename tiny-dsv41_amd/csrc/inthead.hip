@@ -27,6 +27,7 @@
 #include <type_traits>
 
 #include "mfma_tile.h"
+#include "ring_rule.h"
 #include "row_scan.h"
 
 namespace dsv41 {
@@ -376,7 +377,6 @@ __global__ __launch_bounds__(64 * SPLIT, SPLIT * PER_CU / 4) void head_kernel(Pa
 // A workgroup takes a run of groups, up to four at a time, against all tokens, 32 NB at most: wave (wv, wt) group wv's 64 rows
 // and half of the tokens.  Stages of 128 columns go straight to a ring of RING in LDS, RING - 1 of them on their way from
 // memory throughout; one barrier a stage says that it has come and that the one before it is free.
-constexpr int RING = 3;  // (32 tokens a stage, and four stages: no faster)
 // load_lds of what is read once: 7168 -> 129280, 128 tokens 216 us without the hint, 197 with it
 __device__ __forceinline__ void load_lds_once(v4i rs, uint32_t voff, uint32_t lds_addr) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen nt lds" ::"v"(voff), "s"(rs),
@@ -445,7 +445,7 @@ __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) v
 #pragma unroll
       for (int j = 0; j < NB; ++j) acc[i][j] = intx4{0, 0, 0, 0};
     for (int k = 0; k < nst; ++k) {
-      wait_loads<(RING - 2) * LOADS>();
+      wait_loads<stage_wait(LOADS)>();
       barrier();
       if (k == 0) load_lds(srs, (uint32_t)(g * GROUP * 4 + lane * 16), lds0 + (uint32_t)(RING * STAGE + wid * BM * 4));
       load_stage();
@@ -466,7 +466,9 @@ __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) v
       }
       at = at == (RING - 1) * STAGE ? 0 : at + STAGE;
     }
-    if (nst < RING) wait_loads<(RING - 1) * LOADS>();  // (longer rows have waited for the scales by now)
+    // (longer rows have waited for the scales by now)
+    static_assert(scales_wait(2, LOADS) < 0);
+    if (nst == 1) wait_loads<scales_wait(1, LOADS)>();
     if (some) {
 #pragma unroll
       for (int j = 0; j < NB; ++j) {
