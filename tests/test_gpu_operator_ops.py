@@ -186,3 +186,35 @@ def test_calls_on_two_streams_at_once():
     torch.cuda.synchronize()
     for i, o in outs:
         assert torch.equal(o.nan_to_num(), want[i].nan_to_num())
+
+
+CONSTANTS = ["repetition_penalties", "presence_penalties", "frequency_penalties", "bias"]
+
+
+def _op_of(x, **named):
+    a = dict(history=torch.zeros(2, 4, dtype=torch.int64), bias_ids=torch.zeros(3, dtype=torch.int64), bias=torch.zeros(3))
+    a = {k: v.to(x.device) for k, v in a.items()} | named
+    return OPS.process_logits(x, a["history"], None, None, 1.0, 0.0, 0.0, *(a.get(k) for k in CONSTANTS[:3]), a["bias_ids"], a["bias"],
+                              None, None, 0.0)
+
+
+def _refuses_gradients_of_constants(device):
+    # process_logits refuses them too: the op has no gradient to give
+    x = torch.zeros(2, 40, device=device)
+    for name in CONSTANTS:
+        t = torch.ones(3 if name == "bias" else 2, device=device, requires_grad=True)
+        for logits in (x, x.clone().requires_grad_()):
+            with pytest.raises(NotImplementedError, match=f"{name} has no gradient"):
+                _op_of(logits, **{name: t})
+            assert _op_of(logits, **{name: t.detach()})[0].requires_grad == logits.requires_grad
+            with torch.no_grad():
+                assert not _op_of(logits, **{name: t})[0].requires_grad
+
+
+def test_gradients_of_constants_are_refused_in_tracing():
+    _refuses_gradients_of_constants("meta")
+
+
+@pytest.mark.gpu
+def test_gradients_of_constants_are_refused():
+    _refuses_gradients_of_constants(DEV)

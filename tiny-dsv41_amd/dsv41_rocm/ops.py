@@ -242,7 +242,14 @@ def _process_logits_fake(logits, *arguments):
             torch.empty(logits.shape[0], dtype=torch.int32, device=logits.device))
 
 
+_PROCESS_CONSTANTS = {7: "repetition_penalties", 8: "presence_penalties", 9: "frequency_penalties", 11: "bias"}
+
+
 def _process_logits_setup(ctx, inputs, output):
+    # (inside the op no gradient is recorded, so it cannot tell)
+    for i, name in _PROCESS_CONSTANTS.items():
+        if ctx.needs_input_grad[i]:
+            raise NotImplementedError(f"{name} has no gradient: detach it")
     tensors = [t if isinstance(t, torch.Tensor) else None for t in inputs]
     ctx.save_for_backward(*tensors)
     ctx.numbers = [None if isinstance(t, torch.Tensor) else t for t in inputs]
