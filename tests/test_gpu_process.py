@@ -479,3 +479,36 @@ def test_longest_lists_of_bf16_rows():
     want = x.float()
     want[0, 8999] = want[0, 8999] - 524287.0
     assert torch.equal(process_logits(x, history=h, frequency_penalty=1.0), want.bfloat16())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("hist", [None, 0])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("rows", [4, 1030])
+def test_penalties_of_rows_without_a_history(dtype, hist, masked, rows):
+    # looked at all the same: the row of an invalid one holds NaN, its gradient too, and a checked call raises
+    V = 8200
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    x = torch.randn(rows, V, generator=g, device=DEV).to(dtype)
+    a = {} if hist is None else {"history": torch.zeros(rows, 0, dtype=torch.int64, device=DEV)}
+    if masked:
+        a["token_mask"] = torch.full((1, (V + 31) // 32), 0x55555555, dtype=torch.int32, device=DEV)
+        a["fill"] = -5.0
+    want = process_logits(x, **a)
+    up = torch.randn(rows, V, generator=g, device=DEV).to(dtype)
+    slope = torch.where(torch.arange(V, device=DEV) % 2 == 0, up, 0.0) if masked else up
+    for name, value in (("repetition_penalty", 0.0), ("repetition_penalty", INF), ("presence_penalty", math.nan),
+                        ("frequency_penalty", -INF)):
+        knob = torch.rand(rows, generator=g, device=DEV) + 0.5
+        assert torch.equal(process_logits(x, **a, **{name: knob}), want)
+        knob[rows - 2] = value
+        with pytest.raises(ValueError, match="repetition penalties must be finite and positive, the other penalties finite"):
+            process_logits(x, **a, **{name: knob})
+        leaf = x.clone().requires_grad_()
+        y = process_logits(leaf, **a, **{name: knob}, check=False)
+        (grad,) = torch.autograd.grad(y, leaf, up)
+        own = x.clone()
+        process_logits(own, **a, **{name: knob}, check=False, out=own)
+        good = torch.arange(rows, device=DEV) != rows - 2
+        for got, right in ((y.detach(), want), (own, want), (grad, slope)):
+            assert bool(got[rows - 2].isnan().all()) and torch.equal(got[good], right[good])

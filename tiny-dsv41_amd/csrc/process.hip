@@ -68,6 +68,7 @@ struct Params {
   const int32_t* mask_rows;
   float fill;
   int32_t* status;
+  bool knobs_of_rows() const { return rps || press || freqs; }
 };
 
 // What the lists say of an element: how often it was said, whether it is in the history at all, and its entry of the
@@ -571,7 +572,7 @@ void launch_lists(const Params& p, hipStream_t s) {
 }
 template <typename T, bool INPLACE>
 void launch(const Params& p, hipStream_t s) {
-  const bool lists = p.n_bias || p.history;
+  const bool lists = p.n_bias || p.history || p.knobs_of_rows();
   if (lists && p.mask) launch_lists<T, true, INPLACE>(p, s);
   else if (lists) launch_lists<T, false, INPLACE>(p, s);
   else if (p.mask) launch<T, false, true, INPLACE, false>(p, s);
@@ -581,8 +582,9 @@ template <typename T>
 void launch_grad(Params p, hipStream_t s) {
   const dim3 grid = grid_of(p, sizeof(T) == 4 ? SLICE : SHORT_SLICE);
   const size_t lds = (size_t)p.n_bias * sizeof(int);
-  if (p.history && p.mask) hipLaunchKernelGGL((process_grad_kernel<T, true, true>), grid, dim3(NT), lds, s, p);
-  else if (p.history) hipLaunchKernelGGL((process_grad_kernel<T, true, false>), grid, dim3(NT), lds, s, p);
+  const bool lists = p.history || p.knobs_of_rows();
+  if (lists && p.mask) hipLaunchKernelGGL((process_grad_kernel<T, true, true>), grid, dim3(NT), lds, s, p);
+  else if (lists) hipLaunchKernelGGL((process_grad_kernel<T, true, false>), grid, dim3(NT), lds, s, p);
   else if (p.mask) hipLaunchKernelGGL((process_grad_kernel<T, false, true>), grid, dim3(NT), lds, s, p);
   else hipLaunchKernelGGL((process_grad_kernel<T, false, false>), grid, dim3(NT), lds, s, p);
 }
@@ -648,10 +650,11 @@ int run(const dsv41_process_desc* d, bool grad, void* stream) {
     p.hist_len = d->hist_len;
     p.lens = d->history_lens;
     p.prompt_lens = d->history_prompt_lens;
-    p.rps = d->repetition_penalties;
-    p.press = d->presence_penalties;
-    p.freqs = d->frequency_penalties;
   }
+  // (rows' knobs are looked at without a history, too)
+  p.rps = d->repetition_penalties;
+  p.press = d->presence_penalties;
+  p.freqs = d->frequency_penalties;
   p.rp = d->repetition_penalty;
   p.pres = d->presence_penalty;
   p.freq = d->frequency_penalty;
