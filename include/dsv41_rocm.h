@@ -668,7 +668,8 @@ typedef struct dsv41_int_head_desc {
   int32_t vocab;
   const void* x;          /* bf16 [n_tokens, hidden] */
   int64_t x_row_stride;   /* in elements */
-  const int8_t* w;        /* the head's tiles, as dsv41_quantize_rows_run leaves them, 16-byte aligned */
+  const int8_t* w;        /* the head's tiles, as dsv41_quantize_rows_run leaves them, 16-byte aligned; a head that */
+                          /* holds -128, as that never leaves, has at most 132104 columns, or its sums wrap         */
   const float* scales;    /* [vocab], 16-byte aligned */
   void* out;              /* [n_tokens, vocab] */
   int64_t out_row_stride; /* in elements; rows that begin at multiples of 16 bytes are written faster */

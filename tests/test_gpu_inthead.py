@@ -186,6 +186,23 @@ def test_largest_sums(n):
         head_logits(torch.zeros(1, h + 1, device=DEV), Int8Head.from_quantized(w[:, :1].expand(70, h + 1), torch.ones(70, device=DEV)))
 
 
+@pytest.mark.parametrize("n", [2, 70, 200])
+def test_largest_sums_of_the_lowest_integer(n):
+    # 127 times -128, as often as 32 bits hold, in either sign: 132104 * 127 * 128 = 2^31 - 1024
+    h = 132104
+    x = torch.full((n, h), 127.0, dtype=torch.bfloat16, device=DEV)
+    x[1] = -127.0
+    w = torch.full((70, h), -128, dtype=torch.int8, device=DEV)
+    got = head_logits(x, Int8Head.from_quantized(w, torch.ones(70, device=DEV)))
+    want = float(2 ** 31 - 1024)
+    assert bool((got[0] == -want).all()) and bool((got[1] == want).all())
+    wide = torch.full((3, h + 1), 127, dtype=torch.int8, device=DEV)
+    Int8Head.from_quantized(wide, torch.ones(3, device=DEV))
+    wide[2, h] = -128
+    with pytest.raises(NotImplementedError, match="-128"):
+        Int8Head.from_quantized(wide, torch.ones(3, device=DEV))
+
+
 def test_accuracy_against_the_bf16_head():
     # rounding to 127 steps: each factor is off by half a step of its row's maximum at most, so a logit by
     # (|x|_1 max|w| + |w|_1 max|x|) / 254 and a quarter of a step's product a column

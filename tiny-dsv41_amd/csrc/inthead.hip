@@ -37,7 +37,7 @@ using TL = Tile<SQUARE>;
 using rows::bf16_t;
 constexpr int BM = TL::BV;
 constexpr int LINE = ROWB;            // columns are padded to whole lines
-constexpr int MAX_COLUMNS = 133120;   // 2^31 / 127^2 = 133144, in whole lines
+constexpr int MAX_COLUMNS = 133120;   // 2^31 / 127^2 = 133144, in whole lines (132104 where the head holds -128)
 constexpr int QUANT_NT = 256;
 // Tokens of head_kernel, and of ring_kernel.  17 tokens of 7168 -> 129280 (fp32): 176 us by the first, 161 by the second; 16
 // tokens 159 and 159, one 152 and 155.  128 tokens: 188 by the second, 214 by gemm_kernel; of 2048 -> 151936 82 and 98.

@@ -20,6 +20,7 @@ from ._check import any_set
 from .scores import fit_int32, launch, refuse_capture, refuse_tangents, written
 
 LINE, GROUP = 128, 64  # columns and rows are rounded up to these
+LOWEST_COLUMNS = (2 ** 31 - 1) // (127 * 128)  # of rows that hold -128: their products' sums fit 32 bits
 
 _OUT_DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 
@@ -36,7 +37,8 @@ class Int8Head:
 
     @staticmethod
     def from_quantized(weight: torch.Tensor, scales: torch.Tensor) -> "Int8Head":
-        """The head of int8 rows and their scales that a checkpoint holds, laid out for the kernels (a copy)."""
+        """The head of int8 rows and their scales that a checkpoint holds, laid out for the kernels (a copy).  Rows of more
+        than 132104 columns may not hold -128."""
         if not (weight.is_cuda and scales.is_cuda):
             raise ValueError("weight and scales must be on the GPU (libdsv41hip has no CPU path)")
         if weight.ndim != 2 or weight.dtype != torch.int8 or 0 in weight.shape:
@@ -44,6 +46,8 @@ class Int8Head:
         if scales.shape != weight.shape[:1] or not scales.is_floating_point():
             raise ValueError("scales must have one value per row of weight")
         v, h = weight.shape
+        if h > LOWEST_COLUMNS and int(weight.amin()) == -128:
+            raise NotImplementedError(f"rows that hold -128 have at most {LOWEST_COLUMNS} columns: more overflow a 32-bit sum")
         tiles = torch.zeros(_rounded(v, GROUP), _rounded(h, LINE), dtype=torch.int8, device=weight.device)
         tiles[:v, :h] = weight
         # group, (tile, row in four) of a group, four in a tile; column tile, 16 columns of it
