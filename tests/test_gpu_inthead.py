@@ -309,3 +309,25 @@ def test_refusals_on_the_gpu():
         head_logits(d, head, out=torch.empty(1, 50, device=DEV).expand(3, 50))
     with pytest.raises(ValueError, match="one value per row"):
         Int8Head.from_quantized(torch.zeros(3, 4, dtype=torch.int8, device=DEV), torch.ones(4, device=DEV))
+
+
+@pytest.mark.parametrize("n", [3, 40, 200])
+def test_out_beside_what_is_read(n):
+    # an out over the hidden states or the head is refused; columns beside them in the same buffer are not
+    x, w = _inputs(n, 128, 64)
+    head = quantize_head(w.to(DEV))
+    want = head_logits(x.to(DEV), head, dtype=torch.bfloat16)
+    both = torch.empty(n, 128 + 64, dtype=torch.bfloat16, device=DEV)
+    both[:, :128] = x.to(DEV)
+    hidden = both[:, :128]
+    for out in (both[:, 64:128], both[:, :64], both.view(-1)[100:100 + 64 * n].view(n, 64)):
+        with pytest.raises(ValueError, match="out overlaps"):
+            head_logits(hidden, head, out=out)
+    scales = torch.ones(64 * n + 64, device=DEV)
+    with pytest.raises(ValueError, match="out overlaps"):
+        head_logits(hidden, Int8Head(head.tiles, scales[:64], 64, 128), out=scales[60:60 + 64 * n].view(n, 64))
+    tiles = torch.zeros(8192 + 256 * n, dtype=torch.int8, device=DEV)
+    with pytest.raises(ValueError, match="out overlaps"):
+        head_logits(hidden, Int8Head(tiles[:8192], head.scales, 64, 128), out=tiles[4096:4096 + 256 * n].view(torch.float32).view(n, 64))
+    head_logits(hidden, head, out=both[:, 128:])
+    assert torch.equal(both[:, 128:], want) and torch.equal(both[:, :128].cpu(), x)

@@ -17,7 +17,7 @@ import torch
 
 from . import _lib
 from ._check import any_set
-from .scores import fit_int32, launch, refuse_capture, refuse_tangents, written
+from .scores import fit_int32, launch, overlap, refuse_capture, refuse_tangents, written
 
 LINE, GROUP = 128, 64  # columns and rows are rounded up to these
 LOWEST_COLUMNS = (2 ** 31 - 1) // (127 * 128)  # of rows that hold -128: their products' sums fit 32 bits
@@ -155,8 +155,8 @@ def head_logits(
     scales in fp32.  A row's logits do not depend on the batch it is in.
 
     The result's rows begin at multiples of 64 elements, so that of a vocabulary that is none it is a
-    view; ``out`` (rows at any stride that holds them) takes it instead.  There is no gradient: hidden states
-    that require one are refused where it is recorded (:func:`selected_log_probs` is the learner's head).
+    view; ``out`` (rows at any stride that holds them, in memory of their own) takes it instead.  There is no gradient:
+    hidden states that require one are refused where it is recorded (:func:`selected_log_probs` is the learner's head).
 
     With ``check`` the call synchronises and raises ``ValueError`` for hidden states with a NaN or an
     infinity; without, their rows are NaN.
@@ -172,6 +172,8 @@ def head_logits(
             raise ValueError("out must have contiguous rows that do not overlap")
         if out.requires_grad and torch.is_grad_enabled():
             raise NotImplementedError("the 8-bit head has no gradient: call under no_grad")
+        if overlap(out, x, head.tiles, head.scales):
+            raise ValueError("out overlaps the hidden states or the head")
     elif dtype not in _OUT_DTYPES:
         raise ValueError("logits are torch.float32 or torch.bfloat16")
     else:

@@ -105,16 +105,38 @@ def written(t) -> None:
         torch.autograd.graph.increment_version(t)
 
 
-def overlap(a, b) -> bool:
-    """Whether the memory that two tensors of nonnegative strides reach over meets."""
-    def extent(t):
-        last = sum((n - 1) * step for n, step in zip(t.shape, t.stride()))
-        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+def _extent(t):
+    """The addresses that a tensor of nonnegative strides reaches over."""
+    n = t.numel()
+    if n and not t.is_contiguous():
+        n = 1 + sum((m - 1) * step for m, step in zip(t.shape, t.stride()))
+    begin = t.data_ptr()
+    return begin, begin + n * t.element_size()
 
-    if a.numel() == 0 or b.numel() == 0 or a.device != b.device:
-        return False
-    (a0, a1), (b0, b1) = extent(a), extent(b)
-    return a0 < b1 and b0 < a1
+
+def overlap(out, *others) -> bool:
+    """Whether the memory that ``out`` reaches over meets that of others on its device; of matrices whose rows are as far
+    apart, whether their rows do (columns side by side of one buffer do not)."""
+    begin, end = _extent(out)
+    for t in others:
+        b, e = _extent(t)
+        if begin < e and b < end and begin != end and b != e and _rows_meet(out, t, b - begin):
+            return True
+    return False
+
+
+def _rows_meet(a, b, apart):
+    """:func:`overlap` of two whose extents do; ``b`` begins ``apart`` bytes behind ``a``."""
+    if not (a.ndim == b.ndim == 2 and a.stride(1) == b.stride(1) == 1):
+        return True
+    step = a.stride(0) * a.element_size()
+    width_a, width_b = (t.shape[1] * t.element_size() for t in (a, b))
+    if step != b.stride(0) * b.element_size() or step < max(width_a, width_b):
+        return True
+    # b's row j begins `past` bytes behind the begin of a's row j + ahead, and may reach into the next one
+    ahead, past = divmod(apart, step)
+    meet = lambda shift: max(0, shift) < min(a.shape[0], b.shape[0] + shift)
+    return past < width_a and meet(ahead) or past + width_b > step and meet(ahead + 1)
 
 
 def vector(t, dtype, shape, device):
