@@ -512,3 +512,11 @@ def test_penalties_of_rows_without_a_history(dtype, hist, masked, rows):
         good = torch.arange(rows, device=DEV) != rows - 2
         for got, right in ((y.detach(), want), (own, want), (grad, slope)):
             assert bool(got[rows - 2].isnan().all()) and torch.equal(got[good], right[good])
+
+
+def test_an_out_that_is_no_tensor_is_refused():
+    x = torch.zeros(2, 40, device=DEV)
+    for logits in (x, x.clone().requires_grad_()):
+        for bad in (3, [x], "out"):
+            with pytest.raises(ValueError, match="out must have the shape"):
+                process_logits(logits, out=bad)

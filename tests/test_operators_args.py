@@ -10,7 +10,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from dsv41_rocm import (Int8Head, _lib, head_logits, process_logits, quantize_head, token_embedding,
+from dsv41_rocm import (Int8Head, _lib, head_logits, process, process_logits, quantize_head, token_embedding,
                         token_embedding_backward)
 
 HEADER = Path(__file__).resolve().parents[1] / "include" / "dsv41_rocm.h"
@@ -252,6 +252,29 @@ def test_embed_grad_workspace():
 def test_ids_that_are_no_tensor_are_refused():
     with pytest.raises(ValueError, match="integers"):
         token_embedding_backward(torch.zeros(2, 5), [1, 2], 5)
+
+
+def test_lists_that_are_no_tensors_are_refused():
+    # by name, whatever else there is to refuse
+    x, ids = torch.zeros(2, 10), torch.zeros(2, 3, dtype=torch.int64)
+
+    def arguments(**kw):
+        names = ("history", "history_lens", "history_prompt_lens", "repetition_penalty", "presence_penalty", "frequency_penalty",
+                 "bias_ids", "bias", "token_mask", "mask_rows", "fill")
+        neutral = {"repetition_penalty": 1.0, "presence_penalty": 0.0, "frequency_penalty": 0.0, "fill": 0.0}
+        return process._arguments(x, *(kw.get(n, neutral.get(n)) for n in names))
+
+    for bad in ([[1, 2, 3], [4, 5, 6]], 7, "ids"):
+        with pytest.raises(ValueError, match="history must have shape"):
+            arguments(history=bad)
+        with pytest.raises(ValueError, match="bias_ids and bias must have shape"):
+            arguments(bias_ids=ids, bias=bad)
+        with pytest.raises(ValueError, match="bias_ids and bias must have shape"):
+            arguments(bias_ids=bad, bias=x[:, :3])
+        with pytest.raises(ValueError, match="token_mask must be"):
+            arguments(token_mask=bad)
+        with pytest.raises(ValueError, match="out must have the shape"):
+            process._output(bad, x)
 
 
 def test_host_tensors_are_refused():

@@ -84,7 +84,7 @@ def _arguments(logits, history, history_lens, history_prompt_lens, repetition_pe
     pres, press = _knob(presence_penalty, "presence_penalty", 0.0, rows, dev)
     freq, freqs = _knob(frequency_penalty, "frequency_penalty", 0.0, rows, dev)
     if history is not None:
-        if history.ndim != 2 or history.shape[0] != rows:
+        if not isinstance(history, torch.Tensor) or history.ndim != 2 or history.shape[0] != rows:
             raise ValueError("history must have shape [rows, history_length]")
         history = _rows_of(_integers(history, "history", torch.int64, dev))
         if history_lens is not None:
@@ -94,6 +94,8 @@ def _arguments(logits, history, history_lens, history_prompt_lens, repetition_pe
     elif history_lens is not None or history_prompt_lens is not None:
         raise ValueError("history_lens and history_prompt_lens require a history")
     if bias is not None and bias_ids is not None:
+        if not (isinstance(bias, torch.Tensor) and isinstance(bias_ids, torch.Tensor)):
+            raise ValueError("bias_ids and bias must have shape [rows, entries] or [entries]")
         if bias.requires_grad and torch.is_grad_enabled():
             raise NotImplementedError("bias has no gradient: detach it")
         refuse_tangents("biases", bias)
@@ -274,9 +276,9 @@ def process_logits(
     refuse_capture(check)
     tracked = torch.is_grad_enabled() and logits.requires_grad
     if out is not None:
+        out = _output(out, logits)
         if tracked or torch.is_grad_enabled() and out.requires_grad:
             raise ValueError("a call with out has no gradient: leave it out, or call under no_grad")
-        out = _output(out, logits)
         status = forward(logits, numbers, tensors, out, check)
         written(out)
     elif tracked:
