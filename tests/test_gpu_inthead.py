@@ -331,3 +331,14 @@ def test_out_beside_what_is_read(n):
         head_logits(hidden, Int8Head(tiles[:8192], head.scales, 64, 128), out=tiles[4096:4096 + 256 * n].view(torch.float32).view(n, 64))
     head_logits(hidden, head, out=both[:, 128:])
     assert torch.equal(both[:, 128:], want) and torch.equal(both[:, :128].cpu(), x)
+
+
+def test_heads_and_outs_of_other_types_are_refused():
+    x, w = _inputs(3, 200, 50)
+    head = quantize_head(w.to(DEV))
+    for bad in (w.to(DEV), None, (head.tiles, head.scales)):
+        with pytest.raises(ValueError, match="Int8Head"):
+            head_logits(x.to(DEV), bad)
+    for bad in (3, [x]):
+        with pytest.raises(ValueError, match="out must be"):
+            head_logits(x.to(DEV), head, out=bad)

@@ -10,7 +10,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from dsv41_rocm import (Int8Head, _lib, head_logits, process, process_logits, quantize_head, token_embedding,
+from dsv41_rocm import (Int8Head, _lib, head_logits, inthead, process, process_logits, quantize_head, token_embedding,
                         token_embedding_backward)
 
 HEADER = Path(__file__).resolve().parents[1] / "include" / "dsv41_rocm.h"
@@ -275,6 +275,22 @@ def test_lists_that_are_no_tensors_are_refused():
             arguments(token_mask=bad)
         with pytest.raises(ValueError, match="out must have the shape"):
             process._output(bad, x)
+
+
+def test_heads_and_outs_that_are_no_tensors_are_refused():
+    x, ids = torch.zeros(2, 10), torch.zeros(2, dtype=torch.int64)
+    for bad in ([[1]], 3, None):
+        with pytest.raises(ValueError, match="weight must be int8"):
+            Int8Head.from_quantized(bad, x[0])
+        with pytest.raises(ValueError, match="weight must be int8"):
+            Int8Head.from_quantized(x.to(torch.int8), bad)
+        with pytest.raises(ValueError, match="Int8Head"):
+            inthead._check_head(bad, x)
+    with pytest.raises(ValueError, match="Int8Head"):
+        inthead._check_head(x, x)
+    for bad in ([1], 3):
+        with pytest.raises(ValueError, match="out must be"):
+            token_embedding_backward(x, ids, out=bad)
 
 
 def test_host_tensors_are_refused():

@@ -113,6 +113,8 @@ def token_embedding_backward(
         raise ValueError("ids must be integers")
     if not isinstance(grad, torch.Tensor) or grad.ndim < 1 or grad.shape[-1] == 0 or grad.shape[:-1] != ids.shape:
         raise ValueError("grad must have the shape of ids and the hidden size")
+    if out is not None and not isinstance(out, torch.Tensor):
+        raise ValueError("out must be fp32 or bf16 [vocabulary_size, hidden] on the GPU of grad")
     if not grad.is_cuda:
         raise ValueError("grad must be on the GPU (libdsv41hip has no CPU path)")
     refuse_tangents("gradients", grad)

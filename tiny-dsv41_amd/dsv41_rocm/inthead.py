@@ -39,6 +39,8 @@ class Int8Head:
     def from_quantized(weight: torch.Tensor, scales: torch.Tensor) -> "Int8Head":
         """The head of int8 rows and their scales that a checkpoint holds, laid out for the kernels (a copy).  Rows of more
         than 132104 columns may not hold -128."""
+        if not (isinstance(weight, torch.Tensor) and isinstance(scales, torch.Tensor)):
+            raise ValueError("weight must be int8 [vocab, hidden], with one scale per row")
         if not (weight.is_cuda and scales.is_cuda):
             raise ValueError("weight and scales must be on the GPU (libdsv41hip has no CPU path)")
         if weight.ndim != 2 or weight.dtype != torch.int8 or 0 in weight.shape:
@@ -106,6 +108,8 @@ def quantize_head(weight: torch.Tensor, *, check: bool = True) -> Int8Head:
 
 
 def _check_head(head, x):
+    if not isinstance(head, Int8Head):
+        raise ValueError("the head must be an Int8Head: make it with quantize_head or Int8Head.from_quantized")
     v, h = head.vocab, head.hidden
     if x.shape[1] != h:
         raise ValueError("hidden must be [tokens, hidden] and the head [vocab, hidden]")
@@ -162,11 +166,11 @@ def head_logits(
     infinity; without, their rows are NaN.
     """
     x = _rows(hidden, "hidden")
-    n, v = x.shape[0], head.vocab
     _check_head(head, x)
+    n, v = x.shape[0], head.vocab
     given = out
     if out is not None:
-        if out.shape != (n, v) or out.dtype not in _OUT_DTYPES or out.device != x.device:
+        if not isinstance(out, torch.Tensor) or out.shape != (n, v) or out.dtype not in _OUT_DTYPES or out.device != x.device:
             raise ValueError("out must be fp32 or bf16 [tokens, vocab] on the GPU of the hidden states")
         if v > 1 and out.stride(1) != 1 or n > 1 and out.stride(0) < v:
             raise ValueError("out must have contiguous rows that do not overlap")
