@@ -671,7 +671,7 @@ typedef struct dsv41_int_head_desc {
   const int8_t* w;        /* the head's tiles, as dsv41_quantize_rows_run leaves them, 16-byte aligned; a head that */
                           /* holds -128, as that never leaves, has at most 132104 columns, or its sums wrap         */
   const float* scales;    /* [vocab], 16-byte aligned */
-  void* out;              /* [n_tokens, vocab] */
+  void* out;              /* [n_tokens, vocab], in memory of its own: x is read while it is written */
   int64_t out_row_stride; /* in elements; rows that begin at multiples of 16 bytes are written faster */
   int32_t out_dtype;      /* DSV41_DTYPE_F32 or DSV41_DTYPE_BF16 */
   int32_t* out_status;    /* [n_tokens] or NULL */

@@ -334,8 +334,8 @@ __global__ __launch_bounds__(SUM_NT) void sum_kernel(GradParams p) {
 #pragma unroll
   for (int j = 0; j < G; ++j) s[j] = 0.f;
   constexpr int U = 16;  // rows in flight
-  // Onto a gradient of the same type, finished ids' rows are read beside them: 16384 bf16 rows of 7168 take 172 us,
-  // 185 where each waits for its own.
+  // Onto a gradient of the same type, finished ids' rows are read beside them: 16384 bf16 rows of 7168, all three kernels,
+  // 111 us, 121 where each waits for its own (7027 ids, log-uniform and spread over 129280); uniform ids 158 and 170.
   constexpr bool EARLY = ONTO && std::is_same<TG, TO>::value;
 #pragma unroll
   for (int c = 0; c < CHUNK; c += U) {

@@ -9,18 +9,22 @@
 //
 // The columns are padded to a multiple of 128 (one cache line of a row), those of q with zeros.
 //
-// head_kernel, up to 16 tokens, is bound by reading w once: one token, 7168 -> 129280, 130 us (7.1 TB/s, what a
-// nontemporal read reaches).  A workgroup takes 64 rows of w, its four waves every fourth k-step of their columns;
+// Times below are of calls, the quantization's launch (3 to 12 us) included, unless they say "kernel".
+//
+// head_kernel, up to 16 tokens, is bound by reading w once: one token, 7168 -> 129280, kernel 130 us (7.1 TB/s, what a
+// nontemporal read reaches), call 135.  A workgroup takes 64 rows of w, its four waves every fourth k-step of their columns;
 // fragments go from memory to registers with no LDS between, so the rows lie in memory as tiles of a fragment's lanes.
 // (Row-major, each load of a wave met 16 lines, and the loads' rate was the bound: 203 us.)  The waves' integer sums
 // meet in LDS.
-// ring_kernel, up to 128 tokens, shares the tokens' tiles among up to 256 rows of w, by LDS: in head_kernel, whose
-// workgroups read them from L2 for every 64 rows, 64 tokens of 7168 -> 129280 took 205 us, and 170 here; of 2048 -> 151936
-// 73 and 69.
+// ring_kernel, up to 128 tokens, shares the tokens' tiles among up to 256 rows of w, by LDS: 64 tokens of 7168 -> 129280 164
+// us, of 2048 -> 151936 67.  Builds whose head_kernel took them, with the tokens' tiles read from L2 for every 64 rows: 205
+// and 73, and for every 128 of long rows 178 to 185.
 // gemm_kernel, above, has the schedule of the bf16 products (mfma_tile.h): eight waves whose pairs multiply and read in
 // turns, stages of 128 columns loaded straight to LDS, tiles of 256 rows x 192, 256 or 320 tokens.  4096 tokens of 7168 ->
-// 129280: 2.69 ms, 2.8 POP/s, the matrix cores busy 71% of the cycles at 1.75 GHz (power); of 2048 -> 151936 1.11 ms,
-// 2.3 POP/s: a tile there has 16 stages, and a fifth of its time is the conversion and stores of its logits.
+// 129280: bf16 2.61 ms, 2.9 POP/s, fp32 2.90; of 2048 -> 151936 bf16 1.10, 2.3 POP/s, fp32 1.35.  Power bounds the long rows
+// (300 tokens in tiles of 256: the matrix cores busy 71% of the cycles at 1.73 GHz).  Of 2048 columns a tile has 16 stages,
+// and a fifth of its time is the conversion and stores of its logits; of 1024 columns that is nearly half, of fewer more: 4096
+// tokens of 1024, 512 and 256 columns -> 151936 take 712, 555 and 457 us in bf16, 944, 777 and 690 in fp32.
 
 #include <algorithm>
 #include <iterator>
@@ -39,8 +43,9 @@ constexpr int BM = TL::BV;
 constexpr int LINE = ROWB;            // columns are padded to whole lines
 constexpr int MAX_COLUMNS = 133120;   // 2^31 / 127^2 = 133144, in whole lines (132104 where the head holds -128)
 constexpr int QUANT_NT = 256;
-// Tokens of head_kernel, and of ring_kernel.  17 tokens of 7168 -> 129280 (fp32): 176 us by the first, 161 by the second; 16
-// tokens 159 and 159, one 152 and 155.  128 tokens: 188 by the second, 214 by gemm_kernel; of 2048 -> 151936 82 and 98.
+// Tokens of head_kernel (a fragment's, at most), and of ring_kernel.  By the first and the second, fp32: 16 tokens of 7168 ->
+// 129280 149 and 150 us, 8 141 and 144, one 135 and 140; of 2048 -> 151936 55 and 58, 53 and 55, 51 and 53.  By the second and
+// gemm_kernel: 17 tokens of 7168 149 and 155, 128 183 and 184; of 2048 57 and 71, 80 and 88.
 constexpr int FEW = 16, RING_TOKENS = 128;
 
 typedef int intx4 __attribute__((ext_vector_type(4)));
@@ -179,9 +184,11 @@ __global__ __launch_bounds__(QUANT_NT) void quantize_kernel(const bf16_t* x, int
 
 // -------------------------------------------------------------------------------- few tokens
 // waves of a workgroup, steps of theirs in registers, workgroups of a CU: of one token, 2048 -> 151936 and 7168 -> 129280,
-// 52 and 151 us; eight waves 54 and 155, two (four workgroups) 57 and 153, five steps ahead 60 and 152.
+// quantized by a launch before it, 51 and 135 us; eight waves (one workgroup) 51 and 138, two (four workgroups) 57 and 138,
+// five steps ahead 53 and 137.
 constexpr int SPLIT = 4, DEPTH = 4, PER_CU = 2;
-// tokens that head_kernel quantizes itself (of eight: one token 48.9 us for 47.7), their columns, LDS bytes that shift banks
+// tokens that head_kernel quantizes itself (with room for eight, one token took 48.9 us for 47.7 on one build), their columns,
+// LDS bytes that shift banks
 constexpr int OWN = 4, OWN_COLUMNS = 64 * SPLIT * 8, OWN_PAD = 64;
 
 struct Params {
@@ -216,7 +223,7 @@ __device__ __forceinline__ void swap_halves(uint32_t& a, uint32_t& b) {
 }
 // 64 neighbouring logits, from column v on, of each of 16 tokens: lane (quad, token) has columns 16 quad .. + 15 in
 // c0 .. c3.  The quads exchange theirs, so that a store of 16 bytes a lane writes 64 neighbouring bytes of a token's row
-// (4096 tokens, 2048 -> 151936: fp32 1573 us without, bf16 1133).  All lanes take part; those of tokens that do not
+// (4096 tokens, 2048 -> 151936, fp32: 1331 us, 1573 on the build before).  All lanes take part; those of tokens that do not
 // exist (there == false) store nothing.  `wide`: rows begin at multiples of 16 bytes.
 template <typename T>
 __device__ __forceinline__ void store_logits(T* row, int v, int V, bool there, bool wide, const intx4& c0, const intx4& c1,
@@ -377,7 +384,7 @@ __global__ __launch_bounds__(64 * SPLIT, SPLIT * PER_CU / 4) void head_kernel(Pa
 // A workgroup takes a run of groups, up to four at a time, against all tokens, 32 NB at most: wave (wv, wt) group wv's 64 rows
 // and half of the tokens.  Stages of 128 columns go straight to a ring of RING in LDS, RING - 1 of them on their way from
 // memory throughout; one barrier a stage says that it has come and that the one before it is free.
-// load_lds of what is read once: 7168 -> 129280, 128 tokens 216 us without the hint, 197 with it
+// load_lds of what is read once: 7168 -> 129280, 128 tokens 208 us without the hint, 183 with it; 64 tokens 189 and 164
 __device__ __forceinline__ void load_lds_once(v4i rs, uint32_t voff, uint32_t lds_addr) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen nt lds" ::"v"(voff), "s"(rs),
                "s"(lds_addr)
@@ -483,7 +490,7 @@ __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) v
 
 // ------------------------------------------------------------------------------- many tokens
 // W1: blocks of 16 tokens of a wave beyond its first two: tiles of 192 tokens (1), 256 (2) or 320 (3).  ONCE: one tile has all
-// tokens, so that no other reads the weights again (256 tokens of 7168 -> 129280 256 us without the hint, 237 with it).
+// tokens, so that no other reads the weights again (256 tokens of 7168 -> 129280 250 us without the hint, 224 with it).
 template <typename T, int W1, bool ONCE>
 __global__ __launch_bounds__(NT, 1) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_kernel(Params p, bool wide) {
   constexpr int WT = 2 + W1, BN = 64 * WT, AHEAD = 6 + W1;  // loads of a wave's four regions
@@ -692,14 +699,16 @@ int check_head(const dsv41_int_head_desc* d) {
 
 size_t scales_at(const dsv41_int_head_desc* d) { return (size_t)((d->n_tokens + 15) / 16 * 16) * padded_of(d->hidden); }
 
-// What a block of rows costs against a tile of 128 + 64 W1 tokens, 256 tokens' being 1.  Tiles of 256 or 192 and of 320, us:
-// 300 tokens of 7168 -> 129280 (fp32) 337 and 281, of 2048 -> 151936 143 and 138, 600 tokens 553 and 500, 247 and 230; but
-// 4096 tokens of 7168 3026 and 3050.  Of 256 and 192: 576 tokens of 2048 -> 151936 (bf16) 195 and 167; but 256 tokens 99
-// and 110, 1100 tokens 330 and 344, 4096 tokens 1136 and 1221.
+// What a block of rows costs against a tile of 128 + 64 W1 tokens, 256 tokens' being 1.  Tiles of 192, 256 and 320, us: 256
+// tokens of 7168 -> 129280 (fp32) 299, 226 and 247, 300 tokens 313, 352 and 256, 600 570, 519 and 468, 4096 3192, 2903 and
+// 2900; of 2048 -> 151936 256 tokens (bf16) 105, 93 and 102, 300 (fp32) 129, 162 and 129, 576 (bf16) 174, 195 and 176, 600
+// (fp32) 248, 221 and 209, 1100 (bf16) 345, 311 and 327, 4096 (bf16) 1220, 1096 and 1087.  The stores of short rows' logits
+// have no part in it: 4096 tokens of 256, 512 and 1024 columns (bf16) take the tiles of 256, 458, 555 and 709, where those
+// of 320 take 427, 516 and 678.
 constexpr double TILE_COST[4] = {0, 0.85, 1.0, 1.2};
 
-// Whether head_kernel quantizes the tokens: 2048 -> 151936, one and four tokens 47.7 and 48.8 us, 50.4 and 51.7 by a launch
-// before it; of 7168 -> 129280 one token, whose parts a thread would hold together, 136.4 and 134.9.
+// Whether head_kernel quantizes the tokens: 2048 -> 151936, one and four tokens 48.6 and 49.5 us, 51.3 and 51.9 by a launch
+// before it; of 7168 -> 129280 one token, whose parts a thread held together on a build that did so, 136.4 and 134.9.
 bool own_quantization(int n, int cols) { return n <= OWN && cols <= OWN_COLUMNS && cols % 8 == 0; }
 
 // As many workgroups as fit on the GPU together take the same number of groups each.

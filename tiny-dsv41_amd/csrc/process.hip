@@ -20,11 +20,14 @@
 // read for the history's ids while the gradient's own are on their way.
 //
 // Slices begin at memory lines of the result, so rows of an odd vocabulary are written by whole lines: 500 bf16 rows of
-// 151851 copied in 51 us (5.9 TB/s of read and write), as many of 151936 in 53.  2048 fp32 rows: 434 us (5.7 TB/s),
-// with masks 443, with histories of 4096 464; bf16 214, 219 and 262.  256 to 1024 threads and slices of 8192 to 16384 ids, before the loads of a slice went
-// together: 512 and 8192 the best or within 3% (2048 fp32 rows with histories 477; 1024 and 16384: 506, 256 and 8192: 778).
-// What bounds it: memory, and beside long histories of bf16 rows the instructions of reading the lists, once a slice
-// (2048 ids cost 500 rows 12 us).
+// 151851 copied in 51 us (5.9 TB/s of read and write), as many of 151936 in 50.  2048 fp32 rows of 151936: 432 us (5.8
+// TB/s), with masks 441, with histories of 2048 and 4096 440 and 464 (452 where they are ragged, three quarters of that); bf16 213,
+// 218, 239 and 265.  256 to 1024 threads and slices of 8192 to 16384 ids, timed before the loads of a slice went together:
+// 512 and 8192 the best or within 3% (2048 fp32 rows with ragged histories 477; 1024 and 16384: 506, 256 and 8192: 778).
+// The gradient: 500 fp32 rows of 151851 111 us, with masks 114, with histories of 2048 146, with both 150; bf16 56, 63, 90
+// and 91; 1000 fp32 rows of 151936 214 us (5.7 TB/s), with masks 219, with histories of 4096 334.
+// What bounds it: memory, and beside long histories the instructions of reading the lists, once a slice (2048 ids cost
+// 500 bf16 rows 16 to 18 us), in the gradient the single logits, too.
 
 #include <math.h>
 
@@ -337,7 +340,7 @@ __device__ __forceinline__ void load_groups(const T* x, bool inside, const uint3
 // `batch(first, ids)` for every AHEAD entries of a thread; the first ones were loaded ahead of the slice itself, as loads come back
 // in order.
 // (EACH: loads that wait for one another.  In the gradient and with short words they are better so, 500 bf16 rows by 2 us
-// each; 2048 fp32 rows take 459 us that way and 452 with all of them together.)
+// each; 2048 fp32 rows with ragged histories take 459 us that way and 452 with all of them together.)
 template <bool EACH>
 __device__ __forceinline__ void load_ahead(const Row& r, int j0, uint2 (&ids)[AHEAD]) {
 #pragma unroll
@@ -561,8 +564,8 @@ void launch(Params p, hipStream_t s) {
   hipLaunchKernelGGL((process_kernel<T, LISTS, MASK, INPLACE, SHORT>), grid, dim3(NT), lds, s, p);
 }
 // Words of 16 bits take what they hold of bf16 rows' lists, in batches that fill the GPU with the longer slices too.  With
-// histories of 2048 and 4096 and in place with 2048, us, 32 and 16 bits: 2048 rows 244 and 236, 286 and 262, 257 and 226; 500
-// rows 66 and 64, 78 and 71, 57 and 50; 200 rows 27.7 and 27.6, 32.4 and 30.7, 27.2 and 24.8.
+// histories of 2048 and 4096 and in place with 2048, us, 32 and 16 bits: 2048 rows 244 and 238, 288 and 264, 257 and 227; 500
+// rows 68 and 66, 80 and 74, 57 and 50; 200 rows 26.3 and 26.5, 31.0 and 29.5, 26.4 and 23.9.
 template <typename T, bool MASK, bool INPLACE>
 void launch_lists(const Params& p, hipStream_t s) {
   if constexpr (sizeof(T) == 2)
