@@ -17,8 +17,8 @@
 // (Row-major, each load of a wave met 16 lines, and the loads' rate was the bound: 203 us.)  The waves' integer sums
 // meet in LDS.
 // ring_kernel, up to 128 tokens, shares the tokens' tiles among up to 256 rows of w, by LDS: 64 tokens of 7168 -> 129280 164
-// us, of 2048 -> 151936 67.  Builds whose head_kernel took them, with the tokens' tiles read from L2 for every 64 rows: 205
-// and 73, and for every 128 of long rows 178 to 185.
+// us, of 2048 -> 151936 67.  Earlier, head_kernel took them, with the tokens' tiles read from L2 for every 64 rows: 205 and
+// 73, and for every 128 of long rows 178 to 185.
 // gemm_kernel, above, has the schedule of the bf16 products (mfma_tile.h): eight waves whose pairs multiply and read in
 // turns, stages of 128 columns loaded straight to LDS, tiles of 256 rows x 192, 256 or 320 tokens.  4096 tokens of 7168 ->
 // 129280: bf16 2.61 ms, 2.9 POP/s, fp32 2.90; of 2048 -> 151936 bf16 1.10, 2.3 POP/s, fp32 1.35.  Power bounds the long rows
@@ -187,7 +187,7 @@ __global__ __launch_bounds__(QUANT_NT) void quantize_kernel(const bf16_t* x, int
 // quantized by a launch before it, 51 and 135 us; eight waves (one workgroup) 51 and 138, two (four workgroups) 57 and 138,
 // five steps ahead 53 and 137.
 constexpr int SPLIT = 4, DEPTH = 4, PER_CU = 2;
-// tokens that head_kernel quantizes itself (with room for eight, one token took 48.9 us for 47.7 on one build), their columns,
+// tokens that head_kernel quantizes itself (with room for eight, one token took 48.9 us instead of 47.7), their columns,
 // LDS bytes that shift banks
 constexpr int OWN = 4, OWN_COLUMNS = 64 * SPLIT * 8, OWN_PAD = 64;
 
@@ -223,7 +223,7 @@ __device__ __forceinline__ void swap_halves(uint32_t& a, uint32_t& b) {
 }
 // 64 neighbouring logits, from column v on, of each of 16 tokens: lane (quad, token) has columns 16 quad .. + 15 in
 // c0 .. c3.  The quads exchange theirs, so that a store of 16 bytes a lane writes 64 neighbouring bytes of a token's row
-// (4096 tokens, 2048 -> 151936, fp32: 1331 us, 1573 on the build before).  All lanes take part; those of tokens that do not
+// (4096 tokens, 2048 -> 151936, fp32: 1331 us, 1573 without).  All lanes take part; those of tokens that do not
 // exist (there == false) store nothing.  `wide`: rows begin at multiples of 16 bytes.
 template <typename T>
 __device__ __forceinline__ void store_logits(T* row, int v, int V, bool there, bool wide, const intx4& c0, const intx4& c1,
@@ -708,7 +708,7 @@ size_t scales_at(const dsv41_int_head_desc* d) { return (size_t)((d->n_tokens + 
 constexpr double TILE_COST[4] = {0, 0.85, 1.0, 1.2};
 
 // Whether head_kernel quantizes the tokens: 2048 -> 151936, one and four tokens 48.6 and 49.5 us, 51.3 and 51.9 by a launch
-// before it; of 7168 -> 129280 one token, whose parts a thread held together on a build that did so, 136.4 and 134.9.
+// before it; of 7168 -> 129280 one token, whose parts a thread then has to hold together, 136.4 and 134.9.
 bool own_quantization(int n, int cols) { return n <= OWN && cols <= OWN_COLUMNS && cols % 8 == 0; }
 
 // As many workgroups as fit on the GPU together take the same number of groups each.
